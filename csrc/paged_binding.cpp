@@ -1,0 +1,188 @@
+// Torch-facing wrappers of the paged KV cache (csrc/paged_kernels.h).  What a call looks at on the host is checked before the
+// device, so that a refused call is refused anywhere.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <pybind11/pybind11.h>
+#include <torch/extension.h>
+
+#include <cmath>
+
+#include "paged_kernels.h"
+
+namespace py = pybind11;
+using namespace penny;
+
+namespace {
+using OptTensor = c10::optional<at::Tensor>;
+
+cudaStream_t cur() { return at::cuda::getCurrentCUDAStream().stream(); }
+void need(bool ok, const char* msg) { TORCH_CHECK(ok, "penny: ", msg); }
+void ck(cudaError_t rc, const char* what) { TORCH_CHECK(rc == cudaSuccess, "penny: ", what, ": ", cudaGetErrorString(rc)); }
+bool aligned(const at::Tensor& t) { return ((uintptr_t)t.data_ptr() & 15) == 0; }
+bool ints(const at::Tensor& t, int64_t n) { return t.scalar_type() == at::kInt && t.is_contiguous() && t.dim() == 1 && t.numel() == n; }
+bool no_grad(const at::Tensor& t) { return !t.requires_grad() || !at::GradMode::is_enabled(); }
+
+PagedType type_of(const at::Tensor& t, const char* msg) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return PAGED_BF16;
+    case at::kHalf: return PAGED_FP16;
+    case at::kFloat8_e4m3fn: return PAGED_E4M3;
+    default: need(false, msg); return PAGED_BF16;
+  }
+}
+
+// k and v as a pool, with the scales that its type needs.
+PagedPool pool_of(const at::Tensor& k, const at::Tensor& v, PagedType type, PagedType cache, const OptTensor& k_scale, const OptTensor& v_scale) {
+  need(k.dim() == 4 && v.sizes() == k.sizes() && v.strides() == k.strides() && v.scalar_type() == k.scalar_type(),
+       "paged caches: k and v [pages, page_size, kv_heads, dim] of one type, shape and strides");
+  need(k.size(0) >= 1 && k.size(1) >= 1 && k.size(2) >= 1 && k.size(0) < (1ll << 31) && k.size(1) < (1ll << 31), "paged caches: pages and heads");
+  need(cache == PAGED_E4M3 || cache == type, "paged caches: of the projection's type or e4m3");
+  need(k.stride(3) == 1 && aligned(k) && aligned(v), "paged caches: contiguous in dim, 16-byte aligned");
+  const int64_t size = k.element_size();
+  for (int i = 0; i < 3; ++i) need(k.stride(i) * size % 16 == 0 && k.stride(i) >= 0, "paged caches: strides of whole 16 bytes");
+  need(k_scale.has_value() == (cache == PAGED_E4M3) && v_scale.has_value() == (cache == PAGED_E4M3), "k_scale and v_scale: beside e4m3 caches, and only there");
+  PagedPool p = {k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), nullptr, nullptr,
+                 (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)k.size(3)};
+  if (cache == PAGED_E4M3) {
+    for (const at::Tensor* s : {&*k_scale, &*v_scale})
+      need(s->scalar_type() == at::kFloat && s->is_contiguous() && s->dim() == 1 && s->numel() == k.size(2), "k_scale and v_scale: [kv_heads] fp32");
+    p.k_scale = k_scale->data_ptr<float>();
+    p.v_scale = v_scale->data_ptr<float>();
+  }
+  return p;
+}
+void on_device(const at::Tensor& first, std::initializer_list<const at::Tensor*> rest, const char* msg) {
+  bool ok = first.is_cuda();
+  for (const at::Tensor* t : rest) ok = ok && t->device() == first.device();
+  need(ok, msg);
+}
+int sms_of(int device) {
+  int sms = 0;
+  ck(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "device");
+  return sms;
+}
+}  // namespace
+
+void bind_paged(py::module_& m) {
+  m.attr("PAGED_MAX_ROWS") = kPagedMaxRows;
+  // Tokens come (news[r] > 0) and leave (news[r] < 0, the last ones): table, lengths, free and free_count in place; returns or
+  // fills (slots [tokens] int64, positions [tokens] int32, offsets [rows + 1] int32, granted [rows] bool).
+  m.def("page_tables", [](at::Tensor table, at::Tensor lengths, at::Tensor free, at::Tensor free_count, at::Tensor news, int64_t page_size,
+                          int64_t tokens, c10::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>> out) {
+    need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1, "page_tables: table [rows, pages of a row] int32");
+    const int64_t R = table.size(0), W = table.size(1);
+    need(R <= kPagedMaxRows, "page_tables: more than PAGED_MAX_ROWS rows");
+    need((W == 1 || table.stride(1) == 1) && (R == 1 || table.stride(0) >= W), "page_tables: a table with contiguous rows that do not overlap");
+    need(ints(lengths, R) && ints(news, R), "page_tables: lengths and new tokens [rows] int32");
+    need(free.dim() == 1 && free.numel() >= 1 && free.numel() < (1ll << 31) && ints(free, free.numel()) && ints(free_count, 1),
+         "page_tables: free [pages] and free_count [1] int32");
+    need(page_size >= 1 && page_size < (1ll << 30) && W < (1ll << 31), "page_tables: page size");
+    need(tokens >= 0 && tokens < (1ll << 31) - 8, "page_tables: tokens");
+    for (const at::Tensor* t : {&lengths, &free, &free_count, &table})
+      need(t->data_ptr() != news.data_ptr(), "page_tables: new tokens in a tensor of their own");
+    if (out.has_value()) {
+      const auto& [slots, positions, offsets, granted] = *out;
+      need(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.dim() == 1 && slots.numel() == tokens && ints(positions, tokens) &&
+               ints(offsets, R + 1) && granted.scalar_type() == at::kBool && granted.is_contiguous() && granted.dim() == 1 && granted.numel() == R,
+           "page_tables: out is (slots [tokens] int64, positions [tokens] int32, offsets [rows + 1] int32, granted [rows] bool)");
+      need(aligned(slots) && aligned(positions), "page_tables: 16-byte aligned slots and positions");
+    }
+    on_device(table, {&lengths, &free, &free_count, &news}, "page_tables expects tensors on one CUDA device");
+    const at::cuda::OptionalCUDAGuard guard(table.device());
+    if (!out.has_value()) {
+      const auto i32 = table.options();
+      out = std::make_tuple(at::empty({tokens}, i32.dtype(at::kLong)), at::empty({tokens}, i32), at::empty({R + 1}, i32), at::empty({R}, i32.dtype(at::kBool)));
+    }
+    const auto& [slots, positions, offsets, granted] = *out;
+    on_device(table, {&slots, &positions, &offsets, &granted}, "page_tables expects tensors on one CUDA device");
+    const PageTables a = {table.data_ptr<int>(), table.stride(0), lengths.data_ptr<int>(), free.data_ptr<int>(), free_count.data_ptr<int>(),
+                          news.data_ptr<int>(), (long long*)slots.data_ptr<int64_t>(), positions.data_ptr<int>(), offsets.data_ptr<int>(),
+                          granted.data_ptr<bool>(), (int)R, (int)W, (int)free.numel(), (int)page_size, (int)tokens};
+    ck(launch_page_tables(a, cur()), "page_tables");
+    return *out;
+  }, py::arg("table"), py::arg("lengths"), py::arg("free"), py::arg("free_count"), py::arg("new"), py::arg("page_size"), py::arg("tokens"),
+     py::arg("out") = py::none());
+  // qkv [tokens, (heads + 2 kv_heads) dim]: q and k rotated in place or into out [tokens, (heads + kv_heads) dim], k and v to their slots.
+  m.def("paged_append", [](at::Tensor qkv, at::Tensor k, at::Tensor v, at::Tensor slots, at::Tensor positions, int64_t heads, double theta,
+                           OptTensor out, OptTensor k_scale, OptTensor v_scale) {
+    const PagedType type = type_of(qkv, "paged_append: bf16 or fp16 qkv"), cache = type_of(k, "paged_append: bf16, fp16 or e4m3 caches");
+    need(type != PAGED_E4M3, "paged_append: bf16 or fp16 qkv");
+    const PagedPool pool = pool_of(k, v, type, cache, k_scale, v_scale);
+    const int64_t D = pool.dim, T = qkv.size(0);
+    for (int i = 0; i < 3; ++i) need(k.size(i) == 1 || k.stride(i) > 0, "paged_append: caches whose rows do not overlap");
+    need(D % 16 == 0 && D >= 16 && D <= 256, "paged_append: dim a multiple of 16, up to 256");
+    need(heads >= 0 && heads < (1 << 20) && qkv.dim() == 2 && qkv.size(1) == (heads + 2 * pool.heads) * D && T < (1ll << 31),
+         "paged_append: qkv must be [tokens, (heads + 2 kv_heads) dim]");
+    need(qkv.stride(1) == 1 && (T <= 1 || qkv.stride(0) >= qkv.size(1)) && qkv.stride(0) % 8 == 0 && aligned(qkv),
+         "paged_append: rows of qkv contiguous, 16-byte aligned");
+    need(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.dim() == 1 && slots.numel() == T && ints(positions, T),
+         "paged_append: slots [tokens] int64, positions [tokens] int32");
+    need(theta > 0 && std::isfinite(theta), "paged_append: theta above zero");
+    need(no_grad(qkv), "paged_append: no gradients");
+    if (out.has_value())
+      need(out->scalar_type() == qkv.scalar_type() && out->dim() == 2 && out->size(0) == T && out->size(1) == (heads + pool.heads) * D &&
+               out->stride(1) == 1 && (T <= 1 || out->stride(0) >= out->size(1)) && out->stride(0) % 8 == 0 && aligned(*out),
+           "paged_append: out must be [tokens, (heads + kv_heads) dim], like qkv");
+    on_device(qkv, {&k, &v, &slots, &positions}, "paged_append expects tensors on one CUDA device");
+    if (out.has_value()) on_device(qkv, {&*out}, "paged_append expects tensors on one CUDA device");
+    if (k_scale.has_value()) on_device(qkv, {&*k_scale, &*v_scale}, "paged_append expects tensors on one CUDA device");
+    const at::cuda::OptionalCUDAGuard guard(qkv.device());
+    ck(launch_paged_append(qkv.data_ptr(), qkv.stride(0), out.has_value() ? out->data_ptr() : nullptr, out.has_value() ? out->stride(0) : 0, type, pool,
+                           cache, (const long long*)slots.data_ptr<int64_t>(), positions.data_ptr<int>(), (int)T, (int)heads, theta, cur()),
+       "paged_append");
+  }, py::arg("qkv"), py::arg("k"), py::arg("v"), py::arg("slots"), py::arg("positions"), py::arg("heads"), py::arg("theta"),
+     py::arg("out") = py::none(), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none());
+  m.def("paged_attention_workspace_bytes", [](int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_len, int64_t window) {
+    need(rows >= 1 && kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && dim >= 1 && max_len >= 1 && window >= 0,
+         "paged_attention_workspace_bytes: rows, heads and lengths");
+    need(rows < (1 << 24) && heads < (1 << 20) && max_len < (1ll << 31), "paged_attention_workspace_bytes: rows, heads and lengths");
+    return (int64_t)paged_attention_workspace_bytes((int)rows, (int)heads, (int)kv_heads, (int)dim, (int)max_len, (int)std::min<int64_t>(window, 1ll << 30),
+                                                    sms_of(at::cuda::current_device()));
+  }, py::arg("rows"), py::arg("heads"), py::arg("kv_heads"), py::arg("dim"), py::arg("max_len"), py::arg("window") = 0);
+  // q [rows, heads, dim], one token of every row, attends to the row's last `window` positions (0: all of them).
+  m.def("paged_attention", [](at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor table, at::Tensor lengths, OptTensor out, OptTensor lse,
+                              c10::optional<double> scale, int64_t window, OptTensor k_scale, OptTensor v_scale, OptTensor workspace) {
+    const PagedType type = type_of(q, "paged_attention: bf16 or fp16 q"), cache = type_of(k, "paged_attention: bf16, fp16 or e4m3 caches");
+    need(type != PAGED_E4M3, "paged_attention: bf16 or fp16 q");
+    const PagedPool pool = pool_of(k, v, type, cache, k_scale, v_scale);
+    need(q.dim() == 3 && q.size(2) == pool.dim, "paged_attention: q must be [rows, heads, dim]");
+    const int64_t B = q.size(0), H = q.size(1);
+    need(B < (1 << 24) && H < (1 << 20) && H >= 1 && H % pool.heads == 0, "paged_attention: heads a multiple of the caches'");
+    need(pool.dim == 64 || pool.dim == 128 || pool.dim == 256, "paged_attention: dim 64, 128 or 256");
+    auto rows_ok = [&](const at::Tensor& t) { return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned(t); };
+    need(rows_ok(q), "paged_attention: heads of q contiguous, 16-byte aligned");
+    need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B && table.size(1) >= 1 && table.size(1) < (1ll << 31) &&
+             (table.size(1) == 1 || table.stride(1) == 1),
+         "paged_attention: table [rows, pages of a row] int32 with contiguous rows");
+    need(ints(lengths, B), "paged_attention: lengths [rows] int32");
+    need(window >= 0, "paged_attention: a window of no or some positions");
+    need(!scale.has_value() || std::isfinite(*scale), "paged_attention: a finite scale");
+    need(no_grad(q), "paged_attention: no gradients");
+    if (out.has_value())
+      need(out->scalar_type() == q.scalar_type() && out->sizes() == q.sizes() && rows_ok(*out) && (H == 1 || out->stride(1) >= pool.dim) &&
+               (B <= 1 || out->stride(0) >= pool.dim),
+           "paged_attention: out like q");
+    if (lse.has_value())
+      need(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->dim() == 2 && lse->size(0) == B && lse->size(1) == H, "paged_attention: lse [rows, heads] fp32");
+    if (workspace.has_value()) need(workspace->is_contiguous() && aligned(*workspace), "paged_attention: 16-byte aligned contiguous workspace");
+    on_device(q, {&k, &v, &table, &lengths}, "paged_attention expects tensors on one CUDA device");
+    for (const OptTensor* t : {&out, &lse, &k_scale, &v_scale, &workspace})
+      if (t->has_value()) on_device(q, {&**t}, "paged_attention expects tensors on one CUDA device");
+    const at::cuda::OptionalCUDAGuard guard(q.device());
+    if (!out.has_value()) out = at::empty({B, H, pool.dim}, q.options());
+    if (B == 0) return *out;
+    const int sms = sms_of(q.get_device());
+    const int win = (int)std::min<int64_t>(window, 1ll << 30);
+    const int max_len = (int)std::min<int64_t>(table.size(1) * pool.page_size, 0x7fff0000ll);
+    const size_t bytes = paged_attention_workspace_bytes((int)B, (int)H, pool.heads, pool.dim, max_len, win, sms);
+    if (workspace.has_value()) need(workspace->nbytes() >= bytes, "workspace too small (paged_attention_workspace_bytes)");
+    else if (bytes > 0) workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    const PagedAttention a = {q.data_ptr(), q.stride(0), q.stride(1), out->data_ptr(), out->stride(0), out->stride(1),
+                              lse.has_value() ? lse->data_ptr<float>() : nullptr, table.data_ptr<int>(), table.stride(0), lengths.data_ptr<int>(),
+                              (int)B, (int)H, (int)table.size(1), win, scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)pool.dim)};
+    ck(launch_paged_attention(a, type, pool, cache, workspace.has_value() ? workspace->data_ptr() : nullptr, sms, cur()), "paged_attention");
+    return *out;
+  }, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("table"), py::arg("lengths"), py::arg("out") = py::none(), py::arg("lse") = py::none(),
+     py::arg("scale") = py::none(), py::arg("window") = 0, py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(),
+     py::arg("workspace") = py::none());
+}

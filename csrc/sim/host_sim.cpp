@@ -25,6 +25,7 @@
 #include "../algos.h"
 #include "../gemm_tile_order.h"
 #include "../decode_attn_plan.h"
+#include "../paged_plan.h"
 #include "../decode_gemm_plan.h"
 #include "../all_reduce_oneshot.cuh"
 #include "../all_reduce_ring.cuh"
@@ -364,6 +365,30 @@ int penny_decode_attn_cut(const int* positions, int B, int Hkv, int max_len, int
   const int len = piece_len(total, top, B, Hkv, slots);
   for (int r = 0; r < B; ++r) pieces[r] = pieces_of(cut_rows(positions[r], max_len), len);
   return grid_extra(B * Hkv, slots, max_len);
+}
+// The paged KV cache's index arithmetic (paged_plan.h).
+int penny_page_div(int size, int n) { return penny::paged::div_page(penny::paged::page_div(size), n); }
+int penny_pages_of(int size, int n) { return penny::paged::pages_of(penny::paged::page_div(size), n); }
+long long penny_page_place(int page, int pages, int pos, int size, long long page_step, long long pos_step) {
+  return penny::paged::place_of(page, pages, pos, penny::paged::page_div(size), page_step, pos_step);
+}
+long long penny_page_place_of_slot(long long slot, int pages, int size, long long page_step, long long pos_step) {
+  return penny::paged::place_of_slot(slot, pages, size, page_step, pos_step);
+}
+// first and end of what every row attends to, its pieces as the kernel counts them; returns the pieces beyond one per (row,
+// item) that the launcher's grid has room for.
+long long penny_paged_cut(const int* lengths, int rows, int items_per_row, int max_len, int window, int slots, int* first, int* end, int* pieces) {
+  using namespace penny::paged;
+  long long total = 0;
+  for (int r = 0; r < rows; ++r) {
+    const Seen s = seen_of(lengths[r], max_len, window);
+    first[r] = s.first;
+    end[r] = s.end;
+    total += s.end - s.first;
+  }
+  const int len = piece_len(total, items_per_row, slots);
+  for (int r = 0; r < rows; ++r) pieces[r] = pieces_of(end[r] - first[r], len);
+  return extra_pieces(rows, items_per_row, slots, window > 0 && window < max_len ? window : max_len);
 }
 // Tile -> (row block, column block) of the persistent GEMM kernels; pair_rank < 0
 // selects the single-CTA kernel, 0 / 1 the CTA of a pair.  Returns the number of

@@ -6,6 +6,8 @@
     y = P.all_reduce(x, algo="nvls")
     out, res = P.all_reduce_rmsnorm(partial, weight, residual)
 
+    cache = P.PagedKVCache(layers, rows, max_len, kv_heads)    # KV cache in pages, no communicator needed (ops/paged.py)
+
 With a GPU the calls go to the native communicator (symmetric heap + peer-memory
 kernels); without one they go to the gloo backend with the same semantics, which
 is what the CPU test tier runs.  The reference exposes the same operations as
@@ -16,6 +18,8 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+
+from .paged import PagedKVCache, PageStep, page_tables, paged_append, paged_attention  # noqa: F401
 
 _BACKEND = None
 

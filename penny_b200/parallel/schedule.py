@@ -149,3 +149,38 @@ def decode_attn_cut(positions, kv_heads: int, max_len: int, sms: int = 148):
     pos, pieces = (ctypes.c_int * n)(*positions), (ctypes.c_int * n)()
     extra = sim_lib().penny_decode_attn_cut(pos, n, kv_heads, max_len, sms, pieces)
     return None if extra < 0 else (list(pieces), extra)
+
+
+def page_div(page_size: int, position: int) -> int:
+    """The page of a position, as the kernels of the paged KV cache divide (csrc/paged_plan.h)."""
+    return sim_lib().penny_page_div(page_size, position)
+
+
+def pages_of(page_size: int, length: int) -> int:
+    """Pages that hold `length` positions (csrc/paged_plan.h)."""
+    return sim_lib().penny_pages_of(page_size, length)
+
+
+def page_place(page: int, pages: int, position: int, page_size: int, page_step: int, position_step: int) -> int:
+    """Where a position lies in a pool, -1 if the pool does not have its page (csrc/paged_plan.h)."""
+    f = sim_lib().penny_page_place
+    f.restype, f.argtypes = ctypes.c_longlong, [ctypes.c_int] * 4 + [ctypes.c_longlong] * 2
+    return f(page, pages, position, page_size, page_step, position_step)
+
+
+def slot_place(slot: int, pages: int, page_size: int, page_step: int, position_step: int) -> int:
+    """The same for a slot."""
+    f = sim_lib().penny_page_place_of_slot
+    f.restype, f.argtypes = ctypes.c_longlong, [ctypes.c_longlong] + [ctypes.c_int] * 2 + [ctypes.c_longlong] * 2
+    return f(slot, pages, page_size, page_step, position_step)
+
+
+def paged_cut(lengths, items_per_row: int, max_len: int, window: int = 0, slots: int = 296):
+    """The paged attention's cut of a batch's rows (csrc/paged_plan.h): ([first, end) of every row, pieces of every row, pieces
+    beyond one per (row, item) that the grid has room for)."""
+    n = len(lengths)
+    lens, first, end, pieces = (ctypes.c_int * n)(*lengths), (ctypes.c_int * n)(), (ctypes.c_int * n)(), (ctypes.c_int * n)()
+    lib = sim_lib()
+    lib.penny_paged_cut.restype = ctypes.c_longlong
+    extra = lib.penny_paged_cut(lens, n, items_per_row, max_len, window, slots, first, end, pieces)
+    return list(zip(first, end)), list(pieces), extra

@@ -39,12 +39,16 @@ CUDA_SOURCES = [
     "csrc/gemm_tile_sm100.cu",
     "csrc/moe_dispatch_combine.cu",
     "csrc/moe_routing.cu",
+    "csrc/paged_tables.cu",
+    "csrc/paged_append.cu",
+    "csrc/paged_attention.cu",
 ]
 CPP_SOURCES = [
     "csrc/torch_interface.cpp",
     "csrc/custom_all_reduce_binding.cpp",
     "csrc/gemm_binding.cpp",
     "csrc/decode_binding.cpp",
+    "csrc/paged_binding.cpp",
     "csrc/bootstrap.cpp",
     "csrc/symm_heap.cpp",
 ]

@@ -5,21 +5,24 @@
 // (fp32); lse = the logarithm of the sum.  Rows without positions: zeros, -inf.  Positions on a page that the pool does not
 // have count as not there.
 //
-//   * The heads of a KV head share its keys and values: G = Hq / Hkv query rows are the M side of mma.sync (m16n8k16), whose
-//     second eight rows stay empty up to G = 8; more than 16 go to several CTAs.  (The 128 rows of a tcgen05 tile would be
-//     empty; the bound is the cache's stream.)
-//   * A CTA is four warps, each with a private three-stage cp.async pipeline over tiles of 4 KB of K and 4 KB of V (16
-//     positions of 128 bf16 values).  A lane looks up one position's page a tile ahead, so any page size and any strides will
-//     do; what lies outside the row is filled with zeros and never read (stale rows may hold anything).
+//   * The heads of a KV head share its keys and values.  Keys and values are the M side of mma.sync (m16n8k16), the G = Hq / Hkv
+//     query heads its N side: S^T = K Q^T, O^T = V^T P^T, so eight heads fill a product (sixteen take two, more go to several
+//     CTAs), and P^T is S^T's accumulators, transposed in registers.  (The 128 rows of a tcgen05 tile would be empty; the bound is
+//     the cache's stream.)
+//   * All warps of the GPU get an equal share of the batch: for every head group the tiles (4 KB of K and 4 KB of V: 16 positions
+//     of 128 bf16 values) of all rows in a line, cut every `share` tiles (paged_plan.h; every CTA sums over the lengths by
+//     itself).  A warp walks its part of the line with a private three-stage cp.async pipeline that does not drain between
+//     rows.  A lane looks up one position's page a tile ahead, so any page size and any strides will do; what lies outside
+//     a row is filled with zeros and never read (stale rows may hold anything).
+//   * A row that lies in one warp's part is finished from its registers, the parts of one that spans warps of a CTA
+//     meet in shared memory, those of several CTAs in a workspace, which a second kernel joins.  No counters: a workspace
+//     holds nothing between calls.
 //   * e4m3 caches: fp16 is exact for them, so they meet q as fp16, each row of q divided by the power of two of its
 //     largest value (exact; the score's factor takes it back).  A lane's four bytes of K are two adjacent pairs: the dims inside a
 //     16-byte chunk are permuted on both sides of the product.  V's bytes are transposed in pairs by ldmatrix and separated
 //     into even and odd dims.
 //   * P is rounded to the type of the product (bf16: 2^-8 of each weight at most, averaged over the positions; the sum is of the
 //     unrounded ones); q, scores, maxima and sums are not rounded.
-//   * Rows are cut into pieces of the batch's total over the CTAs that the GPU holds (paged_plan.h), found by every CTA from the
-//     lengths on the device.  A second kernel joins the pieces of cut rows; no counters, so a workspace holds nothing between
-//     calls.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -39,17 +42,34 @@ using attn::ldmatrix_x4;
 using attn::ldmatrix_x4_trans;
 using attn::mma_bf16;
 
-constexpr int kWarps = 4, kStages = 3;
+#ifndef PW
+#define PW 4
+#define PS 3
+#define TB 4096
+#endif
+constexpr int kWarps = PW;
+constexpr float kSlack = 8.f;  // weights of up to 2^8
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <int D, bool kE4M3>
+template <bool kWide>
+struct MaskOf {
+  using type = uint32_t;
+};
+template <>
+struct MaskOf<true> {
+  using type = unsigned long long;
+};
+
+template <int D, bool kE4M3, int kBlocks>
 struct Tile {
   static constexpr int kRow = kE4M3 ? D : 2 * D;               // bytes of a position
-  static constexpr int kPos = 4096 / kRow > 16 ? 4096 / kRow : 16;
+  static constexpr int kPos = TB / kRow > 16 ? TB / kRow : 16;
   static constexpr int kChunks = kRow / 16;                    // 16-byte chunks of a position
   static constexpr int kPerPass = 32 / kChunks;                // positions that a warp's 32 chunks cover
   static constexpr int kStage = 2 * kPos * kRow;
+  static constexpr int kStages = kBlocks == 2 || kStage > 8192 ? 2 : PS;
   static constexpr int kSmem = kWarps * kStages * kStage;
+  using Mask = typename MaskOf<(kPos > 32)>::type;
   // where chunk c of position r lies: eight positions' equal chunks in eight different 16-byte banks
   static __device__ __forceinline__ uint32_t at(int r, int c) {
     if constexpr (kRow == 64) return (uint32_t)((r >> 1) * 128 + ((((r & 1) << 2) | (c ^ ((r >> 1) & 3))) << 4));
@@ -78,6 +98,17 @@ __device__ __forceinline__ uint32_t e4m3_hi(uint32_t x) {
   asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, h;}" : "=r"(r) : "r"(x));
   return r;
 }
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// an 8 x 8 matrix of 16-bit values, transposed in the warp's registers
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
 __device__ __forceinline__ float2 to_f32(__nv_bfloat162 v) { return __bfloat1622float2(v); }
 __device__ __forceinline__ float2 to_f32(__half2 v) { return __half22float2(v); }
 template <typename T>
@@ -93,432 +124,582 @@ struct Pair<__half> {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16(lo, hi); }
 };
 
-struct Cut {   // where a CTA's piece comes from and goes to
-  int row, item, piece, pieces;
-};
-// Meta of the joining kernel: the CTA of a row's first piece of item 0, and how many pieces the row has.
 struct Params {
   PagedAttention a;
   PagedPool pool;
   PageDiv div;
-  int group;           // G
-  int items_per_row;   // (KV head, head group) pairs of a row
-  int max_len, slots;  // slots 0: rows are whole
-  int2* meta;
-  float* part_o;   // per piece kRows rows of dim
-  float2* part_ml; // maximum (base 2), sum
+  int group;              // G
+  int items;              // (KV head, head group) pairs
+  int max_len;
+  uint32_t page_step, pos_step, step_bytes;  // strides in units of step_bytes
+  int2* tails;            // per CTA: the row that begins in it and does not end in it, how many teams follow; row -1: none
+  float4* parts;          // per CTA two parts: of a row that began before it, of one that ends after it
+  float2* part_ml;        // their maxima (base 2) and sums
 };
 
-// The piece of CTA `idx`.  Called by all threads; row -1: none.
-__device__ __forceinline__ Cut find_cut(const Params& p, int idx) {
-  __shared__ long long s_sum[kWarps];
-  __shared__ int s_cnt[kWarps];
-  __shared__ Cut s_cut;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+template <int D, int kBlocks>
+struct Part {
+  static constexpr int kFrags = kBlocks * (D / 16);  // MMA accumulators of O^T: 16 dims x 8 heads, a float4 a lane
+  static constexpr int kRows = 8 * kBlocks;
+};
+
+// The share of a team's warps, and where this one begins.  Called by all threads.
+template <int kWarps>
+__device__ __forceinline__ int find_walk(const Params& p, int tile, Walk& w) {
+  __shared__ long long s_sum[kWarps], s_at[kWarps];
+  __shared__ int s_row[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, team = (int)blockIdx.x / p.items, teams = (int)gridDim.x / p.items;
   const int per = (p.a.rows + kWarps * 32 - 1) / (kWarps * 32), r0 = min(p.a.rows, tid * per), r1 = min(p.a.rows, r0 + per);
-  auto seen = [&](int r) {
-    const Seen s = seen_of(p.a.lengths[r], p.max_len, p.a.window);
-    return s.end - s.first;
+  auto seen = [&](int r) { return seen_of(p.a.lengths[r], p.max_len, p.a.window); };
+  auto units = [&](int r) {
+    const Seen s = seen(r);
+    return units_of(s.end - s.first, tile);
   };
-  long long sum = 0;
-  for (int r = r0; r < r1; ++r) sum += seen(r);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_sum[warp] = sum;
-  if (tid == 0) s_cut.row = -1;
-  __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += s_sum[w];
-  const int len = piece_len(total, p.items_per_row, p.slots);
-  int mine = 0;
-  for (int r = r0; r < r1; ++r) mine += pieces_of(seen(r), len);
-  int incl = mine;
+  long long mine = 0;
+  for (int r = r0; r < r1; ++r) mine += units(r);
+  long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) s_cnt[warp] = incl;
+  if (lane == 31) s_sum[warp] = incl;
+  if (lane == 0) s_row[warp] = -1;
   __syncthreads();
-  int first = incl - mine;
-  for (int w = 0; w < warp; ++w) first += s_cnt[w];
-  long long at = idx - (long long)first * p.items_per_row;
-  if (at >= 0 && at < (long long)mine * p.items_per_row) {
-    for (int r = r0; r < r1; ++r) {
-      const int n = pieces_of(seen(r), len);
-      if (at < (long long)n * p.items_per_row) {
-        const int piece = (int)at / p.items_per_row;
-        s_cut = {r, (int)at - piece * p.items_per_row, piece, n};
-        break;
+  long long total = 0, x = incl - mine;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) x += s_sum[i];
+    total += s_sum[i];
+  }
+  const int share = share_of(total, teams * kWarps);
+  for (int r = r0; r < r1; ++r) {
+    const int n = units(r);
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const long long begin = ((long long)team * kWarps + i) * share;
+      if (begin >= x && begin < x + n) {
+        s_row[i] = r;
+        s_at[i] = begin - x;
       }
-      at -= (long long)n * p.items_per_row;
     }
+    x += n;
   }
   __syncthreads();
-  return s_cut;
+  w.row = s_row[warp];
+  w.left = 0;
+  if (w.row >= 0) {
+    enter_row(w, tile, seen);
+    w.at = (int)s_at[warp];
+    w.left = (int)min((long long)share, total - ((long long)team * kWarps + warp) * share);
+  }
+  return share;
 }
 
-// kRows: query rows of a CTA, 8 or 16.
-template <int D, typename T, bool kE4M3, int kRows>
+// One accumulator of O^T, divided by the sums and rounded, to its 16 dims of up to eight heads: this thread holds dims g and g + 8
+// (e4m3: 2 g and 2 g + 1) of heads 2 t and 2 t + 1.  Called by whole warps.  out: the first head's dims.
+template <typename T, bool kE4M3>
+__device__ __forceinline__ void store_frag(T* out, long long head_stride, int heads, int lane, const float4& o, const float (&inv)[2]) {
+  const uint32_t lo = transpose8x8(Pair<T>::pack(o.x * inv[0], o.y * inv[1])), hi = transpose8x8(Pair<T>::pack(o.z * inv[0], o.w * inv[1]));
+  const int g = lane >> 2, t = lane & 3;  // now head g
+  if (g >= heads) return;
+  T* to = out + g * head_stride;
+  if constexpr (kE4M3) {
+    *reinterpret_cast<uint2*>(to + 4 * t) = make_uint2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+  } else {
+    *reinterpret_cast<uint32_t*>(to + 2 * t) = lo;
+    *reinterpret_cast<uint32_t*>(to + 8 + 2 * t) = hi;
+  }
+}
+__device__ __forceinline__ float inverse(float top, float sum, float factor) { return top == -INFINITY ? 0.f * sum : factor / sum; }
+
+// kBlocks: blocks of eight query heads of a CTA, 1 or 2.
+template <int D, typename T, bool kE4M3, int kBlocks>
 __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_constant__ Params p) {
-  using L = Tile<D, kE4M3>;
+  using L = Tile<D, kE4M3, kBlocks>;
   using T2 = typename Pair<T>::type;
-  constexpr int kHalves = kRows / 8, kLook = (L::kPos + 31) / 32, kSteps = D / 16, kNC = L::kPos / 8;
-  constexpr bool kBf16 = !kE4M3 && sizeof(T2) == 4 && __is_same(T, __nv_bfloat16);
+  using P = Part<D, kBlocks>;
+  using Mask = typename L::Mask;
+  constexpr int kRows = P::kRows, kLook = (L::kPos + 31) / 32, kSteps = D / 16, kGroups = L::kPos / 16, kStages = L::kStages;
+  constexpr bool kBf16 = !kE4M3 && __is_same(T, __nv_bfloat16);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
+  __shared__ float2 s_ml[2][kWarps][kRows];  // of a warp's first part and of its last
+  __shared__ int s_head[kWarps];             // a part of a row that began before: 0 none, 1 it ends here, 2 it does not
+  __shared__ int2 s_tail[kWarps];            // a row that does not end here (-1: none), its units still to come
   pdl_launch_dependents();
   pdl_wait();
-  Cut cut;
-  if (p.slots > 0) {
-    cut = find_cut(p, (int)blockIdx.x);
-    if (cut.row < 0) return;
-  } else {
-    cut.row = (int)blockIdx.x / p.items_per_row;
-    cut.item = (int)blockIdx.x - cut.row * p.items_per_row;
-    cut.piece = 0;
-    cut.pieces = 1;
-  }
-  const int b = cut.row, groups = (p.group + kRows - 1) / kRows, kh = cut.item / groups, h0 = (cut.item - kh * groups) * kRows;
-  const int heads = min(kRows, p.group - h0);  // valid rows of this CTA
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if (p.slots > 0 && cut.piece == 0 && cut.item == 0 && threadIdx.x == 0) p.meta[b] = make_int2((int)blockIdx.x, cut.pieces);
-
-  const Seen seen = seen_of(p.a.lengths[b], p.max_len, p.a.window);
-  const int n = seen.end - seen.first;
-  const int per = ((n + cut.pieces - 1) / cut.pieces + L::kPos - 1) / L::kPos * L::kPos;
-  const int t0 = (int)min((long long)seen.first + (long long)cut.piece * per, (long long)seen.end), t1 = min(seen.end, t0 + min(per, n));
-  const int tiles = (t1 - t0 + L::kPos - 1) / L::kPos;
+  Walk load;
+  const int share = find_walk<kWarps>(p, L::kPos, load);
+  Walk w = load;
+  const int item = (int)blockIdx.x % p.items, groups = (p.group + kRows - 1) / kRows, kh = item / groups, h0 = (item - kh * groups) * kRows;
+  const int heads = min(kRows, p.group - h0), head0 = kh * p.group + h0;  // of this CTA
   const uint32_t wbase = attn::smem_u32_local(smem_raw) + warp * (kStages * L::kStage);
-  const int* table = p.a.table + (long long)b * p.a.table_stride;
+  float4* heads_area = reinterpret_cast<float4*>(smem_raw + L::kSmem);                                  // [warps][frags][32]
+  auto tail_area = [&](int i) { return reinterpret_cast<float4*>(smem_raw + i * (kStages * L::kStage)); };  // a drained pipeline's space
   constexpr int kSize = kE4M3 ? 1 : 2;
+  const long long pos_bytes = p.pool.pos_stride * kSize;
   const char* kbase = reinterpret_cast<const char*>(p.pool.k) + kh * p.pool.head_stride * kSize + (lane % L::kChunks) * 16;
   const char* vbase = reinterpret_cast<const char*>(p.pool.v) + kh * p.pool.head_stride * kSize + (lane % L::kChunks) * 16;
-  const long long page_bytes = p.pool.page_stride * kSize, pos_bytes = p.pool.pos_stride * kSize;
 
-  // tile j of this warp: positions [t0 + (warp + 4 j) kPos, + kPos).  The page of this lane's position(s), -1: not there.
-  int page[kLook];
-  auto look = [&](int j) {
-    const int start = t0 + (warp + kWarps * j) * L::kPos;
+  auto seen = [&](int row) { return seen_of(p.a.lengths[row], p.max_len, p.a.window); };
+
+  // ---- loading: the pages of the next tile are looked up while the one before is requested ----
+  int page[kLook], load_pos = -L::kPos, load_tiles = 0, load_end = 0;  // load_tiles: of the part, the next one and those behind it
+  const int* table = nullptr;
+  auto look = [&]() {
+    load_pos += L::kPos;
+    if (--load_tiles <= 0) {
+      while (load.left > 0 && load_tiles <= 0) {
+        const WalkPart part = next_part(load, L::kPos, seen);
+        load_tiles = part.to - part.from;
+        load_pos = load.first + part.from * L::kPos;
+      }
+      if (load_tiles <= 0) return;  // no more
+      load_end = load.end;
+      table = p.a.table + load.row * p.a.table_stride;
+    }
 #pragma unroll
     for (int i = 0; i < kLook; ++i) {
-      const int pos = start + i * 32 + lane;
-      page[i] = i * 32 + lane < L::kPos && warp + kWarps * j < tiles && pos < t1 ? table[div_page(p.div, pos)] : -1;
+      const int pos = load_pos + i * 32 + lane % L::kPos;
+      page[i] = pos < load_end ? table[div_page(p.div, pos)] : -1;
     }
   };
-  // requests tile j; the mask of its positions that are there
-  auto issue = [&](int j) {
-    unsigned long long mask = 0;
-    if (warp + kWarps * j < tiles) {
-      const int start = t0 + (warp + kWarps * j) * L::kPos;
-      const uint32_t sb = wbase + (j % kStages) * L::kStage;
-      long long off[kLook];
+  int stage_in = 0, stage_out = 0;
+  // requests the next tile; the mask of its positions that are there
+  auto issue = [&]() {
+    Mask mask = 0;
+    if (load_tiles > 0) {
+      const uint32_t sb = wbase + stage_in * L::kStage;
+      uint32_t off[kLook];
+      bool one = true;  // all of it on one page
 #pragma unroll
       for (int i = 0; i < kLook; ++i) {
-        const int pos = start + i * 32 + lane;
-        off[i] = place_of(page[i], p.pool.pages, pos, p.div, page_bytes, pos_bytes);
-        mask |= (unsigned long long)__ballot_sync(0xffffffffu, off[i] >= 0) << (32 * i);
+        off[i] = step_of(page[i], p.pool.pages, load_pos + i * 32 + lane % L::kPos, p.div, p.page_step, p.pos_step);
+        const uint32_t there = __ballot_sync(0xffffffffu, off[i] != kNoStep);
+        mask |= (Mask)(L::kPos < 32 ? there & ((1u << L::kPos % 32) - 1) : there) << (i * 32 % (8 * (int)sizeof(Mask)));
+        one = one && there == 0xffffffffu && __all_sync(0xffffffffu, page[i] == __shfl_sync(0xffffffffu, page[0], 0));
       }
+      const int r0 = lane / L::kChunks, c = lane % L::kChunks;
+      if (one) {
+        const unsigned long long by = (unsigned long long)__shfl_sync(0xffffffffu, off[0], 0) * p.step_bytes + r0 * pos_bytes;
+        const char *kp = kbase + by, *vp = vbase + by;
 #pragma unroll
-      for (int i = 0; i < L::kPos / L::kPerPass; ++i) {
-        const int r = i * L::kPerPass + lane / L::kChunks;
-        const long long o = __shfl_sync(0xffffffffu, off[(i * L::kPerPass) / 32], r & 31);
-        const uint32_t s = sb + L::at(r, lane % L::kChunks);
-        cp_async16(s, kbase + (o < 0 ? 0 : o), o >= 0);
-        cp_async16(s + L::kPos * L::kRow, vbase + (o < 0 ? 0 : o), o >= 0);
-      }
-    }
-    cp_async_commit();  // always: keeps the group count in step with j
-    return mask;
-  };
-  look(0);
-  unsigned long long mask0 = issue(0);
-  look(1);
-  unsigned long long mask1 = issue(1);
-  look(2);
-
-  // ---- q as MMA A fragments, and what turns a score into the exponent of two ----
-  uint32_t qa[kSteps][2 * kHalves];
-  float qs[kHalves];
-#pragma unroll
-  for (int r = 0; r < kHalves; ++r) {
-    const int h = r * 8 + g;
-    const T* q = reinterpret_cast<const T*>(p.a.q) + b * p.a.q_stride + (long long)(kh * p.group + h0 + min(h, heads - 1)) * p.a.q_head_stride;
-    qs[r] = p.a.scale * kLog2e;
-    if constexpr (kE4M3) {
-      float x[kSteps][4], top = 0.f;
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        const uint2 raw = *reinterpret_cast<const uint2*>(q + k * 16 + 4 * t);
-        const float2 lo = to_f32(*reinterpret_cast<const T2*>(&raw.x)), hi = to_f32(*reinterpret_cast<const T2*>(&raw.y));
-        x[k][0] = lo.x, x[k][1] = lo.y, x[k][2] = hi.x, x[k][3] = hi.y;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[k][i]));
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = (__float_as_int(top) >> 23) & 255;
-      const bool plain = e < 1 || e > 253;  // zeros, infinities
-      const float down = plain ? 1.f : __int_as_float((254 - e) << 23);
-      qs[r] *= p.pool.k_scale[kh] * (plain ? 1.f : __int_as_float(e << 23));
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        qa[k][r] = pack_f16(x[k][0] * down, x[k][1] * down);
-        qa[k][kHalves + r] = pack_f16(x[k][2] * down, x[k][3] * down);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        qa[k][r] = *reinterpret_cast<const uint32_t*>(q + k * 16 + 2 * t);
-        qa[k][kHalves + r] = *reinterpret_cast<const uint32_t*>(q + k * 16 + 8 + 2 * t);
-      }
-    }
-  }
-  auto mma = [&](float (&d)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {  // a: row g (and g + 8), k low, then k high
-    const uint32_t a1 = kHalves == 2 ? a[1] : 0u, a2 = a[kHalves], a3 = kHalves == 2 ? a[3] : 0u;
-    if constexpr (kBf16) mma_bf16(d, a[0], a1, a2, a3, b0, b1);
-    else mma_f16(d, a[0], a1, a2, a3, b0, b1);
-  };
-  auto pack_p = [&](float lo, float hi) {
-    if constexpr (kBf16) return attn::pack2(lo, hi);
-    else return pack_f16(lo, hi);
-  };
-
-  float m[kHalves], l[kHalves], o[D / 8][4];
-#pragma unroll
-  for (int r = 0; r < kHalves; ++r) m[r] = -INFINITY, l[r] = 0.f;
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-
-  const int my_tiles = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-  for (int j = 0; j < my_tiles; ++j) {
-    __syncwarp();  // everyone is done with the stage that tile j + 2 overwrites
-    const unsigned long long mask2 = issue(j + 2);
-    look(j + 3);
-    cp_async_wait<2>();
-    __syncwarp();
-    const uint32_t sb = wbase + (j % kStages) * L::kStage;
-    // ---- S = Q K^T, eight positions at a time ----
-    float s[kNC][4];
-#pragma unroll
-    for (int c = 0; c < kNC; ++c) {
-      s[c][0] = s[c][1] = s[c][2] = s[c][3] = 0.f;
-#pragma unroll
-      for (int k4 = 0; k4 < L::kChunks / 4; ++k4) {
-        uint32_t kb[4];
-        ldmatrix_x4(sb + L::at(c * 8 + (lane & 7), k4 * 4 + (lane >> 3)), kb);
-        if constexpr (kE4M3) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mma(s[c], qa[k4 * 4 + i], e4m3_lo(kb[i]), e4m3_hi(kb[i]));
-        } else {
-          mma(s[c], qa[k4 * 2], kb[0], kb[1]);
-          mma(s[c], qa[k4 * 2 + 1], kb[2], kb[3]);
+        for (int i = 0; i < L::kPos / L::kPerPass; ++i) {
+          const uint32_t s = sb + L::at(i * L::kPerPass + r0, c);
+          cp_async16(s, kp, true);
+          cp_async16(s + L::kPos * L::kRow, vp, true);
+          kp += L::kPerPass * pos_bytes;
+          vp += L::kPerPass * pos_bytes;
         }
-      }
-    }
-    // ---- running softmax; this thread holds positions c * 8 + 2 t, + 1 of rows g and g + 8 ----
-    uint32_t pa[kNC / 2][2 * kHalves];
-#pragma unroll
-    for (int r = 0; r < kHalves; ++r) {
-      float top = m[r];
-#pragma unroll
-      for (int c = 0; c < kNC; ++c) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float& x = s[c][2 * r + e];
-          x = (mask0 >> (c * 8 + 2 * t + e)) & 1 ? x * qs[r] : -INFINITY;
-          top = fmaxf(top, x);
-        }
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float base = top == -INFINITY ? 0.f : top;  // nothing there yet: weights of zero
-      const float corr = exp2f(m[r] - base);
-      m[r] = top;
-      l[r] *= corr;
-#pragma unroll
-      for (int c = 0; c < kNC; ++c) {
-        const float p0 = exp2f(s[c][2 * r] - base), p1 = exp2f(s[c][2 * r + 1] - base);
-        l[r] += p0 + p1;
-        pa[c / 2][(c & 1) * kHalves + r] = pack_p(p0, p1);
-      }
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) o[i][2 * r] *= corr, o[i][2 * r + 1] *= corr;
-    }
-    // ---- O += P V, 16 positions at a time ----
-#pragma unroll
-    for (int c = 0; c < kNC / 2; ++c) {
-      const int row = c * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-#pragma unroll
-      for (int d = 0; d < L::kChunks / 2; ++d) {
-        uint32_t vb[4];
-        ldmatrix_x4_trans(sb + L::kPos * L::kRow + L::at(row, d * 2 + (lane >> 4)), vb);
-        if constexpr (kE4M3) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t x = __byte_perm(vb[2 * i], 0, 0x3120), y = __byte_perm(vb[2 * i + 1], 0, 0x3120);
-            mma(o[(d * 2 + i) * 2], pa[c], e4m3_lo(x), e4m3_lo(y));
-            mma(o[(d * 2 + i) * 2 + 1], pa[c], e4m3_hi(x), e4m3_hi(y));
-          }
-        } else {
-          mma(o[2 * d], pa[c], vb[0], vb[1]);
-          mma(o[2 * d + 1], pa[c], vb[2], vb[3]);
-        }
-      }
-    }
-    mask0 = mask1;
-    mask1 = mask2;
-  }
-  cp_async_wait<0>();
-
-  // ---- the four warps' sums join in shared memory (the pipelines' space) ----
-  __syncthreads();
-  float* sm_o = reinterpret_cast<float*>(smem_raw);             // [warps][kRows][D]
-  float2* sm_ml = reinterpret_cast<float2*>(sm_o + kWarps * kRows * D);  // [warps][kRows]
-#pragma unroll
-  for (int r = 0; r < kHalves; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const int h = warp * kRows + r * 8 + g;
-    if (r * 8 + g < heads) {
-      float* to = sm_o + h * D;
-      if constexpr (kE4M3) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-          *reinterpret_cast<float4*>(to + i * 16 + 4 * t) =
-              make_float4(o[2 * i][2 * r], o[2 * i + 1][2 * r], o[2 * i][2 * r + 1], o[2 * i + 1][2 * r + 1]);
       } else {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(to + i * 8 + 2 * t) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+        for (int i = 0; i < L::kPos / L::kPerPass; ++i) {
+          const int r = i * L::kPerPass + r0;
+          const uint32_t o = __shfl_sync(0xffffffffu, off[(i * L::kPerPass) / 32], r & 31);
+          const bool ok = o != kNoStep;
+          const unsigned long long by = ok ? (unsigned long long)o * p.step_bytes : 0;
+          const uint32_t s = sb + L::at(r, c);
+          cp_async16(s, kbase + by, ok);
+          cp_async16(s + L::kPos * L::kRow, vbase + by, ok);
+        }
       }
-      if (t == 0) sm_ml[h] = make_float2(m[r], l[r]);
     }
+    stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+    cp_async_commit();  // always: keeps the group count in step with the tiles
+    return mask;
+  };
+  Mask masks[kStages];  // of the tiles in flight
+  look();
+#pragma unroll
+  for (int j = 0; j + 1 < kStages; ++j) {
+    masks[j] = issue();
+    look();
   }
-  __syncthreads();
-  const float v_scale = kE4M3 ? p.pool.v_scale[kh] : 1.f;
-  for (int i = threadIdx.x; i < heads * (D / 4); i += kWarps * 32) {
-    const int h = i / (D / 4), d = (i - h * (D / 4)) * 4;
-    float top = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  if (lane == 0) {
+    s_head[warp] = 0;
+    s_tail[warp] = make_int2(-1, 0);
+  }
+
+  uint32_t qb[kBlocks][kSteps][2];
+  float qs[kBlocks][2];
+  // q of a row as MMA B fragments (head g of a block), and what turns the scores of heads 2 t and 2 t + 1 into exponents of two
+  auto load_q = [&](int row) {
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_ml[w * kRows + h].x);
-    const float base = top == -INFINITY ? 0.f : top;
+    for (int nb = 0; nb < kBlocks; ++nb) {
+      const int h = min(nb * 8 + g, heads - 1);
+      const T* q = reinterpret_cast<const T*>(p.a.q) + row * p.a.q_stride + (head0 + h) * p.a.q_head_stride;
+      if constexpr (kE4M3) {
+        float x[kSteps][4], top = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float2 ml = sm_ml[w * kRows + h];
-      const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * kRows + h) * D + d);
-      const float f = exp2f(ml.x - base);
-      sum += f * ml.y;
-      acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
+        for (int k = 0; k < kSteps; ++k) {
+          const uint2 raw = *reinterpret_cast<const uint2*>(q + k * 16 + 4 * t);
+          const float2 lo = to_f32(*reinterpret_cast<const T2*>(&raw.x)), hi = to_f32(*reinterpret_cast<const T2*>(&raw.y));
+          x[k][0] = lo.x, x[k][1] = lo.y, x[k][2] = hi.x, x[k][3] = hi.y;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[k][i]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = (__float_as_int(top) >> 23) & 255;
+        const bool plain = e < 1 || e > 253;  // zeros, infinities
+        const float down = plain ? 1.f : __int_as_float((254 - e) << 23);
+        const float factor = p.a.scale * kLog2e * p.pool.k_scale[kh] * (plain ? 1.f : __int_as_float(e << 23));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) qs[nb][i] = __shfl_sync(0xffffffffu, factor, (2 * t + i) * 4);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          qb[nb][k][0] = pack_f16(x[k][0] * down, x[k][1] * down);
+          qb[nb][k][1] = pack_f16(x[k][2] * down, x[k][3] * down);
+        }
+      } else {
+        qs[nb][0] = qs[nb][1] = p.a.scale * kLog2e;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          qb[nb][k][0] = *reinterpret_cast<const uint32_t*>(q + k * 16 + 2 * t);
+          qb[nb][k][1] = *reinterpret_cast<const uint32_t*>(q + k * 16 + 8 + 2 * t);
+        }
+      }
     }
-    if (cut.pieces == 1) {
-      const int head = kh * p.group + h0 + h;
-      const float inv = top == -INFINITY ? 0.f : v_scale / sum;
-      const uint2 raw = make_uint2(Pair<T>::pack(acc[0] * inv, acc[1] * inv), Pair<T>::pack(acc[2] * inv, acc[3] * inv));
-      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.a.out) + b * p.a.out_stride + head * p.a.out_head_stride + d) = raw;
-      if (d == 0 && p.a.lse) p.a.lse[(long long)b * p.a.heads + head] = (top + log2f(sum)) * kLn2;
+  };
+  auto mma = [&](float (&d)[4], const uint32_t (&a)[4], const uint32_t (&bb)[2]) {
+    if constexpr (kBf16) mma_bf16(d, a[0], a[1], a[2], a[3], bb[0], bb[1]);
+    else mma_f16(d, a[0], a[1], a[2], a[3], bb[0], bb[1]);
+  };
+  T* const out = reinterpret_cast<T*>(p.a.out);
+  auto out_of = [&](int row, int head) { return out + row * p.a.out_stride + head * p.a.out_head_stride; };
+
+  // ---- this warp's share, row by row ----
+  while (w.left > 0) {
+    const WalkPart part = next_part(w, L::kPos, seen);
+    const int n = part.to - part.from;
+    if (w.units == 1) {  // an empty row
+      const float zero[2] = {0.f, 0.f};
+      for (int f = 0; f < P::kFrags; ++f)
+        store_frag<T, kE4M3>(out_of(w.row, head0 + f / kSteps * 8) + f % kSteps * 16, p.a.out_head_stride, heads - f / kSteps * 8, lane,
+                             make_float4(0.f, 0.f, 0.f, 0.f), zero);
+      if (p.a.lse && lane < heads) p.a.lse[(long long)w.row * p.a.heads + head0 + lane] = -INFINITY;
+      continue;
+    }
+    if (n <= 0) continue;
+    load_q(w.row);
+    // per block of heads: the base (m: minus infinity before the first) of heads 2 t and 2 t + 1, this thread's share of their sums, O^T
+    float m[kBlocks][2], base[kBlocks][2], limit[kBlocks][2], l[kBlocks][2], o[kBlocks][kSteps][4];
+#pragma unroll
+    for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) m[nb][i] = limit[nb][i] = -INFINITY, base[nb][i] = l[nb][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) o[nb][k][0] = o[nb][k][1] = o[nb][k][2] = o[nb][k][3] = 0.f;
+    }
+    for (int j = 0; j < n; ++j) {
+      __syncwarp();  // everyone is done with the stage that the next tile overwrites
+      masks[kStages - 1] = issue();
+      look();
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const uint32_t sb = wbase + stage_out * L::kStage;
+      stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1;
+      // ---- S^T = K Q^T, 16 positions at a time: this thread holds positions g and g + 8 of heads 2 t and 2 t + 1 ----
+      float s[kBlocks][kGroups][4];
+#pragma unroll
+      for (int c = 0; c < kGroups; ++c) {
+#pragma unroll
+        for (int nb = 0; nb < kBlocks; ++nb) s[nb][c][0] = s[nb][c][1] = s[nb][c][2] = s[nb][c][3] = 0.f;
+        const int row = c * 16 + (lane & 15);
+#pragma unroll
+        for (int k2 = 0; k2 < L::kChunks / 2; ++k2) {
+          uint32_t a[4];
+          ldmatrix_x4(sb + L::at(row, k2 * 2 + (lane >> 4)), a);
+          if constexpr (kE4M3) {  // a chunk is 16 dims
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t x[4] = {e4m3_lo(a[2 * i]), e4m3_lo(a[2 * i + 1]), e4m3_hi(a[2 * i]), e4m3_hi(a[2 * i + 1])};
+#pragma unroll
+              for (int nb = 0; nb < kBlocks; ++nb) mma(s[nb][c], x, qb[nb][k2 * 2 + i]);
+            }
+          } else {
+#pragma unroll
+            for (int nb = 0; nb < kBlocks; ++nb) mma(s[nb][c], a, qb[nb][k2]);
+          }
+        }
+      }
+      // ---- weights exp2(score - base); the base follows the maximum when a score exceeds it by more than kSlack ----
+      uint32_t pb[kBlocks][kGroups][2];
+#pragma unroll
+      for (int nb = 0; nb < kBlocks; ++nb) {
+        bool above = false;
+        // exponents against the base as it is; minus infinity where nothing is
+#pragma unroll
+        for (int c = 0; c < kGroups; ++c) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[nb][c][u] = fmaf(s[nb][c][u], qs[nb][u & 1], -base[nb][u & 1]);
+        }
+        if (masks[0] != (Mask)~(Mask)0 >> (8 * (int)sizeof(Mask) - L::kPos)) {
+          const Mask mask = masks[0] >> g;
+#pragma unroll
+          for (int c = 0; c < kGroups; ++c) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s[nb][c][u] = (mask >> (c * 16 + u / 2 * 8)) & 1 ? s[nb][c][u] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kGroups; ++c) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) above = above || s[nb][c][u] > limit[nb][u & 1];
+        }
+        if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < kGroups; ++c) top = fmaxf(top, fmaxf(s[nb][c][i], s[nb][c][2 + i]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            if (top > (m[nb][i] == -INFINITY ? -INFINITY : 0.f)) {
+              const float next = base[nb][i] + top, by = base[nb][i] - next, corr = exp2f(m[nb][i] - next);
+              m[nb][i] = base[nb][i] = next;
+              limit[nb][i] = kSlack;
+              l[nb][i] *= corr;
+#pragma unroll
+              for (int k = 0; k < kSteps; ++k) o[nb][k][i] *= corr, o[nb][k][2 + i] *= corr;
+#pragma unroll
+              for (int c = 0; c < kGroups; ++c) s[nb][c][i] += by, s[nb][c][2 + i] += by;
+            }
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kGroups; ++c) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float p0 = exp2_ftz(s[nb][c][2 * u]), p1 = exp2_ftz(s[nb][c][2 * u + 1]);
+            l[nb][0] += p0;
+            l[nb][1] += p1;
+            pb[nb][c][u] = transpose8x8(kBf16 ? attn::pack2(p0, p1) : pack_f16(p0, p1));
+          }
+        }
+      }
+      // ---- O^T += V^T P^T, 16 positions at a time ----
+#pragma unroll
+      for (int c = 0; c < kGroups; ++c) {
+#pragma unroll
+        for (int d = 0; d < L::kChunks / 2; ++d) {
+          uint32_t a[4];
+          const uint32_t vb = sb + L::kPos * L::kRow;
+          if constexpr (kE4M3) {  // two chunks of 16 dims: their even dims are rows 0 to 7, the odd ones rows 8 to 15
+            ldmatrix_x4_trans(vb + L::at(c * 16 + (lane & 15), d * 2 + (lane >> 4)), a);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t lo = __byte_perm(a[2 * i], 0, 0x3120), hi = __byte_perm(a[2 * i + 1], 0, 0x3120);
+              const uint32_t x[4] = {e4m3_lo(lo), e4m3_hi(lo), e4m3_lo(hi), e4m3_hi(hi)};
+#pragma unroll
+              for (int nb = 0; nb < kBlocks; ++nb) mma(o[nb][d * 2 + i], x, pb[nb][c]);
+            }
+          } else {
+            ldmatrix_x4_trans(vb + L::at(c * 16 + (lane & 7) + (lane >> 4) * 8, d * 2 + ((lane >> 3) & 1)), a);
+#pragma unroll
+            for (int nb = 0; nb < kBlocks; ++nb) mma(o[nb][d], a, pb[nb][c]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i + 1 < kStages; ++i) masks[i] = masks[i + 1];
+    }
+#pragma unroll
+    for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[nb][i] += __shfl_xor_sync(0xffffffffu, l[nb][i], x);
+      }
+    }
+    if (part.begins && part.ends) {
+      const float v_scale = kE4M3 ? p.pool.v_scale[kh] : 1.f;
+#pragma unroll
+      for (int nb = 0; nb < kBlocks; ++nb) {
+        const float inv[2] = {inverse(m[nb][0], l[nb][0], v_scale), inverse(m[nb][1], l[nb][1], v_scale)};
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+          store_frag<T, kE4M3>(out_of(w.row, head0 + nb * 8) + k * 16, p.a.out_head_stride, heads - nb * 8, lane,
+                               make_float4(o[nb][k][0], o[nb][k][1], o[nb][k][2], o[nb][k][3]), inv);
+        if (p.a.lse && g == 0) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (nb * 8 + 2 * t + i < heads) p.a.lse[(long long)w.row * p.a.heads + head0 + nb * 8 + 2 * t + i] = (m[nb][i] + log2f(l[nb][i])) * kLn2;
+        }
+      }
     } else {
-      const long long slot = (long long)blockIdx.x * kRows + h;
-      *reinterpret_cast<float4*>(p.part_o + slot * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      if (d == 0) p.part_ml[slot] = make_float2(top, sum);
+      __syncwarp();  // (the last tile was read by all)
+      float4* area = part.begins ? tail_area(warp) : heads_area + warp * (P::kFrags * 32);
+#pragma unroll
+      for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+          area[(nb * kSteps + k) * 32 + lane] = make_float4(o[nb][k][0], o[nb][k][1], o[nb][k][2], o[nb][k][3]);
+        if (g == 0) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) s_ml[part.begins][warp][nb * 8 + 2 * t + i] = make_float2(m[nb][i], l[nb][i]);
+        }
+      }
+      if (lane == 0) {
+        if (part.begins) s_tail[warp] = make_int2(w.row, w.units - w.at);
+        else s_head[warp] = part.ends ? 1 : 2;
+      }
     }
   }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // ---- parts that meet inside the CTA: a chain begins with a warp's last part, or with what the CTA before left ----
+  int2 tail = make_int2(-1, 0);
+  for (int first = -1; first < kWarps; ++first) {
+    int2 row = make_int2(-1, 0);
+    if (first >= 0) {
+      row = s_tail[first];
+      if (row.x < 0) continue;
+    } else if (s_head[0] == 0) {
+      continue;
+    }
+    int last = first;  // the chain's last warp
+    bool done = false;
+    while (!done && last + 1 < kWarps && s_head[last + 1] != 0) done = s_head[++last] == 1;
+    const bool whole = first >= 0 && done;
+    const float v_scale = kE4M3 && whole ? p.pool.v_scale[kh] : 1.f;
+    const long long slot = 2ll * blockIdx.x + (first >= 0);
+    for (int f = warp; f < P::kFrags; f += kWarps) {
+      const int nb = f / kSteps, h = nb * 8 + 2 * t;
+      float top[2] = {-INFINITY, -INFINITY}, base[2], sum[2] = {0.f, 0.f};
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = max(0, first); i <= last; ++i) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) top[e] = fmaxf(top[e], s_ml[i == first][i][h + e].x);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) base[e] = top[e] == -INFINITY ? 0.f : top[e];
+      for (int i = max(0, first); i <= last; ++i) {
+        const float2 a = s_ml[i == first][i][h], b = s_ml[i == first][i][h + 1];
+        const float fa = exp2f(a.x - base[0]), fb = exp2f(b.x - base[1]);
+        const float4 v = (i == first ? tail_area(i) : heads_area + i * (P::kFrags * 32))[f * 32 + lane];
+        sum[0] += fa * a.y;
+        sum[1] += fb * b.y;
+        acc.x += fa * v.x, acc.y += fb * v.y, acc.z += fa * v.z, acc.w += fb * v.w;
+      }
+      if (whole) {
+        const float inv[2] = {inverse(top[0], sum[0], v_scale), inverse(top[1], sum[1], v_scale)};
+        store_frag<T, kE4M3>(out_of(row.x, head0 + nb * 8) + f % kSteps * 16, p.a.out_head_stride, heads - nb * 8, lane, acc, inv);
+        if (p.a.lse && f % kSteps == 0 && g == 0) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (h + e < heads) p.a.lse[(long long)row.x * p.a.heads + head0 + h + e] = (top[e] + log2f(sum[e])) * kLn2;
+        }
+      } else {
+        p.parts[(slot * P::kFrags + f) * 32 + lane] = acc;
+        if (f % kSteps == 0 && g == 0) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) p.part_ml[slot * kRows + h + e] = make_float2(top[e], sum[e]);
+        }
+      }
+    }
+    if (first >= 0 && !done) {
+      const long long behind = (long long)(kWarps - 1 - first) * share;  // units of the row that this CTA's later warps have
+      tail = make_int2(row.x, (int)((row.y - behind + (long long)kWarps * share - 1) / ((long long)kWarps * share)));
+    }
+  }
+  if (threadIdx.x == 0 && (int)gridDim.x > p.items) p.tails[blockIdx.x] = tail;
 }
 
-// Joins the pieces of a cut row: a CTA per (row, query head), D / 4 threads per piece, 512 / D pieces at a time.
-template <int D, typename T, bool kE4M3, int kRows>
-__global__ void __launch_bounds__(128) k_paged_join(const __grid_constant__ Params p) {
-  constexpr int kLanes = D / 4, kSets = 128 / kLanes;
-  __shared__ float4 s_o[128];
-  __shared__ float2 s_ml[kSets];
+// Joins the parts of a row that spans teams: block c has the row that begins in CTA c and ends in the same item's CTA of a later team.
+template <int D, typename T, bool kE4M3, int kBlocks>
+__global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Params p) {
+  using P = Part<D, kBlocks>;
+  constexpr int kSteps = D / 16, kAhead = 6;
   pdl_launch_dependents();
   pdl_wait();
-  const int b = (int)blockIdx.x / p.a.heads, head = (int)blockIdx.x - b * p.a.heads;
-  const int2 meta = p.meta[b];
-  if (meta.y == 1) return;
-  const int groups = (p.group + kRows - 1) / kRows, kh = head / p.group, hg = (head - kh * p.group) / kRows;
-  const int h = head - kh * p.group - hg * kRows;
-  const int set = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-  auto slot_of = [&](int i) { return ((long long)meta.x + i * p.items_per_row + kh * groups + hg) * kRows + h; };
-  float top = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = set; i0 < meta.y; i0 += 4 * kSets) {
-    float2 ml[4];
-    float4 v[4];
+  const int2 row = p.tails[blockIdx.x];
+  if (row.x < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int item = (int)blockIdx.x % p.items, groups = (p.group + P::kRows - 1) / P::kRows, kh = item / groups, h0 = (item - kh * groups) * P::kRows;
+  const int heads = min(P::kRows, p.group - h0), head0 = kh * p.group + h0, n = 1 + row.y;
+  const float v_scale = kE4M3 ? p.pool.v_scale[kh] : 1.f;
+  for (int f = warp; f < P::kFrags; f += (int)blockDim.x / 32) {
+    const int nb = f / kSteps, h = nb * 8 + 2 * t;
+    float top[2] = {-INFINITY, -INFINITY}, base[2], sum[2] = {0.f, 0.f};
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < n; i0 += kAhead) {
+      float4 ml[kAhead], v[kAhead];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u * kSets;
-      ml[u] = i < meta.y ? p.part_ml[slot_of(i)] : make_float2(-INFINITY, 0.f);
-      v[u] = i < meta.y ? *reinterpret_cast<const float4*>(p.part_o + slot_of(i) * D + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u;
+        const long long slot = 2ll * (blockIdx.x + i * p.items) + (i == 0);
+        ml[u] = i < n ? *reinterpret_cast<const float4*>(p.part_ml + slot * P::kRows + h) : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+        v[u] = i < n ? p.parts[(slot * P::kFrags + f) * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float next[2] = {top[0], top[1]};
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) next[0] = fmaxf(next[0], ml[u].x), next[1] = fmaxf(next[1], ml[u].z);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        base[e] = next[e] == -INFINITY ? 0.f : next[e];
+        const float corr = exp2f(top[e] - base[e]);
+        sum[e] *= corr;
+        if (e == 0) acc.x *= corr, acc.z *= corr;
+        else acc.y *= corr, acc.w *= corr;
+        top[e] = next[e];
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const float fa = exp2f(ml[u].x - base[0]), fb = exp2f(ml[u].z - base[1]);
+        sum[0] += fa * ml[u].y;
+        sum[1] += fb * ml[u].w;
+        acc.x += fa * v[u].x, acc.y += fb * v[u].y, acc.z += fa * v[u].z, acc.w += fb * v[u].w;
+      }
     }
-    float next = top;
+    const float inv[2] = {inverse(top[0], sum[0], v_scale), inverse(top[1], sum[1], v_scale)};
+    T* out = reinterpret_cast<T*>(p.a.out) + row.x * p.a.out_stride + (head0 + nb * 8) * p.a.out_head_stride + f % kSteps * 16;
+    store_frag<T, kE4M3>(out, p.a.out_head_stride, heads - nb * 8, lane, acc, inv);
+    if (p.a.lse && f % kSteps == 0 && g == 0) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) next = fmaxf(next, ml[u].x);
-    const float base = next == -INFINITY ? 0.f : next, corr = exp2f(top - base);
-    sum *= corr;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] *= corr;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float f = exp2f(ml[u].x - base);
-      sum += f * ml[u].y;
-      acc[0] += f * v[u].x, acc[1] += f * v[u].y, acc[2] += f * v[u].z, acc[3] += f * v[u].w;
+      for (int e = 0; e < 2; ++e)
+        if (h + e < heads) p.a.lse[(long long)row.x * p.a.heads + head0 + h + e] = (top[e] + log2f(sum[e])) * kLn2;
     }
-    top = next;
   }
-  s_o[threadIdx.x] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-  if (lane == 0) s_ml[set] = make_float2(top, sum);
-  __syncthreads();
-  if (set > 0) return;
-  top = -INFINITY, sum = 0.f, acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
-#pragma unroll
-  for (int i = 0; i < kSets; ++i) top = fmaxf(top, s_ml[i].x);
-  const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-  for (int i = 0; i < kSets; ++i) {
-    const float f = exp2f(s_ml[i].x - base);
-    const float4 v = s_o[i * kLanes + lane];
-    sum += f * s_ml[i].y;
-    acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
-  }
-  const float inv = top == -INFINITY ? 0.f : (kE4M3 ? p.pool.v_scale[kh] : 1.f) / sum;
-  const uint2 raw = make_uint2(Pair<T>::pack(acc[0] * inv, acc[1] * inv), Pair<T>::pack(acc[2] * inv, acc[3] * inv));
-  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.a.out) + b * p.a.out_stride + head * p.a.out_head_stride + lane * 4) = raw;
-  if (lane == 0 && p.a.lse) p.a.lse[(long long)b * p.a.heads + head] = (top + log2f(sum)) * kLn2;
 }
 
-struct Shape {
-  int rows, items_per_row;
-  long long items, extra;
-};
-Shape shape_of(int batch, int heads, int kv_heads, int max_len, int window, int slots) {
-  Shape s;
-  const int group = heads / kv_heads;
-  s.rows = group > 8 ? 16 : 8;
-  s.items_per_row = kv_heads * ((group + s.rows - 1) / s.rows);
-  s.items = (long long)batch * s.items_per_row;
-  s.extra = extra_pieces(batch, s.items_per_row, slots, window > 0 && window < max_len ? window : max_len);
-  return s;
-}
-size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+int blocks_of(int group) { return group > 8 ? 2 : 1; }
+int items_of(int kv_heads, int group) { return kv_heads * ((group + 8 * blocks_of(group) - 1) / (8 * blocks_of(group))); }
+// CTAs of a launch over rows that can be as long as `most`.
+long long ctas_of(int rows, int items, int most, int tile, int slots) { return (long long)items * teams_of(rows, items, units_of(most, tile), kWarps, slots); }
+// CTAs that the GPU holds at a time.
+int slots_of(int stage_bytes, int sms) { return stage_bytes > 8192 ? sms : 2 * sms; }
+int most_seen(int max_len, int window) { return window > 0 && window < max_len ? window : max_len; }
 
-template <int D, typename T, bool kE4M3, int kRows>
-cudaError_t launch(Params p, const Shape& s, cudaStream_t stream) {
-  auto* kernel = k_paged_attention<D, T, kE4M3, kRows>;
-  constexpr int smem = Tile<D, kE4M3>::kSmem;
-  static_assert(smem >= kWarps * kRows * (D * 4 + 8), "the join of the warps fits the pipelines' space");
+template <int D, typename T, bool kE4M3, int kBlocks>
+cudaError_t launch(Params p, void* workspace, int sms, cudaStream_t stream) {
+  using P = Part<D, kBlocks>;
+  auto* kernel = k_paged_attention<D, T, kE4M3, kBlocks>;
+  constexpr int smem = Tile<D, kE4M3, kBlocks>::kSmem + kWarps * P::kFrags * 512;
+  static_assert(smem <= 227 << 10 && Tile<D, kE4M3, kBlocks>::kStages * Tile<D, kE4M3, kBlocks>::kStage >= P::kFrags * 512, "shared memory");
   cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(kernel), smem).rc;
   if (rc != cudaSuccess) return rc;
-  rc = launch_kernel_ex(kernel, dim3((unsigned)(s.items + s.extra)), dim3(kWarps * 32), (size_t)smem, stream, true, 1, p);
-  if (rc != cudaSuccess || s.extra == 0) return rc;
-  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kRows>, dim3((unsigned)p.a.rows * p.a.heads), dim3(128), 0, stream, true, 1, p);
+  const long long ctas = ctas_of(p.a.rows, p.items, most_seen(p.max_len, p.a.window), Tile<D, kE4M3, kBlocks>::kPos, slots_of(Tile<D, kE4M3, kBlocks>::kStage, sms));
+  if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
+  p.tails = reinterpret_cast<int2*>(workspace);
+  p.parts = reinterpret_cast<float4*>(p.tails + (ctas + 1) / 2 * 2);
+  p.part_ml = reinterpret_cast<float2*>(p.parts + ctas * 2 * P::kFrags * 32);
+  rc = launch_kernel_ex(kernel, dim3((unsigned)ctas), dim3(kWarps * 32), (size_t)smem, stream, true, 1, p);
+  if (rc != cudaSuccess || ctas == p.items) return rc;  // (a single team finishes its rows)
+  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kBlocks>, dim3((unsigned)ctas), dim3(P::kFrags * 32 < 256 ? P::kFrags * 32 : 256), 0, stream, true, 1, p);
 }
 
 }  // namespace
 
 size_t paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int max_len, int window, int sms) {
-  const Shape s = shape_of(rows, heads, kv_heads, max_len, window, 2 * sms);
-  if (s.extra == 0) return 0;
-  const size_t parts = (size_t)(s.items + s.extra) * s.rows;
-  return round16(rows * sizeof(int2)) + parts * (dim * sizeof(float) + sizeof(float2));
+  const int group = heads / kv_heads, blocks = blocks_of(group);
+  // (of all cache types: the smallest tile, one or two CTAs an SM)
+  const int items = items_of(kv_heads, group), most = most_seen(max_len, window);
+  const long long one = ctas_of(rows, items, most, 16, sms), two = ctas_of(rows, items, most, 16, 2 * sms);
+  const size_t ctas = (size_t)(one > two ? one : two);
+  return ctas == (size_t)items ? 0 : (ctas + 1) * (sizeof(int2) + 2 * blocks * ((size_t)(dim / 16) * 512 + 8 * sizeof(float2)));
 }
 
 cudaError_t launch_paged_attention(const PagedAttention& a, PagedType type, const PagedPool& pool, PagedType cache, void* workspace, int sms,
@@ -527,21 +708,20 @@ cudaError_t launch_paged_attention(const PagedAttention& a, PagedType type, cons
       (cache != PAGED_E4M3 && cache != type))
     return cudaErrorInvalidValue;
   const long long cap = (long long)a.width * pool.page_size;
-  Params p;
+  Params p = {};
   p.a = a;
   p.pool = pool;
   p.div = page_div(pool.page_size);
   p.group = a.heads / pool.heads;
-  p.max_len = (int)(cap < 0x7fff0000ll ? cap : 0x7fff0000ll);
-  const int slots = 2 * sms;
-  const Shape s = shape_of(a.rows, a.heads, pool.heads, p.max_len, a.window, slots);
-  if (s.items + s.extra > 0x7fffffffll || (long long)a.rows * a.heads > 0x7fffffffll) return cudaErrorInvalidValue;
-  p.items_per_row = s.items_per_row;
-  p.slots = s.extra > 0 ? slots : 0;
-  p.meta = reinterpret_cast<int2*>(workspace);
-  p.part_o = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + round16(a.rows * sizeof(int2)));
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)(s.items + s.extra) * s.rows * pool.dim);
-#define PENNY_PAGED_ROWS(D, T, E) (s.rows == 8 ? launch<D, T, E, 8>(p, s, stream) : launch<D, T, E, 16>(p, s, stream))
+  p.max_len = (int)(cap < kMaxLen ? cap : kMaxLen);
+  p.items = items_of(pool.heads, p.group);
+  if ((long long)a.rows * units_of(most_seen(p.max_len, a.window), 16) > kMaxUnits) return cudaErrorInvalidValue;
+  const Steps st = steps_of(pool.pages, pool.page_size, pool.page_stride, pool.pos_stride, cache == PAGED_E4M3 ? 1 : 2);
+  if (st.bytes == 0) return cudaErrorInvalidValue;
+  p.page_step = st.page;
+  p.pos_step = st.pos;
+  p.step_bytes = st.bytes;
+#define PENNY_PAGED_ROWS(D, T, E) (p.group <= 8 ? launch<D, T, E, 1>(p, workspace, sms, stream) : launch<D, T, E, 2>(p, workspace, sms, stream))
 #define PENNY_PAGED_TYPE(D)                                                                                                   \
   (cache == PAGED_E4M3 ? (type == PAGED_BF16 ? PENNY_PAGED_ROWS(D, __nv_bfloat16, true) : PENNY_PAGED_ROWS(D, __half, true)) \
                        : (type == PAGED_BF16 ? PENNY_PAGED_ROWS(D, __nv_bfloat16, false) : PENNY_PAGED_ROWS(D, __half, false)))

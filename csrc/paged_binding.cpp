@@ -8,6 +8,7 @@
 #include <cmath>
 
 #include "paged_kernels.h"
+#include "paged_plan.h"
 
 namespace py = pybind11;
 using namespace penny;
@@ -149,6 +150,8 @@ void bind_paged(py::module_& m) {
     const int64_t B = q.size(0), H = q.size(1);
     need(B < (1 << 24) && H < (1 << 20) && H >= 1 && H % pool.heads == 0, "paged_attention: heads a multiple of the caches'");
     need(pool.dim == 64 || pool.dim == 128 || pool.dim == 256, "paged_attention: dim 64, 128 or 256");
+    need(paged::steps_of(pool.pages, pool.page_size, pool.page_stride, pool.pos_stride, (int)k.element_size()).bytes > 0,
+         "paged_attention: caches that reach over 2^32 times what divides their strides");
     auto rows_ok = [&](const at::Tensor& t) { return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned(t); };
     need(rows_ok(q), "paged_attention: heads of q contiguous, 16-byte aligned");
     need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B && table.size(1) >= 1 && table.size(1) < (1ll << 31) &&
@@ -174,6 +177,7 @@ void bind_paged(py::module_& m) {
     const int sms = sms_of(q.get_device());
     const int win = (int)std::min<int64_t>(window, 1ll << 30);
     const int max_len = (int)std::min<int64_t>(table.size(1) * pool.page_size, 0x7fff0000ll);
+    need(B * (int64_t)paged::units_of(win > 0 && win < max_len ? win : max_len, 16) <= paged::kMaxUnits, "paged_attention: a table for over 2^34 positions");
     const size_t bytes = paged_attention_workspace_bytes((int)B, (int)H, pool.heads, pool.dim, max_len, win, sms);
     if (workspace.has_value()) need(workspace->nbytes() >= bytes, "workspace too small (paged_attention_workspace_bytes)");
     else if (bytes > 0) workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));

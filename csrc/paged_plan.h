@@ -47,21 +47,88 @@ PENNY_ATTN_HD Seen seen_of(int length, int max_len, int window) {
   return {window > 0 && end > window ? end - window : 0, end};
 }
 
-// How the rows of a batch are cut: into pieces of `len` positions or a little more, so that all (row, head group) pairs
-// together make about `slots` CTAs.  The lengths are on the device; the launcher makes the grid for the most pieces that
-// any lengths can ask for, and every CTA counts through the cut by itself.
-constexpr int kMinPiece = 256, kMaxPieces = 128;
+// How a batch is shared out.  A row's (KV head, head group) pairs are its items; a team is one CTA for each item, so that a page's
+// heads are read at about the same time (apart from each other 64 rows of 16000 positions took 632 us instead of 607).  The
+// rows lie in a line, each a unit for its start (its output, its q) and one for every tile of positions; every warp of a
+// team's CTAs gets `share` units, at least kMinShare.  The lengths are on the device, and every CTA sums over them by itself.
+constexpr int kMinShare = 4;
+constexpr long long kMaxLen = 0x7fff0000, kMaxUnits = 1ll << 30;  // (shares fit 32 bits)
 
-PENNY_ATTN_HD int piece_len(long long total, int items_per_row, int slots) {
-  const long long len = (total * items_per_row + slots - 1) / slots;
-  return len < kMinPiece ? kMinPiece : len > 0x7fffffff ? 0x7fffffff : (int)len;
+PENNY_ATTN_HD int units_of(int positions, int tile) { return 1 + (positions + tile - 1) / tile; }
+PENNY_ATTN_HD int share_of(long long units, int warps) {
+  const long long share = (units + warps - 1) / warps;
+  return share < kMinShare ? kMinShare : (int)share;
 }
-PENNY_ATTN_HD int pieces_of(int rows, int len) { return attn::at_most(kMaxPieces, attn::at_least(1, rows / len)); }
-// CTAs beyond one per (row, head group): floor(rows / len) summed over the rows is at most total / len, so all pieces of all
-// head groups are at most `slots` and one for each pair; no more than the longest row can have either.
-inline long long extra_pieces(long long rows, int items_per_row, int slots, int most_seen) {
-  const long long by_len = rows * items_per_row * (pieces_of(most_seen, kMinPiece) - 1);
-  return by_len < slots ? by_len : slots;
+// Teams of a launch: as many as the GPU holds (`slots` CTAs), in more rounds where that leaves over a tenth of it empty; no more
+// than there are shares, if every row has `units` units.
+inline int teams_of(long long rows, int items, long long units, int warps, int slots) {
+  int best = 1;
+  double used = 0;
+  for (int rounds = 1; rounds <= 8 && used < 0.9; ++rounds) {
+    const int teams = slots * rounds / items;
+    const double now = (double)teams * items / ((double)slots * rounds);
+    if (teams > 0 && now > used) best = teams, used = now;
+  }
+  const long long most = (rows * units + (long long)warps * kMinShare - 1) / ((long long)warps * kMinShare);
+  return most < best ? (int)most : best;
+}
+
+// What a warp has of the line: where it stands in a row, and what is left of its share.
+struct Walk {
+  int row;
+  int at, units;   // units of the row that lie behind, and all of them
+  int first, end;  // positions
+  int left;        // units of the share
+};
+// A part of a row: its tiles [from, to); begins and ends: the row does.
+struct WalkPart {
+  int from, to;
+  bool begins, ends;
+};
+template <class SeenOf>  // SeenOf(row): what a row attends to
+PENNY_ATTN_HD void enter_row(Walk& w, int tile, SeenOf seen) {
+  const Seen s = seen(w.row);
+  w.first = s.first;
+  w.end = s.end;
+  w.units = units_of(s.end - s.first, tile);
+}
+// The next part of the share (w.left > 0): all that it has of one row.  Without tiles: an empty row, which begins and ends, or a
+// row's start alone, which is nothing (the next warp's part begins the row).
+template <class SeenOf>
+PENNY_ATTN_HD WalkPart next_part(Walk& w, int tile, SeenOf seen) {
+  if (w.at == w.units) {
+    ++w.row;
+    w.at = 0;
+    enter_row(w, tile, seen);
+  }
+  const int from = w.at, to = attn::at_most(w.units, w.at + w.left);
+  w.left -= to - from;
+  w.at = to;
+  const bool some = to > 1 || w.units == 1;
+  return {attn::at_least(0, from - 1), to - 1, from <= 1 && some, to == w.units && some};
+}
+
+// A pool's strides in a unit so large that a place in it fits 32 bits: the largest power of two that divides both.  bytes 0:
+// no such unit (more than 2^32 - 1 times what divides the strides).
+struct Steps {
+  uint32_t page, pos, bytes;
+};
+inline Steps steps_of(long long pages, long long page_size, long long page_stride, long long pos_stride, int value_bytes) {
+  long long page = page_stride * value_bytes, pos = pos_stride * value_bytes;
+  uint32_t bytes = 1;
+  // (the strides of a single page or position say nothing)
+  if (pages == 1) page = 0;
+  if (page_size == 1) pos = 0;
+  while (bytes < (1u << 30) && ((page | pos) & 1) == 0 && (page | pos) != 0) page >>= 1, pos >>= 1, bytes <<= 1;
+  const long long limit = 0xffffffffll;
+  if (page > limit || pos > limit || (pages - 1) * page > limit || (page_size - 1) * pos > limit || (pages - 1) * page + (page_size - 1) * pos >= limit)
+    return {0, 0, 0};
+  return {(uint32_t)page, (uint32_t)pos, bytes};
+}
+constexpr uint32_t kNoStep = 0xffffffffu;
+// place_of in such units; kNoStep: the pool does not have the page.
+PENNY_ATTN_HD uint32_t step_of(int page, int pages, int pos, const PageDiv& d, uint32_t page_step, uint32_t pos_step) {
+  return (uint32_t)page < (uint32_t)pages ? (uint32_t)page * page_step + (uint32_t)(pos - div_page(d, pos) * (int)d.size) * pos_step : kNoStep;
 }
 
 }  // namespace paged

@@ -375,20 +375,47 @@ long long penny_page_place(int page, int pages, int pos, int size, long long pag
 long long penny_page_place_of_slot(long long slot, int pages, int size, long long page_step, long long pos_step) {
   return penny::paged::place_of_slot(slot, pages, size, page_step, pos_step);
 }
-// first and end of what every row attends to, its pieces as the kernel counts them; returns the pieces beyond one per (row,
-// item) that the launcher's grid has room for.
-long long penny_paged_cut(const int* lengths, int rows, int items_per_row, int max_len, int window, int slots, int* first, int* end, int* pieces) {
+uint32_t penny_page_steps(long long pages, long long page_size, long long page_stride, long long pos_stride, int value_bytes, uint32_t* page, uint32_t* pos) {
+  const penny::paged::Steps s = penny::paged::steps_of(pages, page_size, page_stride, pos_stride, value_bytes);
+  *page = s.page;
+  *pos = s.pos;
+  return s.bytes;
+}
+uint32_t penny_page_step_of(int page, int pages, int pos, int size, uint32_t page_step, uint32_t pos_step) {
+  return penny::paged::step_of(page, pages, pos, penny::paged::page_div(size), page_step, pos_step);
+}
+int penny_paged_teams(long long rows, int items, long long units, int warps, int slots) { return penny::paged::teams_of(rows, items, units, warps, slots); }
+// The walk of warp `warp` of `warps` of an item: its parts (row, first tile, last tile, begins | 2 ends | 4 empty, units of the row
+// behind the part) in order, and its tiles' first positions.  Returns the number of parts; -1: too many for `most`.
+int penny_paged_walk(const int* lengths, int rows, int max_len, int window, int tile, int warps, int warp, int* parts, int most, int* tiles,
+                     int most_tiles, int* num_tiles, int* share_out) {
   using namespace penny::paged;
-  long long total = 0;
-  for (int r = 0; r < rows; ++r) {
-    const Seen s = seen_of(lengths[r], max_len, window);
-    first[r] = s.first;
-    end[r] = s.end;
-    total += s.end - s.first;
+  auto seen = [&](int r) { return seen_of(lengths[r], max_len, window); };
+  auto units = [&](int r) { return units_of(seen(r).end - seen(r).first, tile); };
+  long long total = 0, x = 0;
+  for (int r = 0; r < rows; ++r) total += units(r);
+  const int share = share_of(total, warps);
+  const long long begin = (long long)warp * share;
+  *num_tiles = 0;
+  *share_out = share;
+  if (begin >= total) return 0;
+  Walk w = {};
+  while (begin >= x + units(w.row)) x += units(w.row++);
+  enter_row(w, tile, seen);
+  w.at = (int)(begin - x);
+  w.left = (int)(total - begin < share ? total - begin : share);
+  int n = 0;
+  while (w.left > 0) {
+    const WalkPart p = next_part(w, tile, seen);
+    if (n >= most) return -1;
+    for (int i = p.from; i < p.to; ++i) {
+      if (*num_tiles >= most_tiles) return -1;
+      tiles[(*num_tiles)++] = w.first + i * tile;
+    }
+    int* to = parts + 5 * n++;
+    to[0] = w.row, to[1] = p.from, to[2] = p.to, to[3] = p.begins | p.ends << 1 | (w.units == 1) << 2, to[4] = w.units - w.at;
   }
-  const int len = piece_len(total, items_per_row, slots);
-  for (int r = 0; r < rows; ++r) pieces[r] = pieces_of(end[r] - first[r], len);
-  return extra_pieces(rows, items_per_row, slots, window > 0 && window < max_len ? window : max_len);
+  return n;
 }
 // Tile -> (row block, column block) of the persistent GEMM kernels; pair_rank < 0
 // selects the single-CTA kernel, 0 / 1 the CTA of a pair.  Returns the number of

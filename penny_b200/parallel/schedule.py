@@ -175,12 +175,37 @@ def slot_place(slot: int, pages: int, page_size: int, page_step: int, position_s
     return f(slot, pages, page_size, page_step, position_step)
 
 
-def paged_cut(lengths, items_per_row: int, max_len: int, window: int = 0, slots: int = 296):
-    """The paged attention's cut of a batch's rows (csrc/paged_plan.h): ([first, end) of every row, pieces of every row, pieces
-    beyond one per (row, item) that the grid has room for)."""
-    n = len(lengths)
-    lens, first, end, pieces = (ctypes.c_int * n)(*lengths), (ctypes.c_int * n)(), (ctypes.c_int * n)(), (ctypes.c_int * n)()
-    lib = sim_lib()
-    lib.penny_paged_cut.restype = ctypes.c_longlong
-    extra = lib.penny_paged_cut(lens, n, items_per_row, max_len, window, slots, first, end, pieces)
-    return list(zip(first, end)), list(pieces), extra
+def page_steps(pages: int, page_size: int, page_stride: int, position_stride: int, value_bytes: int):
+    """A pool's strides in the unit in which its places fit 32 bits: (unit in bytes, page step, position step), None if there is none
+    (csrc/paged_plan.h)."""
+    f, page, pos = sim_lib().penny_page_steps, ctypes.c_uint32(), ctypes.c_uint32()
+    f.restype, f.argtypes = ctypes.c_uint32, [ctypes.c_longlong] * 4 + [ctypes.c_int] + [ctypes.POINTER(ctypes.c_uint32)] * 2
+    unit = f(pages, page_size, page_stride, position_stride, value_bytes, ctypes.byref(page), ctypes.byref(pos))
+    return (unit, page.value, pos.value) if unit else None
+
+
+def page_step_of(page: int, pages: int, position: int, page_size: int, page_step: int, position_step: int):
+    """page_place in such units; None for a page that the pool does not have."""
+    f = sim_lib().penny_page_step_of
+    f.restype, f.argtypes = ctypes.c_uint32, [ctypes.c_int] * 4 + [ctypes.c_uint32] * 2
+    at = f(page, pages, position, page_size, page_step, position_step)
+    return None if at == 0xffffffff else at
+
+
+def paged_teams(rows: int, items: int, units: int, warps: int = 4, slots: int = 296) -> int:
+    """Teams of CTAs of a paged attention launch (csrc/paged_plan.h)."""
+    f = sim_lib().penny_paged_teams
+    f.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
+    return f(rows, items, units, warps, slots)
+
+
+def paged_walk(lengths, max_len: int, warps: int, warp: int, window: int = 0, tile: int = 16):
+    """What one of the paged attention's warps of an item does (csrc/paged_plan.h): (its parts: (row, first tile, last tile, begins,
+    ends, empty row, units of the row behind the part), its tiles' first positions, every warp's share)."""
+    n, most = len(lengths), 1 << 16
+    parts, tiles, num, share = (ctypes.c_int * (5 * most))(), (ctypes.c_int * most)(), ctypes.c_int(), ctypes.c_int()
+    got = sim_lib().penny_paged_walk((ctypes.c_int * n)(*lengths), n, max_len, window, tile, warps, warp, parts, most, tiles, most,
+                                     ctypes.byref(num), ctypes.byref(share))
+    assert got >= 0, "a walk longer than this function's arrays"
+    rows = [parts[5 * i:5 * i + 5] for i in range(got)]
+    return [(r, a, b, bool(f & 1), bool(f & 2), bool(f & 4), z) for r, a, b, f, z in rows], tiles[:num.value], share.value

@@ -32,27 +32,76 @@ def test_places_of_bad_pages_and_slots():
     assert at(2 ** 33 + 3, 2 ** 30, 16, 16, 1) == 2 ** 33 + 3
 
 
-@pytest.mark.parametrize("max_len", [1, 255, 256, 511, 512, 1024, 4352, 100000, 2 ** 31 - 2 ** 16])
-@pytest.mark.parametrize("items", [1, 2, 8, 20])
-def test_every_piece_has_a_cta(max_len, items):
-    rng = random.Random(max_len + items)
-    for B in (1, 2, 3, 7, 37, 64, 130, 300, 1000):
-        for window in (0, 1, 300, 5000):
+@pytest.mark.parametrize("pages,page,page_stride,pos_stride,size", [
+    (100, 16, 16 * 8 * 128, 8 * 128, 2), (100, 16, 16 * 8 * 128, 128, 2), (7, 24, 24 * 64 + 16, 64, 1), (1, 5, 12345, 64, 1), (1, 1, 3, 5, 2), (5, 1, 8, 999, 2),
+    (2 ** 22, 16, 16 * 1024, 1024, 2), (2 ** 15, 16, 80 * 2 * 16 * 1024, 1024, 2), (3, 16, 0, 64, 2)])
+def test_steps(pages, page, page_stride, pos_stride, size):
+    unit, a, b = schedule.page_steps(pages, page, page_stride, pos_stride, size)
+    rng = random.Random(pages)
+    for pg in {0, pages - 1, rng.randrange(pages)}:
+        for pos in (0, page - 1, 3 * page + page // 2):
+            at = schedule.page_step_of(pg, pages, pos, page, a, b)
+            assert at * unit == schedule.page_place(pg, pages, pos, page, page_stride * size, pos_stride * size)
+    for pg in (-1, pages, 2 ** 31 - 1, -2 ** 31):
+        assert schedule.page_step_of(pg, pages, 0, page, a, b) is None
+
+
+def test_no_steps():
+    assert schedule.page_steps(2 ** 31 - 1, 16, 16 * 24 + 8, 24, 2) is None      # 16 bytes divide the strides: 64 GB at most
+    assert schedule.page_steps(2 ** 26, 16, 16 * 24, 24, 2)[0] == 16
+
+
+def _walks(lengths, max_len, teams, window, tile=16):
+    """Every warp's walk, and that together they are the batch: every tile once, whole rows finished by one warp, the others by a warp
+    that begins them, warps in the middle and one that ends them."""
+    per, warps = 4, 4 * teams
+    seen = [(max(0, min(n, max_len) - window) if window else 0, max(0, min(n, max_len))) for n in lengths]
+    tiles = [-(-(b - a) // tile) for a, b in seen]
+    covered, empties, open_row, counts = {}, set(), None, {}
+    for w in range(warps):
+        parts, starts, share = schedule.paged_walk(lengths, max_len, warps, w, window, tile)
+        assert starts == [seen[r][0] + tile * i for r, a, b, *_ in parts for i in range(a, b)]
+        real = [p for p in parts if p[2] > p[1] or p[5]]
+        for k, (r, a, b, begins, ends, empty, behind) in enumerate(real):
+            if empty:
+                assert tiles[r] == 0 and r not in empties and begins and ends
+                empties.add(r)
+                continue
+            assert covered.get(r, 0) == a and b <= tiles[r] and begins == (a == 0) and ends == (b == tiles[r]) and behind == tiles[r] - b
+            covered[r] = b
+            assert begins or k == 0                 # one part of an earlier row, the first
+            assert ends or k == len(real) - 1       # one part of a later row, the last
+            if not begins:
+                assert open_row == r
+            open_row = None if ends else r
+            if begins and not ends:
+                later = -(-(behind - (per - 1 - w % per) * share) // (per * share))  # teams that follow, as the kernel counts them
+                counts[r] = (w // per, max(0, later))
+            if ends and not begins:
+                first, later = counts[r]
+                assert first + later == w // per
+    assert open_row is None
+    assert all(covered.get(r, 0) == tiles[r] for r in range(len(lengths)))
+    assert empties == {r for r in range(len(lengths)) if tiles[r] == 0}
+
+
+@pytest.mark.parametrize("teams", [1, 2, 5, 37, 296])
+@pytest.mark.parametrize("window", [0, 1, 100])
+def test_every_tile_once(teams, window):
+    rng = random.Random(teams)
+    top = 2 ** 31 - 1
+    for B in (1, 2, 5, 40, 300):
+        for max_len in (1, 16, 17, 300, 5000):
             inside = [rng.randrange(max_len + 1) for _ in range(B)]
-            edges = [max_len, 0, -1, -2 ** 31, 2 ** 31 - 1, max_len + 1]
-            for lengths in [inside] + [[min(e, 2 ** 31 - 1)] * B for e in edges] + [[min(rng.choice(edges), 2 ** 31 - 1)] + inside[1:]]:
-                seen, pieces, extra = schedule.paged_cut(lengths, items, max_len, window)
-                for (first, end), n in zip(seen, lengths):
-                    assert end == max(0, min(n, max_len)) and first == (max(0, end - window) if window else 0)
-                assert all(1 <= p <= 128 for p in pieces)
-                assert sum(pieces) * items <= B * items + extra  # every piece of every row has a CTA
-                assert extra <= 296
+            for lengths in (inside, [0] * B, [max_len] * B, [top] * B, [-1] + inside[1:], [-2 ** 31] * (B - 1) + [max_len], [max_len] + [1] * (B - 1)):
+                _walks(lengths, max_len, teams, window, tile=rng.choice([16, 32, 64]))
 
 
-def test_the_cut():
-    assert schedule.paged_cut([200], 1, 4096)[1:] == ([1], 15)
-    assert schedule.paged_cut([2048], 1, 4096)[1] == [8]
-    assert schedule.paged_cut([100001] * 2, 8, 100032)[1] == [18, 18]
-    assert schedule.paged_cut([2048] * 64, 8, 2560)[1] == [1] * 64       # the rows fill the GPU by themselves
-    assert schedule.paged_cut([60000] + [100] * 63, 8, 65536)[1] == [33] + [1] * 63
-    assert schedule.paged_cut([255] * 3, 8, 256)[2] == 0                  # no row can be cut: no second kernel
+def test_teams():
+    assert schedule.paged_teams(64, 8, 129) == 37 and schedule.paged_teams(1, 1, 14) == 1 and schedule.paged_teams(1, 8, 129) == 9
+    for items in list(range(1, 400)) + [1000, 4096]:
+        teams = schedule.paged_teams(1000, items, 1000)
+        ctas = teams * items
+        assert teams >= 1 and ctas <= max(items, 8 * 296)
+        rounds = -(-ctas // 296)
+        assert ctas >= 0.85 * rounds * 296 or items > 8 * 296  # the GPU is filled

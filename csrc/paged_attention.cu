@@ -42,34 +42,20 @@ using attn::ldmatrix_x4;
 using attn::ldmatrix_x4_trans;
 using attn::mma_bf16;
 
-#ifndef PW
-#define PW 4
-#define PS 3
-#define TB 4096
-#endif
-constexpr int kWarps = PW;
+constexpr int kWarps = 4;
 constexpr float kSlack = 8.f;  // weights of up to 2^8
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-template <bool kWide>
-struct MaskOf {
-  using type = uint32_t;
-};
-template <>
-struct MaskOf<true> {
-  using type = unsigned long long;
-};
 
 template <int D, bool kE4M3, int kBlocks>
 struct Tile {
   static constexpr int kRow = kE4M3 ? D : 2 * D;               // bytes of a position
-  static constexpr int kPos = TB / kRow > 16 ? TB / kRow : 16;
+  static constexpr int kPos = kRow <= 128 ? 32 : 16;
   static constexpr int kChunks = kRow / 16;                    // 16-byte chunks of a position
   static constexpr int kPerPass = 32 / kChunks;                // positions that a warp's 32 chunks cover
   static constexpr int kStage = 2 * kPos * kRow;
-  static constexpr int kStages = kBlocks == 2 || kStage > 8192 ? 2 : PS;
+  static constexpr uint32_t kAll = 0xffffffffu >> (32 - kPos);  // the mask of a full tile
+  static constexpr int kStages = kBlocks == 2 || kStage > 8192 ? 2 : kStage < 8192 ? 5 : 3;
   static constexpr int kSmem = kWarps * kStages * kStage;
-  using Mask = typename MaskOf<(kPos > 32)>::type;
   // where chunk c of position r lies: eight positions' equal chunks in eight different 16-byte banks
   static __device__ __forceinline__ uint32_t at(int r, int c) {
     if constexpr (kRow == 64) return (uint32_t)((r >> 1) * 128 + ((((r & 1) << 2) | (c ^ ((r >> 1) & 3))) << 4));
@@ -129,7 +115,7 @@ struct Params {
   PagedPool pool;
   PageDiv div;
   int group;              // G
-  int items;              // (KV head, head group) pairs
+  int items, groups;      // (KV head, head group) pairs, head groups of a KV head
   int max_len;
   uint32_t page_step, pos_step, step_bytes;  // strides in units of step_bytes
   int2* tails;            // per CTA: the row that begins in it and does not end in it, how many teams follow; row -1: none
@@ -143,64 +129,46 @@ struct Part {
   static constexpr int kRows = 8 * kBlocks;
 };
 
-// The share of a team's warps, and where this one begins.  Called by all threads.
-template <int kWarps>
+// The share of an item's warps, and where this one begins.  Called by whole warps, each of which sums over all rows (no barrier).
 __device__ __forceinline__ int find_walk(const Params& p, int tile, Walk& w) {
-  __shared__ long long s_sum[kWarps], s_at[kWarps];
-  __shared__ int s_row[kWarps];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, team = (int)blockIdx.x / p.items, teams = (int)gridDim.x / p.items;
-  const int per = (p.a.rows + kWarps * 32 - 1) / (kWarps * 32), r0 = min(p.a.rows, tid * per), r1 = min(p.a.rows, r0 + per);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (p.a.rows + 31) / 32, r0 = min(p.a.rows, lane * per), r1 = min(p.a.rows, r0 + per);
   auto seen = [&](int r) { return seen_of(p.a.lengths[r], p.max_len, p.a.window); };
   auto units = [&](int r) {
     const Seen s = seen(r);
     return units_of(s.end - s.first, tile);
   };
-  long long mine = 0;
+  int mine = 0;
+#pragma unroll 4
   for (int r = r0; r < r1; ++r) mine += units(r);
-  long long incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) s_sum[warp] = incl;
-  if (lane == 0) s_row[warp] = -1;
-  __syncthreads();
-  long long total = 0, x = incl - mine;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < warp) x += s_sum[i];
-    total += s_sum[i];
-  }
-  const int share = share_of(total, teams * kWarps);
-  for (int r = r0; r < r1; ++r) {
-    const int n = units(r);
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const long long begin = ((long long)team * kWarps + i) * share;
-      if (begin >= x && begin < x + n) {
-        s_row[i] = r;
-        s_at[i] = begin - x;
-      }
-    }
-    x += n;
-  }
-  __syncthreads();
-  w.row = s_row[warp];
+  const int total = __shfl_sync(0xffffffffu, incl, 31), share = share_of(total, (int)gridDim.y * kWarps);
+  const long long begin = (long long)(blockIdx.y * kWarps + warp) * share;
   w.left = 0;
-  if (w.row >= 0) {
-    enter_row(w, tile, seen);
-    w.at = (int)s_at[warp];
-    w.left = (int)min((long long)share, total - ((long long)team * kWarps + warp) * share);
+  if (begin >= total) return share;
+  int row = r0, at = (int)begin - (incl - mine);
+  const bool here = at >= 0 && at < mine;
+  if (here && per > 1) {
+    for (int n; at >= (n = units(row)); ++row) at -= n;
   }
+  const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+  w.row = __shfl_sync(0xffffffffu, row, from);
+  w.at = __shfl_sync(0xffffffffu, at, from);
+  w.left = min(share, total - (int)begin);
+  enter_row(w, tile, seen);
   return share;
 }
 
-// One accumulator of O^T, divided by the sums and rounded, to its 16 dims of up to eight heads: this thread holds dims g and g + 8
+// One accumulator of O^T, rounded, to its 16 dims of up to eight heads: this thread holds dims g and g + 8
 // (e4m3: 2 g and 2 g + 1) of heads 2 t and 2 t + 1.  Called by whole warps.  out: the first head's dims.
 template <typename T, bool kE4M3>
-__device__ __forceinline__ void store_frag(T* out, long long head_stride, int heads, int lane, const float4& o, const float (&inv)[2]) {
-  const uint32_t lo = transpose8x8(Pair<T>::pack(o.x * inv[0], o.y * inv[1])), hi = transpose8x8(Pair<T>::pack(o.z * inv[0], o.w * inv[1]));
+__device__ __forceinline__ void store_frag(T* out, long long head_stride, int heads, int lane, const float4& o) {
+  const uint32_t lo = transpose8x8(Pair<T>::pack(o.x, o.y)), hi = transpose8x8(Pair<T>::pack(o.z, o.w));
   const int g = lane >> 2, t = lane & 3;  // now head g
   if (g >= heads) return;
   T* to = out + g * head_stride;
@@ -219,8 +187,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   using L = Tile<D, kE4M3, kBlocks>;
   using T2 = typename Pair<T>::type;
   using P = Part<D, kBlocks>;
-  using Mask = typename L::Mask;
-  constexpr int kRows = P::kRows, kLook = (L::kPos + 31) / 32, kSteps = D / 16, kGroups = L::kPos / 16, kStages = L::kStages;
+  constexpr int kRows = P::kRows, kSteps = D / 16, kGroups = L::kPos / 16, kStages = L::kStages;
   constexpr bool kBf16 = !kE4M3 && __is_same(T, __nv_bfloat16);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ float2 s_ml[2][kWarps][kRows];  // of a warp's first part and of its last
@@ -230,92 +197,96 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   Walk load;
-  const int share = find_walk<kWarps>(p, L::kPos, load);
+  const int share = find_walk(p, L::kPos, load);
   Walk w = load;
-  const int item = (int)blockIdx.x % p.items, groups = (p.group + kRows - 1) / kRows, kh = item / groups, h0 = (item - kh * groups) * kRows;
+  const int kh = kBlocks == 1 ? (int)blockIdx.x : (int)blockIdx.x / p.groups, h0 = kBlocks == 1 ? 0 : ((int)blockIdx.x - kh * p.groups) * kRows;
   const int heads = min(kRows, p.group - h0), head0 = kh * p.group + h0;  // of this CTA
+  const int cta = (int)(blockIdx.y * gridDim.x + blockIdx.x);
   const uint32_t wbase = attn::smem_u32_local(smem_raw) + warp * (kStages * L::kStage);
   float4* heads_area = reinterpret_cast<float4*>(smem_raw + L::kSmem);                                  // [warps][frags][32]
   auto tail_area = [&](int i) { return reinterpret_cast<float4*>(smem_raw + i * (kStages * L::kStage)); };  // a drained pipeline's space
   constexpr int kSize = kE4M3 ? 1 : 2;
-  const long long pos_bytes = p.pool.pos_stride * kSize;
+  const uint32_t pos_bytes = p.pos_step * p.step_bytes;
   const char* kbase = reinterpret_cast<const char*>(p.pool.k) + kh * p.pool.head_stride * kSize + (lane % L::kChunks) * 16;
   const char* vbase = reinterpret_cast<const char*>(p.pool.v) + kh * p.pool.head_stride * kSize + (lane % L::kChunks) * 16;
 
   auto seen = [&](int row) { return seen_of(p.a.lengths[row], p.max_len, p.a.window); };
 
-  // ---- loading: the pages of the next tile are looked up while the one before is requested ----
-  int page[kLook], load_pos = -L::kPos, load_tiles = 0, load_end = 0;  // load_tiles: of the part, the next one and those behind it
+  // ---- loading: 64 entries of the row's table in the lanes' registers, the next 32 on their way ----
+  int load_pos = 0, load_tiles = 0, ids_at = 0, ids[2] = {-1, -1};
   const int* table = nullptr;
-  auto look = [&]() {
-    load_pos += L::kPos;
-    if (--load_tiles <= 0) {
-      while (load.left > 0 && load_tiles <= 0) {
-        const WalkPart part = next_part(load, L::kPos, seen);
-        load_tiles = part.to - part.from;
-        load_pos = load.first + part.from * L::kPos;
-      }
-      if (load_tiles <= 0) return;  // no more
-      load_end = load.end;
-      table = p.a.table + load.row * p.a.table_stride;
-    }
-#pragma unroll
-    for (int i = 0; i < kLook; ++i) {
-      const int pos = load_pos + i * 32 + lane % L::kPos;
-      page[i] = pos < load_end ? table[div_page(p.div, pos)] : -1;
-    }
-  };
+  auto load_ids = [&](int at) { return at + lane < pages_of(p.div, load.end) ? table[at + lane] : -1; };
   int stage_in = 0, stage_out = 0;
   // requests the next tile; the mask of its positions that are there
   auto issue = [&]() {
-    Mask mask = 0;
+    uint32_t mask = 0;
+    if (load_tiles == 0) {
+      while (load.left > 0 && load_tiles <= 0) {
+        const WalkPart part = next_part(load, L::kPos, seen);
+        load_tiles = max(0, part.to - part.from);
+        load_pos = load.first + part.from * L::kPos;
+      }
+      if (load_tiles > 0) {
+        table = p.a.table + load.row * p.a.table_stride;
+        ids_at = div_page(p.div, load_pos);
+        ids[0] = load_ids(ids_at);
+        ids[1] = load_ids(ids_at + 32);
+      }
+    }
     if (load_tiles > 0) {
       const uint32_t sb = wbase + stage_in * L::kStage;
-      uint32_t off[kLook];
-      bool one = true;  // all of it on one page
-#pragma unroll
-      for (int i = 0; i < kLook; ++i) {
-        off[i] = step_of(page[i], p.pool.pages, load_pos + i * 32 + lane % L::kPos, p.div, p.page_step, p.pos_step);
-        const uint32_t there = __ballot_sync(0xffffffffu, off[i] != kNoStep);
-        mask |= (Mask)(L::kPos < 32 ? there & ((1u << L::kPos % 32) - 1) : there) << (i * 32 % (8 * (int)sizeof(Mask)));
-        one = one && there == 0xffffffffu && __all_sync(0xffffffffu, page[i] == __shfl_sync(0xffffffffu, page[0], 0));
-      }
       const int r0 = lane / L::kChunks, c = lane % L::kChunks;
-      if (one) {
-        const unsigned long long by = (unsigned long long)__shfl_sync(0xffffffffu, off[0], 0) * p.step_bytes + r0 * pos_bytes;
-        const char *kp = kbase + by, *vp = vbase + by;
+      const int page0 = div_page(p.div, load_pos) - ids_at;
+      if (page0 >= 32) {  // (a tile has 32 pages at most)
+        ids_at += 32;
+        ids[0] = ids[1];
+        ids[1] = load_ids(ids_at + 32);
+      }
 #pragma unroll
-        for (int i = 0; i < L::kPos / L::kPerPass; ++i) {
-          const uint32_t s = sb + L::at(i * L::kPerPass + r0, c);
-          cp_async16(s, kp, true);
-          cp_async16(s + L::kPos * L::kRow, vp, true);
-          kp += L::kPerPass * pos_bytes;
-          vp += L::kPerPass * pos_bytes;
-        }
-      } else {
+      for (int part = 0; part < L::kPos; part += 16) {
+        const int from = load_pos + part, at0 = div_page(p.div, from) - ids_at;
+        constexpr int kPasses = 16 / L::kPerPass;
+        if (from + 16 <= load.end && div_page(p.div, from + 15) - ids_at == at0) {  // all of it on one page
+          const int id = __shfl_sync(0xffffffffu, at0 < 32 ? ids[0] : ids[1], at0 & 31);
+          const uint32_t off = step_of(id, p.pool.pages, from, p.div, p.page_step, p.pos_step);
+          const bool ok = off != kNoStep;
+          if (ok) mask |= 0xffffu << part;
+          const unsigned long long by = ok ? (unsigned long long)off * p.step_bytes + (unsigned long long)pos_bytes * r0 : 0;
+          const char *kp = kbase + by, *vp = vbase + by;
+          const uint32_t pass_bytes = ok ? pos_bytes * L::kPerPass : 0;
 #pragma unroll
-        for (int i = 0; i < L::kPos / L::kPerPass; ++i) {
-          const int r = i * L::kPerPass + r0;
-          const uint32_t o = __shfl_sync(0xffffffffu, off[(i * L::kPerPass) / 32], r & 31);
-          const bool ok = o != kNoStep;
-          const unsigned long long by = ok ? (unsigned long long)o * p.step_bytes : 0;
-          const uint32_t s = sb + L::at(r, c);
-          cp_async16(s, kbase + by, ok);
-          cp_async16(s + L::kPos * L::kRow, vbase + by, ok);
+          for (int i = 0; i < kPasses; ++i) {
+            const uint32_t s = sb + L::at(part + i * L::kPerPass + r0, c);
+            cp_async16(s, kp + (unsigned long long)pass_bytes * i, ok);
+            cp_async16(s + L::kPos * L::kRow, vp + (unsigned long long)pass_bytes * i, ok);
+          }
+        } else {
+          const int pos = from + lane % 16, at = div_page(p.div, pos) - ids_at;
+          const int lo = __shfl_sync(0xffffffffu, ids[0], at & 31), hi = __shfl_sync(0xffffffffu, ids[1], at & 31);
+          const uint32_t off = step_of(pos < load.end ? (at < 32 ? lo : hi) : -1, p.pool.pages, pos, p.div, p.page_step, p.pos_step);
+          mask |= (__ballot_sync(0xffffffffu, off != kNoStep) & 0xffffu) << part;
+#pragma unroll
+          for (int i = 0; i < kPasses; ++i) {
+            const int r = i * L::kPerPass + r0;
+            const uint32_t o = __shfl_sync(0xffffffffu, off, r);
+            const bool ok = o != kNoStep;
+            const unsigned long long by = ok ? (unsigned long long)o * p.step_bytes : 0;
+            const uint32_t s = sb + L::at(part + r, c);
+            cp_async16(s, kbase + by, ok);
+            cp_async16(s + L::kPos * L::kRow, vbase + by, ok);
+          }
         }
       }
+      load_pos += L::kPos;
+      --load_tiles;
     }
     stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
     cp_async_commit();  // always: keeps the group count in step with the tiles
     return mask;
   };
-  Mask masks[kStages];  // of the tiles in flight
-  look();
+  uint32_t masks[kStages];  // of the tiles in flight
 #pragma unroll
-  for (int j = 0; j + 1 < kStages; ++j) {
-    masks[j] = issue();
-    look();
-  }
+  for (int j = 0; j + 1 < kStages; ++j) masks[j] = issue();
   if (lane == 0) {
     s_head[warp] = 0;
     s_tail[warp] = make_int2(-1, 0);
@@ -374,10 +345,9 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
     const WalkPart part = next_part(w, L::kPos, seen);
     const int n = part.to - part.from;
     if (w.units == 1) {  // an empty row
-      const float zero[2] = {0.f, 0.f};
       for (int f = 0; f < P::kFrags; ++f)
         store_frag<T, kE4M3>(out_of(w.row, head0 + f / kSteps * 8) + f % kSteps * 16, p.a.out_head_stride, heads - f / kSteps * 8, lane,
-                             make_float4(0.f, 0.f, 0.f, 0.f), zero);
+                             make_float4(0.f, 0.f, 0.f, 0.f));
       if (p.a.lse && lane < heads) p.a.lse[(long long)w.row * p.a.heads + head0 + lane] = -INFINITY;
       continue;
     }
@@ -395,7 +365,6 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
     for (int j = 0; j < n; ++j) {
       __syncwarp();  // everyone is done with the stage that the next tile overwrites
       masks[kStages - 1] = issue();
-      look();
       cp_async_wait<kStages - 1>();
       __syncwarp();
       const uint32_t sb = wbase + stage_out * L::kStage;
@@ -435,8 +404,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
 #pragma unroll
           for (int u = 0; u < 4; ++u) s[nb][c][u] = fmaf(s[nb][c][u], qs[nb][u & 1], -base[nb][u & 1]);
         }
-        if (masks[0] != (Mask)~(Mask)0 >> (8 * (int)sizeof(Mask) - L::kPos)) {
-          const Mask mask = masks[0] >> g;
+        if (masks[0] != L::kAll) {
+          const uint32_t mask = masks[0] >> g;
 #pragma unroll
           for (int c = 0; c < kGroups; ++c) {
 #pragma unroll
@@ -457,7 +426,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
             if (top > (m[nb][i] == -INFINITY ? -INFINITY : 0.f)) {
-              const float next = base[nb][i] + top, by = base[nb][i] - next, corr = exp2f(m[nb][i] - next);
+              const float next = base[nb][i] + top, by = base[nb][i] - next, corr = exp2_ftz(m[nb][i] - next);
               m[nb][i] = base[nb][i] = next;
               limit[nb][i] = kSlack;
               l[nb][i] *= corr;
@@ -521,7 +490,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
           store_frag<T, kE4M3>(out_of(w.row, head0 + nb * 8) + k * 16, p.a.out_head_stride, heads - nb * 8, lane,
-                               make_float4(o[nb][k][0], o[nb][k][1], o[nb][k][2], o[nb][k][3]), inv);
+                               make_float4(o[nb][k][0] * inv[0], o[nb][k][1] * inv[1], o[nb][k][2] * inv[0], o[nb][k][3] * inv[1]));
         if (p.a.lse && g == 0) {
 #pragma unroll
           for (int i = 0; i < 2; ++i)
@@ -550,62 +519,68 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   cp_async_wait<0>();
   __syncthreads();
 
-  // ---- parts that meet inside the CTA: a chain begins with a warp's last part, or with what the CTA before left ----
+  // ---- parts that meet inside the CTA: a chain begins with a warp's last part, or with what the team before left ----
+  static_assert(kWarps == 4, "a lane for every part and head of eight");
   int2 tail = make_int2(-1, 0);
-  for (int first = -1; first < kWarps; ++first) {
-    int2 row = make_int2(-1, 0);
-    if (first >= 0) {
-      row = s_tail[first];
-      if (row.x < 0) continue;
-    } else if (s_head[0] == 0) {
-      continue;
-    }
+#pragma unroll 1
+  for (int first = s_head[0] != 0 ? -1 : 0; first < kWarps; ++first) {
+    const int2 row = first >= 0 ? s_tail[first] : make_int2(0, 0);
+    if (row.x < 0) continue;
     int last = first;  // the chain's last warp
     bool done = false;
     while (!done && last + 1 < kWarps && s_head[last + 1] != 0) done = s_head[++last] == 1;
     const bool whole = first >= 0 && done;
     const float v_scale = kE4M3 && whole ? p.pool.v_scale[kh] : 1.f;
-    const long long slot = 2ll * blockIdx.x + (first >= 0);
-    for (int f = warp; f < P::kFrags; f += kWarps) {
-      const int nb = f / kSteps, h = nb * 8 + 2 * t;
-      float top[2] = {-INFINITY, -INFINITY}, base[2], sum[2] = {0.f, 0.f};
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i = max(0, first); i <= last; ++i) {
+    const long long slot = 2ll * cta + (first >= 0);
+    // lane 8 i + h: what head h of warp i's part is multiplied by
+    const int i = lane >> 3, h8 = lane & 7;
+    float by[kBlocks];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) top[e] = fmaxf(top[e], s_ml[i == first][i][h + e].x);
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) base[e] = top[e] == -INFINITY ? 0.f : top[e];
-      for (int i = max(0, first); i <= last; ++i) {
-        const float2 a = s_ml[i == first][i][h], b = s_ml[i == first][i][h + 1];
-        const float fa = exp2f(a.x - base[0]), fb = exp2f(b.x - base[1]);
-        const float4 v = (i == first ? tail_area(i) : heads_area + i * (P::kFrags * 32))[f * 32 + lane];
-        sum[0] += fa * a.y;
-        sum[1] += fb * b.y;
-        acc.x += fa * v.x, acc.y += fb * v.y, acc.z += fa * v.z, acc.w += fb * v.w;
-      }
+    for (int nb = 0; nb < kBlocks; ++nb) {
+      const int h = nb * 8 + h8;
+      const float2 ml = i >= first && i <= last ? s_ml[i == first][i][h] : make_float2(-INFINITY, 0.f);
+      float top = fmaxf(ml.x, __shfl_xor_sync(0xffffffffu, ml.x, 8));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+      by[nb] = exp2_ftz(ml.x - (top == -INFINITY ? 0.f : top));
+      float sum = by[nb] * ml.y;
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
       if (whole) {
-        const float inv[2] = {inverse(top[0], sum[0], v_scale), inverse(top[1], sum[1], v_scale)};
-        store_frag<T, kE4M3>(out_of(row.x, head0 + nb * 8) + f % kSteps * 16, p.a.out_head_stride, heads - nb * 8, lane, acc, inv);
-        if (p.a.lse && f % kSteps == 0 && g == 0) {
+        by[nb] *= inverse(top, sum, v_scale);
+        if (warp == 0 && lane < 8 && h < heads && p.a.lse) p.a.lse[(long long)row.x * p.a.heads + head0 + h] = (top + log2f(sum)) * kLn2;
+      } else if (warp == 0 && lane < 8) {
+        p.part_ml[slot * kRows + h] = make_float2(top, sum);
+      }
+    }
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (h + e < heads) p.a.lse[(long long)row.x * p.a.heads + head0 + h + e] = (top[e] + log2f(sum[e])) * kLn2;
-        }
-      } else {
-        p.parts[(slot * P::kFrags + f) * 32 + lane] = acc;
-        if (f % kSteps == 0 && g == 0) {
+    for (int nb = 0; nb < kBlocks; ++nb) {
+      float fa[kWarps], fb[kWarps];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) p.part_ml[slot * kRows + h + e] = make_float2(top[e], sum[e]);
+      for (int u = 0; u < kWarps; ++u) {
+        fa[u] = __shfl_sync(0xffffffffu, by[nb], u * 8 + 2 * t);
+        fb[u] = __shfl_sync(0xffffffffu, by[nb], u * 8 + 2 * t + 1);
+      }
+#pragma unroll 1
+      for (int k = warp; k < kSteps; k += kWarps) {
+        const int f = nb * kSteps + k;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < kWarps; ++u) {
+          if (u < first || u > last) continue;
+          const float4 v = (u == first ? tail_area(u) : heads_area + u * (P::kFrags * 32))[f * 32 + lane];
+          acc.x += fa[u] * v.x, acc.y += fb[u] * v.y, acc.z += fa[u] * v.z, acc.w += fb[u] * v.w;
         }
+        if (whole) store_frag<T, kE4M3>(out_of(row.x, head0 + nb * 8) + k * 16, p.a.out_head_stride, heads - nb * 8, lane, acc);
+        else p.parts[(slot * P::kFrags + f) * 32 + lane] = acc;
       }
     }
     if (first >= 0 && !done) {
-      const long long behind = (long long)(kWarps - 1 - first) * share;  // units of the row that this CTA's later warps have
-      tail = make_int2(row.x, (int)((row.y - behind + (long long)kWarps * share - 1) / ((long long)kWarps * share)));
+      // units of the row behind this CTA
+      const uint32_t behind = (uint32_t)(row.y - (kWarps - 1 - first) * share), each = (uint32_t)(kWarps * share);
+      tail = make_int2(row.x, (int)((behind + each - 1) / each));
     }
   }
-  if (threadIdx.x == 0 && (int)gridDim.x > p.items) p.tails[blockIdx.x] = tail;
+  if (threadIdx.x == 0 && gridDim.y > 1) p.tails[cta] = tail;
 }
 
 // Joins the parts of a row that spans teams: block c has the row that begins in CTA c and ends in the same item's CTA of a later team.
@@ -615,10 +590,11 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Para
   constexpr int kSteps = D / 16, kAhead = 6;
   pdl_launch_dependents();
   pdl_wait();
-  const int2 row = p.tails[blockIdx.x];
+  const int cta = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+  const int2 row = p.tails[cta];
   if (row.x < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int item = (int)blockIdx.x % p.items, groups = (p.group + P::kRows - 1) / P::kRows, kh = item / groups, h0 = (item - kh * groups) * P::kRows;
+  const int kh = kBlocks == 1 ? (int)blockIdx.x : (int)blockIdx.x / p.groups, h0 = kBlocks == 1 ? 0 : ((int)blockIdx.x - kh * p.groups) * P::kRows;
   const int heads = min(P::kRows, p.group - h0), head0 = kh * p.group + h0, n = 1 + row.y;
   const float v_scale = kE4M3 ? p.pool.v_scale[kh] : 1.f;
   for (int f = warp; f < P::kFrags; f += (int)blockDim.x / 32) {
@@ -630,7 +606,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Para
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int i = i0 + u;
-        const long long slot = 2ll * (blockIdx.x + i * p.items) + (i == 0);
+        const long long slot = 2ll * (cta + (long long)i * gridDim.x) + (i == 0);
         ml[u] = i < n ? *reinterpret_cast<const float4*>(p.part_ml + slot * P::kRows + h) : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
         v[u] = i < n ? p.parts[(slot * P::kFrags + f) * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
       }
@@ -640,7 +616,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Para
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         base[e] = next[e] == -INFINITY ? 0.f : next[e];
-        const float corr = exp2f(top[e] - base[e]);
+        const float corr = exp2_ftz(top[e] - base[e]);
         sum[e] *= corr;
         if (e == 0) acc.x *= corr, acc.z *= corr;
         else acc.y *= corr, acc.w *= corr;
@@ -648,7 +624,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Para
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const float fa = exp2f(ml[u].x - base[0]), fb = exp2f(ml[u].z - base[1]);
+        const float fa = exp2_ftz(ml[u].x - base[0]), fb = exp2_ftz(ml[u].z - base[1]);
         sum[0] += fa * ml[u].y;
         sum[1] += fb * ml[u].w;
         acc.x += fa * v[u].x, acc.y += fb * v[u].y, acc.z += fa * v[u].z, acc.w += fb * v[u].w;
@@ -656,7 +632,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Para
     }
     const float inv[2] = {inverse(top[0], sum[0], v_scale), inverse(top[1], sum[1], v_scale)};
     T* out = reinterpret_cast<T*>(p.a.out) + row.x * p.a.out_stride + (head0 + nb * 8) * p.a.out_head_stride + f % kSteps * 16;
-    store_frag<T, kE4M3>(out, p.a.out_head_stride, heads - nb * 8, lane, acc, inv);
+    store_frag<T, kE4M3>(out, p.a.out_head_stride, heads - nb * 8, lane, make_float4(acc.x * inv[0], acc.y * inv[1], acc.z * inv[0], acc.w * inv[1]));
     if (p.a.lse && f % kSteps == 0 && g == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
@@ -686,9 +662,10 @@ cudaError_t launch(Params p, void* workspace, int sms, cudaStream_t stream) {
   p.tails = reinterpret_cast<int2*>(workspace);
   p.parts = reinterpret_cast<float4*>(p.tails + (ctas + 1) / 2 * 2);
   p.part_ml = reinterpret_cast<float2*>(p.parts + ctas * 2 * P::kFrags * 32);
-  rc = launch_kernel_ex(kernel, dim3((unsigned)ctas), dim3(kWarps * 32), (size_t)smem, stream, true, 1, p);
+  const dim3 grid((unsigned)p.items, (unsigned)(ctas / p.items));
+  rc = launch_kernel_ex(kernel, grid, dim3(kWarps * 32), (size_t)smem, stream, true, 1, p);
   if (rc != cudaSuccess || ctas == p.items) return rc;  // (a single team finishes its rows)
-  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kBlocks>, dim3((unsigned)ctas), dim3(P::kFrags * 32 < 256 ? P::kFrags * 32 : 256), 0, stream, true, 1, p);
+  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kBlocks>, grid, dim3(P::kFrags * 32 < 256 ? P::kFrags * 32 : 256), 0, stream, true, 1, p);
 }
 
 }  // namespace
@@ -715,9 +692,10 @@ cudaError_t launch_paged_attention(const PagedAttention& a, PagedType type, cons
   p.group = a.heads / pool.heads;
   p.max_len = (int)(cap < kMaxLen ? cap : kMaxLen);
   p.items = items_of(pool.heads, p.group);
+  p.groups = p.items / pool.heads;
   if ((long long)a.rows * units_of(most_seen(p.max_len, a.window), 16) > kMaxUnits) return cudaErrorInvalidValue;
   const Steps st = steps_of(pool.pages, pool.page_size, pool.page_stride, pool.pos_stride, cache == PAGED_E4M3 ? 1 : 2);
-  if (st.bytes == 0) return cudaErrorInvalidValue;
+  if (st.bytes == 0 || (unsigned long long)st.pos * st.bytes > 1u << 26) return cudaErrorInvalidValue;  // (a tile's rows are counted in 32 bits of bytes)
   p.page_step = st.page;
   p.pos_step = st.pos;
   p.step_bytes = st.bytes;

@@ -152,6 +152,7 @@ void bind_paged(py::module_& m) {
     need(pool.dim == 64 || pool.dim == 128 || pool.dim == 256, "paged_attention: dim 64, 128 or 256");
     need(paged::steps_of(pool.pages, pool.page_size, pool.page_stride, pool.pos_stride, (int)k.element_size()).bytes > 0,
          "paged_attention: caches that reach over 2^32 times what divides their strides");
+    need(pool.page_size == 1 || pool.pos_stride * k.element_size() <= 1 << 26, "paged_attention: positions of a page at most 64 MB apart");
     auto rows_ok = [&](const at::Tensor& t) { return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned(t); };
     need(rows_ok(q), "paged_attention: heads of q contiguous, 16-byte aligned");
     need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B && table.size(1) >= 1 && table.size(1) < (1ll << 31) &&

@@ -52,13 +52,10 @@ PENNY_ATTN_HD Seen seen_of(int length, int max_len, int window) {
 // rows lie in a line, each a unit for its start (its output, its q) and one for every tile of positions; every warp of a
 // team's CTAs gets `share` units, at least kMinShare.  The lengths are on the device, and every CTA sums over them by itself.
 constexpr int kMinShare = 4;
-constexpr long long kMaxLen = 0x7fff0000, kMaxUnits = 1ll << 30;  // (shares fit 32 bits)
+constexpr long long kMaxLen = 0x7fff0000, kMaxUnits = 1ll << 30;  // (all rows' units, and a share more, fit 32 bits)
 
 PENNY_ATTN_HD int units_of(int positions, int tile) { return 1 + (positions + tile - 1) / tile; }
-PENNY_ATTN_HD int share_of(long long units, int warps) {
-  const long long share = (units + warps - 1) / warps;
-  return share < kMinShare ? kMinShare : (int)share;
-}
+PENNY_ATTN_HD int share_of(int units, int warps) { return attn::at_least(kMinShare, (int)(((uint32_t)units + warps - 1) / (uint32_t)warps)); }
 // Teams of a launch: as many as the GPU holds (`slots` CTAs), in more rounds where that leaves over a tenth of it empty; no more
 // than there are shares, if every row has `units` units.
 inline int teams_of(long long rows, int items, long long units, int warps, int slots) {

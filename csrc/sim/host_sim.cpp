@@ -394,7 +394,7 @@ int penny_paged_walk(const int* lengths, int rows, int max_len, int window, int 
   auto units = [&](int r) { return units_of(seen(r).end - seen(r).first, tile); };
   long long total = 0, x = 0;
   for (int r = 0; r < rows; ++r) total += units(r);
-  const int share = share_of(total, warps);
+  const int share = share_of((int)total, warps);
   const long long begin = (long long)warp * share;
   *num_tiles = 0;
   *share_out = share;

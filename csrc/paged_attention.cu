@@ -370,11 +370,16 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
       const uint32_t sb = wbase + stage_out * L::kStage;
       stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1;
       // ---- S^T = K Q^T, 16 positions at a time: this thread holds positions g and g + 8 of heads 2 t and 2 t + 1 ----
+      // (even and odd steps apart: a chain of products into one accumulator is the longest wait of a tile)
       float s[kBlocks][kGroups][4];
 #pragma unroll
       for (int c = 0; c < kGroups; ++c) {
+        float odd[kBlocks][4];
 #pragma unroll
-        for (int nb = 0; nb < kBlocks; ++nb) s[nb][c][0] = s[nb][c][1] = s[nb][c][2] = s[nb][c][3] = 0.f;
+        for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[nb][c][u] = odd[nb][u] = 0.f;
+        }
         const int row = c * 16 + (lane & 15);
 #pragma unroll
         for (int k2 = 0; k2 < L::kChunks / 2; ++k2) {
@@ -385,12 +390,17 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
             for (int i = 0; i < 2; ++i) {
               const uint32_t x[4] = {e4m3_lo(a[2 * i]), e4m3_lo(a[2 * i + 1]), e4m3_hi(a[2 * i]), e4m3_hi(a[2 * i + 1])};
 #pragma unroll
-              for (int nb = 0; nb < kBlocks; ++nb) mma(s[nb][c], x, qb[nb][k2 * 2 + i]);
+              for (int nb = 0; nb < kBlocks; ++nb) mma(i ? odd[nb] : s[nb][c], x, qb[nb][k2 * 2 + i]);
             }
           } else {
 #pragma unroll
-            for (int nb = 0; nb < kBlocks; ++nb) mma(s[nb][c], a, qb[nb][k2]);
+            for (int nb = 0; nb < kBlocks; ++nb) mma(k2 & 1 ? odd[nb] : s[nb][c], a, qb[nb][k2]);
           }
+        }
+#pragma unroll
+        for (int nb = 0; nb < kBlocks; ++nb) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[nb][c][u] += odd[nb][u];
         }
       }
       // ---- weights exp2(score - base); the base follows the maximum when a score exceeds it by more than kSlack ----

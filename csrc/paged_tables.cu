@@ -17,45 +17,51 @@
 #include "paged_plan.h"
 #include "pdl.h"
 
+#include <stdint.h>
+
 namespace penny {
 namespace {
 using namespace paged;
 
-constexpr int kTokensPerThread = 4;
+constexpr int kTokensPerThread = 4, kCluster = 8;
+static_assert(kPagedMaxRows <= 8 * 1024, "rows of a thread");
 
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Exclusive sums over the block's threads, and the whole in `total`.
+// Sums hold at 2^31 - 1 (of terms that do so themselves: in any order the same).
+constexpr uint32_t kTop = 0x7fffffffu;
+__device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) { return min(a + b, kTop); }
+
+// Exclusive sums over the block's threads, and the whole in `total`.  The first call of a kernel needs no barrier in front.
 template <int N>
-__device__ __forceinline__ void block_sums(long long (&v)[N], long long (&total)[N]) {
-  __shared__ long long part[N][32];
+__device__ __forceinline__ void block_sums(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t (&part)[N][32]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  long long own[N];
-  __syncthreads();  // (part is free again)
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    own[i] = v[i];
+    uint32_t incl = v[i];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, v[i], o);
-      if (lane >= o) v[i] += u;
+      const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl = add(incl, u);
     }
-    if (lane == 31) part[i][warp] = v[i];
+    if (lane == 31) part[i][warp] = incl;
+    const uint32_t before = __shfl_up_sync(0xffffffffu, incl, 1);
+    v[i] = lane > 0 ? before : 0;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    long long w = lane < warps ? part[i][lane] : 0;
-    const long long mine = w;
+    uint32_t incl = lane < warps ? part[i][lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += u;
+      const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl = add(incl, u);
     }
-    total[i] = __shfl_sync(0xffffffffu, w, 31);
-    v[i] += __shfl_sync(0xffffffffu, w - mine, warp) - own[i];
+    total[i] = __shfl_sync(0xffffffffu, incl, 31);
+    const uint32_t before = __shfl_sync(0xffffffffu, incl, max(0, warp - 1));
+    if (warp > 0) v[i] = add(v[i], before);
   }
 }
 
@@ -70,6 +76,8 @@ __device__ __forceinline__ int row_at(const int* at, int rows, int x) {
   return lo;
 }
 
+// kPer: rows of a thread, one behind the other.
+template <int kPer>
 __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const PageDiv div, int cluster) {
   extern __shared__ int smem[];
   // per row: where its tokens begin, its length (-1 - length: not granted), its first new page's number among all new
@@ -80,59 +88,75 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
   const int tid = threadIdx.x, rank = blockIdx.x;
   const long long most = min((long long)a.width * a.page_size, 2147483647ll);
   const int count = max(0, min(*a.free_count, a.pages));
-  const int per = (a.rows + blockDim.x - 1) / blockDim.x, r0 = min(a.rows, tid * per), r1 = min(a.rows, r0 + per);
-  auto old_of = [&](int r) { return (int)max(0ll, min((long long)a.lengths[r], most)); };
+  const int r0 = tid * kPer;
   auto gone_of = [&](int old, int n) { return n < 0 ? pages_of(div, old) - pages_of(div, (int)max(0ll, (long long)old + n)) : 0; };
+  __shared__ uint32_t s_two[2][32], s_one[1][32], s_popped;
+  if (tid == 0) s_popped = 0;
 
-  long long sums[2] = {0, 0}, totals[2];
-  for (int r = r0; r < r1; ++r) {
-    const int n = a.news[r], old = old_of(r);
-    sums[0] += max(0, n);
-    sums[1] += gone_of(old, n);
+  int old[kPer], n[kPer];
+  uint32_t sums[2] = {0, 0}, totals[2];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const bool in = r0 + i < a.rows;
+    old[i] = in ? (int)max(0ll, min((long long)a.lengths[r0 + i], most)) : 0;
+    n[i] = in ? a.news[r0 + i] : 0;
   }
-  block_sums(sums, totals);
-  long long end = sums[0];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    sums[0] = add(sums[0], max(0, n[i]));
+    sums[1] = add(sums[1], gone_of(old[i], n[i]));
+  }
+  block_sums(sums, totals, s_two);
   // (more pages than the pool has: a table that holds some twice; what the stack cannot take is dropped)
-  const int pushed = (int)min(totals[1], (long long)(a.pages - count));
-  long long gone = sums[1], need[1] = {0}, all_need[1];
-  for (int r = r0; r < r1; ++r) {
-    const int n = a.news[r], old = old_of(r);
-    s_off[r] = (int)min(end, 2147483647ll);
-    s_gone[r] = (int)min(gone, 2147483647ll);
-    end += max(0, n);
-    gone += gone_of(old, n);
-    const bool fits = n > 0 && old + (long long)n <= most && end <= a.tokens;
-    s_old[r] = fits || n <= 0 ? old : -1 - old;
-    if (fits) need[0] += pages_of(div, old + n) - pages_of(div, old);
+  const int pushed = (int)min(totals[1], (uint32_t)(a.pages - count));
+  const uint32_t pages_there = (uint32_t)(count + pushed);
+  uint32_t end = sums[0], gone = sums[1], need[1] = {0}, all_need[1];
+  bool granted[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (r0 + i < a.rows) {
+      s_off[r0 + i] = (int)end;
+      s_gone[r0 + i] = (int)gone;
+    }
+    if (rank == 0 && r0 + i < a.rows) a.offsets[r0 + i] = (int)end;
+    end = add(end, max(0, n[i]));
+    gone = add(gone, gone_of(old[i], n[i]));
+    granted[i] = n[i] <= 0 || (old[i] + (long long)n[i] <= most && end <= (uint32_t)a.tokens);
+    if (n[i] > 0 && granted[i]) need[0] = add(need[0], pages_of(div, old[i] + n[i]) - pages_of(div, old[i]));
   }
-  block_sums(need, all_need);
-  long long taken = need[0], popped_here = 0;
-  for (int r = r0; r < r1; ++r) {
-    const int n = a.news[r];
-    s_new[r] = (int)min(taken, 2147483647ll);
-    if (n > 0 && s_old[r] >= 0) {
-      const int pages = pages_of(div, s_old[r] + n) - pages_of(div, s_old[r]);
-      taken += pages;
-      if (pages > 0 && taken > count + pushed) s_old[r] = -1 - s_old[r];
-      else popped_here += pages;
+  block_sums(need, all_need, s_one);
+  uint32_t taken = need[0], last = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t first = taken;
+    if (n[i] > 0 && granted[i]) {
+      const int pages = pages_of(div, old[i] + n[i]) - pages_of(div, old[i]);
+      taken = add(taken, pages);
+      // (once a row is refused, all behind it that need pages are: the last one that is not has the sum)
+      granted[i] = pages == 0 || taken <= pages_there;
+      if (granted[i] && pages > 0) last = taken;
+    }
+    if (r0 + i < a.rows) {
+      s_new[r0 + i] = (int)first;
+      s_old[r0 + i] = granted[i] ? old[i] : -1 - old[i];
     }
   }
-  long long popped[1] = {popped_here}, all_popped[1];
-  block_sums(popped, all_popped);
+  last = __reduce_max_sync(0xffffffffu, last);
+  if ((tid & 31) == 0 && last > 0) atomicMax(&s_popped, last);
   if (cluster > 1) cluster_barrier();
   else __syncthreads();
 
   // ---- the rows' own state, from here on nobody reads it ----
   if (rank == 0) {
-    for (int r = r0; r < r1; ++r) {
-      const int n = a.news[r], old = s_old[r] >= 0 ? s_old[r] : -1 - s_old[r];
-      a.granted[r] = s_old[r] >= 0;
-      a.offsets[r] = s_off[r];
-      a.lengths[r] = n > 0 ? (s_old[r] >= 0 ? old + n : old) : (int)max(0ll, (long long)old + n);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (r0 + i >= a.rows) break;
+      a.granted[r0 + i] = granted[i];
+      a.lengths[r0 + i] = granted[i] ? (int)max(0ll, (long long)old[i] + n[i]) : old[i];
     }
     if (tid == 0) {
-      a.offsets[a.rows] = (int)min(totals[0], 2147483647ll);
-      *a.free_count = count + pushed - (int)all_popped[0];
+      a.offsets[a.rows] = (int)totals[0];
+      *a.free_count = count + pushed - (int)s_popped;
     }
   }
 
@@ -149,7 +173,7 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
   const int threads = cluster * blockDim.x, me = rank * blockDim.x + tid;
   for (int k = me; k < pushed; k += threads) a.free_pages[count + pushed - 1 - k] = released(k);
 
-  const int total = (int)min(totals[0], (long long)a.tokens);
+  const int total = (int)min(totals[0], (uint32_t)a.tokens);
   for (long long j0 = (long long)me * kTokensPerThread; j0 < a.tokens; j0 += (long long)threads * kTokensPerThread) {
     long long slot[kTokensPerThread];
     int pos[kTokensPerThread];
@@ -193,11 +217,21 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
 cudaError_t launch_page_tables(const PageTables& a, cudaStream_t stream) {
   if (a.rows < 1 || a.rows > kPagedMaxRows || a.width < 1 || a.page_size < 1 || a.pages < 1 || a.tokens < 0) return cudaErrorInvalidValue;
   const size_t smem = (size_t)a.rows * 4 * sizeof(int);
-  const cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(k_page_tables), kPagedMaxRows * 4 * (int)sizeof(int)).rc;
-  if (rc != cudaSuccess) return rc;
-  const int work = max(a.rows, a.tokens / kTokensPerThread);
-  const int threads = work <= 256 ? 256 : 1024, cluster = a.tokens <= 4096 ? 1 : 8;
-  return launch_kernel_ex(k_page_tables, dim3(cluster), dim3(threads), smem, stream, true, cluster, a, page_div(a.page_size), cluster);
+  // One CTA for a decode step (64 rows: 3.9 us); a cluster where tokens or pages of many rows are to be written (4000 rows, 125,000
+  // tokens in 15,000 pages: of eight CTAs 13 us, one 50).
+  const int threads = a.rows <= 256 && a.tokens <= 1024 ? 256 : 1024, cluster = a.tokens <= 4096 && a.rows <= 1024 ? 1 : kCluster;
+  const int per = (a.rows + threads - 1) / threads;
+#define PENNY_PAGE_TABLES(N)                                                                                                          \
+  do {                                                                                                                                \
+    const cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(k_page_tables<N>), kPagedMaxRows * 4 * (int)sizeof(int)).rc;     \
+    if (rc != cudaSuccess) return rc;                                                                                                 \
+    return launch_kernel_ex(k_page_tables<N>, dim3(cluster), dim3(threads), smem, stream, true, cluster, a, page_div(a.page_size),     \
+                            cluster);                                                                                                 \
+  } while (0)
+  if (per == 1) PENNY_PAGE_TABLES(1);
+  if (per <= 4) PENNY_PAGE_TABLES(4);
+  PENNY_PAGE_TABLES(8);
+#undef PENNY_PAGE_TABLES
 }
 
 }  // namespace penny

@@ -42,7 +42,7 @@ def page_tables(table, lengths, free, free_count, new, page_size: int, tokens: i
     passes these two tests; one that is not keeps its length, and its slots are -1.  A row that gets no tokens is granted.
     At most 8192 rows.  `tokens` may exceed the sum of new (a captured step's fixed number).  Entries of a table row behind its
     pages, and of free from free_count on, say nothing."""
-    return PageStep(*ops.page_tables(table, lengths, free, free_count, new, page_size, tokens, out))
+    return PageStep._make(ops.page_tables(table, lengths, free, free_count, new, page_size, tokens, out))
 
 
 def paged_append(qkv, k, v, slots, positions, heads: int, theta: float, out=None, k_scale=None, v_scale=None) -> None:

@@ -98,6 +98,7 @@ class LlamaSPPrefill:
         self.gathered = e(tokens, H) if backend == "nccl" and not self.cpu else None
         self.full = e(tokens, H) if backend == "nccl" and not self.cpu else None
         self.scale = 1.0 / math.sqrt(D)
+        self._pages = None  # (cache, step) of the forward at work
         # one rank: nothing to gather or scatter, so the linears are plain GEMMs whose epilogues take the
         # residual add, silu * mul and the norms (see _forward_local)
         self.local = backend == "penny" and world == 1 and not self.cpu and (2 * self.F) % 128 == 0
@@ -141,8 +142,12 @@ class LlamaSPPrefill:
             residual_out.copy_(z.to(residual_out.dtype))      # the norm below uses the unrounded sum, like the kernel
         out.copy_((z * torch.rsqrt(z.pow(2).mean(-1, keepdim=True) + self.cfg.eps) * weight.float()).to(out.dtype))
 
-    def _rope(self):
+    def _rope(self, li: int):
         cfg, D = self.cfg, self.cfg.head_dim
+        if self._pages is not None:  # the same rotation, and k and v into the pages
+            cache, step = self._pages
+            cache.append(li, self.qkv, step, self.Hq, cfg.rope_theta)
+            return
         if not self.cpu:
             ops.rope_rows(self.qkv, self.Hq, self.Hkv, D, 0, cfg.rope_theta)
             return
@@ -162,9 +167,9 @@ class LlamaSPPrefill:
         g, u = self.gu[:, :self.F].float(), self.gu[:, self.F:].float()
         self.act.copy_((F_.silu(g) * u).to(self.act.dtype))
 
-    def _attention(self):
+    def _attention(self, li: int):
         cfg, D, T = self.cfg, self.cfg.head_dim, self.T
-        self._rope()
+        self._rope(li)
         q = self.qkv[:, :self.Hq * D].view(T, self.Hq, D).permute(1, 0, 2).unsqueeze(0)
         k = self.qkv[:, self.Hq * D:(self.Hq + self.Hkv) * D].view(T, self.Hkv, D).permute(1, 0, 2).unsqueeze(0)
         v = self.qkv[:, (self.Hq + self.Hkv) * D:].view(T, self.Hkv, D).permute(1, 0, 2).unsqueeze(0)
@@ -189,7 +194,7 @@ class LlamaSPPrefill:
         ops.norm_prep(x, self.layers[0]["norm1"], res, h, ss)
         for li, l in enumerate(self.layers):
             self._gemm(h, l["wqkv"], self.qkv, sumsq=ss)
-            attn = self._attention()
+            attn = self._attention(li)
             ss = self._gemm(attn, l["wo"], h, 2, residual=res, norm_w=l["norm2"], sumsq_out=self.sumsq[1])
             self._gemm(h, l["wgu"], self.act, 1, sumsq=ss)
             if li + 1 < len(self.layers):
@@ -199,15 +204,29 @@ class LlamaSPPrefill:
                 self._gemm(self.act, l["wd"], h, 2, residual=res)
         return res
 
-    def forward(self, x_shard: torch.Tensor) -> torch.Tensor:
-        """x_shard: this rank's [T / world, hidden] rows of the residual stream; returns the same rows after all layers."""
+    def forward(self, x_shard: torch.Tensor, pages=None) -> torch.Tensor:
+        """x_shard: this rank's [T / world, hidden] rows of the residual stream; returns the same rows after all layers.
+
+        pages: (cache, step), a PagedKVCache of this rank's KV heads and the PageStep of its `advance` that let these T tokens, and no
+        others, come to a row that was empty: the keys and values are left there for the decode.  step.granted is looked at
+        here (which waits for the device), except under stream capture."""
+        self._pages = None
+        if pages is not None:
+            cache, step = pages
+            if self.cpu:
+                raise ValueError("a cache in pages needs the GPU")
+            if (len(cache.k), cache.kv_heads, cache.head_dim) != (self.L, self.Hkv, self.cfg.head_dim) or step.slots.numel() != self.T:
+                raise ValueError(f"pages of {self.L} layers with {self.Hkv} KV heads of {self.cfg.head_dim}, a step of {self.T} tokens")
+            if not torch.cuda.is_current_stream_capturing() and not bool(step.granted.all()):
+                raise RuntimeError("the cache had no pages for this prompt")
+            self._pages = pages
         if self.local and x_shard.is_contiguous() and x_shard.data_ptr() % 16 == 0:
             return self._forward_local(x_shard)
         res = x_shard.clone()
         self._add_rmsnorm(res, None, self.layers[0]["norm1"], self.h, None)
         for li, l in enumerate(self.layers):
             self._col(self.h, l["wqkv"], self.qkv)
-            self._row(self._attention(), l["wo"], self.part)
+            self._row(self._attention(li), l["wo"], self.part)
             self._add_rmsnorm(self.part, res, l["norm2"], self.h, res)          # res += o_proj; h = norm(res)
             self._col(self.h, l["wgu"], self.gu)
             self._silu_mul()

@@ -17,6 +17,10 @@ stream serialization, so inside the captured CUDA graph a kernel's prologue and
 the loads of its constant operands (weights, old KV-cache rows) overlap the
 tail of the kernel before it.
 
+`page_size` above 0: the KV cache lies in pages (ops/paged.py), which sequences share a pool of.
+One launch per step takes pages for the new tokens and finds their slots, and the attention kernel
+becomes three: RoPE + append through the slots, attention over the pages, join of its parts.
+
 Column-parallel qkv / gate-up / lm_head, row-parallel o_proj / down (Megatron
 layout); 4 query heads + 1 KV head, 1792 FFN columns and 16032 vocabulary rows
 per GPU at TP=8.  The two all-reduces per layer are the fused kernels of this
@@ -38,6 +42,7 @@ from typing import Optional
 import torch
 
 from .._ext import ops
+from ..ops.paged import PagedKVCache, PageStep
 
 
 @dataclass
@@ -77,7 +82,11 @@ class LlamaTPDecoder:
     def __init__(self, cfg: LlamaConfig, comm=None, rank: int = 0, world: int = 1, max_batch: int = 64,
                  max_len: int = 2560, backend: str = "penny", proto: str = "auto", seed: int = 0,
                  use_graph: bool = True, full_init: bool = False, process_group=None, linears: str = "auto",
-                 pdl: bool = True):
+                 pdl: bool = True, page_size: int = 0, pages: Optional[int] = None, cache_dtype: Optional[torch.dtype] = None):
+        """page_size > 0: KV cache in pages of that many positions, `pages` of them (by default enough for max_batch sequences
+        of max_len), of cache_dtype (bf16 or e4m3)."""
+        if page_size < 0 or (page_size == 0 and (pages is not None or cache_dtype is not None)):
+            raise ValueError("pages and cache_dtype belong to a cache in pages: page_size above 0")
         assert cfg.heads % world == 0 and cfg.kv_heads % world == 0 and cfg.ffn % world == 0
         assert cfg.vocab % world == 0 and cfg.head_dim == 128 and (cfg.ffn // world) % 64 == 0
         assert backend in ("penny", "penny_unfused", "nccl") and linears in ("auto", "penny", "cublas")
@@ -175,8 +184,19 @@ class LlamaTPDecoder:
         self.argmax_ws = torch.zeros(ops.argmax_workspace_bytes(B), dtype=torch.uint8, device=self.dev)
         self.pairs_all = torch.empty(world * 2 * B, dtype=torch.float32, device=self.dev)
         self.next_tokens = torch.zeros(B, dtype=torch.int64, device=self.dev)
-        self.kcache = [torch.zeros(B, self.Hkv, max_len, D, dtype=dt, device=self.dev) for _ in range(cfg.layers)]
-        self.vcache = [torch.zeros(B, self.Hkv, max_len, D, dtype=dt, device=self.dev) for _ in range(cfg.layers)]
+        self.paged: Optional[PagedKVCache] = None
+        if page_size > 0:
+            self.paged = PagedKVCache(cfg.layers, B, max_len, self.Hkv, D, page_size, pages, cache_dtype or dt, device=self.dev)
+            self.page_step = PageStep(torch.full((B,), -1, dtype=torch.int64, device=self.dev), torch.zeros(B, dtype=torch.int32, device=self.dev),
+                                      torch.zeros(B + 1, dtype=torch.int32, device=self.dev), torch.ones(B, dtype=torch.bool, device=self.dev))
+            self.one_each = torch.ones(B, dtype=torch.int32, device=self.dev)
+            self.served = torch.ones(B, dtype=torch.bool, device=self.dev)  # rows that had a page for every token so far
+            self._host_served = torch.ones(B, dtype=torch.bool).pin_memory()
+            self.page_workspace = self.paged.workspace(self.Hq)
+            self.kcache = self.vcache = []
+        else:
+            self.kcache = [torch.zeros(B, self.Hkv, max_len, D, dtype=dt, device=self.dev) for _ in range(cfg.layers)]
+            self.vcache = [torch.zeros(B, self.Hkv, max_len, D, dtype=dt, device=self.dev) for _ in range(cfg.layers)]
         self.splits = self.attention_splits(B * self.Hkv, max_len)
         # (the folded step has the rows cut by their lengths: how many partial rows that takes at most)
         self.pieces = ops.decode_attn_balanced_splits(B, self.Hkv) if self.fold else 1
@@ -199,6 +219,8 @@ class LlamaTPDecoder:
         self.kernels_per_step = cfg.layers * per_layer + norms + 1 + (2 if world > 1 else 0) + own_head
         if self.fold:
             self.kernels_per_step = 5 * cfg.layers + 3
+        if self.paged is not None:  # + page tables; append, attention and (where rows can be cut) join for the attention
+            self.kernels_per_step += 1 + cfg.layers * (2 if self.page_workspace.numel() else 1)
 
     @staticmethod
     def tiled_linears(cfg: LlamaConfig, batch: int) -> frozenset:
@@ -300,10 +322,20 @@ class LlamaTPDecoder:
         """Random K/V rows for positions [0, kv_len) and random current tokens."""
         assert kv_len < self.max_len
         g = torch.Generator(device=self.dev).manual_seed(seed + 17 * self.rank)
+        if self.paged is not None:
+            self.paged.advance(-self.paged.lengths, 0)
+            step = self.paged.advance(torch.full_like(self.paged.lengths, kv_len), self.B * kv_len)
+            self.served.fill_(True)
+            if not bool(step.granted.all()):
+                raise RuntimeError(f"{self.paged.pages} pages of {self.paged.page_size} positions do not hold {self.B} x {kv_len}")
         for li in range(self.cfg.layers):
-            for cache in (self.kcache[li], self.vcache[li]):
-                cache[:, :, :kv_len].copy_(torch.randn(self.B, self.Hkv, kv_len, self.cfg.head_dim, device=self.dev,
-                                                       generator=g, dtype=torch.float32).to(torch.bfloat16))
+            for cache in (self.paged.k[li], self.paged.v[li]) if self.paged is not None else (self.kcache[li], self.vcache[li]):
+                rows = torch.randn(self.B, self.Hkv, kv_len, self.cfg.head_dim, device=self.dev, generator=g, dtype=torch.float32)
+                if self.paged is not None:
+                    rows = rows.transpose(1, 2).reshape(self.B * kv_len, self.Hkv, -1).to(cache.dtype)
+                    cache.view(torch.uint8).view(-1, self.Hkv, rows.shape[2] * rows.element_size())[step.slots] = rows.view(torch.uint8)
+                else:
+                    cache[:, :, :kv_len].copy_(rows.to(torch.bfloat16))
         self.positions.fill_(kv_len)
         gt = torch.Generator(device=self.dev).manual_seed(seed)
         self.tokens.copy_(torch.randint(0, self.cfg.vocab, (self.B,), device=self.dev, generator=gt))
@@ -331,6 +363,18 @@ class LlamaTPDecoder:
         for r in range(0, B, 1024):
             ops.gemm_decode(x[r:r + 1024], w, out[r:r + 1024], silu_pairs, 0, self.pdl, -1, 0, push)
 
+    def _attention(self, li, pieces, balance=False):
+        """RoPE, append and attention of layer li: self.qkv -> self.attn."""
+        theta = self.cfg.rope_theta
+        if self.paged is None:
+            ops.decode_attention_fused(self.qkv, self.kcache[li], self.vcache[li], self.positions, self.attn, self.workspace, self.Hq, self.Hkv,
+                                       pieces, self.scale, theta, self.pdl, balance=balance)
+            return
+        heads = (self.Hq, self.cfg.head_dim)
+        self.paged.append(li, self.qkv, self.page_step, self.Hq, theta)
+        self.paged.attend(li, self.qkv[:, :self.Hq * self.cfg.head_dim].unflatten(1, heads), out=self.attn.unflatten(1, heads), scale=self.scale,
+                          workspace=self.page_workspace)
+
     def _layers_folded(self, tokens):
         """One rank: five launches per layer, q/k/v, gate/up and head on the tiled or on the decode GEMM (`tiled_linears`).  x
         holds the residual stream times the next norm's weight, sumsq its sums of squares; the linear that reads x scales its
@@ -345,9 +389,7 @@ class LlamaTPDecoder:
         ops.norm_prep(self.embed, self.layers[0]["norm1"], res, x, ss, ids=tokens)
         for li, L in enumerate(self.layers):
             scaled("qkv", L["wqkv"], self.qkv, ss)
-            ops.decode_attention_fused(self.qkv, self.kcache[li], self.vcache[li], self.positions, self.attn,
-                                       self.workspace, self.Hq, self.Hkv, self.pieces, self.scale, self.cfg.rope_theta,
-                                       pdl, balance=True)
+            self._attention(li, self.pieces, balance=True)
             ss = self.sumsq[1]
             ops.gemm_decode(self.attn, L["wo"], x, pdl=pdl, residual=res, norm_w=L["norm2"], sumsq_out=ss)
             scaled("gate_up", L["wgu"], self.act, ss, silu=True)
@@ -366,9 +408,7 @@ class LlamaTPDecoder:
                 self._linear(self.x, L["wqkv"], self.qkv)
             else:
                 torch.matmul(self.x, L["wqkv"].t(), out=self.qkv)
-            ops.decode_attention_fused(self.qkv, self.kcache[li], self.vcache[li], self.positions, self.attn,
-                                       self.workspace, self.Hq, self.Hkv, self.splits, self.scale, cfg.rope_theta,
-                                       self.pdl)
+            self._attention(li, self.splits)
             if self.linears == "penny":
                 self._linear(self.attn, L["wo"], self.parts[0], push=self._push)
             else:
@@ -397,6 +437,9 @@ class LlamaTPDecoder:
                 torch.matmul(self.x, self.lm_head.t(), out=self.logits)
 
     def _step_impl(self, warm_up: bool = False, separate: bool = False, host: bool = False):
+        if self.paged is not None:
+            self.paged.advance(self.one_each, self.B, out=self.page_step)
+            torch.logical_and(self.served, self.page_step.granted, out=self.served)
         if self.fold and not separate:
             self._layers_folded(self._host_in if host else self.tokens)
         else:
@@ -420,6 +463,7 @@ class LlamaTPDecoder:
     def capture(self):
         """Warm up (cuBLAS handles, scratch growth) and capture the step in a CUDA graph."""
         saved = (self.positions.clone(), self.tokens.clone())
+        pages = None if self.paged is None else (self.paged.snapshot(), self.served.clone())
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -443,6 +487,21 @@ class LlamaTPDecoder:
             torch.cuda.synchronize()
         self.positions.copy_(saved[0])
         self.tokens.copy_(saved[1])
+        if pages is not None:
+            self.paged.restore(pages[0])
+            self.served.copy_(pages[1])
+
+    def check_pages(self):
+        """Raises if a sequence had no page for one of its tokens (the pool is empty, or it has max_len of them): its tokens from that
+        one on are wrong.  Waits for the device; step() and decode() call it, after step_device() it is the caller's."""
+        if self.paged is not None:
+            self._raise_unserved(self.served.cpu())
+
+    def _raise_unserved(self, served):
+        if not bool(served.all()):
+            rows = (~served).nonzero().flatten().tolist()
+            raise RuntimeError(f"no page for a token of sequences {rows[:8]}{'...' if len(rows) > 8 else ''}: {self.paged.pages} pages of "
+                               f"{self.paged.page_size} positions, {self.max_len} positions a sequence")
 
     def step_device(self):
         """One decode step on the device buffers: self.tokens -> self.next_tokens."""
@@ -465,7 +524,11 @@ class LlamaTPDecoder:
             self.tokens.copy_(self._host_in, non_blocking=True)
             self.step_device()
             self._host_out.copy_(self.next_tokens, non_blocking=True)
+        if self.paged is not None:
+            self._host_served.copy_(self.served, non_blocking=True)
         torch.cuda.current_stream().synchronize()
+        if self.paged is not None:
+            self._raise_unserved(self._host_served)
         return self._host_out
 
     def decode(self, steps: int) -> torch.Tensor:
@@ -474,6 +537,7 @@ class LlamaTPDecoder:
         for _ in range(steps):
             self.step_device()
             out.append(self.next_tokens.clone())
+        self.check_pages()
         return torch.stack(out)
 
     # ------------------------------------------------------- fp32 torch oracle

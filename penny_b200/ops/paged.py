@@ -121,6 +121,24 @@ class PagedKVCache:
         return paged_attention(q, self.k[layer], self.v[layer], self.table, self.lengths, out, lse, scale, window, self.k_scale[layer],
                                self.v_scale[layer], workspace)
 
+    def snapshot(self):
+        """Which pages and lengths the rows have, for `restore` (the pages' contents are not kept)."""
+        return tuple(t.clone() for t in (self.table, self.lengths, self.free, self.free_count))
+
+    def restore(self, snapshot) -> None:
+        for t, old in zip((self.table, self.lengths, self.free, self.free_count), snapshot):
+            t.copy_(old)
+
+    def rows_of(self, layer: int, row: int, length: int):
+        """(k, v) [kv_heads, length, head_dim] of a row's first positions, e4m3 ones times their scales in fp32: a copy, for looking at."""
+        at = torch.arange(length, device=self.device)
+        pages, within = self.table[row].long()[at // self.page_size], at % self.page_size
+        got = []
+        for pool, scale in ((self.k[layer], self.k_scale[layer]), (self.v[layer], self.v_scale[layer])):
+            rows = pool.view(torch.uint8)[pages, within].view(pool.dtype) if self.e4m3 else pool[pages, within]
+            got.append((rows.float() * scale[:, None] if self.e4m3 else rows).transpose(0, 1).contiguous())
+        return tuple(got)
+
     def workspace(self, heads: int, window: int = 0) -> torch.Tensor:
         """A workspace for `attend` with q of `heads` heads."""
         with torch.cuda.device(self.device):

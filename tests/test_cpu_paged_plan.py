@@ -85,13 +85,13 @@ def _walks(lengths, max_len, teams, window, tile=16):
     assert empties == {r for r in range(len(lengths)) if tiles[r] == 0}
 
 
-@pytest.mark.parametrize("teams", [1, 2, 5, 37, 296])
+@pytest.mark.parametrize("teams", [1, 2, 37])
 @pytest.mark.parametrize("window", [0, 1, 100])
 def test_every_tile_once(teams, window):
     rng = random.Random(teams)
     top = 2 ** 31 - 1
-    for B in (1, 2, 5, 40, 300):
-        for max_len in (1, 16, 17, 300, 5000):
+    for B in (1, 2, 5, 40):
+        for max_len in (1, 17, 300, 5000):
             inside = [rng.randrange(max_len + 1) for _ in range(B)]
             for lengths in (inside, [0] * B, [max_len] * B, [top] * B, [-1] + inside[1:], [-2 ** 31] * (B - 1) + [max_len], [max_len] + [1] * (B - 1)):
                 _walks(lengths, max_len, teams, window, tile=rng.choice([16, 32, 64]))

@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   __shared__ int s_head[kWarps];             // a part of a row that began before: 0 none, 1 it ends here, 2 it does not
   __shared__ int2 s_tail[kWarps];            // a row that does not end here (-1: none), its units still to come
   pdl_launch_dependents();
-  pdl_wait();
+  bool waited = !p.a.early;
+  if (waited) pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   Walk load;
   const int share = find_walk(p, L::kPos, load);
@@ -234,6 +235,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
       }
     }
     if (load_tiles > 0) {
+      if (!waited && load_pos + L::kPos >= load.end) {  // the tile of the row's last position
+        pdl_wait();
+        waited = true;
+      }
       const uint32_t sb = wbase + stage_in * L::kStage;
       const int r0 = lane / L::kChunks, c = lane % L::kChunks;
       const int page0 = div_page(p.div, load_pos) - ids_at;
@@ -287,6 +292,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   uint32_t masks[kStages];  // of the tiles in flight
 #pragma unroll
   for (int j = 0; j + 1 < kStages; ++j) masks[j] = issue();
+  if (!waited) pdl_wait();
+  waited = true;
   if (lane == 0) {
     s_head[warp] = 0;
     s_tail[warp] = make_int2(-1, 0);

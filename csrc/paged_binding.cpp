@@ -151,7 +151,7 @@ void bind_paged(py::module_& m) {
   }, py::arg("rows"), py::arg("heads"), py::arg("kv_heads"), py::arg("dim"), py::arg("max_len"), py::arg("window") = 0);
   // q [rows, heads, dim], one token of every row, attends to the row's last `window` positions (0: all of them).
   m.def("paged_attention", [](at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor table, at::Tensor lengths, OptTensor out, OptTensor lse,
-                              c10::optional<double> scale, int64_t window, OptTensor k_scale, OptTensor v_scale, OptTensor workspace) {
+                              c10::optional<double> scale, int64_t window, OptTensor k_scale, OptTensor v_scale, OptTensor workspace, bool early) {
     const PagedType type = type_of(q, "paged_attention: bf16 or fp16 q"), cache = type_of(k, "paged_attention: bf16, fp16 or e4m3 caches");
     need(type != PAGED_E4M3, "paged_attention: bf16 or fp16 q");
     const PagedPool pool = pool_of(k, v, type, cache, k_scale, v_scale);
@@ -193,10 +193,10 @@ void bind_paged(py::module_& m) {
     else if (bytes > 0) workspace = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, q.device(), c10::nullopt);
     const PagedAttention a = {q.data_ptr(), q.stride(0), q.stride(1), out->data_ptr(), out->stride(0), out->stride(1),
                               lse.has_value() ? lse->data_ptr<float>() : nullptr, table.data_ptr<int>(), table.stride(0), lengths.data_ptr<int>(),
-                              (int)B, (int)H, (int)table.size(1), win, scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)pool.dim)};
+                              (int)B, (int)H, (int)table.size(1), win, scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)pool.dim), early};
     ck(launch_paged_attention(a, type, pool, cache, workspace.has_value() ? workspace->data_ptr() : nullptr, sms, cur()), "paged_attention");
     return *out;
   }, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("table"), py::arg("lengths"), py::arg("out") = py::none(), py::arg("lse") = py::none(),
      py::arg("scale") = py::none(), py::arg("window") = 0, py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(),
-     py::arg("workspace") = py::none());
+     py::arg("workspace") = py::none(), py::arg("early") = false);
 }

@@ -49,6 +49,9 @@ struct PagedAttention {
   const int* lengths;
   int rows, heads, width, window;
   float scale;
+  // Kernels that may still run when this one starts (programmatic dependent launch) write, of what it reads, q and the keys and values
+  // of the rows' last positions alone: the rest is read before they end.
+  bool early;
 };
 size_t paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int max_len, int window, int sms);
 cudaError_t launch_paged_attention(const PagedAttention& a, PagedType type, const PagedPool& pool, PagedType cache, void* workspace,

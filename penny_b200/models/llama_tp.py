@@ -371,9 +371,10 @@ class LlamaTPDecoder:
                                        pieces, self.scale, theta, self.pdl, balance=balance)
             return
         heads = (self.Hq, self.cfg.head_dim)
+        # (early: the tables are complete since the launch without programmatic dependency at the step's start)
         self.paged.append(li, self.qkv, self.page_step, self.Hq, theta)
         self.paged.attend(li, self.qkv[:, :self.Hq * self.cfg.head_dim].unflatten(1, heads), out=self.attn.unflatten(1, heads), scale=self.scale,
-                          workspace=self.page_workspace)
+                          workspace=self.page_workspace, early=True)
 
     def _layers_folded(self, tokens):
         """One rank: five launches per layer, q/k/v, gate/up and head on the tiled or on the decode GEMM (`tiled_linears`).  x
@@ -439,7 +440,7 @@ class LlamaTPDecoder:
     def _step_impl(self, warm_up: bool = False, separate: bool = False, host: bool = False):
         if self.paged is not None:
             self.paged.advance(self.one_each, self.B, out=self.page_step)
-            torch.logical_and(self.served, self.page_step.granted, out=self.served)
+            torch.logical_and(self.served, self.page_step.granted, out=self.served)  # (and nothing behind it starts before the tables are done)
         if self.fold and not separate:
             self._layers_folded(self._host_in if host else self.tokens)
         else:

@@ -55,7 +55,7 @@ def paged_append(qkv, k, v, slots, positions, heads: int, theta: float, out=None
 
 
 def paged_attention(q, k, v, table, lengths, out=None, lse=None, scale: Optional[float] = None, window: int = 0, k_scale=None, v_scale=None,
-                    workspace=None) -> torch.Tensor:
+                    workspace=None, early: bool = False) -> torch.Tensor:
     """softmax(scale q K^T) V of one token per row: q [rows, heads, dim] (bf16 or fp16) over the last `window` (0: all) of
     lengths[r] positions on the row's pages; scale: 1 / sqrt(dim) by default.  Returns out, like q.
 
@@ -65,8 +65,10 @@ def paged_attention(q, k, v, table, lengths, out=None, lse=None, scale: Optional
     zeros and -inf; a length past the table row counts as the table row; positions on a page that the pool does not have count as
     not there.  Rows may share pages.  workspace: `paged_attention_workspace_bytes(rows, heads, kv_heads, dim, max_len, window)`
     bytes with max_len = table.size(1) * page_size, for callers that must not allocate; its contents mean nothing between calls,
-    but two calls that may run at the same time need one each."""
-    return ops.paged_attention(q, k, v, table, lengths, out, lse, scale, window, k_scale, v_scale, workspace)
+    but two calls that may run at the same time need one each.  early: for a step whose kernels overlap (this library's are launched with
+    programmatic dependency): those that may still run when this one starts, back to the last launch without it, write of what
+    it reads only q and the keys and values of each row's last position; the other rows, lengths and table are then read before they end."""
+    return ops.paged_attention(q, k, v, table, lengths, out, lse, scale, window, k_scale, v_scale, workspace, early)
 
 
 class PagedKVCache:
@@ -115,11 +117,12 @@ class PagedKVCache:
         """`paged_append` to this cache's `layer` at the step's slots and positions."""
         paged_append(qkv, self.k[layer], self.v[layer], step.slots, step.positions, heads, theta, out, self.k_scale[layer], self.v_scale[layer])
 
-    def attend(self, layer: int, q: torch.Tensor, out=None, lse=None, scale: Optional[float] = None, window: int = 0, workspace=None) -> torch.Tensor:
+    def attend(self, layer: int, q: torch.Tensor, out=None, lse=None, scale: Optional[float] = None, window: int = 0, workspace=None,
+               early: bool = False) -> torch.Tensor:
         """`paged_attention` of q [rows, heads, head_dim] over this cache's `layer`, all positions of lengths (those of the
         step that `advance` made room for included: append before)."""
         return paged_attention(q, self.k[layer], self.v[layer], self.table, self.lengths, out, lse, scale, window, self.k_scale[layer],
-                               self.v_scale[layer], workspace)
+                               self.v_scale[layer], workspace, early)
 
     def snapshot(self):
         """Which pages and lengths the rows have, for `restore` (the pages' contents are not kept)."""

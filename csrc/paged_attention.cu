@@ -118,7 +118,6 @@ struct Params {
   int items, groups;      // (KV head, head group) pairs, head groups of a KV head
   int max_len;
   uint32_t page_step, pos_step, step_bytes;  // strides in units of step_bytes
-  int2* tails;            // per CTA: the row that begins in it and does not end in it, how many teams follow; row -1: none
   float4* parts;          // per CTA two parts: of a row that began before it, of one that ends after it
   float2* part_ml;        // their maxima (base 2) and sums
 };
@@ -129,13 +128,14 @@ struct Part {
   static constexpr int kRows = 8 * kBlocks;
 };
 
-// The share of an item's warps, and where this one begins.  Called by whole warps, each of which sums over all rows (no barrier).
-__device__ __forceinline__ int find_walk(const Params& p, int tile, Walk& w) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// The row of unit `unit` of the line and how far behind the row's first it is; `unit` of `share`, the units of a warp.  False: behind the
+// line's end.  Called by whole warps, each of which sums over all rows (no barrier).
+template <class UnitOf>
+__device__ __forceinline__ bool locate(const Params& p, int tile, UnitOf unit, int& row, int& at, int& share, int& total) {
+  const int lane = threadIdx.x & 31;
   const int per = (p.a.rows + 31) / 32, r0 = min(p.a.rows, lane * per), r1 = min(p.a.rows, r0 + per);
-  auto seen = [&](int r) { return seen_of(p.a.lengths[r], p.max_len, p.a.window); };
   auto units = [&](int r) {
-    const Seen s = seen(r);
+    const Seen s = seen_of(p.a.lengths[r], p.max_len, p.a.window);
     return units_of(s.end - s.first, tile);
   };
   int mine = 0;
@@ -147,21 +147,19 @@ __device__ __forceinline__ int find_walk(const Params& p, int tile, Walk& w) {
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  const int total = __shfl_sync(0xffffffffu, incl, 31), share = share_of(total, (int)gridDim.y * kWarps);
-  const long long begin = (long long)(blockIdx.y * kWarps + warp) * share;
-  w.left = 0;
-  if (begin >= total) return share;
-  int row = r0, at = (int)begin - (incl - mine);
+  total = __shfl_sync(0xffffffffu, incl, 31);
+  share = share_of(total, (int)gridDim.y * kWarps);
+  const long long begin = unit(share);
+  if (begin >= total) return false;
+  row = r0, at = (int)begin - (incl - mine);
   const bool here = at >= 0 && at < mine;
   if (here && per > 1) {
     for (int n; at >= (n = units(row)); ++row) at -= n;
   }
   const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-  w.row = __shfl_sync(0xffffffffu, row, from);
-  w.at = __shfl_sync(0xffffffffu, at, from);
-  w.left = min(share, total - (int)begin);
-  enter_row(w, tile, seen);
-  return share;
+  row = __shfl_sync(0xffffffffu, row, from);
+  at = __shfl_sync(0xffffffffu, at, from);
+  return true;
 }
 
 // One accumulator of O^T, rounded, to its 16 dims of up to eight heads: this thread holds dims g and g + 8
@@ -192,13 +190,26 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ float2 s_ml[2][kWarps][kRows];  // of a warp's first part and of its last
   __shared__ int s_head[kWarps];             // a part of a row that began before: 0 none, 1 it ends here, 2 it does not
-  __shared__ int2 s_tail[kWarps];            // a row that does not end here (-1: none), its units still to come
-  pdl_launch_dependents();
+  __shared__ int s_tail[kWarps];             // a row that does not end here, -1: none
+  // (dependents may start once all CTAs are behind the wait: the joining kernel reads the lengths before its own)
   bool waited = !p.a.early;
-  if (waited) pdl_wait();
+  auto wait = [&]() {
+    pdl_wait();
+    pdl_launch_dependents();
+    waited = true;
+  };
+  if (waited) wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  Walk load;
-  const int share = find_walk(p, L::kPos, load);
+  auto seen = [&](int row) { return seen_of(p.a.lengths[row], p.max_len, p.a.window); };
+  Walk load = {};
+  {
+    const int me = (int)blockIdx.y * kWarps + warp;
+    int share, total;
+    if (locate(p, L::kPos, [&](int each) { return (long long)me * each; }, load.row, load.at, share, total)) {
+      load.left = min(share, total - me * share);
+      enter_row(load, L::kPos, seen);
+    }
+  }
   Walk w = load;
   const int kh = kBlocks == 1 ? (int)blockIdx.x : (int)blockIdx.x / p.groups, h0 = kBlocks == 1 ? 0 : ((int)blockIdx.x - kh * p.groups) * kRows;
   const int heads = min(kRows, p.group - h0), head0 = kh * p.group + h0;  // of this CTA
@@ -211,7 +222,6 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   const char* kbase = reinterpret_cast<const char*>(p.pool.k) + kh * p.pool.head_stride * kSize + (lane % L::kChunks) * 16;
   const char* vbase = reinterpret_cast<const char*>(p.pool.v) + kh * p.pool.head_stride * kSize + (lane % L::kChunks) * 16;
 
-  auto seen = [&](int row) { return seen_of(p.a.lengths[row], p.max_len, p.a.window); };
 
   // ---- loading: 64 entries of the row's table in the lanes' registers, the next 32 on their way ----
   int load_pos = 0, load_tiles = 0, ids_at = 0, ids[2] = {-1, -1};
@@ -236,8 +246,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
     }
     if (load_tiles > 0) {
       if (!waited && load_pos + L::kPos >= load.end) {  // the tile of the row's last position
-        pdl_wait();
-        waited = true;
+        wait();
       }
       const uint32_t sb = wbase + stage_in * L::kStage;
       const int r0 = lane / L::kChunks, c = lane % L::kChunks;
@@ -292,11 +301,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   uint32_t masks[kStages];  // of the tiles in flight
 #pragma unroll
   for (int j = 0; j + 1 < kStages; ++j) masks[j] = issue();
-  if (!waited) pdl_wait();
-  waited = true;
+  if (!waited) wait();
   if (lane == 0) {
     s_head[warp] = 0;
-    s_tail[warp] = make_int2(-1, 0);
+    s_tail[warp] = -1;
   }
 
   uint32_t qb[kBlocks][kSteps][2];
@@ -351,7 +359,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   while (w.left > 0) {
     const WalkPart part = next_part(w, L::kPos, seen);
     const int n = part.to - part.from;
-    if (w.units == 1) {  // an empty row
+    if (w.first == w.end) {  // an empty row
       for (int f = 0; f < P::kFrags; ++f)
         store_frag<T, kE4M3>(out_of(w.row, head0 + f / kSteps * 8) + f % kSteps * 16, p.a.out_head_stride, heads - f / kSteps * 8, lane,
                              make_float4(0.f, 0.f, 0.f, 0.f));
@@ -528,7 +536,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
         }
       }
       if (lane == 0) {
-        if (part.begins) s_tail[warp] = make_int2(w.row, w.units - w.at);
+        if (part.begins) s_tail[warp] = w.row;
         else s_head[warp] = part.ends ? 1 : 2;
       }
     }
@@ -538,11 +546,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
 
   // ---- parts that meet inside the CTA: a chain begins with a warp's last part, or with what the team before left ----
   static_assert(kWarps == 4, "a lane for every part and head of eight");
-  int2 tail = make_int2(-1, 0);
 #pragma unroll 1
   for (int first = s_head[0] != 0 ? -1 : 0; first < kWarps; ++first) {
-    const int2 row = first >= 0 ? s_tail[first] : make_int2(0, 0);
-    if (row.x < 0) continue;
+    const int row = first >= 0 ? s_tail[first] : 0;
+    if (row < 0) continue;
     int last = first;  // the chain's last warp
     bool done = false;
     while (!done && last + 1 < kWarps && s_head[last + 1] != 0) done = s_head[++last] == 1;
@@ -564,7 +571,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
       if (whole) {
         by[nb] *= inverse(top, sum, v_scale);
-        if (warp == 0 && lane < 8 && h < heads && p.a.lse) p.a.lse[(long long)row.x * p.a.heads + head0 + h] = (top + log2f(sum)) * kLn2;
+        if (warp == 0 && lane < 8 && h < heads && p.a.lse) p.a.lse[(long long)row * p.a.heads + head0 + h] = (top + log2f(sum)) * kLn2;
       } else if (warp == 0 && lane < 8) {
         p.part_ml[slot * kRows + h] = make_float2(top, sum);
       }
@@ -587,73 +594,77 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
           const float4 v = (u == first ? tail_area(u) : heads_area + u * (P::kFrags * 32))[f * 32 + lane];
           acc.x += fa[u] * v.x, acc.y += fb[u] * v.y, acc.z += fa[u] * v.z, acc.w += fb[u] * v.w;
         }
-        if (whole) store_frag<T, kE4M3>(out_of(row.x, head0 + nb * 8) + k * 16, p.a.out_head_stride, heads - nb * 8, lane, acc);
+        if (whole) store_frag<T, kE4M3>(out_of(row, head0 + nb * 8) + k * 16, p.a.out_head_stride, heads - nb * 8, lane, acc);
         else p.parts[(slot * P::kFrags + f) * 32 + lane] = acc;
       }
     }
-    if (first >= 0 && !done) {
-      // units of the row behind this CTA
-      const uint32_t behind = (uint32_t)(row.y - (kWarps - 1 - first) * share), each = (uint32_t)(kWarps * share);
-      tail = make_int2(row.x, (int)((behind + each - 1) / each));
-    }
   }
-  if (threadIdx.x == 0 && gridDim.y > 1) p.tails[cta] = tail;
 }
 
-// Joins the parts of a row that spans teams: block c has the row that begins in CTA c and ends in the same item's CTA of a later team.
+// Joins the parts of a row that spans teams: a block has the row that begins in its team (if there is one that does not end there), and
+// finds out before it waits.  A warp takes an accumulator of O^T, or, with more warps than those, every so many-th part of it.
+constexpr int kJoinThreads = 512;
 template <int D, typename T, bool kE4M3, int kBlocks>
-__global__ void __launch_bounds__(256) k_paged_join(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_constant__ Params p) {
   using P = Part<D, kBlocks>;
-  constexpr int kSteps = D / 16, kAhead = 6;
+  constexpr int kSteps = D / 16, kAhead = 4, kTile = Tile<D, kE4M3, kBlocks>::kPos;
+  __shared__ float4 s_acc[kJoinThreads], s_ml[kJoinThreads];
   pdl_launch_dependents();
+  int row, at, share, total, behind = 0;
+  if (locate(p, kTile, [&](int each) { return ((long long)blockIdx.y + 1) * kWarps * each; }, row, at, share, total)) {
+    const Seen s = seen_of(p.a.lengths[row], p.max_len, p.a.window);
+    const int each = kWarps * share, end = ((int)blockIdx.y + 1) * each;
+    behind = teams_behind(end - each, end, end - at, units_of(s.end - s.first, kTile));
+  }
   pdl_wait();
-  const int cta = (int)(blockIdx.y * gridDim.x + blockIdx.x);
-  const int2 row = p.tails[cta];
-  if (row.x < 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (behind == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warps = blockDim.x / 32;
   const int kh = kBlocks == 1 ? (int)blockIdx.x : (int)blockIdx.x / p.groups, h0 = kBlocks == 1 ? 0 : ((int)blockIdx.x - kh * p.groups) * P::kRows;
-  const int heads = min(P::kRows, p.group - h0), head0 = kh * p.group + h0, n = 1 + row.y;
+  const int heads = min(P::kRows, p.group - h0), head0 = kh * p.group + h0, n = 1 + behind;
+  const int sets = max(1, warps / P::kFrags), set = warp / P::kFrags;
+  const long long cta = blockIdx.y * gridDim.x + blockIdx.x;
   const float v_scale = kE4M3 ? p.pool.v_scale[kh] : 1.f;
-  for (int f = warp; f < P::kFrags; f += (int)blockDim.x / 32) {
+  for (int f = warp % P::kFrags; f < P::kFrags; f += warps) {
     const int nb = f / kSteps, h = nb * 8 + 2 * t;
-    float top[2] = {-INFINITY, -INFINITY}, base[2], sum[2] = {0.f, 0.f};
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < n; i0 += kAhead) {
+    auto take = [&](const float4& ml, const float4& v) {  // maxima and sums of two heads, their values
+      const float next[2] = {fmaxf(top[0], ml.x), fmaxf(top[1], ml.z)};
+      const float base[2] = {next[0] == -INFINITY ? 0.f : next[0], next[1] == -INFINITY ? 0.f : next[1]};
+      const float a = exp2_ftz(top[0] - base[0]), b = exp2_ftz(top[1] - base[1]), c = exp2_ftz(ml.x - base[0]), d = exp2_ftz(ml.z - base[1]);
+      sum[0] = sum[0] * a + ml.y * c, sum[1] = sum[1] * b + ml.w * d;
+      acc.x = acc.x * a + v.x * c, acc.y = acc.y * b + v.y * d, acc.z = acc.z * a + v.z * c, acc.w = acc.w * b + v.w * d;
+      top[0] = next[0], top[1] = next[1];
+    };
+    for (int i0 = set; i0 < n; i0 += kAhead * sets) {
       float4 ml[kAhead], v[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int i = i0 + u;
-        const long long slot = 2ll * (cta + (long long)i * gridDim.x) + (i == 0);
-        ml[u] = i < n ? *reinterpret_cast<const float4*>(p.part_ml + slot * P::kRows + h) : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
-        v[u] = i < n ? p.parts[(slot * P::kFrags + f) * 32 + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      float next[2] = {top[0], top[1]};
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) next[0] = fmaxf(next[0], ml[u].x), next[1] = fmaxf(next[1], ml[u].z);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        base[e] = next[e] == -INFINITY ? 0.f : next[e];
-        const float corr = exp2_ftz(top[e] - base[e]);
-        sum[e] *= corr;
-        if (e == 0) acc.x *= corr, acc.z *= corr;
-        else acc.y *= corr, acc.w *= corr;
-        top[e] = next[e];
+        const int i = i0 + u * sets;
+        const long long slot = 2 * (cta + (long long)i * gridDim.x) + (i == 0);
+        if (i < n) {
+          ml[u] = *reinterpret_cast<const float4*>(p.part_ml + slot * P::kRows + h);
+          v[u] = p.parts[(slot * P::kFrags + f) * 32 + lane];
+        }
       }
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const float fa = exp2_ftz(ml[u].x - base[0]), fb = exp2_ftz(ml[u].z - base[1]);
-        sum[0] += fa * ml[u].y;
-        sum[1] += fb * ml[u].w;
-        acc.x += fa * v[u].x, acc.y += fb * v[u].y, acc.z += fa * v[u].z, acc.w += fb * v[u].w;
-      }
+      for (int u = 0; u < kAhead; ++u)
+        if (i0 + u * sets < n) take(ml[u], v[u]);
+    }
+    if (sets > 1) {
+      s_acc[threadIdx.x] = acc;
+      s_ml[threadIdx.x] = make_float4(top[0], sum[0], top[1], sum[1]);
+      __syncthreads();
+      if (set > 0) return;
+      for (int i = 1; i < sets; ++i) take(s_ml[threadIdx.x + i * P::kFrags * 32], s_acc[threadIdx.x + i * P::kFrags * 32]);
     }
     const float inv[2] = {inverse(top[0], sum[0], v_scale), inverse(top[1], sum[1], v_scale)};
-    T* out = reinterpret_cast<T*>(p.a.out) + row.x * p.a.out_stride + (head0 + nb * 8) * p.a.out_head_stride + f % kSteps * 16;
+    T* out = reinterpret_cast<T*>(p.a.out) + row * p.a.out_stride + (head0 + nb * 8) * p.a.out_head_stride + f % kSteps * 16;
     store_frag<T, kE4M3>(out, p.a.out_head_stride, heads - nb * 8, lane, make_float4(acc.x * inv[0], acc.y * inv[1], acc.z * inv[0], acc.w * inv[1]));
     if (p.a.lse && f % kSteps == 0 && g == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if (h + e < heads) p.a.lse[(long long)row.x * p.a.heads + head0 + h + e] = (top[e] + log2f(sum[e])) * kLn2;
+        if (h + e < heads) p.a.lse[(long long)row * p.a.heads + head0 + h + e] = (top[e] + log2f(sum[e])) * kLn2;
     }
   }
 }
@@ -676,13 +687,14 @@ cudaError_t launch(Params p, void* workspace, int sms, cudaStream_t stream) {
   if (rc != cudaSuccess) return rc;
   const long long ctas = ctas_of(p.a.rows, p.items, most_seen(p.max_len, p.a.window), Tile<D, kE4M3, kBlocks>::kPos, slots_of(Tile<D, kE4M3, kBlocks>::kStage, sms));
   if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
-  p.tails = reinterpret_cast<int2*>(workspace);
-  p.parts = reinterpret_cast<float4*>(p.tails + (ctas + 1) / 2 * 2);
+  p.parts = reinterpret_cast<float4*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.parts + ctas * 2 * P::kFrags * 32);
   const dim3 grid((unsigned)p.items, (unsigned)(ctas / p.items));
   rc = launch_kernel_ex(kernel, grid, dim3(kWarps * 32), (size_t)smem, stream, true, 1, p);
   if (rc != cudaSuccess || ctas == p.items) return rc;  // (a single team finishes its rows)
-  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kBlocks>, grid, dim3(P::kFrags * 32 < 256 ? P::kFrags * 32 : 256), 0, stream, true, 1, p);
+  // few rows are cut into many parts each (2 rows of 100001: 18)
+  const int warps = (int)grid.y > 4 * p.a.rows ? kJoinThreads / 32 : 8;
+  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kBlocks>, grid, dim3((P::kFrags < warps && p.a.rows >= (int)grid.y ? P::kFrags : warps) * 32), 0, stream, true, 1, p);
 }
 
 }  // namespace
@@ -693,7 +705,7 @@ size_t paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int di
   const int items = items_of(kv_heads, group), most = most_seen(max_len, window);
   const long long one = ctas_of(rows, items, most, 16, sms), two = ctas_of(rows, items, most, 16, 2 * sms);
   const size_t ctas = (size_t)(one > two ? one : two);
-  return ctas == (size_t)items ? 0 : (ctas + 1) * (sizeof(int2) + 2 * blocks * ((size_t)(dim / 16) * 512 + 8 * sizeof(float2)));
+  return ctas == (size_t)items ? 0 : ctas * 2 * blocks * ((size_t)(dim / 16) * 512 + 8 * sizeof(float2));
 }
 
 cudaError_t launch_paged_attention(const PagedAttention& a, PagedType type, const PagedPool& pool, PagedType cache, void* workspace, int sms,

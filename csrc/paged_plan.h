@@ -51,10 +51,11 @@ PENNY_ATTN_HD Seen seen_of(int length, int max_len, int window) {
 // heads are read at about the same time (apart from each other 64 rows of 16000 positions took 632 us instead of 607).  The
 // rows lie in a line, each a unit for its start (its output, its q) and one for every tile of positions; every warp of a
 // team's CTAs gets `share` units, at least kMinShare.  The lengths are on the device, and every CTA sums over them by itself.
-constexpr int kMinShare = 4;
+// kStart: 96 rows of 1 to 8192 positions, e4m3, in 49.3 / 45.4 / 43.9 / 43.0 us with 1 / 2 / 3 / 5; 256 of 100 25.5 / 27.3 / 27.0 / 25.0.
+constexpr int kMinShare = 4, kStart = 3;
 constexpr long long kMaxLen = 0x7fff0000, kMaxUnits = 1ll << 30;  // (all rows' units, and a share more, fit 32 bits)
 
-PENNY_ATTN_HD int units_of(int positions, int tile) { return 1 + (positions + tile - 1) / tile; }
+PENNY_ATTN_HD int units_of(int positions, int tile) { return positions > 0 ? kStart + (positions + tile - 1) / tile : 1; }
 PENNY_ATTN_HD int share_of(int units, int warps) { return attn::at_least(kMinShare, (int)(((uint32_t)units + warps - 1) / (uint32_t)warps)); }
 // Teams of a launch: as many as the GPU holds (`slots` CTAs), in more rounds where that leaves over a tenth of it empty; no more
 // than there are shares, if every row has `units` units.
@@ -89,7 +90,7 @@ PENNY_ATTN_HD void enter_row(Walk& w, int tile, SeenOf seen) {
   w.end = s.end;
   w.units = units_of(s.end - s.first, tile);
 }
-// The next part of the share (w.left > 0): all that it has of one row.  Without tiles: an empty row, which begins and ends, or a
+// The next part of the share (w.left > 0): all that it has of one row.  Without tiles: an empty row (which begins and ends), or a
 // row's start alone, which is nothing (the next warp's part begins the row).
 template <class SeenOf>
 PENNY_ATTN_HD WalkPart next_part(Walk& w, int tile, SeenOf seen) {
@@ -98,11 +99,17 @@ PENNY_ATTN_HD WalkPart next_part(Walk& w, int tile, SeenOf seen) {
     w.at = 0;
     enter_row(w, tile, seen);
   }
-  const int from = w.at, to = attn::at_most(w.units, w.at + w.left);
-  w.left -= to - from;
-  w.at = to;
-  const bool some = to > 1 || w.units == 1;
-  return {attn::at_least(0, from - 1), to - 1, from <= 1 && some, to == w.units && some};
+  const int from = attn::at_least(0, w.at - kStart), end = attn::at_most(w.units, w.at + w.left), to = attn::at_least(0, end - kStart);
+  w.left -= end - w.at;
+  w.at = end;
+  const bool some = to > from || w.first == w.end;
+  return {from, to, from == 0 && some, end == w.units && some};
+}
+// What lies across the end of a team's share, [begin, end) of the line: the row that has unit `end` starts at unit `start`.  How many
+// teams behind it have a part of the row, if its first tile is the team's; 0: the row is another team's.
+PENNY_ATTN_HD int teams_behind(int begin, int end, int start, int units) {
+  const int first = start + kStart, behind = start + units - end, each = end - begin;
+  return first >= begin && first < end && behind > 0 ? (behind + each - 1) / each : 0;
 }
 
 // A pool's strides in a unit so large that a place in it fits 32 bits: the largest power of two that divides both.  bytes 0:

@@ -384,6 +384,7 @@ uint32_t penny_page_steps(long long pages, long long page_size, long long page_s
 uint32_t penny_page_step_of(int page, int pages, int pos, int size, uint32_t page_step, uint32_t pos_step) {
   return penny::paged::step_of(page, pages, pos, penny::paged::page_div(size), page_step, pos_step);
 }
+int penny_paged_teams_behind(int begin, int end, int start, int units) { return penny::paged::teams_behind(begin, end, start, units); }
 int penny_paged_teams(long long rows, int items, long long units, int warps, int slots) { return penny::paged::teams_of(rows, items, units, warps, slots); }
 // The walk of warp `warp` of `warps` of an item: its parts (row, first tile, last tile, begins | 2 ends | 4 empty, units of the row
 // behind the part) in order, and its tiles' first positions.  Returns the number of parts; -1: too many for `most`.
@@ -413,7 +414,7 @@ int penny_paged_walk(const int* lengths, int rows, int max_len, int window, int 
       tiles[(*num_tiles)++] = w.first + i * tile;
     }
     int* to = parts + 5 * n++;
-    to[0] = w.row, to[1] = p.from, to[2] = p.to, to[3] = p.begins | p.ends << 1 | (w.units == 1) << 2, to[4] = w.units - w.at;
+    to[0] = w.row, to[1] = p.from, to[2] = p.to, to[3] = p.begins | p.ends << 1 | (w.first == w.end) << 2, to[4] = w.units - w.at;
   }
   return n;
 }

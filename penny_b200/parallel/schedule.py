@@ -199,6 +199,12 @@ def paged_teams(rows: int, items: int, units: int, warps: int = 4, slots: int = 
     return f(rows, items, units, warps, slots)
 
 
+def paged_teams_behind(begin: int, end: int, start: int, units: int) -> int:
+    """Teams behind one with share [begin, end) that have a part of the row that begins in it and lies across its end; 0: there is no
+    such row (csrc/paged_plan.h)."""
+    return sim_lib().penny_paged_teams_behind(begin, end, start, units)
+
+
 def paged_walk(lengths, max_len: int, warps: int, warp: int, window: int = 0, tile: int = 16):
     """What one of the paged attention's warps of an item does (csrc/paged_plan.h): (its parts: (row, first tile, last tile, begins,
     ends, empty row, units of the row behind the part), its tiles' first positions, every warp's share)."""

@@ -58,6 +58,9 @@ def _walks(lengths, max_len, teams, window, tile=16):
     seen = [(max(0, min(n, max_len) - window) if window else 0, max(0, min(n, max_len))) for n in lengths]
     tiles = [-(-(b - a) // tile) for a, b in seen]
     covered, empties, open_row, counts = {}, set(), None, {}
+    line = [0]
+    for n in tiles:
+        line.append(line[-1] + (n + 3 if n else 1))  # three units for a row's start, one for an empty row
     for w in range(warps):
         parts, starts, share = schedule.paged_walk(lengths, max_len, warps, w, window, tile)
         assert starts == [seen[r][0] + tile * i for r, a, b, *_ in parts for i in range(a, b)]
@@ -75,12 +78,19 @@ def _walks(lengths, max_len, teams, window, tile=16):
                 assert open_row == r
             open_row = None if ends else r
             if begins and not ends:
-                later = -(-(behind - (per - 1 - w % per) * share) // (per * share))  # teams that follow, as the kernel counts them
-                counts[r] = (w // per, max(0, later))
+                # teams that follow, as the joining kernel counts them from the line alone
+                begin = w // per * per * share
+                counts[r] = (w // per, schedule.paged_teams_behind(begin, begin + per * share, line[r], line[r + 1] - line[r]) if begin + per * share < line[-1] else 0)
             if ends and not begins:
                 first, later = counts[r]
                 assert first + later == w // per
     assert open_row is None
+    for team in range(teams):  # and a team that begins no row across its end is not taken for one
+        begin, end = team * per * share, (team + 1) * per * share
+        if end < line[-1]:
+            r = max(i for i, x in enumerate(line[:-1]) if x <= end)
+            if schedule.paged_teams_behind(begin, end, line[r], line[r + 1] - line[r]):
+                assert counts[r][0] == team and counts[r][1] > 0
     assert all(covered.get(r, 0) == tiles[r] for r in range(len(lengths)))
     assert empties == {r for r in range(len(lengths)) if tiles[r] == 0}
 

@@ -58,7 +58,7 @@ constexpr long long kMaxLen = 0x7fff0000, kMaxUnits = 1ll << 30;  // (all rows' 
 PENNY_ATTN_HD int units_of(int positions, int tile) { return positions > 0 ? kStart + (positions + tile - 1) / tile : 1; }
 PENNY_ATTN_HD int share_of(int units, int warps) { return attn::at_least(kMinShare, (int)(((uint32_t)units + warps - 1) / (uint32_t)warps)); }
 // Teams of a launch: as many as the GPU holds (`slots` CTAs), in more rounds where that leaves over a tenth of it empty; no more
-// than there are shares, if every row has `units` units.
+// than there are shares of tiles, if every row has `units` units.
 inline int teams_of(long long rows, int items, long long units, int warps, int slots) {
   int best = 1;
   double used = 0;
@@ -67,8 +67,8 @@ inline int teams_of(long long rows, int items, long long units, int warps, int s
     const double now = (double)teams * items / ((double)slots * rounds);
     if (teams > 0 && now > used) best = teams, used = now;
   }
-  const long long most = (rows * units + (long long)warps * kMinShare - 1) / ((long long)warps * kMinShare);
-  return most < best ? (int)most : best;
+  const long long most = (rows * (units - kStart) + (long long)warps * kMinShare - 1) / ((long long)warps * kMinShare);
+  return most < best ? (int)(most > 1 ? most : 1) : best;
 }
 
 // What a warp has of the line: where it stands in a row, and what is left of its share.

@@ -108,7 +108,8 @@ def test_every_tile_once(teams, window):
 
 
 def test_teams():
-    assert schedule.paged_teams(64, 8, 129) == 37 and schedule.paged_teams(1, 1, 14) == 1 and schedule.paged_teams(1, 8, 129) == 9
+    assert schedule.paged_teams(64, 8, 131) == 37 and schedule.paged_teams(1, 1, 19) == 1 and schedule.paged_teams(1, 1, 20) == 2
+    assert schedule.paged_teams(1, 8, 131) == 8 and schedule.paged_teams(5, 3, 1) == 1
     for items in list(range(1, 400)) + [1000, 4096]:
         teams = schedule.paged_teams(1000, items, 1000)
         ctas = teams * items

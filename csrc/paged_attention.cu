@@ -22,7 +22,10 @@
 //     16-byte chunk are permuted on both sides of the product.  V's bytes are transposed in pairs by ldmatrix and separated
 //     into even and odd dims.
 //   * P is rounded to the type of the product (bf16: 2^-8 of each weight at most, averaged over the positions; the sum is of the
-//     unrounded ones); q, scores, maxima and sums are not rounded.
+//     unrounded ones); q, scores, maxima and sums are not rounded.  Weights count from a base near the maximum so far.  With fp16 it
+//     follows when it is exceeded by 2^8, which is seldom (64 rows of 4096, e4m3, 28 of 2 heads: 34.4 us, always 38.1).  With bf16
+//     it follows always, so that the largest weight is one and not off: 64 rows of 2048 are 0.0018 of the output's norm from 64
+//     bits (its own rounding: 0.0017), otherwise 0.0022 (and 0.5 us faster).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -43,7 +46,6 @@ using attn::ldmatrix_x4_trans;
 using attn::mma_bf16;
 
 constexpr int kWarps = 4;
-constexpr float kSlack = 8.f;  // weights of up to 2^8
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int D, bool kE4M3, int kBlocks>
@@ -54,8 +56,20 @@ struct Tile {
   static constexpr int kPerPass = 32 / kChunks;                // positions that a warp's 32 chunks cover
   static constexpr int kStage = 2 * kPos * kRow;
   static constexpr uint32_t kAll = 0xffffffffu >> (32 - kPos);  // the mask of a full tile
-  static constexpr int kStages = kBlocks == 2 || kStage > 8192 ? 2 : kStage < 8192 ? 5 : 3;
-  static constexpr int kSmem = kWarps * kStages * kStage;
+  static constexpr int kFrags = kBlocks * (D / 16);            // MMA accumulators of O^T: 16 dims x 8 heads, a float4 a lane
+  static constexpr int kParts = kWarps * kFrags * 512;         // room for a part of every warp
+  // two CTAs to an SM where three stages (five small ones) or two of them leave room for that, else one; of 228 KB a CTA takes 1 KB
+  // and its static variables besides
+  static constexpr int kOwn = 1024 + kBlocks * 512 + 64, kHalf = (228 << 10) / 2 - kOwn;
+  static constexpr int stages(int most, int limit) {
+    int n = most;
+    while (n > 2 && n * kWarps * kStage + kParts > limit) --n;
+    return n;
+  }
+  static constexpr bool kTwo = 2 * kWarps * kStage + kParts <= kHalf;
+  static constexpr int kStages = stages(kStage < 8192 ? 5 : 3, kTwo ? kHalf : (228 << 10) - kOwn);
+  static constexpr int kPipes = kWarps * kStages * kStage, kSmem = kPipes + kParts;
+  static_assert(kSmem <= (kTwo ? kHalf : (228 << 10) - kOwn) && kStages * kStage >= kFrags * 512, "shared memory");
   // where chunk c of position r lies: eight positions' equal chunks in eight different 16-byte banks
   static __device__ __forceinline__ uint32_t at(int r, int c) {
     if constexpr (kRow == 64) return (uint32_t)((r >> 1) * 128 + ((((r & 1) << 2) | (c ^ ((r >> 1) & 3))) << 4));
@@ -122,12 +136,6 @@ struct Params {
   float2* part_ml;        // their maxima (base 2) and sums
 };
 
-template <int D, int kBlocks>
-struct Part {
-  static constexpr int kFrags = kBlocks * (D / 16);  // MMA accumulators of O^T: 16 dims x 8 heads, a float4 a lane
-  static constexpr int kRows = 8 * kBlocks;
-};
-
 // The row of unit `unit` of the line and how far behind the row's first it is; `unit` of `share`, the units of a warp.  False: behind the
 // line's end.  Called by whole warps, each of which sums over all rows (no barrier).
 template <class UnitOf>
@@ -184,9 +192,9 @@ template <int D, typename T, bool kE4M3, int kBlocks>
 __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_constant__ Params p) {
   using L = Tile<D, kE4M3, kBlocks>;
   using T2 = typename Pair<T>::type;
-  using P = Part<D, kBlocks>;
-  constexpr int kRows = P::kRows, kSteps = D / 16, kGroups = L::kPos / 16, kStages = L::kStages;
+  constexpr int kRows = 8 * kBlocks, kSteps = D / 16, kGroups = L::kPos / 16, kStages = L::kStages;
   constexpr bool kBf16 = !kE4M3 && __is_same(T, __nv_bfloat16);
+  constexpr float kSlack = kBf16 ? 0.f : 8.f;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ float2 s_ml[2][kWarps][kRows];  // of a warp's first part and of its last
   __shared__ int s_head[kWarps];             // a part of a row that began before: 0 none, 1 it ends here, 2 it does not
@@ -215,7 +223,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   const int heads = min(kRows, p.group - h0), head0 = kh * p.group + h0;  // of this CTA
   const int cta = (int)(blockIdx.y * gridDim.x + blockIdx.x);
   const uint32_t wbase = attn::smem_u32_local(smem_raw) + warp * (kStages * L::kStage);
-  float4* heads_area = reinterpret_cast<float4*>(smem_raw + L::kSmem);                                  // [warps][frags][32]
+  float4* heads_area = reinterpret_cast<float4*>(smem_raw + L::kPipes);                                  // [warps][frags][32]
   auto tail_area = [&](int i) { return reinterpret_cast<float4*>(smem_raw + i * (kStages * L::kStage)); };  // a drained pipeline's space
   constexpr int kSize = kE4M3 ? 1 : 2;
   const uint32_t pos_bytes = p.pos_step * p.step_bytes;
@@ -360,7 +368,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
     const WalkPart part = next_part(w, L::kPos, seen);
     const int n = part.to - part.from;
     if (w.first == w.end) {  // an empty row
-      for (int f = 0; f < P::kFrags; ++f)
+      for (int f = 0; f < L::kFrags; ++f)
         store_frag<T, kE4M3>(out_of(w.row, head0 + f / kSteps * 8) + f % kSteps * 16, p.a.out_head_stride, heads - f / kSteps * 8, lane,
                              make_float4(0.f, 0.f, 0.f, 0.f));
       if (p.a.lse && lane < heads) p.a.lse[(long long)w.row * p.a.heads + head0 + lane] = -INFINITY;
@@ -368,12 +376,12 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
     }
     if (n <= 0) continue;
     load_q(w.row);
-    // per block of heads: the base (m: minus infinity before the first) of heads 2 t and 2 t + 1, this thread's share of their sums, O^T
-    float m[kBlocks][2], base[kBlocks][2], limit[kBlocks][2], l[kBlocks][2], o[kBlocks][kSteps][4];
+    // per block of heads: the base (m: minus infinity before there is one) of heads 2 t and 2 t + 1, this thread's share of their sums, O^T
+    float m[kBlocks][2], base[kBlocks][2], l[kBlocks][2], o[kBlocks][kSteps][4];
 #pragma unroll
     for (int nb = 0; nb < kBlocks; ++nb) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) m[nb][i] = limit[nb][i] = -INFINITY, base[nb][i] = l[nb][i] = 0.f;
+      for (int i = 0; i < 2; ++i) m[nb][i] = -INFINITY, base[nb][i] = l[nb][i] = 0.f;
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) o[nb][k][0] = o[nb][k][1] = o[nb][k][2] = o[nb][k][3] = 0.f;
     }
@@ -418,7 +426,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
           for (int u = 0; u < 4; ++u) s[nb][c][u] += odd[nb][u];
         }
       }
-      // ---- weights exp2(score - base); the base follows the maximum when a score exceeds it by more than kSlack ----
+      // ---- weights exp2(score - base); the base goes up to the maximum when a score of the tile is above it by more than kSlack ----
       uint32_t pb[kBlocks][kGroups][2];
 #pragma unroll
       for (int nb = 0; nb < kBlocks; ++nb) {
@@ -440,7 +448,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
 #pragma unroll
         for (int c = 0; c < kGroups; ++c) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) above = above || s[nb][c][u] > limit[nb][u & 1];
+          for (int u = 0; u < 4; ++u) above = above || s[nb][c][u] > (m[nb][u & 1] == -INFINITY ? -INFINITY : kSlack);
         }
         if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
@@ -453,7 +461,6 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
             if (top > (m[nb][i] == -INFINITY ? -INFINITY : 0.f)) {
               const float next = base[nb][i] + top, by = base[nb][i] - next, corr = exp2_ftz(m[nb][i] - next);
               m[nb][i] = base[nb][i] = next;
-              limit[nb][i] = kSlack;
               l[nb][i] *= corr;
 #pragma unroll
               for (int k = 0; k < kSteps; ++k) o[nb][k][i] *= corr, o[nb][k][2 + i] *= corr;
@@ -524,7 +531,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
       }
     } else {
       __syncwarp();  // (the last tile was read by all)
-      float4* area = part.begins ? tail_area(warp) : heads_area + warp * (P::kFrags * 32);
+      float4* area = part.begins ? tail_area(warp) : heads_area + warp * (L::kFrags * 32);
 #pragma unroll
       for (int nb = 0; nb < kBlocks; ++nb) {
 #pragma unroll
@@ -591,11 +598,11 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
 #pragma unroll
         for (int u = 0; u < kWarps; ++u) {
           if (u < first || u > last) continue;
-          const float4 v = (u == first ? tail_area(u) : heads_area + u * (P::kFrags * 32))[f * 32 + lane];
+          const float4 v = (u == first ? tail_area(u) : heads_area + u * (L::kFrags * 32))[f * 32 + lane];
           acc.x += fa[u] * v.x, acc.y += fb[u] * v.y, acc.z += fa[u] * v.z, acc.w += fb[u] * v.w;
         }
         if (whole) store_frag<T, kE4M3>(out_of(row, head0 + nb * 8) + k * 16, p.a.out_head_stride, heads - nb * 8, lane, acc);
-        else p.parts[(slot * P::kFrags + f) * 32 + lane] = acc;
+        else p.parts[(slot * L::kFrags + f) * 32 + lane] = acc;
       }
     }
   }
@@ -606,25 +613,25 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
 constexpr int kJoinThreads = 512;
 template <int D, typename T, bool kE4M3, int kBlocks>
 __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_constant__ Params p) {
-  using P = Part<D, kBlocks>;
-  constexpr int kSteps = D / 16, kAhead = 4, kTile = Tile<D, kE4M3, kBlocks>::kPos;
+  using L = Tile<D, kE4M3, kBlocks>;
+  constexpr int kSteps = D / 16, kAhead = 4, kRows = 8 * kBlocks;
   __shared__ float4 s_acc[kJoinThreads], s_ml[kJoinThreads];
   pdl_launch_dependents();
   int row, at, share, total, behind = 0;
-  if (locate(p, kTile, [&](int each) { return ((long long)blockIdx.y + 1) * kWarps * each; }, row, at, share, total)) {
+  if (locate(p, L::kPos, [&](int each) { return ((long long)blockIdx.y + 1) * kWarps * each; }, row, at, share, total)) {
     const Seen s = seen_of(p.a.lengths[row], p.max_len, p.a.window);
     const int each = kWarps * share, end = ((int)blockIdx.y + 1) * each;
-    behind = teams_behind(end - each, end, end - at, units_of(s.end - s.first, kTile));
+    behind = teams_behind(end - each, end, end - at, units_of(s.end - s.first, L::kPos));
   }
   pdl_wait();
   if (behind == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warps = blockDim.x / 32;
-  const int kh = kBlocks == 1 ? (int)blockIdx.x : (int)blockIdx.x / p.groups, h0 = kBlocks == 1 ? 0 : ((int)blockIdx.x - kh * p.groups) * P::kRows;
-  const int heads = min(P::kRows, p.group - h0), head0 = kh * p.group + h0, n = 1 + behind;
-  const int sets = max(1, warps / P::kFrags), set = warp / P::kFrags;
+  const int kh = kBlocks == 1 ? (int)blockIdx.x : (int)blockIdx.x / p.groups, h0 = kBlocks == 1 ? 0 : ((int)blockIdx.x - kh * p.groups) * kRows;
+  const int heads = min(kRows, p.group - h0), head0 = kh * p.group + h0, n = 1 + behind;
+  const int sets = max(1, warps / L::kFrags), set = warp / L::kFrags;
   const long long cta = blockIdx.y * gridDim.x + blockIdx.x;
   const float v_scale = kE4M3 ? p.pool.v_scale[kh] : 1.f;
-  for (int f = warp % P::kFrags; f < P::kFrags; f += warps) {
+  for (int f = warp % L::kFrags; f < L::kFrags; f += warps) {
     const int nb = f / kSteps, h = nb * 8 + 2 * t;
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -643,8 +650,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_consta
         const int i = i0 + u * sets;
         const long long slot = 2 * (cta + (long long)i * gridDim.x) + (i == 0);
         if (i < n) {
-          ml[u] = *reinterpret_cast<const float4*>(p.part_ml + slot * P::kRows + h);
-          v[u] = p.parts[(slot * P::kFrags + f) * 32 + lane];
+          ml[u] = *reinterpret_cast<const float4*>(p.part_ml + slot * kRows + h);
+          v[u] = p.parts[(slot * L::kFrags + f) * 32 + lane];
         }
       }
 #pragma unroll
@@ -656,7 +663,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_consta
       s_ml[threadIdx.x] = make_float4(top[0], sum[0], top[1], sum[1]);
       __syncthreads();
       if (set > 0) return;
-      for (int i = 1; i < sets; ++i) take(s_ml[threadIdx.x + i * P::kFrags * 32], s_acc[threadIdx.x + i * P::kFrags * 32]);
+      for (int i = 1; i < sets; ++i) take(s_ml[threadIdx.x + i * L::kFrags * 32], s_acc[threadIdx.x + i * L::kFrags * 32]);
     }
     const float inv[2] = {inverse(top[0], sum[0], v_scale), inverse(top[1], sum[1], v_scale)};
     T* out = reinterpret_cast<T*>(p.a.out) + row * p.a.out_stride + (head0 + nb * 8) * p.a.out_head_stride + f % kSteps * 16;
@@ -673,28 +680,24 @@ int blocks_of(int group) { return group > 8 ? 2 : 1; }
 int items_of(int kv_heads, int group) { return kv_heads * ((group + 8 * blocks_of(group) - 1) / (8 * blocks_of(group))); }
 // CTAs of a launch over rows that can be as long as `most`.
 long long ctas_of(int rows, int items, int most, int tile, int slots) { return (long long)items * teams_of(rows, items, units_of(most, tile), kWarps, slots); }
-// CTAs that the GPU holds at a time.
-int slots_of(int stage_bytes, int sms) { return stage_bytes > 8192 ? sms : 2 * sms; }
 int most_seen(int max_len, int window) { return window > 0 && window < max_len ? window : max_len; }
 
 template <int D, typename T, bool kE4M3, int kBlocks>
 cudaError_t launch(Params p, void* workspace, int sms, cudaStream_t stream) {
-  using P = Part<D, kBlocks>;
+  using L = Tile<D, kE4M3, kBlocks>;
   auto* kernel = k_paged_attention<D, T, kE4M3, kBlocks>;
-  constexpr int smem = Tile<D, kE4M3, kBlocks>::kSmem + kWarps * P::kFrags * 512;
-  static_assert(smem <= 227 << 10 && Tile<D, kE4M3, kBlocks>::kStages * Tile<D, kE4M3, kBlocks>::kStage >= P::kFrags * 512, "shared memory");
-  cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(kernel), smem).rc;
+  cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(kernel), L::kSmem).rc;
   if (rc != cudaSuccess) return rc;
-  const long long ctas = ctas_of(p.a.rows, p.items, most_seen(p.max_len, p.a.window), Tile<D, kE4M3, kBlocks>::kPos, slots_of(Tile<D, kE4M3, kBlocks>::kStage, sms));
+  const long long ctas = ctas_of(p.a.rows, p.items, most_seen(p.max_len, p.a.window), L::kPos, L::kTwo ? 2 * sms : sms);
   if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
   p.parts = reinterpret_cast<float4*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.parts + ctas * 2 * P::kFrags * 32);
+  p.part_ml = reinterpret_cast<float2*>(p.parts + ctas * 2 * L::kFrags * 32);
   const dim3 grid((unsigned)p.items, (unsigned)(ctas / p.items));
-  rc = launch_kernel_ex(kernel, grid, dim3(kWarps * 32), (size_t)smem, stream, true, 1, p);
+  rc = launch_kernel_ex(kernel, grid, dim3(kWarps * 32), (size_t)L::kSmem, stream, true, 1, p);
   if (rc != cudaSuccess || ctas == p.items) return rc;  // (a single team finishes its rows)
   // few rows are cut into many parts each (2 rows of 100001: 18)
   const int warps = (int)grid.y > 4 * p.a.rows ? kJoinThreads / 32 : 8;
-  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kBlocks>, grid, dim3((P::kFrags < warps && p.a.rows >= (int)grid.y ? P::kFrags : warps) * 32), 0, stream, true, 1, p);
+  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kBlocks>, grid, dim3((L::kFrags < warps && p.a.rows >= (int)grid.y ? L::kFrags : warps) * 32), 0, stream, true, 1, p);
 }
 
 }  // namespace

@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = (__float_as_int(top) >> 23) & 255;
-        const bool plain = e < 1 || e > 253;  // zeros, infinities
+        const int e = min((__float_as_int(top) >> 23) & 255, 253);  // (one over a power of two above that is none of fp32's)
+        const bool plain = e < 1;  // zeros
         const float down = plain ? 1.f : __int_as_float((254 - e) << 23);
         const float factor = p.a.scale * kLog2e * p.pool.k_scale[kh] * (plain ? 1.f : __int_as_float(e << 23));
 #pragma unroll

@@ -40,6 +40,7 @@ PagedPool pool_of(const at::Tensor& k, const at::Tensor& v, PagedType type, Page
   need(k.size(0) >= 1 && k.size(1) >= 1 && k.size(2) >= 1 && k.size(0) < (1ll << 31) && k.size(1) < (1ll << 31), "paged caches: pages and heads");
   need(cache == PAGED_E4M3 || cache == type, "paged caches: of the projection's type or e4m3");
   need(k.stride(3) == 1 && aligned(k) && aligned(v), "paged caches: contiguous in dim, 16-byte aligned");
+  need(no_grad(k) && no_grad(v), "paged caches: no gradients");
   const int64_t size = k.element_size();
   for (int i = 0; i < 3; ++i) need(k.stride(i) * size % 16 == 0 && k.stride(i) >= 0, "paged caches: strides of whole 16 bytes");
   need(k_scale.has_value() == (cache == PAGED_E4M3) && v_scale.has_value() == (cache == PAGED_E4M3), "k_scale and v_scale: beside e4m3 caches, and only there");
@@ -163,18 +164,22 @@ void bind_paged(py::module_& m) {
          "paged_attention: caches that reach over 2^32 times what divides their strides");
     need(pool.page_size == 1 || pool.pos_stride * k.element_size() <= 1 << 26, "paged_attention: positions of a page at most 64 MB apart");
     auto rows_ok = [&](const at::Tensor& t) { return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned(t); };
+    // rows and heads that do not overlap: one of the two outside the other
+    auto apart = [&](const at::Tensor& t) {
+      const int64_t D = pool.dim, b = B > 1 ? t.stride(0) : INT64_MAX, h = H > 1 ? t.stride(1) : INT64_MAX;
+      if (B <= 1 || H <= 1) return b >= D && h >= D;
+      return (h >= D && b / H >= h) || (b >= D && h / B >= b);
+    };
     need(rows_ok(q), "paged_attention: heads of q contiguous, 16-byte aligned");
     need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B && table.size(1) >= 1 && table.size(1) < (1ll << 31) &&
              (table.size(1) == 1 || table.stride(1) == 1),
          "paged_attention: table [rows, pages of a row] int32 with contiguous rows");
     need(ints(lengths, B), "paged_attention: lengths [rows] int32");
     need(window >= 0, "paged_attention: a window of no or some positions");
-    need(!scale.has_value() || std::isfinite(*scale), "paged_attention: a finite scale");
+    need(!scale.has_value() || std::isfinite((float)*scale), "paged_attention: a finite scale");
     need(no_grad(q), "paged_attention: no gradients");
     if (out.has_value())
-      need(out->scalar_type() == q.scalar_type() && out->sizes() == q.sizes() && rows_ok(*out) && (H == 1 || out->stride(1) >= pool.dim) &&
-               (B <= 1 || out->stride(0) >= pool.dim),
-           "paged_attention: out like q");
+      need(out->scalar_type() == q.scalar_type() && out->sizes() == q.sizes() && rows_ok(*out) && apart(*out), "paged_attention: out like q, its rows apart");
     if (lse.has_value())
       need(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->dim() == 2 && lse->size(0) == B && lse->size(1) == H, "paged_attention: lse [rows, heads] fp32");
     if (workspace.has_value()) need(workspace->is_contiguous() && aligned(*workspace), "paged_attention: 16-byte aligned contiguous workspace");

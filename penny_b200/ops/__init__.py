@@ -19,9 +19,17 @@ from typing import Optional
 
 import torch
 
-from .paged import PagedKVCache, PageStep, page_tables, paged_append, paged_attention  # noqa: F401
-
 _BACKEND = None
+_PAGED = ("PagedKVCache", "PageStep", "page_tables", "paged_append", "paged_attention")
+
+
+def __getattr__(name):
+    # (the paged KV cache needs the extension, the collectives on the gloo backend do not)
+    if name not in _PAGED:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from . import paged
+    globals().update({n: getattr(paged, n) for n in _PAGED})
+    return globals()[name]
 
 
 def init(group=None, heap_bytes: Optional[int] = None, force_cpu: bool = False):

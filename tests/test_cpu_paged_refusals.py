@@ -79,7 +79,10 @@ def _attend(**over):
     (dict(q=torch.zeros(3, 8, 96, dtype=BF), k=torch.zeros(6, 16, 2, 96, dtype=BF)), "dim 64, 128 or 256"), (dict(table=ints(2, 4)), "table"),
     (dict(table=ints(3, 0)), "table"), (dict(table=torch.zeros(3, 4, dtype=torch.int64)), "table"), (dict(table=ints(4, 3).t()), "table"), (dict(lengths=ints(2)), "lengths"),
     (dict(lengths=torch.zeros(3, dtype=torch.int64)), "lengths"), (dict(window=-1), "window"), (dict(scale=float("nan")), "scale"), (dict(out=torch.zeros(3, 8, 64)), "out like q"),
-    (dict(out=torch.zeros(1, 8, 64, dtype=BF).expand(3, 8, 64)), "out like q"), (dict(lse=torch.zeros(3, 8, dtype=BF)), "lse"), (dict(lse=torch.zeros(8, 3).t()), "lse"),
+    (dict(out=torch.zeros(1, 8, 64, dtype=BF).expand(3, 8, 64)), "out like q"), (dict(out=torch.zeros(10 * 64, dtype=BF).as_strided((3, 8, 64), (64, 64, 1))), "apart"),
+    (dict(out=torch.zeros(4000, dtype=BF).as_strided((3, 8, 64), (64 * 7, 64, 1))), "apart"), (dict(scale=1e300), "scale"),
+    (dict(k=torch.zeros(6, 16, 2, 64, dtype=BF, requires_grad=True)), "gradients"), (dict(out=torch.zeros(8, 3, 64, dtype=BF).transpose(0, 1)), "CUDA"),
+    (dict(out=torch.zeros(3, 9, 72, dtype=BF)[:, 1:, :64]), "CUDA"), (dict(lse=torch.zeros(3, 8, dtype=BF)), "lse"), (dict(lse=torch.zeros(8, 3).t()), "lse"),
     (dict(k=torch.zeros(0, 16, 2, 64, dtype=BF)), "pages"), (dict(k=torch.zeros(6, 16, 2, 64, dtype=F8), k_scale=torch.ones(2)), "beside e4m3"),
     (dict(workspace=torch.zeros(65, dtype=torch.uint8)[1:]), "aligned"), (dict(q=torch.zeros(3, 8, 64, dtype=BF, requires_grad=True)), "gradients"), (dict(), "CUDA"),
 ])

@@ -161,6 +161,9 @@ def test_values_without_a_number():
     big["q"] *= 1e30  # past fp16 by far
     out, _ = _run(big, scale=1e-31)
     _check(big, out, _run(big, scale=1e-31)[1], scale=1e-31)
+    big["q"][0, 2, 5] = 3e38  # the largest power of two there is
+    _check(big, *_run(big, scale=1e-41), scale=1e-41)
+    big["q"][0, 2, 5] = 1e30
     big["q"][0, 1] *= 1e-36
     _check(big, *_run(big, scale=1e-31), scale=1e-31)
 
@@ -181,6 +184,44 @@ def test_views_in_place_and_padded(dtype, cache):
     q = c["q"].contiguous()
     c["q"] = q
     assert _run(c, out=q)[0].data_ptr() == q.data_ptr() and torch.equal(q, out)
+
+
+def test_in_place_of_transposed_heads():
+    """out with the heads outside the rows."""
+    c = _case([70, 0, 900], 8, 2, 64, 16, BF, BF, seed=11)
+    out, lse = _run(c)
+    turned = torch.full((8, 3, 64), 3.0, dtype=BF, device="cuda").transpose(0, 1)
+    _run(c, out=turned)
+    assert torch.equal(turned, out)
+
+
+def test_another_order_of_the_same_rows():
+    """Rows in another order, or alone, give what they gave but for where they are cut."""
+    lengths = [900, 1, 0, 333, 5000, 64]
+    c = _case(lengths, 16, 2, 128, 32, BF, E4M3, seed=12)
+    out, lse = _run(c)
+    order = torch.tensor([4, 2, 0, 5, 1, 3], device="cuda")
+    moved = dict(c, q=c["q"][order], table=c["table"][order], lengths=c["lengths"][order])
+    _check(moved, *_run(moved))
+    for b in range(6):
+        alone = dict(c, q=c["q"][b:b + 1], table=c["table"][b:b + 1], lengths=c["lengths"][b:b + 1])
+        _check(alone, *_run(alone))
+
+
+def test_early():
+    """With early set, keys and values of the last positions come from the kernel in front, at every place of a tile."""
+    heads, kv_heads, dim, page = 8, 2, 128, 16
+    for dtype in (BF, HF):
+        c = _case([1, 15, 16, 17, 400, 1000], heads, kv_heads, dim, page, dtype, dtype, seed=13)
+        B = 6
+        last = c["lengths"] - 1
+        slots = c["table"].gather(1, (last // page).long()[:, None])[:, 0].long() * page + last % page
+        for rep in range(3):
+            qkv = torch.randn(B, (heads + 2 * kv_heads) * dim, device="cuda").to(dtype)
+            torch.cuda._sleep(200000)
+            P.paged_append(qkv, c["k"], c["v"], slots, last, heads, 1e4)
+            c["q"] = qkv[:, :heads * dim].unflatten(1, (heads, dim))
+            _check(c, *_run(c, early=True))
 
 
 def test_no_rows():

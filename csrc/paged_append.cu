@@ -9,8 +9,8 @@
 // cosines are computed once and shared by its heads.
 //
 // Bound by memory: every value is read and written once.  A block has a token, a thread two pairs of 16 bytes at a time, the first
-// of which are on their way while the angles are computed.  16384 tokens of 32 + 2 * 8 heads of 128 bf16 values: 75 us, 5.8 TB/s
-// (with the loads behind the angles 88, with four tokens to a block of 448 threads 92); 64 tokens 2.5 us.
+// of which are on their way while the angles are computed.  16384 tokens of 32 + 2 * 8 heads of 128 bf16 values: 71 us, 6.2 TB/s
+// (with the loads behind the angles 88, with four tokens to a block of 448 threads 92); 64 tokens 2.7 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -83,11 +83,11 @@ __device__ __forceinline__ void store8(void* pool, long long at, const float (&x
 
 template <typename T, bool kE4M3>
 __global__ void __launch_bounds__(kMaxThreads) k_paged_append(T* qkv, long long qkv_stride, T* out, long long out_stride, const PagedPool pool,
-                                                              const long long* slots, const int* positions, int heads, int items,
+                                                              const long long* slots, const int* positions, int heads, int items, bool early,
                                                               const paged::PageDiv by_vec, const __grid_constant__ Turns turns) {
   __shared__ float2 s_rot[kMaxHalf];  // cosine, sine: the first pairs of all vectors, the second ones, ... (no two lanes on one bank)
   pdl_launch_dependents();
-  pdl_wait();
+  if (!early) pdl_wait();
   // work items: pairs of 8 values of the q and k heads, then pairs of 8 values of the v heads
   const int half = pool.dim / 2, vecs = half / 8, tid = threadIdx.x, threads = blockDim.x;
   T* const row = qkv + blockIdx.x * qkv_stride;
@@ -107,16 +107,22 @@ __global__ void __launch_bounds__(kMaxThreads) k_paged_append(T* qkv, long long 
       it[u].b = *reinterpret_cast<const uint4*>(x + half);
     }
   };
-  fetch(tid);
+  if (!early) fetch(tid);
   const long long at = paged::place_of_slot(slots[blockIdx.x], pool.pages, pool.page_size, pool.page_stride, pool.pos_stride);
-  if (at < 0) return;
-  for (int d = tid; d < half; d += threads) {
-    const double x = (double)positions[blockIdx.x] * turns.of[d];
-    float sn, cs;
-    sincospif(2.0f * (float)(x - rint(x)), &sn, &cs);
-    s_rot[(d & 7) * vecs + (d >> 3)] = make_float2(cs, sn);
+  if (at >= 0) {
+    for (int d = tid; d < half; d += threads) {
+      const double x = (double)positions[blockIdx.x] * turns.of[d];
+      float sn, cs;
+      sincospif(2.0f * (float)(x - rint(x)), &sn, &cs);
+      s_rot[(d & 7) * vecs + (d >> 3)] = make_float2(cs, sn);
+    }
+  }
+  if (early) {
+    pdl_wait();
+    fetch(tid);
   }
   __syncthreads();
+  if (at < 0) return;
   for (int i0 = tid; i0 < items; i0 += kItems * threads) {
     if (i0 != tid) fetch(i0);
 #pragma unroll
@@ -151,7 +157,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_paged_append(T* qkv, long long 
 
 template <typename T, bool kE4M3>
 cudaError_t launch(void* qkv, long long qkv_stride, void* out, long long out_stride, const PagedPool& pool, const long long* slots,
-                   const int* positions, int tokens, int heads, double theta, cudaStream_t stream) {
+                   const int* positions, int tokens, int heads, double theta, bool early, cudaStream_t stream) {
   Turns turns;
   const double step = std::pow(theta, -2.0 / pool.dim);
   double f = 0.15915494309189533577;  // 1 / (2 pi)
@@ -161,19 +167,19 @@ cudaError_t launch(void* qkv, long long qkv_stride, void* out, long long out_str
   // which an SM holds more (16384 tokens 74 and 76 us)
   const int most = tokens >= 148 * 8 ? 128 : kMaxThreads, threads = std::min(most, (items + 32 * kItems - 1) / (32 * kItems) * 32);
   return launch_kernel_ex(k_paged_append<T, kE4M3>, dim3(tokens), dim3(threads), 0, stream, true, 1, (T*)qkv, qkv_stride, (T*)(out ? out : qkv),
-                          out ? out_stride : qkv_stride, pool, slots, positions, heads, items, paged::page_div(pool.dim / 16), turns);
+                          out ? out_stride : qkv_stride, pool, slots, positions, heads, items, early, paged::page_div(pool.dim / 16), turns);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_append(void* qkv, long long qkv_stride, void* out, long long out_stride, PagedType type, const PagedPool& pool,
                                 PagedType cache, const long long* slots, const int* positions, int tokens, int heads, double theta,
-                                cudaStream_t stream) {
+                                bool early, cudaStream_t stream) {
   if (pool.dim < 16 || pool.dim > 2 * kMaxHalf || pool.dim % 16 != 0 || heads < 0 || pool.heads < 1 || !(theta > 0) || type == PAGED_E4M3 ||
       (cache != PAGED_E4M3 && cache != type))
     return cudaErrorInvalidValue;
   if (tokens < 1) return cudaSuccess;
-#define PENNY_PAGED_APPEND(T, E) launch<T, E>(qkv, qkv_stride, out, out_stride, pool, slots, positions, tokens, heads, theta, stream)
+#define PENNY_PAGED_APPEND(T, E) launch<T, E>(qkv, qkv_stride, out, out_stride, pool, slots, positions, tokens, heads, theta, early, stream)
   if (type == PAGED_BF16)
     return cache == PAGED_E4M3 ? PENNY_PAGED_APPEND(__nv_bfloat16, true) : PENNY_PAGED_APPEND(__nv_bfloat16, false);
   return cache == PAGED_E4M3 ? PENNY_PAGED_APPEND(__half, true) : PENNY_PAGED_APPEND(__half, false);

@@ -22,10 +22,10 @@
 //     16-byte chunk are permuted on both sides of the product.  V's bytes are transposed in pairs by ldmatrix and separated
 //     into even and odd dims.
 //   * P is rounded to the type of the product (bf16: 2^-8 of each weight at most, averaged over the positions; the sum is of the
-//     unrounded ones); q, scores, maxima and sums are not rounded.  Weights count from a base near the maximum so far.  With fp16 it
-//     follows when it is exceeded by 2^8, which is seldom (64 rows of 4096, e4m3, 28 of 2 heads: 34.4 us, always 38.1).  With bf16
-//     it follows always, so that the largest weight is one and not off: 64 rows of 2048 are 0.0018 of the output's norm from 64
-//     bits (its own rounding: 0.0017), otherwise 0.0022 (and 0.5 us faster).
+//     unrounded ones); q, scores, maxima and sums are not rounded.  Weights count from a base near the maximum so far.  Where they are
+//     finer than the output (e4m3 caches with a bf16 q) it follows when it is exceeded by 2^8, which is seldom (64 rows of 4096, 28
+//     of 2 heads: 34.4 us, always 38.1).  Elsewhere it follows always, so that the largest weight is one and not off: 64 rows of 2048,
+//     bf16, are 0.0018 of the output's norm from 64 bits (its own rounding: 0.0017), otherwise 0.0022 (and 0.5 us faster).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   using T2 = typename Pair<T>::type;
   constexpr int kRows = 8 * kBlocks, kSteps = D / 16, kGroups = L::kPos / 16, kStages = L::kStages;
   constexpr bool kBf16 = !kE4M3 && __is_same(T, __nv_bfloat16);
-  constexpr float kSlack = kBf16 ? 0.f : 8.f;
+  constexpr float kSlack = kE4M3 && __is_same(T, __nv_bfloat16) ? 8.f : 0.f;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ float2 s_ml[2][kWarps][kRows];  // of a warp's first part and of its last
   __shared__ int s_head[kWarps];             // a part of a row that began before: 0 none, 1 it ends here, 2 it does not

@@ -115,7 +115,7 @@ void bind_paged(py::module_& m) {
      py::arg("out") = py::none());
   // qkv [tokens, (heads + 2 kv_heads) dim]: q and k rotated in place or into out [tokens, (heads + kv_heads) dim], k and v to their slots.
   m.def("paged_append", [](at::Tensor qkv, at::Tensor k, at::Tensor v, at::Tensor slots, at::Tensor positions, int64_t heads, double theta,
-                           OptTensor out, OptTensor k_scale, OptTensor v_scale) {
+                           OptTensor out, OptTensor k_scale, OptTensor v_scale, bool early) {
     const PagedType type = type_of(qkv, "paged_append: bf16 or fp16 qkv"), cache = type_of(k, "paged_append: bf16, fp16 or e4m3 caches");
     need(type != PAGED_E4M3, "paged_append: bf16 or fp16 qkv");
     const PagedPool pool = pool_of(k, v, type, cache, k_scale, v_scale);
@@ -139,10 +139,10 @@ void bind_paged(py::module_& m) {
     if (k_scale.has_value()) on_device(qkv, {&*k_scale, &*v_scale}, "paged_append expects tensors on one CUDA device");
     const at::cuda::OptionalCUDAGuard guard(qkv.device());
     ck(launch_paged_append(qkv.data_ptr(), qkv.stride(0), out.has_value() ? out->data_ptr() : nullptr, out.has_value() ? out->stride(0) : 0, type, pool,
-                           cache, (const long long*)slots.data_ptr<int64_t>(), positions.data_ptr<int>(), (int)T, (int)heads, theta, cur()),
+                           cache, (const long long*)slots.data_ptr<int64_t>(), positions.data_ptr<int>(), (int)T, (int)heads, theta, early, cur()),
        "paged_append");
   }, py::arg("qkv"), py::arg("k"), py::arg("v"), py::arg("slots"), py::arg("positions"), py::arg("heads"), py::arg("theta"),
-     py::arg("out") = py::none(), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none());
+     py::arg("out") = py::none(), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(), py::arg("early") = false);
   m.def("paged_attention_workspace_bytes", [](int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_len, int64_t window) {
     need(rows >= 1 && kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && dim >= 1 && max_len >= 1 && window >= 0,
          "paged_attention_workspace_bytes: rows, heads and lengths");

@@ -33,10 +33,11 @@ struct PageTables {
 };
 cudaError_t launch_page_tables(const PageTables& a, cudaStream_t stream);
 
-// type: of qkv and out.  out null: in place.
+// type: of qkv and out.  out null: in place.  early: slots and positions are read before the kernels that may still run when this one
+// starts end.
 cudaError_t launch_paged_append(void* qkv, long long qkv_stride, void* out, long long out_stride, PagedType type, const PagedPool& pool,
                                 PagedType cache, const long long* slots, const int* positions, int tokens, int heads, double theta,
-                                cudaStream_t stream);
+                                bool early, cudaStream_t stream);
 
 struct PagedAttention {
   const void* q;  // [rows, heads, dim]

@@ -372,7 +372,7 @@ class LlamaTPDecoder:
             return
         heads = (self.Hq, self.cfg.head_dim)
         # (early: the tables are complete since the launch without programmatic dependency at the step's start)
-        self.paged.append(li, self.qkv, self.page_step, self.Hq, theta)
+        self.paged.append(li, self.qkv, self.page_step, self.Hq, theta, early=True)
         self.paged.attend(li, self.qkv[:, :self.Hq * self.cfg.head_dim].unflatten(1, heads), out=self.attn.unflatten(1, heads), scale=self.scale,
                           workspace=self.page_workspace, early=True)
 

@@ -45,13 +45,13 @@ def page_tables(table, lengths, free, free_count, new, page_size: int, tokens: i
     return PageStep._make(ops.page_tables(table, lengths, free, free_count, new, page_size, tokens, out))
 
 
-def paged_append(qkv, k, v, slots, positions, heads: int, theta: float, out=None, k_scale=None, v_scale=None) -> None:
+def paged_append(qkv, k, v, slots, positions, heads: int, theta: float, out=None, k_scale=None, v_scale=None, early: bool = False) -> None:
     """Rotates q and k of every token of qkv [tokens, (heads + 2 kv_heads) dim] (rotate-half form, in place or into out
     [tokens, (heads + kv_heads) dim]) and stores the rotated k and v at the tokens' slots of the pools k, v [pages, page_size,
     kv_heads, dim].  A token whose slot the pool does not have (-1) is left alone, its row of out too; no two tokens have the
     same slot.  Pools of qkv's type, or e4m3: value / k_scale[head] (v_scale), saturated at 448.  Any strides of whole 16 bytes;
-    dim a multiple of 16, up to 256.  out and qkv do not overlap."""
-    ops.paged_append(qkv, k, v, slots, positions, heads, theta, out, k_scale, v_scale)
+    dim a multiple of 16, up to 256.  out and qkv do not overlap.  early: as in `paged_attention`, for slots and positions."""
+    ops.paged_append(qkv, k, v, slots, positions, heads, theta, out, k_scale, v_scale, early)
 
 
 def paged_attention(q, k, v, table, lengths, out=None, lse=None, scale: Optional[float] = None, window: int = 0, k_scale=None, v_scale=None,
@@ -113,9 +113,11 @@ class PagedKVCache:
         """`page_tables` on this cache: new[r] tokens come to row r or its last -new[r] leave (-lengths[r]: the row is free)."""
         return page_tables(self.table, self.lengths, self.free, self.free_count, new, self.page_size, tokens, out)
 
-    def append(self, layer: int, qkv: torch.Tensor, step: PageStep, heads: int, theta: float, out: Optional[torch.Tensor] = None) -> None:
+    def append(self, layer: int, qkv: torch.Tensor, step: PageStep, heads: int, theta: float, out: Optional[torch.Tensor] = None,
+               early: bool = False) -> None:
         """`paged_append` to this cache's `layer` at the step's slots and positions."""
-        paged_append(qkv, self.k[layer], self.v[layer], step.slots, step.positions, heads, theta, out, self.k_scale[layer], self.v_scale[layer])
+        paged_append(qkv, self.k[layer], self.v[layer], step.slots, step.positions, heads, theta, out, self.k_scale[layer], self.v_scale[layer],
+                     early)
 
     def attend(self, layer: int, q: torch.Tensor, out=None, lse=None, scale: Optional[float] = None, window: int = 0, workspace=None,
                early: bool = False) -> torch.Tensor:

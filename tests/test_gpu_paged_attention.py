@@ -219,7 +219,7 @@ def test_early():
         for rep in range(3):
             qkv = torch.randn(B, (heads + 2 * kv_heads) * dim, device="cuda").to(dtype)
             torch.cuda._sleep(200000)
-            P.paged_append(qkv, c["k"], c["v"], slots, last, heads, 1e4)
+            P.paged_append(qkv, c["k"], c["v"], slots, last, heads, 1e4, early=rep > 0)
             c["q"] = qkv[:, :heads * dim].unflatten(1, (heads, dim))
             _check(c, *_run(c, early=True))
 

@@ -10,15 +10,17 @@
 //     CTAs), and P^T is S^T's accumulators, transposed in registers.  (The 128 rows of a tcgen05 tile would be empty; the bound is
 //     the cache's stream.)
 //   * All warps of the GPU get an equal share of the batch: for every head group the tiles (4 KB of K and 4 KB of V: 16 positions
-//     of 128 bf16 values) of all rows in a line, cut every `share` tiles (paged_plan.h; every CTA sums over the lengths by
+//     of 128 bf16 values) of all rows in a line, cut every `share` tiles (paged_plan.h; every warp sums over the lengths by
 //     itself).  A warp walks its part of the line with a private three-stage cp.async pipeline that does not drain between
-//     rows.  A lane looks up one position's page a tile ahead, so any page size and any strides will do; what lies outside
-//     a row is filled with zeros and never read (stale rows may hold anything).
+//     rows (a CTA for each piece of a row instead took 48 us for 26 at rows of up to 1000 positions of 20 heads of 64).  64 entries
+//     of the row's table stand in the lanes' registers; sixteen positions on one page take one of them, others one each, so
+//     any page size and any strides will do.  What lies outside a row is filled with zeros and never read (stale rows may
+//     hold anything).
 //   * A row that lies in one warp's part is finished from its registers, the parts of one that spans warps of a CTA
 //     meet in shared memory, those of several CTAs in a workspace, which a second kernel joins.  No counters: a workspace
 //     holds nothing between calls.
 //   * e4m3 caches: fp16 is exact for them, so they meet q as fp16, each row of q divided by the power of two of its
-//     largest value (exact; the score's factor takes it back).  A lane's four bytes of K are two adjacent pairs: the dims inside a
+//     largest value (exact, but values under 2^-14 of that keep 2^-25 of it; the score's factor takes it back).  A lane's four bytes of K are two adjacent pairs: the dims inside a
 //     16-byte chunk are permuted on both sides of the product.  V's bytes are transposed in pairs by ldmatrix and separated
 //     into even and odd dims.
 //   * P is rounded to the type of the product (bf16: 2^-8 of each weight at most, averaged over the positions; the sum is of the

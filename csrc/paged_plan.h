@@ -25,12 +25,8 @@ PENNY_ATTN_HD int div_page(const PageDiv& d, int n) { return (int)(((uint64_t)(u
 // pages that hold n positions
 PENNY_ATTN_HD int pages_of(const PageDiv& d, int n) { return n > 0 ? div_page(d, n - 1) + 1 : 0; }
 
-// Where position `pos` lies, in units of the steps, if its page is one of the pool's; -1 if not.  (A table is the caller's memory on
-// the device: what it says is looked at, never trusted.)
-PENNY_ATTN_HD long long place_of(int page, int pages, int pos, const PageDiv& d, long long page_step, long long pos_step) {
-  return (uint32_t)page < (uint32_t)pages ? page * page_step + (pos - div_page(d, pos) * (int)d.size) * pos_step : -1;
-}
-// The same for a slot.
+// Where a slot lies, in units of the steps, if it is one of the pool's; -1 if not.  (Slots and tables are the caller's memory on the
+// device: what they say is looked at, never trusted.)
 PENNY_ATTN_HD long long place_of_slot(long long slot, int pages, int page_size, long long page_step, long long pos_step) {
   if (slot < 0 || slot >= (long long)pages * page_size) return -1;
   const long long page = slot / page_size;
@@ -48,9 +44,10 @@ PENNY_ATTN_HD Seen seen_of(int length, int max_len, int window) {
 }
 
 // How a batch is shared out.  A row's (KV head, head group) pairs are its items; a team is one CTA for each item, so that a page's
-// heads are read at about the same time (apart from each other 64 rows of 16000 positions took 632 us instead of 607).  The
-// rows lie in a line, each a unit for its start (its output, its q) and one for every tile of positions; every warp of a
-// team's CTAs gets `share` units, at least kMinShare.  The lengths are on the device, and every CTA sums over them by itself.
+// heads are read at about the same time (apart from each other 64 rows of 16000 positions, e4m3, took 389 us instead of 340).  The
+// rows lie in a line, each kStart units for its start (q on the way in, the output) and one for every tile of positions, an empty
+// one a single unit; every warp of a team's CTAs gets `share` units, at least kMinShare (4 / 5 / 6: 3 rows of 300 positions 8.2 / 8.9 /
+// 9.7 us).  The lengths are on the device, and every warp sums over them by itself.
 // kStart: 96 rows of 1 to 8192 positions, e4m3, in 49.3 / 45.4 / 43.9 / 43.0 us with 1 / 2 / 3 / 5; 256 of 100 25.5 / 27.3 / 27.0 / 25.0.
 constexpr int kMinShare = 4, kStart = 3;
 constexpr long long kMaxLen = 0x7fff0000, kMaxUnits = 1ll << 30;  // (all rows' units, and a share more, fit 32 bits)
@@ -130,7 +127,7 @@ inline Steps steps_of(long long pages, long long page_size, long long page_strid
   return {(uint32_t)page, (uint32_t)pos, bytes};
 }
 constexpr uint32_t kNoStep = 0xffffffffu;
-// place_of in such units; kNoStep: the pool does not have the page.
+// Where position `pos` lies, in such units, if its page is one of the pool's; kNoStep if not.
 PENNY_ATTN_HD uint32_t step_of(int page, int pages, int pos, const PageDiv& d, uint32_t page_step, uint32_t pos_step) {
   return (uint32_t)page < (uint32_t)pages ? (uint32_t)page * page_step + (uint32_t)(pos - div_page(d, pos) * (int)d.size) * pos_step : kNoStep;
 }

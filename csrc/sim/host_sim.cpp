@@ -369,9 +369,6 @@ int penny_decode_attn_cut(const int* positions, int B, int Hkv, int max_len, int
 // The paged KV cache's index arithmetic (paged_plan.h).
 int penny_page_div(int size, int n) { return penny::paged::div_page(penny::paged::page_div(size), n); }
 int penny_pages_of(int size, int n) { return penny::paged::pages_of(penny::paged::page_div(size), n); }
-long long penny_page_place(int page, int pages, int pos, int size, long long page_step, long long pos_step) {
-  return penny::paged::place_of(page, pages, pos, penny::paged::page_div(size), page_step, pos_step);
-}
 long long penny_page_place_of_slot(long long slot, int pages, int size, long long page_step, long long pos_step) {
   return penny::paged::place_of_slot(slot, pages, size, page_step, pos_step);
 }

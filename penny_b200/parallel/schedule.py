@@ -161,15 +161,8 @@ def pages_of(page_size: int, length: int) -> int:
     return sim_lib().penny_pages_of(page_size, length)
 
 
-def page_place(page: int, pages: int, position: int, page_size: int, page_step: int, position_step: int) -> int:
-    """Where a position lies in a pool, -1 if the pool does not have its page (csrc/paged_plan.h)."""
-    f = sim_lib().penny_page_place
-    f.restype, f.argtypes = ctypes.c_longlong, [ctypes.c_int] * 4 + [ctypes.c_longlong] * 2
-    return f(page, pages, position, page_size, page_step, position_step)
-
-
 def slot_place(slot: int, pages: int, page_size: int, page_step: int, position_step: int) -> int:
-    """The same for a slot."""
+    """Where a slot lies in a pool, -1 if the pool does not have it (csrc/paged_plan.h)."""
     f = sim_lib().penny_page_place_of_slot
     f.restype, f.argtypes = ctypes.c_longlong, [ctypes.c_longlong] + [ctypes.c_int] * 2 + [ctypes.c_longlong] * 2
     return f(slot, pages, page_size, page_step, position_step)
@@ -185,7 +178,7 @@ def page_steps(pages: int, page_size: int, page_stride: int, position_stride: in
 
 
 def page_step_of(page: int, pages: int, position: int, page_size: int, page_step: int, position_step: int):
-    """page_place in such units; None for a page that the pool does not have."""
+    """Where a position lies in a pool, in such units; None for a page that the pool does not have."""
     f = sim_lib().penny_page_step_of
     f.restype, f.argtypes = ctypes.c_uint32, [ctypes.c_int] * 4 + [ctypes.c_uint32] * 2
     at = f(page, pages, position, page_size, page_step, position_step)

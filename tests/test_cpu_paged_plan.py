@@ -18,13 +18,7 @@ def test_page_of_a_position(size):
             assert schedule.pages_of(size, n) == max(0, -(-n // size))
 
 
-def test_places_of_bad_pages_and_slots():
-    place = schedule.page_place
-    assert place(3, 4, 50, 16, 1000, 10) == 3 * 1000 + 2 * 10
-    for page in (-1, 4, 5, -2 ** 31, 2 ** 31 - 1):
-        assert place(page, 4, 50, 16, 1000, 10) == -1
-    # offsets past 32 bits
-    assert place(2 ** 21, 2 ** 21 + 1, 7, 16, 16 * 8 * 128 * 2, 8 * 128 * 2) == 2 ** 21 * 2 ** 15 + 7 * 2 ** 11
+def test_places_of_bad_slots():
     at = schedule.slot_place
     assert at(3 * 24 + 5, 4, 24, 1000, 10) == 3050 and at(4 * 24 - 1, 4, 24, 1000, 10) == 3230
     for slot in (-1, -2 ** 63, 4 * 24, 2 ** 63 - 1, 2 ** 32):
@@ -41,7 +35,7 @@ def test_steps(pages, page, page_stride, pos_stride, size):
     for pg in {0, pages - 1, rng.randrange(pages)}:
         for pos in (0, page - 1, 3 * page + page // 2):
             at = schedule.page_step_of(pg, pages, pos, page, a, b)
-            assert at * unit == schedule.page_place(pg, pages, pos, page, page_stride * size, pos_stride * size)
+            assert at * unit == (pg * page_stride + pos % page * pos_stride) * size
     for pg in (-1, pages, 2 ** 31 - 1, -2 ** 31):
         assert schedule.page_step_of(pg, pages, 0, page, a, b) is None
 

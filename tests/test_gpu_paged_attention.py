@@ -93,7 +93,7 @@ def test_lengths(dtype, cache, dim, heads, kv_heads, page):
 
 @pytest.mark.parametrize("dtype,cache", [(BF, BF), (HF, E4M3)])
 @pytest.mark.parametrize("lengths,heads,kv_heads", [([20000], 4, 1), ([4111, 9], 8, 2), ([70001], 2, 1), ([255, 256, 511, 512, 0, 2600], 16, 1),
-                                                    ([1, 7000] + [40] * 130, 8, 2), ([600] * 300, 8, 8), ([0, 0], 4, 2)])
+                                                    ([1, 7000] + [40] * 130, 8, 2), ([600] * 300, 8, 8), ([0, 0], 4, 2), ([7, 0, 30] * 1500, 2, 1)])
 def test_pieces(dtype, cache, lengths, heads, kv_heads):
     """Rows that are cut into many pieces, one long row among short ones, more rows than a block has threads, whole rows."""
     c = _case(lengths, heads, kv_heads, 128, 16, dtype, cache, seed=1)

@@ -388,10 +388,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
       for (int k = 0; k < kSteps; ++k) o[nb][k][0] = o[nb][k][1] = o[nb][k][2] = o[nb][k][3] = 0.f;
     }
     for (int j = 0; j < n; ++j) {
-      __syncwarp();  // everyone is done with the stage that the next tile overwrites
-      masks[kStages - 1] = issue();
-      cp_async_wait<kStages - 1>();
-      __syncwarp();
+      cp_async_wait<kStages - 2>();
+      __syncwarp();  // all of the tile is there, and everyone is done with the stage that the next request overwrites
       const uint32_t sb = wbase + stage_out * L::kStage;
       stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1;
       // ---- S^T = K Q^T, 16 positions at a time: this thread holds positions g and g + 8 of heads 2 t and 2 t + 1 ----
@@ -428,6 +426,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
           for (int u = 0; u < 4; ++u) s[nb][c][u] += odd[nb][u];
         }
       }
+      masks[kStages - 1] = issue();  // (its instructions fill the wait for the products)
       // ---- weights exp2(score - base); the base goes up to the maximum when a score of the tile is above it by more than kSlack ----
       uint32_t pb[kBlocks][kGroups][2];
 #pragma unroll

@@ -23,7 +23,7 @@ namespace penny {
 namespace {
 using namespace paged;
 
-constexpr int kTokensPerThread = 4, kCluster = 8;
+constexpr int kTokensPerThread = 4;
 static_assert(kPagedMaxRows <= 8 * 1024, "rows of a thread");
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -212,19 +212,36 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
   }
 }
 
+// CTAs of a cluster for many rows or tokens: sixteen where the device has room for one such cluster, else the eight that all have.
+int cluster_of(const void* kernel) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, int> done;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = done[{dev, kernel}];
+  if (n == 0) {
+    const bool may = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+    if (!may) (void)cudaGetLastError();
+    n = may && max_clusters(kernel, 16, 1024, kPagedMaxRows * 4 * sizeof(int)) > 0 ? 16 : 8;
+  }
+  return n;
+}
+
 }  // namespace
 
 cudaError_t launch_page_tables(const PageTables& a, cudaStream_t stream) {
   if (a.rows < 1 || a.rows > kPagedMaxRows || a.width < 1 || a.page_size < 1 || a.pages < 1 || a.tokens < 0) return cudaErrorInvalidValue;
   const size_t smem = (size_t)a.rows * 4 * sizeof(int);
   // One CTA for a decode step (64 rows: 3.9 us); a cluster where tokens or pages of many rows are to be written (4000 rows, 125,000
-  // tokens in 15,000 pages: of eight CTAs 13 us, one 50).
-  const int threads = a.rows <= 256 && a.tokens <= 1024 ? 256 : 1024, cluster = a.tokens <= 4096 && a.rows <= 1024 ? 1 : kCluster;
+  // tokens in 15,000 pages, there and back: of eight CTAs 23.0 us, of sixteen 19.9).
+  const int threads = a.rows <= 256 && a.tokens <= 1024 ? 256 : 1024, big = a.tokens > 4096 || a.rows > 1024;
   const int per = (a.rows + threads - 1) / threads;
 #define PENNY_PAGE_TABLES(N)                                                                                                          \
   do {                                                                                                                                \
     const cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(k_page_tables<N>), kPagedMaxRows * 4 * (int)sizeof(int)).rc;     \
     if (rc != cudaSuccess) return rc;                                                                                                 \
+    const int cluster = big ? cluster_of(reinterpret_cast<const void*>(k_page_tables<N>)) : 1;                                         \
     return launch_kernel_ex(k_page_tables<N>, dim3(cluster), dim3(threads), smem, stream, true, cluster, a, page_div(a.page_size),     \
                             cluster);                                                                                                 \
   } while (0)

@@ -76,13 +76,27 @@ __device__ __forceinline__ int row_at(const int* at, int rows, int x) {
   return lo;
 }
 
+// Values of a thread's rows to shared memory.
+template <int kPer>
+__device__ __forceinline__ void put(int* to, int r0, int rows, const int (&v)[kPer]) {
+#pragma unroll
+  for (int i = 0; i < kPer; i += 4) {
+    if constexpr (kPer % 4 == 0) {
+      if (r0 + i < rows) *reinterpret_cast<int4*>(to + r0 + i) = make_int4(v[i], v[i + 1], v[i + 2], v[i + 3]);  // (up to three behind the last)
+    } else {
+      if (r0 + i < rows) to[r0 + i] = v[i];
+    }
+  }
+}
+
 // kPer: rows of a thread, one behind the other.
 template <int kPer>
 __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const PageDiv div, int cluster) {
   extern __shared__ int smem[];
   // per row: where its tokens begin, its length (-1 - length: not granted), its first new page's number among all new
   // ones, its first released page's among all released
-  int *s_off = smem, *s_old = s_off + a.rows, *s_new = s_old + a.rows, *s_gone = s_new + a.rows;
+  const int stride = (a.rows + 3) / 4 * 4;
+  int *s_off = smem, *s_old = s_off + stride, *s_new = s_old + stride, *s_gone = s_new + stride;
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, rank = blockIdx.x;
@@ -112,13 +126,11 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
   const uint32_t pages_there = (uint32_t)(count + pushed);
   uint32_t end = sums[0], gone = sums[1], need[1] = {0}, all_need[1];
   bool granted[kPer];
+  int first_token[kPer], first_gone[kPer], first_new[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    if (r0 + i < a.rows) {
-      s_off[r0 + i] = (int)end;
-      s_gone[r0 + i] = (int)gone;
-    }
-    if (rank == 0 && r0 + i < a.rows) a.offsets[r0 + i] = (int)end;
+    first_token[i] = (int)end;
+    first_gone[i] = (int)gone;
     end = add(end, max(0, n[i]));
     gone = add(gone, gone_of(old[i], n[i]));
     granted[i] = n[i] <= 0 || (old[i] + (long long)n[i] <= most && end <= (uint32_t)a.tokens);
@@ -128,7 +140,7 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
   uint32_t taken = need[0], last = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const uint32_t first = taken;
+    first_new[i] = (int)taken;
     if (n[i] > 0 && granted[i]) {
       const int pages = pages_of(div, old[i] + n[i]) - pages_of(div, old[i]);
       taken = add(taken, pages);
@@ -136,28 +148,32 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
       granted[i] = pages == 0 || taken <= pages_there;
       if (granted[i] && pages > 0) last = taken;
     }
-    if (r0 + i < a.rows) {
-      s_new[r0 + i] = (int)first;
-      s_old[r0 + i] = granted[i] ? old[i] : -1 - old[i];
-    }
   }
+  int kept[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) kept[i] = granted[i] ? old[i] : -1 - old[i];
+  put<kPer>(s_off, r0, a.rows, first_token);
+  put<kPer>(s_old, r0, a.rows, kept);
+  put<kPer>(s_new, r0, a.rows, first_new);
+  put<kPer>(s_gone, r0, a.rows, first_gone);
   last = __reduce_max_sync(0xffffffffu, last);
   if ((tid & 31) == 0 && last > 0) atomicMax(&s_popped, last);
   if (cluster > 1) cluster_barrier();
   else __syncthreads();
 
   // ---- the rows' own state, from here on nobody reads it ----
-  if (rank == 0) {
+  if ((tid >> 5) % cluster == rank) {  // (every CTA has all rows: each writes its warps' part)
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       if (r0 + i >= a.rows) break;
       a.granted[r0 + i] = granted[i];
+      a.offsets[r0 + i] = first_token[i];
       a.lengths[r0 + i] = granted[i] ? (int)max(0ll, (long long)old[i] + n[i]) : old[i];
     }
-    if (tid == 0) {
-      a.offsets[a.rows] = (int)totals[0];
-      *a.free_count = count + pushed - (int)s_popped;
-    }
+  }
+  if (rank == 0 && tid == 0) {
+    a.offsets[a.rows] = (int)totals[0];
+    *a.free_count = count + pushed - (int)s_popped;
   }
 
   // k-th released page, rows and pages ascending
@@ -174,37 +190,47 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
   for (int k = me; k < pushed; k += threads) a.free_pages[count + pushed - 1 - k] = released(k);
 
   const int total = (int)min(totals[0], (uint32_t)a.tokens);
-  for (long long j0 = (long long)me * kTokensPerThread; j0 < a.tokens; j0 += (long long)threads * kTokensPerThread) {
-    long long slot[kTokensPerThread];
-    int pos[kTokensPerThread];
-    int r = j0 < total ? row_at(s_off, a.rows, (int)j0) : a.rows, page = -1, page_at = -1;
+  // a token to a thread, or four where there are more than threads; their pages are read at the same time
+  const int each = a.tokens <= threads ? 1 : kTokensPerThread;
+  for (long long j0 = (long long)me * each; j0 < a.tokens; j0 += (long long)threads * each) {
+    int row[kTokensPerThread], pos[kTokensPerThread], at[kTokensPerThread], page[kTokensPerThread];
+    bool fresh[kTokensPerThread];
+    int r = j0 < total ? row_at(s_off, a.rows, (int)j0) : a.rows;
 #pragma unroll
     for (int i = 0; i < kTokensPerThread; ++i) {
       const int j = (int)j0 + i;
-      slot[i] = -1;
+      row[i] = -1;
       pos[i] = 0;
-      if (j >= total) continue;
-      while (r + 1 < a.rows && s_off[r + 1] <= j) {
-        ++r;
-        page_at = -1;
-      }
-      const int old = s_old[r];
-      if (old < 0) continue;
-      const int p = old + (j - s_off[r]), at = div_page(div, p), held = pages_of(div, old);
-      if (at != page_at) {
-        page_at = at;
-        page = at < held ? a.table[r * a.table_stride + at] : new_page(s_new[r] + at - held);
-      }
-      if (at >= held && p - at * a.page_size == 0) a.table[r * a.table_stride + at] = page;
-      pos[i] = p;
-      if (page >= 0 && page < a.pages) slot[i] = (long long)page * a.page_size + (p - at * a.page_size);
+      if (i >= each || j >= total) continue;
+      while (r + 1 < a.rows && s_off[r + 1] <= j) ++r;
+      const int had = s_old[r];
+      if (had < 0) continue;
+      row[i] = r;
+      pos[i] = had + (j - s_off[r]);
+      at[i] = div_page(div, pos[i]);
+      page[i] = at[i] - pages_of(div, had);  // of the row's new pages; below zero: one that it had
+      fresh[i] = page[i] >= 0;
     }
-    if (j0 + kTokensPerThread <= a.tokens) {
+#pragma unroll
+    for (int i = 0; i < kTokensPerThread; ++i)
+      if (row[i] >= 0) page[i] = fresh[i] ? new_page(s_new[row[i]] + page[i]) : a.table[row[i] * a.table_stride + at[i]];
+    long long slot[kTokensPerThread];
+#pragma unroll
+    for (int i = 0; i < kTokensPerThread; ++i) {
+      slot[i] = -1;
+      if (row[i] < 0) continue;
+      const int within = pos[i] - at[i] * a.page_size;
+      if (fresh[i] && within == 0) a.table[row[i] * a.table_stride + at[i]] = page[i];
+      if (page[i] >= 0 && page[i] < a.pages) slot[i] = (long long)page[i] * a.page_size + within;
+    }
+    if (each == kTokensPerThread && j0 + kTokensPerThread <= a.tokens) {
 #pragma unroll
       for (int i = 0; i < kTokensPerThread; i += 2) *reinterpret_cast<longlong2*>(a.slots + j0 + i) = make_longlong2(slot[i], slot[i + 1]);
       *reinterpret_cast<int4*>(a.positions + j0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
     } else {
-      for (int i = 0; i < kTokensPerThread && j0 + i < a.tokens; ++i) {
+#pragma unroll
+      for (int i = 0; i < kTokensPerThread; ++i) {
+        if (i >= each || j0 + i >= a.tokens) break;
         a.slots[j0 + i] = slot[i];
         a.positions[j0 + i] = pos[i];
       }
@@ -232,7 +258,7 @@ int cluster_of(const void* kernel) {
 
 cudaError_t launch_page_tables(const PageTables& a, cudaStream_t stream) {
   if (a.rows < 1 || a.rows > kPagedMaxRows || a.width < 1 || a.page_size < 1 || a.pages < 1 || a.tokens < 0) return cudaErrorInvalidValue;
-  const size_t smem = (size_t)a.rows * 4 * sizeof(int);
+  const size_t smem = (size_t)(a.rows + 3) / 4 * 16 * sizeof(int);
   // One CTA for a decode step (64 rows: 3.9 us); a cluster where tokens or pages of many rows are to be written (4000 rows, 125,000
   // tokens in 15,000 pages, there and back: of eight CTAs 23.0 us, of sixteen 19.9).
   const int threads = a.rows <= 256 && a.tokens <= 1024 ? 256 : 1024, big = a.tokens > 4096 || a.rows > 1024;

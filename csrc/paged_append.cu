@@ -9,7 +9,7 @@
 // cosines are computed once and shared by its heads.
 //
 // Bound by memory: every value is read and written once.  A block has a token, a thread two pairs of 16 bytes at a time, the first
-// of which are on their way while the angles are computed.  16384 tokens of 32 + 2 * 8 heads of 128 bf16 values: 71 us, 6.2 TB/s
+// of which are on their way while the angles are computed.  16384 tokens of 32 + 2 * 8 heads of 128 bf16 values: 72 us, 6.1 TB/s
 // (with the loads behind the angles 88, with four tokens to a block of 448 threads 92); 64 tokens 2.7 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -35,16 +35,20 @@ PagedType type_of(const at::Tensor& t, const char* msg) {
 
 // k and v as a pool, with the scales that its type needs.
 PagedPool pool_of(const at::Tensor& k, const at::Tensor& v, PagedType type, PagedType cache, const OptTensor& k_scale, const OptTensor& v_scale) {
-  need(k.dim() == 4 && v.sizes() == k.sizes() && v.strides() == k.strides() && v.scalar_type() == k.scalar_type(),
-       "paged caches: k and v [pages, page_size, kv_heads, dim] of one type, shape and strides");
+  // (the stride of a dimension of one says nothing)
+  bool alike = k.dim() == 4 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type();
+  for (int i = 0; alike && i < 4; ++i) alike = k.size(i) <= 1 || k.stride(i) == v.stride(i);
+  need(alike, "paged caches: k and v [pages, page_size, kv_heads, dim] of one type, shape and strides");
   need(k.size(0) >= 1 && k.size(1) >= 1 && k.size(2) >= 1 && k.size(0) < (1ll << 31) && k.size(1) < (1ll << 31), "paged caches: pages and heads");
   need(cache == PAGED_E4M3 || cache == type, "paged caches: of the projection's type or e4m3");
   need(k.stride(3) == 1 && aligned(k) && aligned(v), "paged caches: contiguous in dim, 16-byte aligned");
   need(no_grad(k) && no_grad(v), "paged caches: no gradients");
   const int64_t size = k.element_size();
-  for (int i = 0; i < 3; ++i) need(k.stride(i) * size % 16 == 0 && k.stride(i) >= 0, "paged caches: strides of whole 16 bytes");
+  for (int i = 0; i < 3; ++i)
+    need(k.size(i) == 1 || (k.stride(i) * size % 16 == 0 && k.stride(i) >= 0), "paged caches: strides of whole 16 bytes");
   need(k_scale.has_value() == (cache == PAGED_E4M3) && v_scale.has_value() == (cache == PAGED_E4M3), "k_scale and v_scale: beside e4m3 caches, and only there");
-  PagedPool p = {k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), nullptr, nullptr,
+  auto stride = [&](int i) -> long long { return k.size(i) == 1 ? 0 : k.stride(i); };
+  PagedPool p = {k.data_ptr(), v.data_ptr(), stride(0), stride(1), stride(2), nullptr, nullptr,
                  (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)k.size(3)};
   if (cache == PAGED_E4M3) {
     for (const at::Tensor* s : {&*k_scale, &*v_scale})
@@ -124,7 +128,7 @@ void bind_paged(py::module_& m) {
     need(D % 16 == 0 && D >= 16 && D <= 256, "paged_append: dim a multiple of 16, up to 256");
     need(heads >= 0 && heads < (1 << 20) && qkv.dim() == 2 && qkv.size(1) == (heads + 2 * pool.heads) * D && T < (1ll << 31),
          "paged_append: qkv must be [tokens, (heads + 2 kv_heads) dim]");
-    need(qkv.stride(1) == 1 && (T <= 1 || qkv.stride(0) >= qkv.size(1)) && qkv.stride(0) % 8 == 0 && aligned(qkv),
+    need(qkv.stride(1) == 1 && (T <= 1 || (qkv.stride(0) >= qkv.size(1) && qkv.stride(0) % 8 == 0)) && aligned(qkv),
          "paged_append: rows of qkv contiguous, 16-byte aligned");
     need(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.dim() == 1 && slots.numel() == T && ints(positions, T),
          "paged_append: slots [tokens] int64, positions [tokens] int32");
@@ -132,7 +136,7 @@ void bind_paged(py::module_& m) {
     need(no_grad(qkv), "paged_append: no gradients");
     if (out.has_value())
       need(out->scalar_type() == qkv.scalar_type() && out->dim() == 2 && out->size(0) == T && out->size(1) == (heads + pool.heads) * D &&
-               out->stride(1) == 1 && (T <= 1 || out->stride(0) >= out->size(1)) && out->stride(0) % 8 == 0 && aligned(*out),
+               out->stride(1) == 1 && (T <= 1 || (out->stride(0) >= out->size(1) && out->stride(0) % 8 == 0)) && aligned(*out),
            "paged_append: out must be [tokens, (heads + kv_heads) dim], like qkv");
     on_device(qkv, {&k, &v, &slots, &positions}, "paged_append expects tensors on one CUDA device");
     if (out.has_value()) on_device(qkv, {&*out}, "paged_append expects tensors on one CUDA device");
@@ -163,7 +167,9 @@ void bind_paged(py::module_& m) {
     need(paged::steps_of(pool.pages, pool.page_size, pool.page_stride, pool.pos_stride, (int)k.element_size()).bytes > 0,
          "paged_attention: caches that reach over 2^32 times what divides their strides");
     need(pool.page_size == 1 || pool.pos_stride * k.element_size() <= 1 << 26, "paged_attention: positions of a page at most 64 MB apart");
-    auto rows_ok = [&](const at::Tensor& t) { return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned(t); };
+    auto rows_ok = [&](const at::Tensor& t) {
+      return t.stride(2) == 1 && (B <= 1 || t.stride(0) % 8 == 0) && (H == 1 || t.stride(1) % 8 == 0) && aligned(t);
+    };
     // rows and heads that do not overlap: one of the two outside the other
     auto apart = [&](const at::Tensor& t) {
       const int64_t D = pool.dim, b = B > 1 ? t.stride(0) : INT64_MAX, h = H > 1 ? t.stride(1) : INT64_MAX;

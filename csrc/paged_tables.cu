@@ -27,7 +27,7 @@ constexpr int kTokensPerThread = 4;
 static_assert(kPagedMaxRows <= 8 * 1024, "rows of a thread");
 
 __device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Sums hold at 2^31 - 1 (of terms that do so themselves: in any order the same).

@@ -195,6 +195,25 @@ def test_in_place_of_transposed_heads():
     assert torch.equal(turned, out)
 
 
+def test_strides_of_single_rows_heads_and_pages():
+    """What the strides of a dimension of one say does not count: of one row, one head, one KV head, one page, pages of one position."""
+    odd = lambda t, dims: t.as_strided(t.shape, [3 if i in dims else s for i, s in enumerate(t.stride())])  # noqa: E731
+    c = _case([300], 1, 1, 64, 16, BF, BF, seed=14)
+    out, lse = _run(c)
+    d = dict(c, q=odd(c["q"].contiguous(), (0, 1)), k=odd(c["k"], (2,)))
+    got, lse2 = _run(d)
+    assert torch.equal(got, out) and torch.equal(lse, lse2)
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    one = dict(q=c["q"], k=odd(c["k"][:1], (0, 2)), v=c["v"][:1].nan_to_num(), table=table, lengths=torch.tensor([1], dtype=torch.int32, device="cuda"))
+    one["k"] = one["k"].nan_to_num()
+    _check(one, *_run(one))
+    c = _case([40, 7], 4, 2, 128, 1, HF, E4M3, seed=15)
+    d = dict(c, k=odd(c["k"], (1,)))
+    out, lse = _run(c)
+    assert torch.equal(_run(d)[0], out)
+    _check(c, out, lse)
+
+
 def test_another_order_of_the_same_rows():
     """Rows in another order, or alone, give what they gave but for where they are cut."""
     lengths = [900, 1, 0, 333, 5000, 64]

@@ -1,4 +1,5 @@
-// Attention of one new token per sequence over a paged KV cache.
+// Attention of one new token per sequence over a paged KV cache.  (The attention over contiguous caches, csrc/decode_attention_fused.cu,
+// rotates and appends its token itself; here csrc/paged_append.cu has done that.)
 //
 //   o[b, h] = sum_j softmax_j(scale * q[b, h] . K_j) V_j,  j in the last `window` of lengths[b] positions (all without one),
 // position j in the pool's page table[b, j / page_size] at j % page_size.  One pass over K and V with a running maximum and sum
@@ -64,8 +65,8 @@ struct Tile {
   static constexpr int kFrags = kBlocks * (D / 16);            // MMA accumulators of O^T: 16 dims x 8 heads, a float4 a lane
   static constexpr int kParts = kWarps * kFrags * 512;         // room for a part of every warp
   // two CTAs to an SM where three stages (five small ones) or two of them leave room for that, else one; of 228 KB a CTA takes 1 KB
-  // and its static variables besides
-  static constexpr int kOwn = 1024 + kBlocks * 512 + 64, kHalf = (228 << 10) / 2 - kOwn;
+  // and its static variables, in whole KB, besides
+  static constexpr int kOwn = 1024 + kBlocks * 1024, kHalf = (228 << 10) / 2 - kOwn;
   static constexpr int stages(int most, int limit) {
     int n = most;
     while (n > 2 && n * kWarps * kStage + kParts > limit) --n;
@@ -235,7 +236,6 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   const char* kbase = reinterpret_cast<const char*>(p.pool.k) + kh * p.pool.head_stride * kSize + (lane % L::kChunks) * 16;
   const char* vbase = reinterpret_cast<const char*>(p.pool.v) + kh * p.pool.head_stride * kSize + (lane % L::kChunks) * 16;
 
-
   // ---- loading: 64 entries of the row's table in the lanes' registers, the next 32 on their way ----
   int load_pos = 0, load_tiles = 0, ids_at = 0, ids[2] = {-1, -1};
   const int* table = nullptr;
@@ -258,9 +258,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
       }
     }
     if (load_tiles > 0) {
-      if (!waited && load_pos + L::kPos >= load.end) {  // the tile of the row's last position
-        wait();
-      }
+      if (!waited && load_pos + L::kPos >= load.end) wait();  // the tile of the row's last position
       const uint32_t sb = wbase + stage_in * L::kStage;
       const int r0 = lane / L::kChunks, c = lane % L::kChunks;
       const int page0 = div_page(p.div, load_pos) - ids_at;

@@ -3,7 +3,7 @@
     penny_b200.parallel   communicators (symmetric heap, NVLS), CustomAllreduce,
                           the gloo CPU backend, the tuner, schedule math
     penny_b200.ops        all_reduce / all_gather / reduce_scatter / exchange /
-                          all_to_all and the fused ops
+                          all_to_all and the fused ops; a KV cache in pages (PagedKVCache)
     penny_b200.models     Llama-3-8B-shaped TP decode and sequence-parallel prefill,
                           Mixtral-shaped EP layer
     penny_b200.utils      initialize_distributed, device-side benchmarking

@@ -136,6 +136,8 @@ struct Params {
   PageDiv div;
   int group;              // G
   int items, groups;      // (KV head, head group) pairs, head groups of a KV head
+  int teams;              // CTAs of an item
+  bool by_row;            // the joining kernel has a block for each row, not for each team
   int max_len;
   uint32_t page_step, pos_step, step_bytes;  // strides in units of step_bytes
   float4* parts;          // per CTA two parts: of a row that began before it, of one that ends after it
@@ -162,7 +164,7 @@ __device__ __forceinline__ bool locate(const Params& p, int tile, UnitOf unit, i
     if (lane >= o) incl += v;
   }
   total = __shfl_sync(0xffffffffu, incl, 31);
-  share = share_of(total, (int)gridDim.y * kWarps);
+  share = share_of(total, p.teams * kWarps);
   const long long begin = unit(share);
   if (begin >= total) return false;
   row = r0, at = (int)begin - (incl - mine);
@@ -618,8 +620,9 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   }
 }
 
-// Joins the parts of a row that spans teams: a block has the row that begins in its team (if there is one that does not end there), and
-// finds out before it waits.  A warp takes an accumulator of O^T, or, with more warps than those, every so many-th part of it.
+// Joins the parts of a row that spans teams: a block has a row, or the row that begins in its team (if there is one that does not end
+// there), and finds out before it waits.  A warp takes an accumulator of O^T, or, with more warps than those, every so many-th part
+// of it; with gridDim.z above one a block has one accumulator.
 constexpr int kJoinThreads = 512;
 template <int D, typename T, bool kE4M3, int kBlocks>
 __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_constant__ Params p) {
@@ -627,22 +630,42 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_consta
   constexpr int kSteps = D / 16, kAhead = 4, kRows = 8 * kBlocks;
   __shared__ float4 s_acc[kJoinThreads], s_ml[kJoinThreads];
   pdl_launch_dependents();
-  int row, at, share, total, behind = 0;
-  if (locate(p, L::kPos, [&](int each) { return ((long long)blockIdx.y + 1) * kWarps * each; }, row, at, share, total)) {
+  int row = (int)blockIdx.y, team = (int)blockIdx.y, behind = 0;  // teams behind the one that begins the row
+  if (p.by_row) {
+    int total = 0, before = 0;
+    for (int r = threadIdx.x & 31; r < p.a.rows; r += 32) {
+      const Seen s = seen_of(p.a.lengths[r], p.max_len, p.a.window);
+      const int n = units_of(s.end - s.first, L::kPos);
+      total += n;
+      before += r < row ? n : 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    const int each = kWarps * share_of(total, p.teams * kWarps);
     const Seen s = seen_of(p.a.lengths[row], p.max_len, p.a.window);
-    const int each = kWarps * share, end = ((int)blockIdx.y + 1) * each;
-    behind = teams_behind(end - each, end, end - at, units_of(s.end - s.first, L::kPos));
+    team = (before + kStart) / each;
+    behind = s.end > s.first ? teams_behind(team * each, (team + 1) * each, before, units_of(s.end - s.first, L::kPos)) : 0;
+  } else {
+    int at, share, total;
+    if (locate(p, L::kPos, [&](int each) { return ((long long)team + 1) * kWarps * each; }, row, at, share, total)) {
+      const Seen s = seen_of(p.a.lengths[row], p.max_len, p.a.window);
+      const int each = kWarps * share, end = (team + 1) * each;
+      behind = teams_behind(end - each, end, end - at, units_of(s.end - s.first, L::kPos));
+    }
   }
   pdl_wait();
   if (behind == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warps = blockDim.x / 32;
   const int kh = kBlocks == 1 ? (int)blockIdx.x : (int)blockIdx.x / p.groups, h0 = kBlocks == 1 ? 0 : ((int)blockIdx.x - kh * p.groups) * kRows;
   const int heads = min(kRows, p.group - h0), head0 = kh * p.group + h0, n = 1 + behind;
-  const int sets = max(1, warps / L::kFrags), set = warp / L::kFrags;
-  const long long cta = blockIdx.y * gridDim.x + blockIdx.x;
+  const int frags = gridDim.z > 1 ? 1 : L::kFrags, sets = max(1, warps / frags), set = warp / frags;
+  const long long cta = (long long)team * gridDim.x + blockIdx.x;
   const float v_scale = kE4M3 ? p.pool.v_scale[kh] : 1.f;
-  for (int f = warp % L::kFrags; f < L::kFrags; f += warps) {
-    const int nb = f / kSteps, h = nb * 8 + 2 * t;
+  for (int f0 = warp % frags; f0 < frags; f0 += warps) {
+    const int f = f0 + (int)blockIdx.z, nb = f / kSteps, h = nb * 8 + 2 * t;
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     auto take = [&](const float4& ml, const float4& v) {  // maxima and sums of two heads, their values
@@ -673,7 +696,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_consta
       s_ml[threadIdx.x] = make_float4(top[0], sum[0], top[1], sum[1]);
       __syncthreads();
       if (set > 0) return;
-      for (int i = 1; i < sets; ++i) take(s_ml[threadIdx.x + i * L::kFrags * 32], s_acc[threadIdx.x + i * L::kFrags * 32]);
+      for (int i = 1; i < sets; ++i) take(s_ml[threadIdx.x + i * frags * 32], s_acc[threadIdx.x + i * frags * 32]);
     }
     const float inv[2] = {inverse(top[0], sum[0], v_scale), inverse(top[1], sum[1], v_scale)};
     T* out = reinterpret_cast<T*>(p.a.out) + row * p.a.out_stride + (head0 + nb * 8) * p.a.out_head_stride + f % kSteps * 16;
@@ -702,12 +725,18 @@ cudaError_t launch(Params p, void* workspace, int sms, cudaStream_t stream) {
   if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
   p.parts = reinterpret_cast<float4*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.parts + ctas * 2 * L::kFrags * 32);
-  const dim3 grid((unsigned)p.items, (unsigned)(ctas / p.items));
+  p.teams = (int)(ctas / p.items);
+  p.by_row = p.a.rows < p.teams;
+  const dim3 grid((unsigned)p.items, (unsigned)p.teams);
   rc = launch_kernel_ex(kernel, grid, dim3(kWarps * 32), (size_t)L::kSmem, stream, true, 1, p);
   if (rc != cudaSuccess || ctas == p.items) return rc;  // (a single team finishes its rows)
-  // few rows are cut into many parts each (2 rows of 100001: 18)
-  const int warps = (int)grid.y > 4 * p.a.rows ? kJoinThreads / 32 : 8;
-  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kBlocks>, grid, dim3((L::kFrags < warps && p.a.rows >= (int)grid.y ? L::kFrags : warps) * 32), 0, stream, true, 1, p);
+  // Fewer rows than teams: a block for each row, and one for each accumulator where rows are in many parts.  A block for each team, with
+  // all accumulators: 1 row of 100000 positions, 4 heads of 1, 296 parts: 37 us, so 20; 40 of 20000 at most: 21, so 18.5.  A block for
+  // each accumulator where a row has 1 or 2 parts: 32 rows of 2048, 32 heads of 8: 55 us, so 47.5.
+  const bool many = p.teams > 4 * p.a.rows;
+  const int warps = p.teams > 16 * p.a.rows ? kJoinThreads / 32 : L::kFrags < 8 && !p.by_row ? L::kFrags : 8;
+  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kBlocks>, dim3(grid.x, p.by_row ? p.a.rows : p.teams, many ? L::kFrags : 1), dim3(warps * 32), 0,
+                          stream, true, 1, p);
 }
 
 }  // namespace

@@ -78,6 +78,13 @@ def _walks(lengths, max_len, teams, window, tile=16):
             if ends and not begins:
                 first, later = counts[r]
                 assert first + later == w // per
+            if begins:
+                # the team of a row's first tile, and those that follow, as the joining kernel counts them for each row
+                each = per * share
+                team = (line[r] + 3) // each
+                assert team == w // per
+                later = schedule.paged_teams_behind(team * each, (team + 1) * each, line[r], line[r + 1] - line[r])
+                assert (later == 0) == (line[r + 1] <= (team + 1) * each) and team + later == (line[r + 1] - 1) // each
     assert open_row is None
     for team in range(teams):  # and a team that begins no row across its end is not taken for one
         begin, end = team * per * share, (team + 1) * per * share

@@ -108,6 +108,17 @@ def test_pieces(dtype, cache, lengths, heads, kv_heads):
             _run(c, workspace=ws[:-16])
 
 
+@pytest.mark.parametrize("dtype,cache", [(BF, BF), (HF, E4M3)])
+@pytest.mark.parametrize("heads,kv_heads,dim,window", [(4, 1, 128, 0), (3, 1, 64, 5000), (34, 2, 64, 0), (8, 1, 256, 0), (32, 2, 256, 700)])
+@pytest.mark.parametrize("lengths", [[0, 30011], [1, 9000, 0, 20, 5001, 0, 0], [7001, 0, 1, 16] * 5, [2000, 1, 0] * 16 + [4999], [800, 0] * 60])
+def test_join(dtype, cache, heads, kv_heads, dim, window, lengths):
+    """Rows in hundreds of parts, in a few and in one, empty rows among them: every way in which the joining kernel shares them out."""
+    c = _case(lengths, heads, kv_heads, dim, 16, dtype, cache, seed=9)
+    out, lse = _run(c, window=window)
+    _check(c, out, lse, window=window, rows=range(min(8, len(lengths))))
+    _check(c, out, lse, window=window, rows=range(max(0, len(lengths) - 8), len(lengths)))
+
+
 @pytest.mark.parametrize("window", [1, 16, 17, 300, 100000])
 @pytest.mark.parametrize("dtype,cache", [(BF, BF), (HF, HF), (BF, E4M3)])
 def test_window(window, dtype, cache):

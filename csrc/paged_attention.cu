@@ -622,12 +622,12 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
 
 // Joins the parts of a row that spans teams: a block has a row, or the row that begins in its team (if there is one that does not end
 // there), and finds out before it waits.  A warp takes an accumulator of O^T, or, with more warps than those, every so many-th part
-// of it; with gridDim.z above one a block has one accumulator.
+// of it; with gridDim.z above one a block has one accumulator.  kAhead: parts requested before the first is used.
 constexpr int kJoinThreads = 512;
-template <int D, typename T, bool kE4M3, int kBlocks>
+template <int D, typename T, bool kE4M3, int kBlocks, int kAhead>
 __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_constant__ Params p) {
   using L = Tile<D, kE4M3, kBlocks>;
-  constexpr int kSteps = D / 16, kAhead = 4, kRows = 8 * kBlocks;
+  constexpr int kSteps = D / 16, kRows = 8 * kBlocks;
   __shared__ float4 s_acc[kJoinThreads], s_ml[kJoinThreads];
   pdl_launch_dependents();
   int row = (int)blockIdx.y, team = (int)blockIdx.y, behind = 0;  // teams behind the one that begins the row
@@ -731,12 +731,13 @@ cudaError_t launch(Params p, void* workspace, int sms, cudaStream_t stream) {
   rc = launch_kernel_ex(kernel, grid, dim3(kWarps * 32), (size_t)L::kSmem, stream, true, 1, p);
   if (rc != cudaSuccess || ctas == p.items) return rc;  // (a single team finishes its rows)
   // Fewer rows than teams: a block for each row, and one for each accumulator where rows are in many parts.  A block for each team, with
-  // all accumulators: 1 row of 100000 positions, 4 heads of 1, 296 parts: 37 us, so 20; 40 of 20000 at most: 21, so 18.5.  A block for
-  // each accumulator where a row has 1 or 2 parts: 32 rows of 2048, 32 heads of 8: 55 us, so 47.5.
-  const bool many = p.teams > 4 * p.a.rows;
-  const int warps = p.teams > 16 * p.a.rows ? kJoinThreads / 32 : L::kFrags < 8 && !p.by_row ? L::kFrags : 8;
-  return launch_kernel_ex(k_paged_join<D, T, kE4M3, kBlocks>, dim3(grid.x, p.by_row ? p.a.rows : p.teams, many ? L::kFrags : 1), dim3(warps * 32), 0,
-                          stream, true, 1, p);
+  // all accumulators: 1 row of 100000 positions, 4 heads of 1, 296 parts: 37 us, so 18.7; 40 of 20000 at most: 21, so 18.5.  A block for
+  // each accumulator where a row has 1 or 2 parts: 32 rows of 2048, 32 heads of 8: 55 us, so 47.5.  Eight parts under way in a warp, or
+  // four with fewer registers, where so many blocks have to find room beside the attention's (8 rows of 2048 20.3 us, so 18.2).
+  const bool many = p.teams > 4 * p.a.rows, long_rows = p.teams > 16 * p.a.rows;
+  const int warps = long_rows ? kJoinThreads / 32 : L::kFrags < 8 && !p.by_row ? L::kFrags : 8;
+  return launch_kernel_ex(many && !long_rows ? k_paged_join<D, T, kE4M3, kBlocks, 4> : k_paged_join<D, T, kE4M3, kBlocks, 8>,
+                          dim3(grid.x, p.by_row ? p.a.rows : p.teams, many ? L::kFrags : 1), dim3(warps * 32), 0, stream, true, 1, p);
 }
 
 }  // namespace

@@ -471,8 +471,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
             if (top > (m[nb][i] == -INFINITY ? -INFINITY : 0.f)) {
-              const float next = base[nb][i] + top, by = base[nb][i] - next, corr = exp2_ftz(m[nb][i] - next);
-              m[nb][i] = base[nb][i] = next;
+              // (the exponents and the base move by the same number, so that the largest exponent is zero, however far apart the numbers of
+              // the scores' size are)
+              const float by = -top, corr = m[nb][i] == -INFINITY ? 0.f : exp2_ftz(by);
+              m[nb][i] = base[nb][i] -= by;
               l[nb][i] *= corr;
 #pragma unroll
               for (int k = 0; k < kSteps; ++k) o[nb][k][i] *= corr, o[nb][k][2 + i] *= corr;

@@ -25,7 +25,10 @@
 //     16-byte chunk are permuted on both sides of the product.  V's bytes are transposed in pairs by ldmatrix and separated
 //     into even and odd dims.
 //   * P is rounded to the type of the product (bf16: 2^-8 of each weight at most, averaged over the positions; the sum is of the
-//     unrounded ones); q, scores, maxima and sums are not rounded.  Weights count from a base near the maximum so far.  Where they are
+//     unrounded ones); q, scores, maxima and sums are not rounded.  fp16 holds nothing under 2^-25 and little under 2^-14, and a long
+//     row has many such weights: the base of fp16 weights stands kShift under the maximum, so that the largest is near 2^15 and a weight
+//     loses 2^-40 of the largest at most (2^-32 where the base may lag).  With a largest weight of one, 25,000 positions of a warp
+//     that stood 17.4 under another one were lost whole.  Weights count from a base near the maximum so far.  Where they are
 //     finer than the output (e4m3 caches with a bf16 q) it follows when it is exceeded by 2^8, which is seldom (64 rows of 4096, 28
 //     of 2 heads: 34.4 us, always 38.1).  Elsewhere it follows always, so that the largest weight is one and not off: 64 rows of 2048,
 //     bf16, are 0.0018 of the output's norm from 64 bits (its own rounding: 0.0017), otherwise 0.0022 (and 0.5 us faster).
@@ -202,7 +205,9 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
   using T2 = typename Pair<T>::type;
   constexpr int kRows = 8 * kBlocks, kSteps = D / 16, kGroups = L::kPos / 16, kStages = L::kStages;
   constexpr bool kBf16 = !kE4M3 && __is_same(T, __nv_bfloat16);
-  constexpr float kSlack = kE4M3 && __is_same(T, __nv_bfloat16) ? 8.f : 0.f;
+  // exponents: how far the base stands under the maximum, and how far a score may be above that before it follows (fp16 weights: up to
+  // 2^(kShift + kSlack) = 2^15)
+  constexpr float kSlack = kE4M3 && __is_same(T, __nv_bfloat16) ? 8.f : 0.f, kShift = kBf16 ? 0.f : 15.f - kSlack;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ float2 s_ml[2][kWarps][kRows];  // of a warp's first part and of its last
   __shared__ int s_head[kWarps];             // a part of a row that began before: 0 none, 1 it ends here, 2 it does not
@@ -438,7 +443,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
         }
       }
       if constexpr (kStages > 2) masks[kStages - 1] = issue();
-      // ---- weights exp2(score - base); the base goes up to the maximum when a score of the tile is above it by more than kSlack ----
+      // ---- weights exp2(score - base); the base goes up when a score of the tile is above base + kShift by more than kSlack ----
       uint32_t pb[kBlocks][kGroups][2];
 #pragma unroll
       for (int nb = 0; nb < kBlocks; ++nb) {
@@ -460,7 +465,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
 #pragma unroll
         for (int c = 0; c < kGroups; ++c) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) above = above || s[nb][c][u] > (m[nb][u & 1] == -INFINITY ? -INFINITY : kSlack);
+          for (int u = 0; u < 4; ++u) above = above || s[nb][c][u] > (m[nb][u & 1] == -INFINITY ? -INFINITY : kShift + kSlack);
         }
         if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
@@ -470,10 +475,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
             for (int c = 0; c < kGroups; ++c) top = fmaxf(top, fmaxf(s[nb][c][i], s[nb][c][2 + i]));
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            if (top > (m[nb][i] == -INFINITY ? -INFINITY : 0.f)) {
-              // (the exponents and the base move by the same number, so that the largest exponent is zero, however far apart the numbers of
-              // the scores' size are)
-              const float by = -top, corr = m[nb][i] == -INFINITY ? 0.f : exp2_ftz(by);
+            if (top > (m[nb][i] == -INFINITY ? -INFINITY : kShift)) {
+              // (the exponents and the base move by the same amount, rounded down: the largest one then is at most kShift and above
+              // kShift - 16, however far apart the numbers of the scores' size are)
+              const float by = __fsub_rd(kShift, top), corr = m[nb][i] == -INFINITY ? 0.f : exp2_ftz(by);
               m[nb][i] = base[nb][i] -= by;
               l[nb][i] *= corr;
 #pragma unroll

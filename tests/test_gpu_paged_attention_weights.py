@@ -1,4 +1,6 @@
-"""Paged attention where the scores are large."""
+"""Paged attention where the weights of a long row are far below its largest one, and where its scores are large."""
+import math
+
 import pytest
 import torch
 
@@ -7,6 +9,44 @@ import penny_b200.ops as P
 pytestmark = pytest.mark.gpu
 BF, HF, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
 STEP = {BF: 2.0 ** -8, HF: 2.0 ** -11}
+
+
+def _dominated(dtype, cache, n, at, gap, dim=64, page=64, heads=296):
+    """One row of n positions for `heads` KV heads (so few CTAs have each that a warp walks a quarter of the row): all scores zero but
+    that of position `at`, about `gap`; its values are zero, the others' two.  Every page but that position's is the same one."""
+    width = -(-n // page)
+    table = torch.zeros(1, width, dtype=torch.int32, device="cuda")
+    table[0, at // page] = 1
+    k, v = torch.zeros(2, page, 1, dim, device="cuda"), torch.full((2, page, 1, dim), 2.0, device="cuda")
+    k[1, at % page, 0, 0], v[1, at % page] = 448 if cache == E4M3 else gap, 0
+    scales = {} if cache != E4M3 else dict(k_scale=torch.full((heads,), gap / 448, device="cuda"), v_scale=torch.ones(heads, device="cuda"))
+    k, v = (t.to(cache).expand(-1, -1, heads, -1) for t in (k, v))
+    q = torch.zeros(1, heads, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    score = float(k[1, at % page, 0, 0].float()) * (float(scales["k_scale"][0]) if scales else 1.0)
+    lse = torch.zeros(1, heads, device="cuda")
+    out = P.paged_attention(q, k, v, table, torch.tensor([n], dtype=torch.int32, device="cuda"), lse=lse, scale=1.0, **scales)
+    tail = (n - 1) * math.exp(-score)
+    return out, lse, 2 * tail / (1 + tail), score + math.log1p(tail)
+
+
+@pytest.mark.parametrize("dtype,cache", [(HF, HF), (HF, E4M3), (BF, E4M3), (BF, BF)])
+@pytest.mark.parametrize("n", [100003, 1600000])
+@pytest.mark.parametrize("where", ["first", "early", "last"])
+@pytest.mark.parametrize("gap", [17.4, 19.0, 12.0])
+def test_one_key_far_above_the_others(dtype, cache, n, where, gap):
+    """A weight is off by half a step of the type that meets V where that type holds it in full; an fp16 one also by 2 ** -25 of what the
+    largest is multiplied by, 2 ** 15, or 2 ** 7 at least where the base lags (bf16 q of an e4m3 cache).  fp32's part: a score's base-2
+    exponent (up to 32) to 2 ** -20, weights and outputs to 2 ** -17.  A warp walks n / 4 positions at most; a lane adds an eighth of
+    their weights one after another to its sum (2 ** -24 of it each: n * 2 ** -29), and each position adds a product to the output
+    (2 ** -23 of it each, for matrix instructions may cut off: n * 2 ** -25)."""
+    at = {"first": 0, "early": n // 8, "last": n - 1}[where]
+    out, lse, want, true = _dominated(dtype, cache, n, at, gap)
+    floor = 0.0 if cache == BF else 2 * n * 2.0 ** (-32 if dtype == BF else -40)
+    bound = (STEP[BF] if cache == BF else STEP[HF]) * want + STEP[dtype] * want + floor + 2.0 ** -25 + (2.0 ** -17 + n * (2.0 ** -29 + 2.0 ** -25)) * want
+    err = (out.double() - want).abs().max().item()
+    assert err <= bound, (err, bound)
+    assert (lse.double() - true).abs().max().item() <= 2.0 ** -16 + n * 2.0 ** -29
 
 
 @pytest.mark.parametrize("dtype,cache", [(HF, HF), (HF, E4M3), (BF, E4M3), (BF, BF)])

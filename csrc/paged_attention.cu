@@ -20,8 +20,9 @@
 //   * A row that lies in one warp's part is finished from its registers, the parts of one that spans warps of a CTA
 //     meet in shared memory, those of several CTAs in a workspace, which a second kernel joins.  No counters: a workspace
 //     holds nothing between calls.
-//   * e4m3 caches: fp16 is exact for them, so they meet q as fp16, each row of q divided by the power of two of its
-//     largest value (exact, but values under 2^-14 of that keep 2^-25 of it; the score's factor takes it back).  A lane's four bytes of K are two adjacent pairs: the dims inside a
+//   * e4m3 caches: fp16 is exact for them, so they meet q as fp16, each row of q times the power of two that brings its largest value
+//     to [2^15, 2^16) (exact for fp16 rows; of bf16 ones values under 2^-29 of the largest keep 2^-40 of it; the score's factor takes it
+//     back).  A lane's four bytes of K are two adjacent pairs: the dims inside a
 //     16-byte chunk are permuted on both sides of the product.  V's bytes are transposed in pairs by ldmatrix and separated
 //     into even and odd dims.
 //   * P is rounded to the type of the product (bf16: 2^-8 of each weight at most, averaged over the positions; the sum is of the
@@ -345,16 +346,15 @@ __global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const __grid_co
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = min((__float_as_int(top) >> 23) & 255, 253);  // (one over a power of two above that is none of fp32's)
-        const bool plain = e < 1;  // zeros
-        const float down = plain ? 1.f : __int_as_float((254 - e) << 23);
-        const float factor = p.a.scale * kLog2e * p.pool.k_scale[kh] * (plain ? 1.f : __int_as_float(e << 23));
+        // times 2^(142 - e), so that the largest is in [2^15, 2^16) (smaller where it is under 2^-111, for both powers to be fp32's)
+        const int e = max((__float_as_int(top) >> 23) & 255, 16);
+        const float up = __int_as_float((269 - e) << 23), factor = p.a.scale * kLog2e * p.pool.k_scale[kh] * __int_as_float((e - 15) << 23);
 #pragma unroll
         for (int i = 0; i < 2; ++i) qs[nb][i] = __shfl_sync(0xffffffffu, factor, (2 * t + i) * 4);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-          qb[nb][k][0] = pack_f16(x[k][0] * down, x[k][1] * down);
-          qb[nb][k][1] = pack_f16(x[k][2] * down, x[k][3] * down);
+          qb[nb][k][0] = pack_f16(x[k][0] * up, x[k][1] * up);
+          qb[nb][k][1] = pack_f16(x[k][2] * up, x[k][3] * up);
         }
       } else {
         qs[nb][0] = qs[nb][1] = p.a.scale * kLog2e;

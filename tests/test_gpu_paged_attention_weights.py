@@ -69,3 +69,26 @@ def test_scores_too_large_for_their_fractions(dtype, cache, size):
         if top.values[h, 0] - top.values[h, 1] > 2.0 ** -10:
             want = v.view(-1, dim)[top.indices[h, 0]].double()  # (the weight and the output rounded)
             assert ((out[0, h].double() - want).abs() <= ((STEP[BF] if cache == BF else STEP[HF]) + STEP[dtype]) * (1 + 2.0 ** -6) * want.abs()).all(), h
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("top", [1.0, 1.9921875, 2.0 ** -12, 60000.0])
+def test_small_values_of_q_beside_a_large_one(dtype, top):
+    """q of an 8-bit cache whose score comes from values far under its largest one, which meets a key of zero: what fp16 holds beside the
+    largest is not lost (values down to 2 ** -29 of it; scores to 2 ** -20, sums and logarithm to as much)."""
+    dim, page = 64, 16
+    small = top * (2.0 ** -20 if dtype == BF else 2.0 ** -9) * (1 + 2.0 ** -7)
+    q = torch.zeros(1, 4, dim, dtype=dtype, device="cuda")
+    q[..., 0], q[0, :, 1] = top, torch.tensor([1.0, 0.5, -0.25, 2.0 ** -8], device="cuda").to(dtype) * torch.tensor(small, device="cuda").to(dtype)
+    k, v = torch.zeros(1, page, 1, dim, device="cuda"), torch.zeros(1, page, 1, dim, device="cuda")
+    k[0, 1, 0, 1] = 448
+    v[0, 1] = 1
+    one, scale = torch.ones(1, device="cuda"), 1.75 / (448 * small)
+    lse = torch.zeros(1, 4, device="cuda")
+    out = P.paged_attention(q, k.to(E4M3), v.to(E4M3), torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([2], dtype=torch.int32, device="cuda"),
+                            lse=lse, scale=scale, k_scale=one, v_scale=one)
+    s = q[0, :, 1].double() * 448 * float(torch.tensor(scale, dtype=torch.float32))
+    true = torch.log1p(s.exp())
+    assert ((lse[0].double() - true).abs() <= 2.0 ** -18).all(), (lse, true)
+    want = torch.sigmoid(s)[:, None]
+    assert ((out[0].double() - want).abs() <= (STEP[HF] + STEP[dtype] + 2.0 ** -17) * want).all()

@@ -42,7 +42,7 @@ from typing import Optional
 import torch
 
 from .._ext import ops
-from ..ops.paged import PagedKVCache, PageStep
+from ..ops.paged import OutOfPages, PagedKVCache, PageStep
 
 
 @dataclass
@@ -84,7 +84,8 @@ class LlamaTPDecoder:
                  use_graph: bool = True, full_init: bool = False, process_group=None, linears: str = "auto",
                  pdl: bool = True, page_size: int = 0, pages: Optional[int] = None, cache_dtype: Optional[torch.dtype] = None):
         """page_size > 0: KV cache in pages of that many positions, `pages` of them (by default enough for max_batch sequences
-        of max_len), of cache_dtype (bf16 or e4m3)."""
+        of max_len), of cache_dtype (bf16 or e4m3).  `positions` are that cache's lengths then; every step lets one token come to every
+        row.  A row for which there is no page is left out of a step, which raises OutOfPages when it has waited for the device."""
         if page_size < 0 or (page_size == 0 and (pages is not None or cache_dtype is not None)):
             raise ValueError("pages and cache_dtype belong to a cache in pages: page_size above 0")
         assert cfg.heads % world == 0 and cfg.kv_heads % world == 0 and cfg.ffn % world == 0
@@ -190,11 +191,15 @@ class LlamaTPDecoder:
             self.page_step = PageStep(torch.full((B,), -1, dtype=torch.int64, device=self.dev), torch.zeros(B, dtype=torch.int32, device=self.dev),
                                       torch.zeros(B + 1, dtype=torch.int32, device=self.dev), torch.ones(B, dtype=torch.bool, device=self.dev))
             self.one_each = torch.ones(B, dtype=torch.int32, device=self.dev)
-            self.served = torch.ones(B, dtype=torch.bool, device=self.dev)  # rows that had a page for every token so far
+            self.served = torch.ones(B, dtype=torch.bool, device=self.dev)  # rows that had a page for every token since the last check
+            # a row's next position is its length, which page_tables counts on where the row is granted its token; what the step's last
+            # kernel counts on says nothing
+            self.positions, self.counted = self.paged.lengths, self.positions
             self._host_served = torch.ones(B, dtype=torch.bool).pin_memory()
             self.page_workspace = self.paged.workspace(self.Hq)
             self.kcache = self.vcache = []
         else:
+            self.counted = self.positions
             self.kcache = [torch.zeros(B, self.Hkv, max_len, D, dtype=dt, device=self.dev) for _ in range(cfg.layers)]
             self.vcache = [torch.zeros(B, self.Hkv, max_len, D, dtype=dt, device=self.dev) for _ in range(cfg.layers)]
         self.splits = self.attention_splits(B * self.Hkv, max_len)
@@ -451,7 +456,7 @@ class LlamaTPDecoder:
         # (one rank: the winners are the tokens, the same kernel hands them on)
         if self.world == 1:
             ops.argmax_rows(self.logits, self.max_val, self.max_idx, 0, self.argmax_ws, None, self.next_tokens, self.tokens,
-                            self.positions, self._host_out if host else None)
+                            self.counted, self._host_out if host else None)
         else:
             ops.argmax_rows(self.logits, self.max_val, self.max_idx, self.rank * self.V, self.argmax_ws, self.pair)
             if self.backend == "nccl":
@@ -459,7 +464,7 @@ class LlamaTPDecoder:
                 dist.all_gather_into_tensor(self.pairs_all, self.pair, group=self.pg)
             else:
                 self.comm.all_gather(self.pair, out=self.pairs_all)
-            ops.sample_finish(self.pairs_all, self.world, self.next_tokens, self.tokens, self.positions)
+            ops.sample_finish(self.pairs_all, self.world, self.next_tokens, self.tokens, self.counted)
 
     def capture(self):
         """Warm up (cuBLAS handles, scratch growth) and capture the step in a CUDA graph."""
@@ -493,16 +498,30 @@ class LlamaTPDecoder:
             self.served.copy_(pages[1])
 
     def check_pages(self):
-        """Raises if a sequence had no page for one of its tokens (the pool is empty, or it has max_len of them): its tokens from that
-        one on are wrong.  Waits for the device; step() and decode() call it, after step_device() it is the caller's."""
+        """Raises OutOfPages if a sequence had no page for one of its tokens since the last check (the pool is empty, or it has max_len of
+        them).  Waits for the device; step() and decode() call it, after step_device() it is the caller's."""
         if self.paged is not None:
-            self._raise_unserved(self.served.cpu())
+            self._raise_unserved(self.served.cpu(), self.next_tokens)
 
-    def _raise_unserved(self, served):
+    def _raise_unserved(self, served, next_tokens):
         if not bool(served.all()):
+            self.served.fill_(True)  # (said once)
             rows = (~served).nonzero().flatten().tolist()
-            raise RuntimeError(f"no page for a token of sequences {rows[:8]}{'...' if len(rows) > 8 else ''}: {self.paged.pages} pages of "
-                               f"{self.paged.page_size} positions, {self.max_len} positions a sequence")
+            raise OutOfPages(f"no page for a token of sequences {rows[:8]}{'...' if len(rows) > 8 else ''}: {self.paged.pages} pages of "
+                             f"{self.paged.page_size} positions, {self.max_len} positions a sequence", rows, next_tokens.clone())
+
+    def release(self, rows):
+        """The sequences of `rows` leave a cache in pages: their pages are free, their lengths zero, and the next step's token of such a row
+        is the first one of a new sequence."""
+        if self.paged is None:
+            raise ValueError("release: a cache in pages has rows that leave")
+        rows = list(rows)
+        if any(not 0 <= r < self.B for r in rows):
+            raise IndexError(f"rows must lie in [0, {self.B})")
+        leave = torch.zeros(self.B, dtype=torch.int32)
+        leave[rows] = -1
+        self.paged.advance(leave.to(self.dev) * self.paged.lengths, 0)
+        self.served[leave.to(self.dev) != 0] = True
 
     def step_device(self):
         """One decode step on the device buffers: self.tokens -> self.next_tokens."""
@@ -515,7 +534,11 @@ class LlamaTPDecoder:
         """Public decode call: `tokens` is a CPU int64 tensor [batch]; returns the
         next token of every sequence as a CPU tensor.  The captured step of one rank
         reads the tokens from pinned memory and leaves the next ones there; the other
-        forms copy them to the device and back around the step."""
+        forms copy them to the device and back around the step.
+
+        A cache in pages: OutOfPages names the rows that had no page for their token.  Those are as they were, their next_tokens
+        say nothing: they may take the same token again when there are pages (`release`).  The others have taken theirs, and
+        next_tokens has what follows."""
         # (on the device an id without an embedding row stops the context)
         if not ops.take_ids(tokens, self._host_in, self.cfg.vocab):
             raise IndexError(f"token ids must lie in [0, {self.cfg.vocab})")
@@ -529,17 +552,20 @@ class LlamaTPDecoder:
             self._host_served.copy_(self.served, non_blocking=True)
         torch.cuda.current_stream().synchronize()
         if self.paged is not None:
-            self._raise_unserved(self._host_served)
+            self._raise_unserved(self._host_served, self._host_out)
         return self._host_out
 
     def decode(self, steps: int) -> torch.Tensor:
-        """Autoregressive greedy decode for `steps` tokens; returns [steps, batch] on the device."""
+        """Autoregressive greedy decode for `steps` tokens; returns [steps, batch] on the device.  OutOfPages has them as next_tokens:
+        of a row that it names as many as its length has grown by count (and the last of them is the token it takes next)."""
         out = []
         for _ in range(steps):
             self.step_device()
             out.append(self.next_tokens.clone())
-        self.check_pages()
-        return torch.stack(out)
+        out = torch.stack(out)
+        if self.paged is not None:
+            self._raise_unserved(self.served.cpu(), out)
+        return out
 
     # ------------------------------------------------------- fp32 torch oracle
     @torch.no_grad()

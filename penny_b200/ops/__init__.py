@@ -20,7 +20,7 @@ from typing import Optional
 import torch
 
 _BACKEND = None
-_PAGED = ("PagedKVCache", "PageStep", "page_tables", "paged_append", "paged_attention")
+_PAGED = ("PagedKVCache", "PageStep", "OutOfPages", "page_tables", "paged_append", "paged_attention")
 
 
 def __getattr__(name):

@@ -30,6 +30,14 @@ class PageStep(NamedTuple):
     granted: torch.Tensor    # [rows] bool
 
 
+class OutOfPages(RuntimeError):
+    """Rows that were not granted a token (no page, or at their longest), and the tokens that the step gave all the same."""
+
+    def __init__(self, said: str, rows: List[int], next_tokens: torch.Tensor):
+        super().__init__(said)
+        self.rows, self.next_tokens = rows, next_tokens
+
+
 def page_tables(table, lengths, free, free_count, new, page_size: int, tokens: int, out: Optional[PageStep] = None) -> PageStep:
     """Lets new[r] tokens come to row r, or its last -new[r] leave, and moves the pages that follow from it.
 

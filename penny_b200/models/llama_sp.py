@@ -208,8 +208,8 @@ class LlamaSPPrefill:
         """x_shard: this rank's [T / world, hidden] rows of the residual stream; returns the same rows after all layers.
 
         pages: (cache, step), a PagedKVCache of this rank's KV heads and the PageStep of its `advance` that let these T tokens, and no
-        others, come to a row that was empty: the keys and values are left there for the decode.  step.granted is looked at
-        here (which waits for the device), except under stream capture."""
+        others, come to a row that was empty: the keys and values are left there for the decode.  That is looked at here (which waits
+        for the device), except under stream capture."""
         self._pages = None
         if pages is not None:
             cache, step = pages
@@ -217,8 +217,13 @@ class LlamaSPPrefill:
                 raise ValueError("a cache in pages needs the GPU")
             if (len(cache.k), cache.kv_heads, cache.head_dim) != (self.L, self.Hkv, self.cfg.head_dim) or step.slots.numel() != self.T:
                 raise ValueError(f"pages of {self.L} layers with {self.Hkv} KV heads of {self.cfg.head_dim}, a step of {self.T} tokens")
-            if not torch.cuda.is_current_stream_capturing() and not bool(step.granted.all()):
-                raise RuntimeError("the cache had no pages for this prompt")
+            if not torch.cuda.is_current_stream_capturing():
+                at = torch.arange(self.T, dtype=torch.int32, device=step.positions.device)
+                granted, prompt = torch.stack([step.granted.all(), ((step.positions == at) & (step.slots >= 0)).all()]).tolist()
+                if not granted:
+                    raise RuntimeError("the cache had no pages for this prompt")
+                if not prompt:  # (the attention covers these tokens alone, all as one sequence from position 0 on)
+                    raise ValueError(f"pages: the {self.T} tokens of one row that was empty before the step")
             self._pages = pages
         if self.local and x_shard.is_contiguous() and x_shard.data_ptr() % 16 == 0:
             return self._forward_local(x_shard)

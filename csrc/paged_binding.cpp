@@ -6,7 +6,10 @@
 #include <pybind11/pybind11.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
+#include <utility>
+#include <vector>
 
 #include "paged_kernels.h"
 #include "paged_plan.h"
@@ -67,6 +70,76 @@ int sms_of(int device) {
   int sms = 0;
   ck(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "device");
   return sms;
+}
+
+// Where a tensor's elements lie: runs of `len` bytes at `n` by `step`, the largest step first; dimensions of one are left out.
+struct Runs {
+  uintptr_t at;
+  std::vector<std::pair<int64_t, int64_t>> dims;  // (n, step in bytes)
+  int64_t len;
+  explicit Runs(const at::Tensor& t) : at((uintptr_t)t.data_ptr()), len(t.element_size()) {
+    for (int i = 0; i < t.dim(); ++i)
+      if (t.size(i) > 1 && (i + 1 < t.dim() || t.stride(i) != 1)) dims.push_back({t.size(i), t.stride(i) * t.element_size()});
+    if (t.dim() > 0 && (t.size(-1) <= 1 || t.stride(-1) == 1)) len *= t.size(-1);
+    std::stable_sort(dims.begin(), dims.end(), [](auto& a, auto& b) { return a.second > b.second; });
+  }
+};
+// From a tensor's first byte to behind its last.
+std::pair<uintptr_t, uintptr_t> bounds(const at::Tensor& t) {
+  int64_t n = 1;
+  for (int i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+  return {(uintptr_t)t.data_ptr(), (uintptr_t)t.data_ptr() + n * t.element_size()};
+}
+// Do runs of a and runs of b, both laid out by dims[i...], meet if b's are `off` bytes further?
+bool meet_at(const Runs& a, const Runs& b, size_t i, int64_t off) {
+  if (i == a.dims.size()) return off < a.len && -off < b.len;
+  const auto [n, step] = a.dims[i];
+  if (step == 0) return meet_at(a, b, i + 1, off);
+  int64_t wa = a.len, wb = b.len;  // of what is inside a step
+  for (size_t j = i + 1; j < a.dims.size(); ++j) wa += (a.dims[j].first - 1) * a.dims[j].second, wb += (a.dims[j].first - 1) * a.dims[j].second;
+  // off + d step in (-wb, wa): one or two d, unless steps overlap
+  auto floor_div = [](int64_t x, int64_t y) { return x >= 0 ? x / y : -((-x + y - 1) / y); };
+  for (int64_t d = std::max(1 - n, floor_div(-wb - off, step)); d < n && off + d * step < wa; ++d)
+    if (off + d * step > -wb && meet_at(a, b, i + 1, off + d * step)) return true;
+  return false;
+}
+bool overlap(const at::Tensor& ta, const at::Tensor& tb) {
+  if (ta.numel() == 0 || tb.numel() == 0) return false;
+  const auto in_a = bounds(ta), in_b = bounds(tb);
+  if (in_a.second <= in_b.first || in_b.second <= in_a.first) return false;
+  const Runs a(ta), b(tb);
+  if (a.dims == b.dims) return meet_at(a, b, 0, (int64_t)(b.at - a.at));
+  // laid out in two ways, within each other's bounds: all runs in order
+  int64_t count = 0;
+  for (const Runs* r : {&a, &b}) {
+    int64_t n = 1;
+    for (auto& d : r->dims) n *= d.first;
+    count += n;
+  }
+  if (count > 1 << 22) return true;
+  std::vector<std::pair<uintptr_t, const Runs*>> runs;
+  for (const Runs* r : {&a, &b}) {
+    std::vector<uintptr_t> at = {r->at};
+    for (auto& d : r->dims) {
+      const size_t n = at.size();
+      for (int64_t i = 1; i < d.first; ++i)
+        for (size_t j = 0; j < n; ++j) at.push_back(at[j] + i * d.second);
+    }
+    for (uintptr_t x : at) runs.push_back({x, r});
+  }
+  std::sort(runs.begin(), runs.end());
+  uintptr_t end_a = 0, end_b = 0;
+  for (auto& [x, r] : runs) {
+    if (x < (r == &a ? end_b : end_a)) return true;
+    (r == &a ? end_a : end_b) = x + r->len;  // (runs of one tensor have one length: the last begun is the last to end)
+  }
+  return false;
+}
+// Every element of b where a has the one of the same indices (the last dimension may be shorter)
+bool same_place(const at::Tensor& a, const at::Tensor& b) {
+  bool same = a.data_ptr() == b.data_ptr();
+  for (int i = 0; same && i + 1 < a.dim(); ++i) same = a.size(i) <= 1 || a.stride(i) == b.stride(i);
+  return same;
 }
 }  // namespace
 
@@ -186,6 +259,7 @@ void bind_paged(py::module_& m) {
     need(no_grad(q), "paged_attention: no gradients");
     if (out.has_value())
       need(out->scalar_type() == q.scalar_type() && out->sizes() == q.sizes() && rows_ok(*out) && apart(*out), "paged_attention: out like q, its rows apart");
+    if (out.has_value()) need(!overlap(*out, q) || same_place(*out, q), "paged_attention: out is q, or apart from it");
     if (lse.has_value())
       need(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->dim() == 2 && lse->size(0) == B && lse->size(1) == H, "paged_attention: lse [rows, heads] fp32");
     if (workspace.has_value()) need(workspace->is_contiguous() && aligned(*workspace), "paged_attention: 16-byte aligned contiguous workspace");

@@ -71,7 +71,8 @@ def paged_attention(q, k, v, table, lengths, out=None, lse=None, scale: Optional
     strides of whole 16 bytes (k's and v's alike); dim 64, 128 or 256; heads a multiple of kv_heads.  lse: [rows, heads] fp32 for
     the logarithm of the weights' sum, with which parts of a context can be joined.  A row of length 0 (or below) gives
     zeros and -inf; a length past the table row counts as the table row; positions on a page that the pool does not have count as
-    not there.  Rows may share pages.  workspace: `paged_attention_workspace_bytes(rows, heads, kv_heads, dim, max_len, window)`
+    not there.  Rows may share pages.  out is q itself or apart from it; out, lse and workspace share nothing with each other or with what
+    else the call reads.  workspace: `paged_attention_workspace_bytes(rows, heads, kv_heads, dim, max_len, window)`
     bytes with max_len = table.size(1) * page_size, for callers that must not allocate; its contents mean nothing between calls,
     but two calls that may run at the same time need one each.  early: for a step whose kernels overlap (this library's are launched with
     programmatic dependency): those that may still run when this one starts, back to the last launch without it, write of what

@@ -1,0 +1,72 @@
+"""Outputs of the paged operators that share memory with what a call reads: refused, without a GPU; what only lies between is not."""
+import random
+
+import pytest
+import torch
+
+import penny_b200.ops as P
+
+BF = torch.bfloat16
+ints = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+
+
+def _attend(q, out):
+    k = torch.zeros(6, 16, 2, 64, dtype=BF)
+    P.paged_attention(q, k, k.clone(), ints(q.shape[0], 4), ints(q.shape[0]), out=out)
+
+
+def _views(n, *offsets_sizes_strides):
+    flat = torch.zeros(n, dtype=BF)
+    return [flat.as_strided(size, stride, offset) for offset, size, stride in offsets_sizes_strides]
+
+
+SIZE = (3, 4, 64)
+
+
+@pytest.mark.parametrize("a,b", [
+    ((0, SIZE, (256, 64, 1)), (64, SIZE, (256, 64, 1))), ((256, SIZE, (256, 64, 1)), (0, SIZE, (256, 64, 1))),     # a head, a row further
+    ((0, SIZE, (256, 64, 1)), (8, SIZE, (256, 64, 1))), ((0, SIZE, (512, 64, 1)), (192, SIZE, (512, 64, 1))),      # a few values; the last head
+    ((0, SIZE, (512, 128, 1)), (568, SIZE, (512, 128, 1))), ((0, SIZE, (256, 64, 1)), (0, SIZE, (64, 192, 1))),     # between heads but for 8; other order
+    ((0, SIZE, (256, 64, 1)), (704, SIZE, (512, 64, 1))), ((0, SIZE, (0, 64, 1)), (128, SIZE, (256, 64, 1))),       # other strides; q of one row for all
+    ((0, (1, 4, 64), (8, 64, 1)), (192, (1, 4, 64), (999, 64, 1))), ((0, (4, 4, 64), (256, 64, 1)), (0, (4, 4, 64), (64, 256, 1))),  # rows for heads
+])
+def test_attention_out_across_q(a, b):
+    q, out = _views(4096, a, b)
+    with pytest.raises(RuntimeError, match="out is q, or apart from it"):
+        _attend(q, out)
+
+
+@pytest.mark.parametrize("a,b", [
+    ((0, SIZE, (256, 64, 1)), (0, SIZE, (256, 64, 1))), ((0, SIZE, (512, 64, 1)), (256, SIZE, (512, 64, 1))),       # in place; beside in the rows
+    ((256, SIZE, (512, 64, 1)), (0, SIZE, (512, 64, 1))), ((0, SIZE, (512, 128, 1)), (64, SIZE, (512, 128, 1))),    # the other side; between heads
+    ((0, SIZE, (512, 128, 1)), (576, SIZE, (512, 128, 1))), ((0, SIZE, (256, 64, 1)), (768, SIZE, (512, 64, 1))),   # a row further; behind
+    ((0, SIZE, (1024, 64, 1)), (256, SIZE, (256, 64, 1))), ((0, (1, 4, 64), (8, 64, 1)), (0, (1, 4, 64), (999, 64, 1))),  # within a row; one row
+])
+def test_attention_out_beside_q(a, b):
+    q, out = _views(4096, a, b)
+    with pytest.raises(RuntimeError, match="CUDA"):  # (past every check of the host but the last)
+        _attend(q, out)
+
+
+def test_attention_out_and_q_at_random():
+    """Layouts within and across each other, against the sets of elements."""
+    rng, n, met = random.Random(3), 0, 0
+    flat, index = torch.zeros(8000, dtype=BF), torch.arange(8000)
+    for _ in range(3000):
+        B, H, D = rng.randint(1, 4), rng.choice([2, 4]), 64
+        lay = lambda: rng.choice([(H * D, D), (2 * H * D, D), (H * 2 * D, 2 * D), (D, B * D), (D, 2 * B * D), (H * D + 8, D),  # noqa: E731
+                                  (rng.randrange(8, 600, 8), rng.randrange(8, 300, 8))])
+        first = lay()
+        views = [((B, H, D), (*s, 1), rng.randrange(0, 1600, 8)) for s in (first, first if rng.random() < 0.6 else lay())]
+        q, out = (flat.as_strided(*v) for v in views)
+        at_q, at_out = (index.as_strided(*v) for v in views)
+        if at_out.unique().numel() < at_out.numel():
+            continue
+        across = bool(torch.isin(at_q, at_out).any()) and not torch.equal(at_q, at_out)
+        with pytest.raises(RuntimeError) as said:
+            _attend(q, out)
+        if "its rows apart" in str(said.value):
+            continue
+        assert ("apart from it" in str(said.value)) == across, views
+        n, met = n + 1, met + across
+    assert n > 1000 and 200 < met < n - 200

@@ -211,6 +211,8 @@ void bind_paged(py::module_& m) {
       need(out->scalar_type() == qkv.scalar_type() && out->dim() == 2 && out->size(0) == T && out->size(1) == (heads + pool.heads) * D &&
                out->stride(1) == 1 && (T <= 1 || (out->stride(0) >= out->size(1) && out->stride(0) % 8 == 0)) && aligned(*out),
            "paged_append: out must be [tokens, (heads + kv_heads) dim], like qkv");
+    if (out.has_value()) need(!overlap(*out, qkv) || same_place(*out, qkv), "paged_append: out is the start of qkv's rows, or apart from them");
+    need(!overlap(k, v), "paged_append: k apart from v");
     on_device(qkv, {&k, &v, &slots, &positions}, "paged_append expects tensors on one CUDA device");
     if (out.has_value()) on_device(qkv, {&*out}, "paged_append expects tensors on one CUDA device");
     if (k_scale.has_value()) on_device(qkv, {&*k_scale, &*v_scale}, "paged_append expects tensors on one CUDA device");

@@ -58,7 +58,8 @@ def paged_append(qkv, k, v, slots, positions, heads: int, theta: float, out=None
     [tokens, (heads + kv_heads) dim]) and stores the rotated k and v at the tokens' slots of the pools k, v [pages, page_size,
     kv_heads, dim].  A token whose slot the pool does not have (-1) is left alone, its row of out too; no two tokens have the
     same slot.  Pools of qkv's type, or e4m3: value / k_scale[head] (v_scale), saturated at 448.  Any strides of whole 16 bytes;
-    dim a multiple of 16, up to 256.  out and qkv do not overlap.  early: as in `paged_attention`, for slots and positions."""
+    dim a multiple of 16, up to 256.  k and v are apart; out is apart from qkv, or the start of its rows.
+    early: as in `paged_attention`, for slots and positions."""
     ops.paged_append(qkv, k, v, slots, positions, heads, theta, out, k_scale, v_scale, early)
 
 

@@ -70,3 +70,30 @@ def test_attention_out_and_q_at_random():
         assert ("apart from it" in str(said.value)) == across, views
         n, met = n + 1, met + across
     assert n > 1000 and 200 < met < n - 200
+
+
+def _append(qkv, out, k=None, v=None):
+    k = torch.zeros(6, 16, 2, 64, dtype=BF) if k is None else k
+    P.paged_append(qkv, k, torch.zeros_like(k) if v is None else v, torch.zeros(qkv.shape[0], dtype=torch.int64), ints(qkv.shape[0]), 4, 1e4, out=out)
+
+
+def test_append_out_across_qkv():
+    for offset, stride in ((64, 512), (512, 512), (128, 1024), (640, 512)):
+        qkv, out = _views(8192, (0, (3, 512), (stride, 1)), (offset, (3, 384), (stride, 1)))
+        with pytest.raises(RuntimeError, match="out is the start of qkv's rows, or apart"):
+            _append(qkv, out)
+    for a, b in (((0, (3, 512), (1024, 1)), (512, (3, 384), (1024, 1))), ((0, (3, 512), (512, 1)), (0, (3, 384), (512, 1))), ((0, (1, 512), (8, 1)), (512, (1, 384), (8, 1)))):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            _append(*_views(8192, a, b))
+
+
+def test_append_k_across_v():
+    pool = torch.zeros(6, 16, 2, 2, 64, dtype=BF)
+    qkv = torch.zeros(3, 512, dtype=BF)
+    for k, v in ((pool[:, :, 0], pool[:, :, 0]), (pool[:5, :, 0], pool[1:, :, 0]), (pool[:, :8, 0], pool[:, 4:12, 0])):
+        with pytest.raises(RuntimeError, match="k apart from v"):
+            _append(qkv, None, k, v)
+    flat = torch.zeros(6, 16, 2, 64, dtype=BF)
+    for k, v in ((pool[:, :, 0], pool[:, :, 1]), (pool[:, :8, 0], pool[:, 8:, 0]), (flat[:3], flat[3:]), (pool[..., 0, :], pool[..., 1, :]), (pool[:, :, 0, :, :32], pool[:, :, 0, :, 32:])):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            _append(qkv[:, :8 * k.shape[3]], None, k, v)

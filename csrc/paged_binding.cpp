@@ -158,14 +158,25 @@ void bind_paged(py::module_& m) {
          "page_tables: free [pages] and free_count [1] int32");
     need(page_size >= 1 && page_size < (1ll << 30) && W < (1ll << 31), "page_tables: page size");
     need(tokens >= 0 && tokens < (1ll << 31) - 8, "page_tables: tokens");
-    for (const at::Tensor* t : {&lengths, &free, &free_count, &table})
-      need(t->data_ptr() != news.data_ptr(), "page_tables: new tokens in a tensor of their own");
     if (out.has_value()) {
       const auto& [slots, positions, offsets, granted] = *out;
       need(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.dim() == 1 && slots.numel() == tokens && ints(positions, tokens) &&
                ints(offsets, R + 1) && granted.scalar_type() == at::kBool && granted.is_contiguous() && granted.dim() == 1 && granted.numel() == R,
            "page_tables: out is (slots [tokens] int64, positions [tokens] int32, offsets [rows + 1] int32, granted [rows] bool)");
       need(aligned(slots) && aligned(positions), "page_tables: 16-byte aligned slots and positions");
+    }
+    {  // (the state is read and written by different CTAs, new by some after others have written)
+      const at::Tensor* all[9] = {&table, &lengths, &free, &free_count, &news};
+      int n = 5;
+      if (out.has_value())
+        for (const at::Tensor* t : {&std::get<0>(*out), &std::get<1>(*out), &std::get<2>(*out), &std::get<3>(*out)}) all[n++] = t;
+      std::pair<uintptr_t, uintptr_t> in[9];
+      for (int i = 0; i < n; ++i) {
+        in[i] = bounds(*all[i]);
+        for (int j = 0; j < i; ++j)
+          need(all[i]->numel() == 0 || all[j]->numel() == 0 || in[i].second <= in[j].first || in[j].second <= in[i].first,
+               "page_tables: table, lengths, free, free_count, new tokens and out in memory of their own");
+      }
     }
     on_device(table, {&lengths, &free, &free_count, &news}, "page_tables expects tensors on one CUDA device");
     const at::cuda::OptionalCUDAGuard guard(table.device());

@@ -42,7 +42,8 @@ def page_tables(table, lengths, free, free_count, new, page_size: int, tokens: i
     """Lets new[r] tokens come to row r, or its last -new[r] leave, and moves the pages that follow from it.
 
     table [rows, pages of a row] int32, lengths [rows] int32: the sequences; free [pages] int32 with free_count [1] int32: a
-    stack of the pages that no row has, its top at free_count - 1.  All four are updated in place.  new: [rows] int32.
+    stack of the pages that no row has, its top at free_count - 1.  All four are updated in place.  new: [rows] int32.  No two of
+    these tensors and of out's share memory.
 
     Pages of tokens that leave are put on the stack first, rows and pages in descending order; then pages are taken from it,
     rows and pages ascending (so what comes and leaves again is back in its old place).  A row is granted its new

@@ -97,3 +97,21 @@ def test_append_k_across_v():
     for k, v in ((pool[:, :, 0], pool[:, :, 1]), (pool[:, :8, 0], pool[:, 8:, 0]), (flat[:3], flat[3:]), (pool[..., 0, :], pool[..., 1, :]), (pool[:, :, 0, :, :32], pool[:, :, 0, :, 32:])):
         with pytest.raises(RuntimeError, match="CUDA"):
             _append(qkv[:, :8 * k.shape[3]], None, k, v)
+
+
+def test_tables_of_their_own():
+    def call(**over):
+        a = dict(table=ints(3, 4), lengths=ints(3), free=ints(10), free_count=ints(1), new=ints(3), page_size=16, tokens=8, out=None) | over
+        P.page_tables(**a)
+    flat = ints(64)
+    slots = torch.zeros(16, dtype=torch.int64)
+    step = lambda **o: tuple((dict(slots=slots[:8], positions=ints(8), offsets=ints(4), granted=torch.zeros(3, dtype=torch.bool)) | o).values())  # noqa: E731
+    for over in (dict(lengths=flat[:3], new=flat[2:5]), dict(free=flat[:10], new=flat[9:12]), dict(free_count=flat[1:2], new=flat[:3]), dict(table=flat[:12].view(3, 4), new=flat[8:11]),
+                 dict(lengths=flat[:3], free=flat[1:11]), dict(new=flat[:3], out=step(positions=flat[:8])), dict(lengths=flat[:3], out=step(offsets=flat[2:6])),
+                 dict(out=step(positions=slots.view(torch.int32)[8:16])), dict(out=step(granted=slots.view(torch.bool)[:3]))):
+        with pytest.raises(RuntimeError, match="of their own"):
+            call(**over)
+    for over in (dict(lengths=flat[:3], new=flat[3:6], free=flat[6:16], free_count=flat[16:17], table=flat[20:32].view(3, 4), out=step(positions=flat[32:40], offsets=flat[40:44])),
+                 dict(tokens=0, out=step(slots=slots[:0], positions=flat[:0])), dict(table=flat[:24].view(3, 8)[:, :4], lengths=flat[24:27])):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call(**over)

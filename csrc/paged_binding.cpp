@@ -86,9 +86,11 @@ struct Runs {
 };
 // From a tensor's first byte to behind its last.
 std::pair<uintptr_t, uintptr_t> bounds(const at::Tensor& t) {
+  const auto sizes = t.sizes(), strides = t.strides();
   int64_t n = 1;
-  for (int i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
-  return {(uintptr_t)t.data_ptr(), (uintptr_t)t.data_ptr() + n * t.element_size()};
+  for (size_t i = 0; i < sizes.size(); ++i) n += (sizes[i] - 1) * strides[i];
+  const uintptr_t at = (uintptr_t)t.data_ptr();
+  return {at, at + n * t.element_size()};
 }
 // Do runs of a and runs of b, both laid out by dims[i...], meet if b's are `off` bytes further?
 bool meet_at(const Runs& a, const Runs& b, size_t i, int64_t off) {

@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <utility>
 #include <vector>
@@ -150,7 +151,8 @@ void bind_paged(py::module_& m) {
   // Tokens come (news[r] > 0) and leave (news[r] < 0, the last ones): table, lengths, free and free_count in place; returns or
   // fills (slots [tokens] int64, positions [tokens] int32, offsets [rows + 1] int32, granted [rows] bool).
   m.def("page_tables", [](at::Tensor table, at::Tensor lengths, at::Tensor free, at::Tensor free_count, at::Tensor news, int64_t page_size,
-                          int64_t tokens, c10::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>> out) {
+                          int64_t tokens, c10::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>> out,
+                          c10::optional<int64_t> max_len) {
     need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1, "page_tables: table [rows, pages of a row] int32");
     const int64_t R = table.size(0), W = table.size(1);
     need(R <= kPagedMaxRows, "page_tables: more than PAGED_MAX_ROWS rows");
@@ -160,6 +162,7 @@ void bind_paged(py::module_& m) {
          "page_tables: free [pages] and free_count [1] int32");
     need(page_size >= 1 && page_size < (1ll << 30) && W < (1ll << 31), "page_tables: page size");
     need(tokens >= 0 && tokens < (1ll << 31) - 8, "page_tables: tokens");
+    need(!max_len.has_value() || *max_len >= 0, "page_tables: max_len");
     if (out.has_value()) {
       const auto& [slots, positions, offsets, granted] = *out;
       need(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.dim() == 1 && slots.numel() == tokens && ints(positions, tokens) &&
@@ -198,11 +201,12 @@ void bind_paged(py::module_& m) {
     on_device(table, {&slots, &positions, &offsets, &granted}, "page_tables expects tensors on one CUDA device");
     const PageTables a = {table.data_ptr<int>(), table.stride(0), lengths.data_ptr<int>(), free.data_ptr<int>(), free_count.data_ptr<int>(),
                           news.data_ptr<int>(), (long long*)slots.data_ptr<int64_t>(), positions.data_ptr<int>(), offsets.data_ptr<int>(),
-                          granted.data_ptr<bool>(), (int)R, (int)W, (int)free.numel(), (int)page_size, (int)tokens};
+                          granted.data_ptr<bool>(), (int)R, (int)W, (int)free.numel(), (int)page_size, (int)tokens,
+                          (int)std::min<int64_t>(max_len.value_or(INT_MAX), INT_MAX)};
     ck(launch_page_tables(a, cur()), "page_tables");
     return *out;
   }, py::arg("table"), py::arg("lengths"), py::arg("free"), py::arg("free_count"), py::arg("new"), py::arg("page_size"), py::arg("tokens"),
-     py::arg("out") = py::none());
+     py::arg("out") = py::none(), py::arg("max_len") = py::none());
   // qkv [tokens, (heads + 2 kv_heads) dim]: q and k rotated in place or into out [tokens, (heads + kv_heads) dim], k and v to their slots.
   m.def("paged_append", [](at::Tensor qkv, at::Tensor k, at::Tensor v, at::Tensor slots, at::Tensor positions, int64_t heads, double theta,
                            OptTensor out, OptTensor k_scale, OptTensor v_scale, bool early) {

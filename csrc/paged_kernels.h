@@ -30,6 +30,7 @@ struct PageTables {
   int *positions, *offsets;
   bool* granted;
   int rows, width, pages, page_size, tokens;
+  int max_len;  // positions that a row may be granted, at most
 };
 cudaError_t launch_page_tables(const PageTables& a, cudaStream_t stream);
 

@@ -6,7 +6,7 @@
 // matter of prefix sums over the rows, so any order of execution gives the same tables:
 //   leaving tokens  the k-th released page, rows and pages ascending, of `pushed` goes to place count + pushed - 1 - k
 //   coming tokens   the k-th new page comes from place count + pushed - 1 - k
-// (What comes and leaves again is back in its old place.)  A row is granted its tokens if the table row holds them, they end
+// (What comes and leaves again is back in its old place.)  A row is granted its tokens if it may be that long, they end
 // inside `tokens`, and the stack has pages for it and all rows before it that pass these two tests.
 //
 // One launch: every CTA of a cluster sums over all rows by itself (8 bytes a row, read from L2), the cluster's barrier stands
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, rank = blockIdx.x;
-  const long long most = min((long long)a.width * a.page_size, 2147483647ll);
+  const long long most = min((long long)a.width * a.page_size, 2147483647ll), longest = min(most, (long long)a.max_len);
   const int count = max(0, min(*a.free_count, a.pages));
   const int r0 = tid * kPer;
   auto gone_of = [&](int old, int n) { return n < 0 ? pages_of(div, old) - pages_of(div, (int)max(0ll, (long long)old + n)) : 0; };
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
     first_gone[i] = (int)gone;
     end = add(end, max(0, n[i]));
     gone = add(gone, gone_of(old[i], n[i]));
-    granted[i] = n[i] <= 0 || (old[i] + (long long)n[i] <= most && end <= (uint32_t)a.tokens);
+    granted[i] = n[i] <= 0 || (old[i] + (long long)n[i] <= longest && end <= (uint32_t)a.tokens);
     if (n[i] > 0 && granted[i]) need[0] = add(need[0], pages_of(div, old[i] + n[i]) - pages_of(div, old[i]));
   }
   block_sums(need, all_need, s_one);

@@ -38,7 +38,8 @@ class OutOfPages(RuntimeError):
         self.rows, self.next_tokens = rows, next_tokens
 
 
-def page_tables(table, lengths, free, free_count, new, page_size: int, tokens: int, out: Optional[PageStep] = None) -> PageStep:
+def page_tables(table, lengths, free, free_count, new, page_size: int, tokens: int, out: Optional[PageStep] = None,
+                max_len: Optional[int] = None) -> PageStep:
     """Lets new[r] tokens come to row r, or its last -new[r] leave, and moves the pages that follow from it.
 
     table [rows, pages of a row] int32, lengths [rows] int32: the sequences; free [pages] int32 with free_count [1] int32: a
@@ -46,12 +47,13 @@ def page_tables(table, lengths, free, free_count, new, page_size: int, tokens: i
     these tensors and of out's share memory.
 
     Pages of tokens that leave are put on the stack first, rows and pages in descending order; then pages are taken from it,
-    rows and pages ascending (so what comes and leaves again is back in its old place).  A row is granted its new
-    tokens if its table row can hold them, they end inside `tokens`, and there are pages for it and every row before it that
-    passes these two tests; one that is not keeps its length, and its slots are -1.  A row that gets no tokens is granted.
+    rows and pages ascending (so what comes and leaves again is back in its old place).  A row is granted its new tokens if its
+    table row can hold them and it gets no longer than max_len (None: what the table row holds), they end inside `tokens`, and there
+    are pages for it and every row before it that passes these tests; one that is not keeps its length, and its slots are -1.  A
+    row that gets no tokens is granted.
     At most 8192 rows.  `tokens` may exceed the sum of new (a captured step's fixed number).  Entries of a table row behind its
     pages, and of free from free_count on, say nothing."""
-    return PageStep._make(ops.page_tables(table, lengths, free, free_count, new, page_size, tokens, out))
+    return PageStep._make(ops.page_tables(table, lengths, free, free_count, new, page_size, tokens, out, max_len))
 
 
 def paged_append(qkv, k, v, slots, positions, heads: int, theta: float, out=None, k_scale=None, v_scale=None, early: bool = False) -> None:
@@ -122,7 +124,7 @@ class PagedKVCache:
 
     def advance(self, new: torch.Tensor, tokens: int, out: Optional[PageStep] = None) -> PageStep:
         """`page_tables` on this cache: new[r] tokens come to row r or its last -new[r] leave (-lengths[r]: the row is free)."""
-        return page_tables(self.table, self.lengths, self.free, self.free_count, new, self.page_size, tokens, out)
+        return page_tables(self.table, self.lengths, self.free, self.free_count, new, self.page_size, tokens, out, self.max_len)
 
     def append(self, layer: int, qkv: torch.Tensor, step: PageStep, heads: int, theta: float, out: Optional[torch.Tensor] = None,
                early: bool = False) -> None:

@@ -242,8 +242,9 @@ void bind_paged(py::module_& m) {
   m.def("paged_attention_workspace_bytes", [](int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_len, int64_t window) {
     need(rows >= 1 && kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && dim >= 1 && max_len >= 1 && window >= 0,
          "paged_attention_workspace_bytes: rows, heads and lengths");
-    need(rows < (1 << 24) && heads < (1 << 20) && max_len < (1ll << 31), "paged_attention_workspace_bytes: rows, heads and lengths");
-    return (int64_t)paged_attention_workspace_bytes((int)rows, (int)heads, (int)kv_heads, (int)dim, (int)max_len, (int)std::min<int64_t>(window, 1ll << 30),
+    need(rows < (1 << 24) && heads < (1 << 20) && dim <= 256, "paged_attention_workspace_bytes: rows, heads and dim");
+    return (int64_t)paged_attention_workspace_bytes((int)rows, (int)heads, (int)kv_heads, (int)dim, (int)std::min<int64_t>(max_len, paged::kMaxLen),
+                                                    (int)std::min<int64_t>(window, 1ll << 30),
                                                     sms_of(at::cuda::current_device()));
   }, py::arg("rows"), py::arg("heads"), py::arg("kv_heads"), py::arg("dim"), py::arg("max_len"), py::arg("window") = 0);
   // q [rows, heads, dim], one token of every row, attends to the row's last `window` positions (0: all of them).
@@ -290,7 +291,7 @@ void bind_paged(py::module_& m) {
     if (B == 0) return *out;
     const int sms = sms_of(q.get_device());
     const int win = (int)std::min<int64_t>(window, 1ll << 30);
-    const int max_len = (int)std::min<int64_t>(table.size(1) * pool.page_size, 0x7fff0000ll);
+    const int max_len = (int)std::min<int64_t>(table.size(1) * pool.page_size, paged::kMaxLen);
     need(B * (int64_t)paged::units_of(win > 0 && win < max_len ? win : max_len, 16) <= paged::kMaxUnits, "paged_attention: a table for over 2^34 positions");
     const size_t bytes = paged_attention_workspace_bytes((int)B, (int)H, pool.heads, pool.dim, max_len, win, sms);
     if (workspace.has_value()) need(workspace->nbytes() >= bytes, "workspace too small (paged_attention_workspace_bytes)");

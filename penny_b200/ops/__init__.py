@@ -20,7 +20,8 @@ from typing import Optional
 import torch
 
 _BACKEND = None
-_PAGED = ("PagedKVCache", "PageStep", "OutOfPages", "page_tables", "paged_append", "paged_attention")
+_PAGED = ("PagedKVCache", "PageStep", "OutOfPages", "page_tables", "paged_append", "paged_attention",
+          "paged_attention_workspace_bytes")
 
 
 def __getattr__(name):

@@ -84,6 +84,11 @@ def paged_attention(q, k, v, table, lengths, out=None, lse=None, scale: Optional
     return ops.paged_attention(q, k, v, table, lengths, out, lse, scale, window, k_scale, v_scale, workspace, early)
 
 
+def paged_attention_workspace_bytes(rows: int, heads: int, kv_heads: int, dim: int, max_len: int, window: int = 0) -> int:
+    """Bytes of a workspace for `paged_attention` on the current device, for tables of max_len positions a row (0: none is needed)."""
+    return ops.paged_attention_workspace_bytes(rows, heads, kv_heads, dim, max_len, window)
+
+
 class PagedKVCache:
     """The pools of `layers` layers, one table for all of them, and the pages that are free.
 

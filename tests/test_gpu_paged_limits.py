@@ -43,3 +43,21 @@ def test_decoder_ends_at_max_len():
     with pytest.raises(RuntimeError, match="50 positions"):
         m.step(torch.tensor([1, 2]))
     assert m.paged.lengths.tolist() == [50, 50]
+
+
+def test_tables_past_two_to_the_31_positions():
+    """A workspace for a table that could hold more positions than a row can have, and the attention with it and without."""
+    c = P.PagedKVCache(1, 1, 2 ** 31, 1, 64, page_size=1 << 16, pages=2)
+    assert c.table.shape[1] * c.page_size == 2 ** 31
+    step = c.advance(_ints(70000), 70000)
+    qkv = torch.randn(70000, 6 * 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).bfloat16()
+    c.append(0, qkv, step, 4, 1e4)
+    q = qkv[-1:, :256].unflatten(1, (4, 64))
+    ws = c.workspace(4)
+    assert ws.numel() == P.paged_attention_workspace_bytes(1, 4, 1, 64, 2 ** 31) == P.paged_attention_workspace_bytes(1, 4, 1, 64, 2 ** 40) > 0
+    out = c.attend(0, q, workspace=ws)
+    assert torch.equal(out, c.attend(0, q))
+    k, v = (t[0].double() for t in c.rows_of(0, 0, 70000))
+    p = (q[0].double() @ k.t() / 8).softmax(-1)
+    want, size = p @ v, p @ v.abs()
+    assert ((out[0].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -12) * size + 2.0 ** -8 * want.abs()).all()  # (a weight and the output rounded)

@@ -88,6 +88,8 @@ class LlamaTPDecoder:
         row.  A row for which there is no page is left out of a step, which raises OutOfPages when it has waited for the device."""
         if page_size < 0 or (page_size == 0 and (pages is not None or cache_dtype is not None)):
             raise ValueError("pages and cache_dtype belong to a cache in pages: page_size above 0")
+        if cache_dtype not in (None, torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError("cache_dtype: bf16 or e4m3, beside a bf16 projection")
         assert cfg.heads % world == 0 and cfg.kv_heads % world == 0 and cfg.ffn % world == 0
         assert cfg.vocab % world == 0 and cfg.head_dim == 128 and (cfg.ffn // world) % 64 == 0
         assert backend in ("penny", "penny_unfused", "nccl") and linears in ("auto", "penny", "cublas")

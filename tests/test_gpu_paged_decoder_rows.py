@@ -93,3 +93,9 @@ def test_release():
             m.release(bad)
     with pytest.raises(ValueError):
         LlamaTPDecoder(LlamaConfig.tiny(), world=1, max_batch=3, max_len=64, full_init=True).release([0])
+
+
+def test_caches_that_the_decoder_cannot_have():
+    for over in (dict(cache_dtype=torch.float16), dict(cache_dtype=torch.float32)):
+        with pytest.raises(ValueError):
+            _model(**over)

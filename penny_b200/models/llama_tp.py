@@ -82,12 +82,14 @@ class LlamaTPDecoder:
     def __init__(self, cfg: LlamaConfig, comm=None, rank: int = 0, world: int = 1, max_batch: int = 64,
                  max_len: int = 2560, backend: str = "penny", proto: str = "auto", seed: int = 0,
                  use_graph: bool = True, full_init: bool = False, process_group=None, linears: str = "auto",
-                 pdl: bool = True, page_size: int = 0, pages: Optional[int] = None, cache_dtype: Optional[torch.dtype] = None):
+                 pdl: bool = True, page_size: int = 0, pages: Optional[int] = None, cache_dtype: Optional[torch.dtype] = None,
+                 cache_scales: Optional[tuple] = None):
         """page_size > 0: KV cache in pages of that many positions, `pages` of them (by default enough for max_batch sequences
-        of max_len), of cache_dtype (bf16 or e4m3).  `positions` are that cache's lengths then; every step lets one token come to every
+        of max_len), of cache_dtype (bf16 or e4m3; cache_scales: its (k_scale, v_scale), as PagedKVCache takes them).  `positions` are
+        that cache's lengths then; every step lets one token come to every
         row.  A row for which there is no page is left out of a step, which raises OutOfPages when it has waited for the device."""
-        if page_size < 0 or (page_size == 0 and (pages is not None or cache_dtype is not None)):
-            raise ValueError("pages and cache_dtype belong to a cache in pages: page_size above 0")
+        if page_size < 0 or (page_size == 0 and (pages is not None or cache_dtype is not None or cache_scales is not None)):
+            raise ValueError("pages, cache_dtype and cache_scales belong to a cache in pages: page_size above 0")
         if cache_dtype not in (None, torch.bfloat16, torch.float8_e4m3fn):
             raise ValueError("cache_dtype: bf16 or e4m3, beside a bf16 projection")
         assert cfg.heads % world == 0 and cfg.kv_heads % world == 0 and cfg.ffn % world == 0
@@ -189,7 +191,8 @@ class LlamaTPDecoder:
         self.next_tokens = torch.zeros(B, dtype=torch.int64, device=self.dev)
         self.paged: Optional[PagedKVCache] = None
         if page_size > 0:
-            self.paged = PagedKVCache(cfg.layers, B, max_len, self.Hkv, D, page_size, pages, cache_dtype or dt, device=self.dev)
+            self.paged = PagedKVCache(cfg.layers, B, max_len, self.Hkv, D, page_size, pages, cache_dtype or dt, *(cache_scales or (None, None)),
+                                      device=self.dev)
             self.page_step = PageStep(torch.full((B,), -1, dtype=torch.int64, device=self.dev), torch.zeros(B, dtype=torch.int32, device=self.dev),
                                       torch.zeros(B + 1, dtype=torch.int32, device=self.dev), torch.ones(B, dtype=torch.bool, device=self.dev))
             self.one_each = torch.ones(B, dtype=torch.int32, device=self.dev)
@@ -336,10 +339,13 @@ class LlamaTPDecoder:
             if not bool(step.granted.all()):
                 raise RuntimeError(f"{self.paged.pages} pages of {self.paged.page_size} positions do not hold {self.B} x {kv_len}")
         for li in range(self.cfg.layers):
-            for cache in (self.paged.k[li], self.paged.v[li]) if self.paged is not None else (self.kcache[li], self.vcache[li]):
+            for i, cache in enumerate((self.paged.k[li], self.paged.v[li]) if self.paged is not None else (self.kcache[li], self.vcache[li])):
                 rows = torch.randn(self.B, self.Hkv, kv_len, self.cfg.head_dim, device=self.dev, generator=g, dtype=torch.float32)
                 if self.paged is not None:
-                    rows = rows.transpose(1, 2).reshape(self.B * kv_len, self.Hkv, -1).to(cache.dtype)
+                    rows = rows.transpose(1, 2).reshape(self.B * kv_len, self.Hkv, -1)
+                    if self.paged.e4m3:
+                        rows = (rows / (self.paged.k_scale, self.paged.v_scale)[i][li][:, None]).clamp(-448, 448)
+                    rows = rows.to(cache.dtype)
                     cache.view(torch.uint8).view(-1, self.Hkv, rows.shape[2] * rows.element_size())[step.slots] = rows.view(torch.uint8)
                 else:
                     cache[:, :, :kv_len].copy_(rows.to(torch.bfloat16))

@@ -121,6 +121,8 @@ class PagedKVCache:
             scales.append(list(s) if isinstance(s, (list, tuple)) else [s] * layers)
             if len(scales[-1]) != layers:
                 raise ValueError("PagedKVCache: one scale tensor for all layers, or one for each")
+            if self.e4m3 and any(t.dtype != torch.float32 or t.shape != (kv_heads,) for t in scales[-1]):
+                raise ValueError("PagedKVCache: scales [kv_heads] fp32")
         self.k_scale, self.v_scale = scales
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=self.device)
         self.lengths = torch.zeros(rows, dtype=torch.int32, device=self.device)

@@ -95,7 +95,29 @@ def test_release():
         LlamaTPDecoder(LlamaConfig.tiny(), world=1, max_batch=3, max_len=64, full_init=True).release([0])
 
 
+@pytest.mark.parametrize("graph", [True, False])
+def test_scales_of_an_8_bit_cache(graph):
+    """Scales that are not one, a tensor for all layers or one for each: logits over what the cache holds, before and after a step."""
+    cfg = LlamaConfig.tiny()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    k = 0.01 + 0.02 * torch.rand(cfg.kv_heads, device="cuda", generator=g)
+    v = [0.01 + 0.02 * torch.rand(cfg.kv_heads, device="cuda", generator=g) for _ in range(cfg.layers)]
+    m = _model(cache_dtype=E4M3, cache_scales=(k, v), use_graph=graph)
+    m.fill_synthetic_kv(40)
+    assert m.paged.k_scale[1] is k and m.paged.v_scale[1] is v[1]
+    for li in (0, 1):
+        for t in m.paged.rows_of(li, 0, 40):  # normal values, 2 ** -4 of each at most from them: and not 50 times too small
+            assert 0.9 < t.std() < 1.1 and t.abs().max() < 6
+    m.capture()
+    out = m.step(torch.tensor([3, 4, 5])).tolist()
+    _near(m, [3, 4, 5], [40, 40, 40], [0, 1, 2])
+    m.step(torch.tensor(out))
+    _near(m, out, [41, 41, 41], [0, 1, 2])
+
+
 def test_caches_that_the_decoder_cannot_have():
-    for over in (dict(cache_dtype=torch.float16), dict(cache_dtype=torch.float32)):
+    one = torch.ones(LlamaConfig.tiny().kv_heads, device="cuda")
+    for over in (dict(cache_dtype=torch.float16), dict(cache_dtype=torch.float32), dict(cache_scales=(one, one)), dict(cache_dtype=E4M3, cache_scales=(one, one[1:])),
+                 dict(cache_dtype=E4M3, cache_scales=(one.double(), one)), dict(page_size=0, cache_scales=(one, one))):
         with pytest.raises(ValueError):
             _model(**over)

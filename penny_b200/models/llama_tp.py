@@ -342,7 +342,7 @@ class LlamaTPDecoder:
             for i, cache in enumerate((self.paged.k[li], self.paged.v[li]) if self.paged is not None else (self.kcache[li], self.vcache[li])):
                 rows = torch.randn(self.B, self.Hkv, kv_len, self.cfg.head_dim, device=self.dev, generator=g, dtype=torch.float32)
                 if self.paged is not None:
-                    rows = rows.transpose(1, 2).reshape(self.B * kv_len, self.Hkv, -1)
+                    rows = rows.transpose(1, 2).reshape(self.B * kv_len, self.Hkv, self.cfg.head_dim)
                     if self.paged.e4m3:
                         rows = (rows / (self.paged.k_scale, self.paged.v_scale)[i][li][:, None]).clamp(-448, 448)
                     rows = rows.to(cache.dtype)

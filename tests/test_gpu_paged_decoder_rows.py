@@ -121,3 +121,19 @@ def test_caches_that_the_decoder_cannot_have():
                  dict(cache_dtype=E4M3, cache_scales=(one.double(), one)), dict(page_size=0, cache_scales=(one, one))):
         with pytest.raises(ValueError):
             _model(**over)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_empty_rows_at_the_start(dtype):
+    """A cache that is filled with nothing: the first tokens are at position 0."""
+    m = _model(cache_dtype=dtype, use_graph=False)
+    m.fill_synthetic_kv(0)
+    assert m.paged.lengths.tolist() == [0] * 3 and int(m.paged.free_count) == m.paged.pages
+    m.step(torch.tensor([3, 4, 5]))
+    # one position: the last layer's attention is its value, as it is stored (which in 8 bits is up to 2 ** -4 from the fp32 model's)
+    value = torch.stack([m.paged.rows_of(m.cfg.layers - 1, b, 1)[1][:, 0] for b in range(3)])
+    assert torch.equal(m.attn.view(3, m.Hkv, -1, m.cfg.head_dim).float(), value.float()[:, :, None].expand(-1, -1, m.Hq // m.Hkv, -1))
+    if dtype == torch.bfloat16:
+        _near(m, [3, 4, 5], [0] * 3, [0, 1, 2])
+        m.step(torch.tensor([7, 8, 9]))
+        _near(m, [7, 8, 9], [1] * 3, [0, 1, 2])

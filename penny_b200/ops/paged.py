@@ -156,8 +156,12 @@ class PagedKVCache:
 
     def rows_of(self, layer: int, row: int, length: int):
         """(k, v) [kv_heads, length, head_dim] of a row's first positions, e4m3 ones times their scales in fp32: a copy, for looking at."""
+        if not 0 <= length <= self.table.shape[1] * self.page_size:
+            raise IndexError(f"rows_of: a row has {self.table.shape[1] * self.page_size} positions at most")
         at = torch.arange(length, device=self.device)
         pages, within = self.table[row].long()[at // self.page_size], at % self.page_size
+        if bool(((pages < 0) | (pages >= self.pages)).any()):
+            raise IndexError("rows_of: positions that are on no page of the pool")
         got = []
         for pool, scale in ((self.k[layer], self.k_scale[layer]), (self.v[layer], self.v_scale[layer])):
             rows = pool.view(torch.uint8)[pages, within].view(pool.dtype) if self.e4m3 else pool[pages, within]

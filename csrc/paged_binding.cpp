@@ -57,6 +57,7 @@ PagedPool pool_of(const at::Tensor& k, const at::Tensor& v, PagedType type, Page
   if (cache == PAGED_E4M3) {
     for (const at::Tensor* s : {&*k_scale, &*v_scale})
       need(s->scalar_type() == at::kFloat && s->is_contiguous() && s->dim() == 1 && s->numel() == k.size(2), "k_scale and v_scale: [kv_heads] fp32");
+    need(no_grad(*k_scale) && no_grad(*v_scale), "paged caches: no gradients");
     p.k_scale = k_scale->data_ptr<float>();
     p.v_scale = v_scale->data_ptr<float>();
   }
@@ -223,7 +224,7 @@ void bind_paged(py::module_& m) {
     need(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.dim() == 1 && slots.numel() == T && ints(positions, T),
          "paged_append: slots [tokens] int64, positions [tokens] int32");
     need(theta > 0 && std::isfinite(theta), "paged_append: theta above zero");
-    need(no_grad(qkv), "paged_append: no gradients");
+    need(no_grad(qkv) && (!out.has_value() || no_grad(*out)), "paged_append: no gradients");
     if (out.has_value())
       need(out->scalar_type() == qkv.scalar_type() && out->dim() == 2 && out->size(0) == T && out->size(1) == (heads + pool.heads) * D &&
                out->stride(1) == 1 && (T <= 1 || (out->stride(0) >= out->size(1) && out->stride(0) % 8 == 0)) && aligned(*out),
@@ -276,7 +277,7 @@ void bind_paged(py::module_& m) {
     need(ints(lengths, B), "paged_attention: lengths [rows] int32");
     need(window >= 0, "paged_attention: a window of no or some positions");
     need(!scale.has_value() || std::isfinite((float)*scale), "paged_attention: a finite scale");
-    need(no_grad(q), "paged_attention: no gradients");
+    need(no_grad(q) && (!out.has_value() || no_grad(*out)) && (!lse.has_value() || no_grad(*lse)), "paged_attention: no gradients");
     if (out.has_value())
       need(out->scalar_type() == q.scalar_type() && out->sizes() == q.sizes() && rows_ok(*out) && apart(*out), "paged_attention: out like q, its rows apart");
     if (out.has_value()) need(!overlap(*out, q) || same_place(*out, q), "paged_attention: out is q, or apart from it");

@@ -9,8 +9,8 @@
 // cosines are computed once and shared by its heads.
 //
 // Bound by memory: every value is read and written once.  A block has a token, a thread two pairs of 16 bytes at a time, the first
-// of which are on their way while the angles are computed.  16384 tokens of 32 + 2 * 8 heads of 128 bf16 values: 72 us, 6.1 TB/s
-// (with the loads behind the angles 88, with four tokens to a block of 448 threads 92); 64 tokens 2.7 us.
+// of which are on their way while the angles are computed.  16384 tokens of 32 + 2 * 8 heads of 128 bf16 values: 72 to 74 us,
+// 6 TB/s (with the loads behind the angles 88, with four tokens to a block of 448 threads 92); 64 tokens 2.9 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -120,6 +120,7 @@ __device__ __forceinline__ void store8(void* pool, long long at, const float (&x
   }
 }
 
+// (64 registers, so that an SM holds eight blocks of 128 threads: 2047 tokens, e4m3, 8.6 us, with 73 registers 10.4)
 template <typename T, bool kE4M3>
 __global__ void __launch_bounds__(kMaxThreads, 4) k_paged_append(T* qkv, long long qkv_stride, T* out, long long out_stride, const PagedPool pool,
                                                               const long long* slots, const int* positions, int heads, int items, bool early,
@@ -203,7 +204,7 @@ cudaError_t launch(void* qkv, long long qkv_stride, void* out, long long out_str
   for (int d = 0; d < pool.dim / 2; ++d, f *= step) turns.of[d] = f;
   const int items = (heads + 2 * pool.heads) * (pool.dim / 16);
   // few tokens: as many threads as have work (64 tokens of 448 items: 2.5 us with 224 threads, 3.0 with 128); many: small blocks, of
-  // which an SM holds more (16384 tokens 74 and 76 us)
+  // which an SM holds more (16384 tokens 3 % less time)
   const int most = tokens >= 148 * 8 ? 128 : kMaxThreads, threads = std::min(most, (items + 32 * kItems - 1) / (32 * kItems) * 32);
   return launch_kernel_ex(k_paged_append<T, kE4M3>, dim3(tokens), dim3(threads), 0, stream, true, 1, (T*)qkv, qkv_stride, (T*)(out ? out : qkv),
                           out ? out_stride : qkv_stride, pool, slots, positions, heads, items, early, paged::page_div(pool.dim / 16), turns);

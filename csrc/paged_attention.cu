@@ -32,10 +32,11 @@
 //     that stood 17.4 under another one were lost whole.  Weights count from a base near the maximum so far.  Where they are
 //     finer than the output (e4m3 caches with a bf16 q) it follows when it is exceeded by 2^8, which is seldom (64 rows of 4096, 28
 //     of 2 heads: 34.4 us, always 38.1).  Elsewhere it follows always, so that the largest weight is one and not off: 64 rows of 2048,
-//     bf16, are 0.0018 of the output's norm from 64 bits (its own rounding: 0.0017), otherwise 0.0022 (and 0.5 us faster).
+//     bf16, are 0.00183 of the output's norm from 64 bits (its own rounding: 0.00166; the rest is P's), otherwise 0.0022 (and 0.5 us
+//     faster).
 //
-// Bound by memory: 64 rows of 2048 positions, 32 of 8 heads of 128, bf16, 84.5 us (6.4 TB/s), 64 of 16000 589 (7.1); few or short rows by
-// a chain of latencies: 6.6 us for one row of 200, 9.7 for one of 2048.
+// Bound by memory: 64 rows of 2048 positions, 32 of 8 heads of 128, bf16, 85 us (6.3 TB/s), 64 of 16000 598 (7.0); few or short rows by
+// a chain of latencies: 6.6 us for one row of 200, 9.4 for one of 2048.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -25,7 +25,7 @@ from .._ext import ops
 class PageStep(NamedTuple):
     """Where the tokens of a step go, rows one behind the other."""
     slots: torch.Tensor      # [tokens] int64: page * page_size + offset; -1 behind the last token and where not granted
-    positions: torch.Tensor  # [tokens] int32: position in the sequence (0 where the slot is -1)
+    positions: torch.Tensor  # [tokens] int32: position in the sequence (0 behind the last token and where not granted)
     offsets: torch.Tensor    # [rows + 1] int32: row r's tokens are [offsets[r], offsets[r + 1])
     granted: torch.Tensor    # [rows] bool
 

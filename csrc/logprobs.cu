@@ -1,0 +1,323 @@
+// Log probabilities of given tokens under the softmax of their logits, its entropy, and its likeliest tokens.
+//
+// With m = max x, Z = sum exp(x - m):  log p(t) = x_t - m - log Z,  entropy = log Z - (sum exp(x - m) (x - m)) / Z.
+// One pass over the logits: every thread keeps a maximum and the two sums (fp32), which are scaled when the maximum grows;
+// threads, warps and the CTAs of a row's cluster are joined by the same rule.  The sums are taken of x - m and not of x, so that an
+// fp32 logit loses nothing against a far maximum.
+//
+// The likeliest tokens are found in the same pass.  Of a CTA's first values the largest ones of 64 groups of lanes are ranked: at least
+// `top` values of the row are as large as the top-th of those, and few others (about 190 of 128256 at a top of 20).  What is as large
+// goes to a list of its warp, as a number that orders by value and then by lowest id; a list that is full keeps its largest `top`, of
+// which the smallest is the new bound (a row in ascending order takes a full list for every 64 values, and stays right).  At the end
+// every number on the lists counts those above it, which is its place.
+//
+// Few rows: a row's cluster has up to eight CTAs, whose sums and lists meet in the first one's shared memory.
+//
+// Bound by memory where rows are many (a value takes about six instructions and one exponential, three quarters of what an SM can do
+// in the time), by latency where they are few.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "logprobs.h"
+#include "pdl.h"
+
+namespace penny {
+namespace {
+
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBatch = 32;  // kBatch: values of a thread at a time
+constexpr int kGroups = 64, kList = 96, kMaxCluster = 8;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+static_assert(kLogprobsMaxTop <= 32 && kGroups == kThreads / 8 && kList >= kLogprobsMaxTop + 64, "lists");
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint32_t of_cta0(const void* p) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_at(p)));
+  return r;
+}
+
+// `kPer` values of 16 bytes
+__device__ __forceinline__ void unpack(const __nv_bfloat16*, const uint4& r, float* x) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack(const __half*, const uint4& r, float* x) {
+  const __half2* p = reinterpret_cast<const __half2*>(&r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(p[i]);
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack(const float*, const uint4& r, float* x) {
+  x[0] = __uint_as_float(r.x), x[1] = __uint_as_float(r.y), x[2] = __uint_as_float(r.z), x[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(float x) { return x; }
+
+// Orders as the values do (NaN on top), equal ones by the lowest id.
+__device__ __forceinline__ unsigned long long key_of(float x, int id) {
+  const uint32_t b = __float_as_uint(x + 0.f);  // (no negative zero)
+  return ((unsigned long long)((int)b < 0 ? ~b : b | 0x80000000u) << 32) | (0xffffffffu - (uint32_t)id);
+}
+__device__ __forceinline__ float value_of(unsigned long long key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ int id_of(unsigned long long key) { return (int)(0xffffffffu - (uint32_t)key); }
+
+// Maximum, sum of exp2(y), sum of exp2(y) y, with y = (x - maximum) log2 e.
+struct Sums {
+  float m, z, e;
+};
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+  const float m = max_nan(a.m, b.m);
+  const float ya = a.m == m ? 0.f : fmaxf((a.m - m) * kLog2e, -1e30f), yb = b.m == m ? 0.f : fmaxf((b.m - m) * kLog2e, -1e30f);
+  if (m != m) return {m, m, m};
+  const float ca = exp2_ftz(ya), cb = exp2_ftz(yb);
+  // (a sum of nothing is zero, and so is what is multiplied by it; zero times a far maximum is not taken)
+  const float ea = ca == 0.f ? 0.f : ca * fmaf(ya, a.z, a.e), eb = cb == 0.f ? 0.f : cb * fmaf(yb, b.z, b.e);
+  return {m, a.z * ca + b.z * cb, ea + eb};
+}
+
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(kThreads, 2) k_token_logprobs(const TokenLogprobs a, int cluster) {
+  constexpr int kPer = 16 / (int)sizeof(T), kVecs = kBatch / kPer;
+  __shared__ Sums s_sums[kWarps], s_parts[kMaxCluster];
+  __shared__ unsigned long long s_list[kTop ? kWarps * kList : 1], s_all[kTop ? kMaxCluster * kLogprobsMaxTop : 1];
+  __shared__ float s_group[kTop ? kGroups : 1], s_bound;
+  __shared__ int s_count[kWarps + 1];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = (int)(blockIdx.x / cluster), rank = (int)(blockIdx.x % cluster);
+  const T* const x0 = reinterpret_cast<const T*>(a.logits) + row * a.row_stride;
+  // [0, head): in front of the first 16-byte boundary, [head + kPer vecs, vocab): behind the last
+  const int head = min(a.vocab, (int)((16 - ((uintptr_t)x0 & 15)) % 16 / sizeof(T))), vecs = (a.vocab - head) / kPer;
+  const int per = (vecs + cluster - 1) / cluster, v0 = min(vecs, rank * per), v1 = min(vecs, v0 + per);
+  const uint4* const xv = reinterpret_cast<const uint4*>(x0 + head);
+
+  Sums s = {-INFINITY, 0.f, 0.f};
+  float bound = -INFINITY;  // values below are not among the top ones
+  unsigned long long floor = 0;  // nor are keys up to this one
+  int count = 0;             // on the warp's list
+  unsigned long long* const list = s_list + (kTop ? warp * kList : 0);
+  auto keep_top = [&]() {  // the list's largest `top`, by counting those above
+    __syncwarp();
+    unsigned long long mine[kList / 32];
+    int place[kList / 32];
+#pragma unroll
+    for (int i = 0; i < kList / 32; ++i) {
+      mine[i] = i * 32 + lane < count ? list[i * 32 + lane] : 0;
+      place[i] = 0;
+    }
+    for (int j = 0; j < count; ++j) {
+      const unsigned long long other = list[j];
+#pragma unroll
+      for (int i = 0; i < kList / 32; ++i) place[i] += other > mine[i];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kList / 32; ++i)
+      if (i * 32 + lane < count && place[i] < a.top) list[place[i]] = mine[i];
+    __syncwarp();
+    if (count >= a.top) {
+      count = a.top;
+      floor = list[a.top - 1];
+      bound = value_of(floor);
+    }
+  };
+  auto offer = [&](float x, int id, bool there) {  // (by whole warps)
+    const unsigned long long key = key_of(x, id);
+    const bool in = there && key > floor && !(x < bound);
+    const uint32_t who = __ballot_sync(0xffffffffu, in);
+    if (who == 0) return;
+    if (in) list[count + __popc(who & ((1u << lane) - 1))] = key;
+    count += __popc(who);
+    if (count + 32 > kList) keep_top();
+  };
+  auto add = [&](const float* x, int n, float top) {
+    if (!(top <= s.m)) s = join(s, {top, 0.f, 0.f});  // (NaN too)
+    if (s.m == -INFINITY) return;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (i >= n) break;
+      // (minus infinity is exp2(-300) = 0 here, which times itself is zero)
+      const float y = max_nan((x[i] - s.m) * kLog2e, -300.f), p = exp2_ftz(y);
+      s.z += p;
+      s.e = fmaf(p, y, s.e);
+    }
+  };
+  // the values of a vector, minus infinity (which changes nothing) behind the end, and their maximum
+  auto values = [&](const uint4& raw, bool there, float (&x)[kPer]) {
+    unpack((const T*)nullptr, raw, x);
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < kPer; ++i) top = max_nan(top, x[i]);
+    if (!there) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] = -INFINITY;
+      top = -INFINITY;
+    }
+    return top;
+  };
+
+  uint4 raw[kVecs];
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const int v = v0 + tid + u * kThreads;
+    raw[u] = v < v1 ? xv[v] : make_uint4(0, 0, 0, 0);
+  }
+  if constexpr (kTop) {  // the bound: the top-th of the groups' largest (minus infinity where groups have nothing)
+    float most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      float x[kPer];
+      most = max_nan(most, values(raw[u], v0 + tid + u * kThreads < v1, x));
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if ((lane & 7) == 0) s_group[tid >> 3] = most;
+    __syncthreads();
+    if (tid < kGroups) {
+      const unsigned long long mine = key_of(s_group[tid], tid);
+      int place = 0;
+      for (int j = 0; j < kGroups; ++j) place += key_of(s_group[j], j) > mine;
+      if (place == a.top - 1) s_bound = s_group[tid];
+    }
+    __syncthreads();
+    bound = s_bound;
+  }
+  for (int base = v0; base < v1; base += kThreads * kVecs) {
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int v = base + tid + u * kThreads, next = v + kThreads * kVecs;
+      const bool there = v < v1;
+      float x[kPer];
+      const float top = values(raw[u], there, x);
+      if (next < v1) raw[u] = xv[next];
+      add(x, kPer, top);
+      if constexpr (kTop) {
+        if (__any_sync(0xffffffffu, !(top < bound))) {
+#pragma unroll 1
+          for (int i = 0; i < kPer; ++i) {
+            float one = x[0];
+#pragma unroll
+            for (int j = 1; j < kPer; ++j) one = i == j ? x[j] : one;
+            offer(one, head + v * kPer + i, there);
+          }
+        }
+      }
+    }
+  }
+  // what is not in whole vectors: the first CTA's first warp
+  if (rank == 0 && warp == 0) {
+    const int tail = head + vecs * kPer, rest = head + a.vocab - tail;  // fewer than 16
+    const int i = lane < head ? lane : tail + lane - head;
+    const bool there = lane < rest;
+    const float x = there ? to_f32(x0[i]) : -INFINITY;
+    add(&x, 1, x);
+    if constexpr (kTop) offer(x, i, there);
+  }
+  // ---- the warps' and the cluster's sums ----
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    s = join(s, {__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.z, o), __shfl_xor_sync(0xffffffffu, s.e, o)});
+  if (lane == 0) s_sums[warp] = s;
+  if constexpr (kTop) {
+    if (count > a.top) keep_top();
+    if (lane == 0) s_count[warp] = count;
+  }
+  if (cluster > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");  // (the first CTA is there)
+  else __syncthreads();
+  if (warp == 0) {
+    s = lane < kWarps ? s_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1)
+      s = join(s, {__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.z, o), __shfl_xor_sync(0xffffffffu, s.e, o)});
+    if (lane == 0) {
+      const uint32_t to = of_cta0(&s_parts[rank]);
+      asm volatile("st.shared::cluster.f32 [%0], %1;\nst.shared::cluster.f32 [%0 + 4], %2;\nst.shared::cluster.f32 [%0 + 8], %3;" ::"r"(to), "f"(s.m),
+                   "f"(s.z), "f"(s.e)
+                   : "memory");
+    }
+  }
+  if constexpr (kTop) {
+    // the lists of the warps, at most `top` numbers each: a thread has one of them and counts those above
+    for (int i = tid; i < kWarps * kLogprobsMaxTop; i += kThreads) {
+      const int w = i / kLogprobsMaxTop, at = i % kLogprobsMaxTop;
+      const uint32_t to = of_cta0(&s_all[rank * kLogprobsMaxTop]);
+      int all = 0, place = 0;
+      const unsigned long long mine = at < s_count[w] ? s_list[w * kList + at] : 0;
+      for (int v = 0; v < kWarps; ++v) {
+        const int n = s_count[v];
+        all += n;
+        for (int j = 0; j < n; ++j) place += s_list[v * kList + j] > mine;
+      }
+      if (at < s_count[w] && place < a.top) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + 8 * place), "l"(mine) : "memory");
+      if (i >= all && i < a.top) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + 8 * i), "l"(0ull) : "memory");  // (fewer than that)
+    }
+  }
+  if (cluster > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+  else __syncthreads();
+  if (rank != 0) return;
+  s = s_parts[0];
+  for (int i = 1; i < cluster; ++i) s = join(s, s_parts[i]);
+  const float log_z = s.m == -INFINITY ? 0.f : logf(s.z);
+  if (tid == 0) {
+    const long long token = a.tokens[row];
+    const bool there = token >= 0 && token < a.vocab;
+    a.logprobs[row] = !there ? __int_as_float(0x7fffffff) : s.m == -INFINITY ? -INFINITY : to_f32(x0[token]) - s.m - log_z;
+    a.entropy[row] = s.m == -INFINITY ? 0.f : log_z - s.e * kLn2 / s.z;
+  }
+  if constexpr (kTop) {
+    for (int i = tid; i < cluster * a.top; i += kThreads) {
+      const unsigned long long mine = s_all[i / a.top * kLogprobsMaxTop + i % a.top];
+      int place = 0;
+      for (int c = 0; c < cluster; ++c)
+        for (int j = 0; j < a.top; ++j) place += s_all[c * kLogprobsMaxTop + j] > mine;
+      if (mine != 0 && place < a.top) {
+        a.top_logprobs[(long long)row * a.top + place] = s.m == -INFINITY ? -INFINITY : value_of(mine) - s.m - log_z;
+        a.top_ids[(long long)row * a.top + place] = id_of(mine);
+      }
+    }
+  }
+}
+
+template <typename T, bool kTop>
+cudaError_t launch(const TokenLogprobs& a, cudaStream_t stream) {
+  // CTAs of a row: as many as keep two on every SM busy, each with 4096 values at least
+  int cluster = 1;
+  while (cluster < kMaxCluster && (long long)a.rows * cluster * 2 <= 2 * 148 && a.vocab / (cluster * 2) >= 4096) cluster *= 2;
+  if ((long long)a.rows * cluster > 0x7fffffffll) return cudaErrorInvalidValue;
+  return launch_kernel_ex(k_token_logprobs<T, kTop>, dim3((unsigned)(a.rows * cluster)), dim3(kThreads), 0, stream, true, cluster, a, cluster);
+}
+
+}  // namespace
+
+cudaError_t launch_token_logprobs(const TokenLogprobs& a, LogitType type, cudaStream_t stream) {
+  if (a.rows < 0 || a.vocab < 1 || a.vocab > (1 << 30) || a.top < 0 || a.top > kLogprobsMaxTop || a.top > a.vocab) return cudaErrorInvalidValue;
+  if (a.rows == 0) return cudaSuccess;
+  switch (type) {
+    case LOGITS_BF16: return a.top > 0 ? launch<__nv_bfloat16, true>(a, stream) : launch<__nv_bfloat16, false>(a, stream);
+    case LOGITS_FP16: return a.top > 0 ? launch<__half, true>(a, stream) : launch<__half, false>(a, stream);
+    default: return a.top > 0 ? launch<float, true>(a, stream) : launch<float, false>(a, stream);
+  }
+}
+
+}  // namespace penny

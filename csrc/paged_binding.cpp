@@ -139,6 +139,88 @@ bool overlap(const at::Tensor& ta, const at::Tensor& tb) {
   }
   return false;
 }
+// The state of a cache's rows and pages, as page_tables takes it; refs may be missing.  Nothing of it shares memory, nor with `more`.
+void check_state(const at::Tensor& table, const at::Tensor& lengths, const at::Tensor& free, const at::Tensor& free_count, const at::Tensor* refs,
+                 int64_t page_size, std::initializer_list<const at::Tensor*> more) {
+  need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1, "table [rows, pages of a row] int32");
+  const int64_t R = table.size(0), W = table.size(1);
+  need(R <= kPagedMaxRows, "more than PAGED_MAX_ROWS rows");
+  need((W == 1 || table.stride(1) == 1) && (R == 1 || table.stride(0) >= W), "a table with contiguous rows that do not overlap");
+  need(ints(lengths, R), "lengths [rows] int32");
+  need(free.dim() == 1 && free.numel() >= 1 && free.numel() < (1ll << 31) && ints(free, free.numel()) && ints(free_count, 1),
+       "free [pages] and free_count [1] int32");
+  need(refs == nullptr || ints(*refs, free.numel()), "refs [pages] int32");
+  need(page_size >= 1 && page_size < (1ll << 30) && W < (1ll << 31), "page size");
+  std::vector<const at::Tensor*> all = {&table, &lengths, &free, &free_count};
+  if (refs != nullptr) all.push_back(refs);
+  const size_t own = all.size();
+  all.insert(all.end(), more.begin(), more.end());
+  std::vector<std::pair<uintptr_t, uintptr_t>> in;
+  for (size_t i = 0; i < all.size(); ++i) {
+    in.push_back(bounds(*all[i]));
+    for (size_t j = 0; j < std::min(i, own); ++j)
+      need(all[i]->numel() == 0 || all[j]->numel() == 0 || in[i].second <= in[j].first || in[j].second <= in[i].first,
+           "table, lengths, free, free_count, refs and the other tensors in memory of their own");
+  }
+}
+// A pool as page_copy sees it: a page's runs of whole 16 bytes, the largest steps outside.
+PageCopy page_layout(const at::Tensor& t) {
+  need(t.dim() == 4 && t.size(0) >= 1 && t.size(1) >= 1 && t.size(2) >= 1 && t.size(3) >= 1 && t.size(0) < (1ll << 31) && t.size(1) < (1ll << 31) &&
+           t.size(2) < (1ll << 31), "page_copy: pools [pages, page_size, kv_heads, dim]");
+  const int64_t size = t.element_size();
+  int64_t run = t.size(3) * size;
+  need((t.size(3) == 1 || t.stride(3) == 1) && run % 16 == 0 && aligned(t), "page_copy: pools contiguous in dim, rows of whole 16 bytes, 16-byte aligned");
+  std::vector<std::pair<int64_t, int64_t>> dims;  // (step in bytes, n)
+  for (int i : {1, 2})
+    if (t.size(i) > 1) dims.push_back({t.stride(i) * size, t.size(i)});
+  std::sort(dims.begin(), dims.end());
+  int64_t end = run;  // of what is inside a step
+  for (auto& [step, n] : dims) {
+    need(step % 16 == 0 && step >= end, "page_copy: pools with strides of whole 16 bytes whose rows do not overlap");
+    end += (n - 1) * step;
+  }
+  const int64_t page = t.size(0) > 1 ? t.stride(0) * size : 0;
+  if (t.size(0) > 1) {
+    // the pages outside of everything else, or between its steps (all other strides whole multiples of what all pages take)
+    bool apart = page >= end;
+    if (!apart && page % 16 == 0) {
+      int64_t inside = run;
+      bool placed = false;
+      apart = true;
+      for (size_t i = 0; i <= dims.size() && apart; ++i) {
+        if (!placed && (i == dims.size() || dims[i].first > page)) {
+          apart = page >= inside;
+          inside += (t.size(0) - 1) * page;
+          placed = true;
+        }
+        if (i == dims.size()) break;
+        apart = apart && dims[i].first >= inside;
+        inside += (dims[i].second - 1) * dims[i].first;
+      }
+    }
+    need(apart && page % 16 == 0, "page_copy: pools with strides of whole 16 bytes whose rows do not overlap");
+  }
+  while (!dims.empty() && dims.front().first == run) {
+    run *= dims.front().second;
+    dims.erase(dims.begin());
+  }
+  need(run < (1ll << 31), "page_copy: pages of less than 2 GB");
+  PageCopy a = {};
+  a.page_bytes = page;
+  a.run_bytes = (int)run;
+  a.inner = a.outer = 1;
+  if (!dims.empty()) a.inner = (int)dims[0].second, a.inner_bytes = dims[0].first;
+  if (dims.size() > 1) a.outer = (int)dims[1].second, a.outer_bytes = dims[1].first;
+  a.pages = (int)t.size(0);
+  return a;
+}
+// A tensor of n values in an allocation of several, `from` bytes behind its start
+at::Tensor part_of(const at::Tensor& all, int64_t from, int64_t n, at::ScalarType type) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  t.unsafeGetTensorImpl()->set_storage_offset(from / (int64_t)c10::elementSize(type));
+  return t;
+}
 // Every element of b where a has the one of the same indices (the last dimension may be shorter)
 bool same_place(const at::Tensor& a, const at::Tensor& b) {
   bool same = a.data_ptr() == b.data_ptr();
@@ -153,7 +235,7 @@ void bind_paged(py::module_& m) {
   // fills (slots [tokens] int64, positions [tokens] int32, offsets [rows + 1] int32, granted [rows] bool).
   m.def("page_tables", [](at::Tensor table, at::Tensor lengths, at::Tensor free, at::Tensor free_count, at::Tensor news, int64_t page_size,
                           int64_t tokens, c10::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>> out,
-                          c10::optional<int64_t> max_len) {
+                          c10::optional<int64_t> max_len, OptTensor refs) {
     need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1, "page_tables: table [rows, pages of a row] int32");
     const int64_t R = table.size(0), W = table.size(1);
     need(R <= kPagedMaxRows, "page_tables: more than PAGED_MAX_ROWS rows");
@@ -164,6 +246,7 @@ void bind_paged(py::module_& m) {
     need(page_size >= 1 && page_size < (1ll << 30) && W < (1ll << 31), "page_tables: page size");
     need(tokens >= 0 && tokens < (1ll << 31) - 8, "page_tables: tokens");
     need(!max_len.has_value() || *max_len >= 0, "page_tables: max_len");
+    need(!refs.has_value() || ints(*refs, free.numel()), "page_tables: refs [pages] int32");
     if (out.has_value()) {
       const auto& [slots, positions, offsets, granted] = *out;
       need(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.dim() == 1 && slots.numel() == tokens && ints(positions, tokens) &&
@@ -172,42 +255,122 @@ void bind_paged(py::module_& m) {
       need(aligned(slots) && aligned(positions), "page_tables: 16-byte aligned slots and positions");
     }
     {  // (the state is read and written by different CTAs, new by some after others have written)
-      const at::Tensor* all[9] = {&table, &lengths, &free, &free_count, &news};
+      const at::Tensor* all[10] = {&table, &lengths, &free, &free_count, &news};
       int n = 5;
+      if (refs.has_value()) all[n++] = &*refs;
       if (out.has_value())
         for (const at::Tensor* t : {&std::get<0>(*out), &std::get<1>(*out), &std::get<2>(*out), &std::get<3>(*out)}) all[n++] = t;
-      std::pair<uintptr_t, uintptr_t> in[9];
+      std::pair<uintptr_t, uintptr_t> in[10];
       for (int i = 0; i < n; ++i) {
         in[i] = bounds(*all[i]);
         for (int j = 0; j < i; ++j)
           need(all[i]->numel() == 0 || all[j]->numel() == 0 || in[i].second <= in[j].first || in[j].second <= in[i].first,
-               "page_tables: table, lengths, free, free_count, new tokens and out in memory of their own");
+               "page_tables: table, lengths, free, free_count, refs, new tokens and out in memory of their own");
       }
     }
     on_device(table, {&lengths, &free, &free_count, &news}, "page_tables expects tensors on one CUDA device");
+    if (refs.has_value()) on_device(table, {&*refs}, "page_tables expects tensors on one CUDA device");
     const at::cuda::OptionalCUDAGuard guard(table.device());
     if (!out.has_value()) {
       // one allocation for the four (of a call of 6.7 us on the host, four took 3)
       const int64_t at1 = (tokens * 8 + 15) / 16 * 16, at2 = at1 + (tokens * 4 + 15) / 16 * 16, at3 = at2 + (R + 1) * 4;
       const at::Tensor all = at::detail::empty_cuda({at3 + R}, at::kByte, table.device(), c10::nullopt);
-      auto part = [&](int64_t from, int64_t n, at::ScalarType type) {
-        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
-        t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
-        t.unsafeGetTensorImpl()->set_storage_offset(from / (int64_t)c10::elementSize(type));
-        return t;
-      };
-      out = std::make_tuple(part(0, tokens, at::kLong), part(at1, tokens, at::kInt), part(at2, R + 1, at::kInt), part(at3, R, at::kBool));
+      out = std::make_tuple(part_of(all, 0, tokens, at::kLong), part_of(all, at1, tokens, at::kInt), part_of(all, at2, R + 1, at::kInt),
+                            part_of(all, at3, R, at::kBool));
     }
     const auto& [slots, positions, offsets, granted] = *out;
     on_device(table, {&slots, &positions, &offsets, &granted}, "page_tables expects tensors on one CUDA device");
     const PageTables a = {table.data_ptr<int>(), table.stride(0), lengths.data_ptr<int>(), free.data_ptr<int>(), free_count.data_ptr<int>(),
                           news.data_ptr<int>(), (long long*)slots.data_ptr<int64_t>(), positions.data_ptr<int>(), offsets.data_ptr<int>(),
                           granted.data_ptr<bool>(), (int)R, (int)W, (int)free.numel(), (int)page_size, (int)tokens,
-                          (int)std::min<int64_t>(max_len.value_or(INT_MAX), INT_MAX)};
+                          (int)std::min<int64_t>(max_len.value_or(INT_MAX), INT_MAX), refs.has_value() ? refs->data_ptr<int>() : nullptr};
     ck(launch_page_tables(a, cur()), "page_tables");
     return *out;
   }, py::arg("table"), py::arg("lengths"), py::arg("free"), py::arg("free_count"), py::arg("new"), py::arg("page_size"), py::arg("tokens"),
-     py::arg("out") = py::none(), py::arg("max_len") = py::none());
+     py::arg("out") = py::none(), py::arg("max_len") = py::none(), py::arg("refs") = py::none());
+  // Rows `target` become copies of rows `source`; returns (copy_from, copy_to [forks] int32, granted [forks] bool).
+  m.def("page_fork", [](at::Tensor table, at::Tensor lengths, at::Tensor free, at::Tensor free_count, at::Tensor refs, at::Tensor source,
+                        at::Tensor target, int64_t page_size) {
+    check_state(table, lengths, free, free_count, &refs, page_size, {&source, &target});
+    const int64_t n = source.numel();
+    need(ints(source, n) && ints(target, n) && n <= kPagedMaxRows, "page_fork: source and target [forks] int32, no more than PAGED_MAX_ROWS");
+    on_device(table, {&lengths, &free, &free_count, &refs, &source, &target}, "page_fork expects tensors on one CUDA device");
+    const at::cuda::OptionalCUDAGuard guard(table.device());
+    const at::Tensor all = at::detail::empty_cuda({n * 9}, at::kByte, table.device(), c10::nullopt);
+    const at::Tensor from = part_of(all, 0, n, at::kInt), to = part_of(all, n * 4, n, at::kInt), granted = part_of(all, n * 8, n, at::kBool);
+    const PageFork a = {table.data_ptr<int>(), table.stride(0), lengths.data_ptr<int>(), free.data_ptr<int>(), free_count.data_ptr<int>(),
+                        refs.data_ptr<int>(), source.data_ptr<int>(), target.data_ptr<int>(), from.data_ptr<int>(), to.data_ptr<int>(),
+                        granted.data_ptr<bool>(), (int)table.size(0), (int)table.size(1), (int)free.numel(), (int)page_size, (int)n};
+    ck(launch_page_fork(a, cur()), "page_fork");
+    return std::make_tuple(from, to, granted);
+  }, py::arg("table"), py::arg("lengths"), py::arg("free"), py::arg("free_count"), py::arg("refs"), py::arg("source"), py::arg("target"),
+     py::arg("page_size"));
+  // The pages in use to the front of the pool; returns (copy_from, copy_to [pages / 2] int32).
+  m.def("page_compact", [](at::Tensor table, at::Tensor lengths, at::Tensor free, at::Tensor free_count, at::Tensor refs, int64_t page_size) {
+    check_state(table, lengths, free, free_count, &refs, page_size, {});
+    on_device(table, {&lengths, &free, &free_count, &refs}, "page_compact expects tensors on one CUDA device");
+    const at::cuda::OptionalCUDAGuard guard(table.device());
+    const int64_t n = free.numel() / 2;
+    const at::Tensor all = at::detail::empty_cuda({n * 8}, at::kByte, table.device(), c10::nullopt);
+    const at::Tensor from = part_of(all, 0, n, at::kInt), to = part_of(all, n * 4, n, at::kInt);
+    const PageCompact a = {table.data_ptr<int>(), table.stride(0), lengths.data_ptr<int>(), free.data_ptr<int>(), free_count.data_ptr<int>(),
+                           refs.data_ptr<int>(), from.data_ptr<int>(), to.data_ptr<int>(), (int)table.size(0), (int)table.size(1),
+                           (int)free.numel(), (int)page_size};
+    ck(launch_page_compact(a, cur()), "page_compact");
+    return std::make_tuple(from, to);
+  }, py::arg("table"), py::arg("lengths"), py::arg("free"), py::arg("free_count"), py::arg("refs"), py::arg("page_size"));
+  // Page copy_from[i] of every pool to page copy_to[i].
+  m.def("page_copy", [](const std::vector<at::Tensor>& pools, at::Tensor copy_from, at::Tensor copy_to) {
+    const int64_t n = copy_from.numel();
+    need(ints(copy_from, n) && ints(copy_to, n) && n < (1ll << 31), "page_copy: copy_from and copy_to [copies] int32");
+    if (pools.empty()) return;
+    const at::Tensor& first = pools[0];
+    PageCopy a = page_layout(first);
+    std::vector<std::pair<std::pair<uintptr_t, uintptr_t>, const at::Tensor*>> in;
+    for (const at::Tensor& t : pools) {
+      bool alike = t.dim() == 4 && t.sizes() == first.sizes() && t.element_size() == first.element_size() && aligned(t);
+      for (int i = 0; alike && i < 4; ++i) alike = t.size(i) <= 1 || t.stride(i) == first.stride(i);
+      need(alike, "page_copy: pools of one shape, size of values and strides");
+      need(no_grad(t), "page_copy: no gradients");
+      in.push_back({bounds(t), &t});
+    }
+    for (const at::Tensor* list : {&copy_from, &copy_to}) in.push_back({bounds(*list), list});
+    std::sort(in.begin(), in.end());
+    for (size_t i = 0; i < in.size(); ++i)
+      for (size_t j = i + 1; j < in.size() && in[j].first.first < in[i].first.second; ++j) {
+        const bool lists = in[i].second->dim() != 4 && in[j].second->dim() != 4;  // (which are only read)
+        need(lists || !overlap(*in[i].second, *in[j].second), "page_copy: pools and lists apart from each other");
+      }
+    on_device(first, {&copy_from, &copy_to}, "page_copy expects tensors on one CUDA device");
+    for (const at::Tensor& t : pools) on_device(first, {&t}, "page_copy expects tensors on one CUDA device");
+    const at::cuda::OptionalCUDAGuard guard(first.device());
+    a.from = copy_from.data_ptr<int>();
+    a.to = copy_to.data_ptr<int>();
+    a.copies = (int)n;
+    for (size_t p = 0; p < pools.size(); p += kPageCopyPools) {
+      a.pools = (int)std::min<size_t>(kPageCopyPools, pools.size() - p);
+      for (int i = 0; i < a.pools; ++i) a.pool[i] = (char*)pools[p + i].data_ptr();
+      ck(launch_page_copy(a, sms_of(first.get_device()), cur()), "page_copy");
+    }
+  }, py::arg("pools"), py::arg("copy_from"), py::arg("copy_to"));
+  // Rows with the same first pages; returns (order [rows], starts [rows + 1], shared [rows]) int32.
+  m.def("page_groups", [](at::Tensor table, at::Tensor lengths, int64_t page_size) {
+    need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1 && table.size(1) < (1ll << 31),
+         "page_groups: table [rows, pages of a row] int32");
+    const int64_t R = table.size(0);
+    need(R <= kPagedMaxRows, "page_groups: more than PAGED_MAX_ROWS rows");
+    need(table.size(1) == 1 || table.stride(1) == 1, "page_groups: a table with contiguous rows");
+    need(ints(lengths, R), "page_groups: lengths [rows] int32");
+    need(page_size >= 1 && page_size < (1ll << 30), "page_groups: page size");
+    on_device(table, {&lengths}, "page_groups expects tensors on one CUDA device");
+    const at::cuda::OptionalCUDAGuard guard(table.device());
+    const at::Tensor all = at::detail::empty_cuda({(3 * R + 1) * 4}, at::kByte, table.device(), c10::nullopt);
+    const at::Tensor order = part_of(all, 0, R, at::kInt), starts = part_of(all, R * 4, R + 1, at::kInt), shared = part_of(all, (2 * R + 1) * 4, R, at::kInt);
+    const PageGroups a = {table.data_ptr<int>(), table.stride(0), lengths.data_ptr<int>(), order.data_ptr<int>(), starts.data_ptr<int>(),
+                          shared.data_ptr<int>(), (int)R, (int)table.size(1), (int)page_size};
+    ck(launch_page_groups(a, cur()), "page_groups");
+    return std::make_tuple(order, starts, shared);
+  }, py::arg("table"), py::arg("lengths"), py::arg("page_size"));
   // qkv [tokens, (heads + 2 kv_heads) dim]: q and k rotated in place or into out [tokens, (heads + kv_heads) dim], k and v to their slots.
   m.def("paged_append", [](at::Tensor qkv, at::Tensor k, at::Tensor v, at::Tensor slots, at::Tensor positions, int64_t heads, double theta,
                            OptTensor out, OptTensor k_scale, OptTensor v_scale, bool early) {

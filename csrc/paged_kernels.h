@@ -31,8 +31,50 @@ struct PageTables {
   bool* granted;
   int rows, width, pages, page_size, tokens;
   int max_len;  // positions that a row may be granted, at most
+  int* refs;    // [pages] or null: how many rows have a page
 };
 cudaError_t launch_page_tables(const PageTables& a, cudaStream_t stream);
+
+// Rows with pages in common (csrc/paged_share.cu): the state of PageTables with refs.
+struct PageFork {
+  int* table;
+  long long table_stride;
+  int *lengths, *free_pages, *free_count, *refs;
+  const int *source, *target;  // [forks]
+  int *copy_from, *copy_to;    // [forks]
+  bool* granted;
+  int rows, width, pages, page_size, forks;
+};
+cudaError_t launch_page_fork(const PageFork& a, cudaStream_t stream);
+
+struct PageCompact {
+  int* table;
+  long long table_stride;
+  const int* lengths;
+  int *free_pages, *free_count, *refs;
+  int *copy_from, *copy_to;  // [pages / 2]
+  int rows, width, pages, page_size;
+};
+cudaError_t launch_page_compact(const PageCompact& a, cudaStream_t stream);
+
+// Pages of `pools` pools of one layout: runs of run_bytes (whole 16 bytes) at outer by outer_bytes and inner by inner_bytes.
+constexpr int kPageCopyPools = 128;  // of a launch
+struct PageCopy {
+  char* pool[kPageCopyPools];
+  const int *from, *to;
+  long long page_bytes, outer_bytes, inner_bytes;
+  int pools, copies, pages, outer, inner, run_bytes;
+};
+cudaError_t launch_page_copy(const PageCopy& a, int sms, cudaStream_t stream);
+
+struct PageGroups {
+  const int* table;
+  long long table_stride;
+  const int* lengths;
+  int *order, *starts, *shared;  // [rows], [rows + 1], [rows]
+  int rows, width, page_size;
+};
+cudaError_t launch_page_groups(const PageGroups& a, cudaStream_t stream);
 
 // type: of qkv and out.  out null: in place.  early: slots and positions are read before the kernels that may still run when this one
 // starts end.

@@ -9,12 +9,19 @@
 // (What comes and leaves again is back in its old place.)  A row is granted its tokens if it may be that long, they end
 // inside `tokens`, and the stack has pages for it and all rows before it that pass these two tests.
 //
+// Pages that several rows have (`refs`, the rows of every page): a row that leaves a page takes one off its count, and the page is
+// released when there is none left.  Counts go down in any order; of the row and page numbers k that leave a released page the largest
+// one stands for it (the count itself takes the number, as -1 - k, until the page is on the stack), so the order on the stack is that
+// of the numbers.  Only a call in which rows leave pays for this.  New pages have one row.  A row whose next token
+// would be written to a page that others have too is not granted.
+//
 // One launch: every CTA of a cluster sums over all rows by itself (8 bytes a row, read from L2), the cluster's barrier stands
 // between the last read of the lengths and their update, then the CTAs share tokens and released pages.  Latency is
 // all there is to it: a few reads and prefix sums one after the other, and 12 bytes written per token.
 #include "kernel_setup.h"
 #include "paged_kernels.h"
 #include "paged_plan.h"
+#include "paged_sums.cuh"
 #include "pdl.h"
 
 #include <stdint.h>
@@ -25,56 +32,6 @@ using namespace paged;
 
 constexpr int kTokensPerThread = 4;
 static_assert(kPagedMaxRows <= 8 * 1024, "rows of a thread");
-
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
-}
-
-// Sums hold at 2^31 - 1 (of terms that do so themselves: in any order the same).
-constexpr uint32_t kTop = 0x7fffffffu;
-__device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) { return min(a + b, kTop); }
-
-// Exclusive sums over the block's threads, and the whole in `total`.  The first call of a kernel needs no barrier in front.
-template <int N>
-__device__ __forceinline__ void block_sums(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t (&part)[N][32]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    uint32_t incl = v[i];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl = add(incl, u);
-    }
-    if (lane == 31) part[i][warp] = incl;
-    const uint32_t before = __shfl_up_sync(0xffffffffu, incl, 1);
-    v[i] = lane > 0 ? before : 0;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    uint32_t incl = lane < warps ? part[i][lane] : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl = add(incl, u);
-    }
-    total[i] = __shfl_sync(0xffffffffu, incl, 31);
-    const uint32_t before = __shfl_sync(0xffffffffu, incl, max(0, warp - 1));
-    if (warp > 0) v[i] = add(v[i], before);
-  }
-}
-
-// The last row r of [0, rows) with at[r] <= x (at is ascending, at[0] <= x).
-__device__ __forceinline__ int row_at(const int* at, int rows, int x) {
-  int lo = 0, hi = rows;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (at[mid] <= x) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
 
 // Values of a thread's rows to shared memory.
 template <int kPer>
@@ -89,8 +46,62 @@ __device__ __forceinline__ void put(int* to, int r0, int rows, const int (&v)[kP
   }
 }
 
+// Takes the references of the rows that leave off the pages' counts, puts the pages that have none left on the stack and returns how
+// many are on it now.  s_old, s_gone: per row its length and the number of its first reference among all `total` that leave.  Called by
+// all threads of the cluster.
+__device__ __noinline__ int leave_shared(const PageTables& a, const PageDiv& div, int cluster, int count, const int* s_old, const int* s_gone, int total) {
+  __shared__ int s_warp[32], s_run;
+  const int tid = threadIdx.x, rank = blockIdx.x, threads = cluster * blockDim.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  auto page_of = [&](int k) {  // -1: none of the pool's
+    const int r = row_at(s_gone, a.rows, k), left = pages_of(div, (int)max(0ll, (long long)s_old[r] + a.news[r]));
+    const int page = a.table[r * a.table_stride + left + (k - s_gone[r])];
+    return (unsigned)page < (unsigned)a.pages ? page : -1;
+  };
+  auto barrier = [&]() {
+    if (cluster > 1) cluster_barrier();
+    else __syncthreads();
+  };
+  for (int k = rank * (int)blockDim.x + tid; k < total; k += threads) {
+    const int page = page_of(k);
+    if (page >= 0) atomicSub(a.refs + page, 1);
+  }
+  barrier();
+  for (int k = rank * (int)blockDim.x + tid; k < total; k += threads) {
+    const int page = page_of(k);
+    if (page >= 0 && __ldcg(a.refs + page) <= 0) atomicMin(a.refs + page, -1 - k);
+  }
+  barrier();
+  if (rank == 0) {  // numbers in descending order onto the stack
+    if (tid == 0) s_run = count;
+    __syncthreads();
+    for (int top = total; top > 0; top -= (int)blockDim.x) {
+      const int k = top - 1 - tid, page = k >= 0 ? page_of(k) : -1;
+      const bool mine = page >= 0 && __ldcg(a.refs + page) == -1 - k;
+      const uint32_t who = __ballot_sync(0xffffffffu, mine);
+      if (lane == 0) s_warp[warp] = __popc(who);
+      __syncthreads();
+      int before = s_run, all = 0;
+      for (int w = 0; w < warps; ++w) {
+        before += w < warp ? s_warp[w] : 0;
+        all += s_warp[w];
+      }
+      const int at = before + __popc(who & ((1u << lane) - 1));
+      if (mine) {
+        if (at < a.pages) a.free_pages[at] = page;
+        a.refs[page] = 0;
+      }
+      __syncthreads();
+      if (tid == 0) s_run = min(a.pages, s_run + all);
+      __syncthreads();
+    }
+    if (tid == 0) *a.free_count = s_run;
+  }
+  barrier();
+  return __ldcg(a.free_count);
+}
+
 // kPer: rows of a thread, one behind the other.
-template <int kPer>
+template <int kPer, bool kRefs>
 __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const PageDiv div, int cluster) {
   extern __shared__ int smem[];
   // per row: where its tokens begin, its length (-1 - length: not granted), its first new page's number among all new
@@ -101,7 +112,7 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
   pdl_wait();
   const int tid = threadIdx.x, rank = blockIdx.x;
   const long long most = min((long long)a.width * a.page_size, 2147483647ll), longest = min(most, (long long)a.max_len);
-  const int count = max(0, min(*a.free_count, a.pages));
+  int count = max(0, min(*a.free_count, a.pages));
   const int r0 = tid * kPer;
   auto gone_of = [&](int old, int n) { return n < 0 ? pages_of(div, old) - pages_of(div, (int)max(0ll, (long long)old + n)) : 0; };
   __shared__ uint32_t s_two[2][32], s_one[1][32], s_popped;
@@ -121,8 +132,23 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
     sums[1] = add(sums[1], gone_of(old[i], n[i]));
   }
   block_sums(sums, totals, s_two);
+  if constexpr (kRefs) {
+    if (totals[1] > 0) {
+      int first[kPer];
+      uint32_t gone = sums[1];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        first[i] = (int)gone;
+        gone = add(gone, gone_of(old[i], n[i]));
+      }
+      put<kPer>(s_old, r0, a.rows, old);
+      put<kPer>(s_gone, r0, a.rows, first);
+      __syncthreads();
+      count = leave_shared(a, div, cluster, count, s_old, s_gone, (int)totals[1]);
+    }
+  }
   // (more pages than the pool has: a table that holds some twice; what the stack cannot take is dropped)
-  const int pushed = (int)min(totals[1], (uint32_t)(a.pages - count));
+  const int pushed = kRefs ? 0 : (int)min(totals[1], (uint32_t)(a.pages - count));
   const uint32_t pages_there = (uint32_t)(count + pushed);
   uint32_t end = sums[0], gone = sums[1], need[1] = {0}, all_need[1];
   bool granted[kPer];
@@ -134,6 +160,13 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
     end = add(end, max(0, n[i]));
     gone = add(gone, gone_of(old[i], n[i]));
     granted[i] = n[i] <= 0 || (old[i] + (long long)n[i] <= longest && end <= (uint32_t)a.tokens);
+    if constexpr (kRefs) {
+      const int at = div_page(div, old[i]);
+      if (granted[i] && n[i] > 0 && old[i] != at * a.page_size) {
+        const int page = a.table[(r0 + i) * a.table_stride + at];
+        granted[i] = (unsigned)page >= (unsigned)a.pages || __ldcg(a.refs + page) <= 1;
+      }
+    }
     if (n[i] > 0 && granted[i]) need[0] = add(need[0], pages_of(div, old[i] + n[i]) - pages_of(div, old[i]));
   }
   block_sums(need, all_need, s_one);
@@ -220,7 +253,10 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
       slot[i] = -1;
       if (row[i] < 0) continue;
       const int within = pos[i] - at[i] * a.page_size;
-      if (fresh[i] && within == 0) a.table[row[i] * a.table_stride + at[i]] = page[i];
+      if (fresh[i] && within == 0) {
+        a.table[row[i] * a.table_stride + at[i]] = page[i];
+        if (kRefs && (unsigned)page[i] < (unsigned)a.pages) a.refs[page[i]] = 1;
+      }
       if (page[i] >= 0 && page[i] < a.pages) slot[i] = (long long)page[i] * a.page_size + within;
     }
     if (each == kTokensPerThread && j0 + kTokensPerThread <= a.tokens) {
@@ -238,22 +274,6 @@ __global__ void __launch_bounds__(1024) k_page_tables(const PageTables a, const 
   }
 }
 
-// CTAs of a cluster for many rows or tokens: sixteen where the device has room for one such cluster, else the eight that all have.
-int cluster_of(const void* kernel) {
-  static std::mutex mu;
-  static std::map<std::pair<int, const void*>, int> done;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  std::lock_guard<std::mutex> lock(mu);
-  int& n = done[{dev, kernel}];
-  if (n == 0) {
-    const bool may = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
-    if (!may) (void)cudaGetLastError();
-    n = may && max_clusters(kernel, 16, 1024, kPagedMaxRows * 4 * sizeof(int)) > 0 ? 16 : 8;
-  }
-  return n;
-}
-
 }  // namespace
 
 cudaError_t launch_page_tables(const PageTables& a, cudaStream_t stream) {
@@ -263,17 +283,22 @@ cudaError_t launch_page_tables(const PageTables& a, cudaStream_t stream) {
   // with 3060 tokens 9.1, in one CTA 10.2; 4000 rows with 42,209 tokens in 5342 pages 16.1, of eight CTAs instead of sixteen 3 more.
   const int threads = a.rows <= 256 && a.tokens <= 1024 ? 256 : 1024, big = a.tokens > 2048 || a.rows > 1024;
   const int per = (a.rows + threads - 1) / threads;
-#define PENNY_PAGE_TABLES(N)                                                                                                          \
+#define PENNY_PAGE_TABLES(N, R)                                                                                                        \
   do {                                                                                                                                \
-    const cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(k_page_tables<N>), kPagedMaxRows * 4 * (int)sizeof(int)).rc;     \
+    const cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(k_page_tables<N, R>), kPagedMaxRows * 4 * (int)sizeof(int)).rc;     \
     if (rc != cudaSuccess) return rc;                                                                                                 \
-    const int cluster = big ? cluster_of(reinterpret_cast<const void*>(k_page_tables<N>)) : 1;                                         \
-    return launch_kernel_ex(k_page_tables<N>, dim3(cluster), dim3(threads), smem, stream, true, cluster, a, page_div(a.page_size),     \
+    const int cluster = big ? cluster_of(reinterpret_cast<const void*>(k_page_tables<N, R>), kPagedMaxRows * 4 * sizeof(int)) : 1;                                         \
+    return launch_kernel_ex(k_page_tables<N, R>, dim3(cluster), dim3(threads), smem, stream, true, cluster, a, page_div(a.page_size),     \
                             cluster);                                                                                                 \
   } while (0)
-  if (per == 1) PENNY_PAGE_TABLES(1);
-  if (per <= 4) PENNY_PAGE_TABLES(4);
-  PENNY_PAGE_TABLES(8);
+  if (a.refs != nullptr) {
+    if (per == 1) PENNY_PAGE_TABLES(1, true);
+    if (per <= 4) PENNY_PAGE_TABLES(4, true);
+    PENNY_PAGE_TABLES(8, true);
+  }
+  if (per == 1) PENNY_PAGE_TABLES(1, false);
+  if (per <= 4) PENNY_PAGE_TABLES(4, false);
+  PENNY_PAGE_TABLES(8, false);
 #undef PENNY_PAGE_TABLES
 }
 

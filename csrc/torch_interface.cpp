@@ -32,6 +32,7 @@ void bind_custom_all_reduce(py::module_& m);  // custom_all_reduce_binding.cpp
 void bind_gemm(py::module_& m);               // gemm_binding.cpp
 void bind_decode(py::module_& m);             // decode_binding.cpp
 void bind_paged(py::module_& m);              // paged_binding.cpp
+void bind_logprobs(py::module_& m);           // logprobs_binding.cpp
 uint32_t* penny_gemm_error_word();            // gemm_binding.cpp
 
 namespace {
@@ -564,4 +565,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_gemm(m);
   bind_decode(m);
   bind_paged(m);
+  bind_logprobs(m);
 }

@@ -7,6 +7,7 @@
     out, res = P.all_reduce_rmsnorm(partial, weight, residual)
 
     cache = P.PagedKVCache(layers, rows, max_len, kv_heads)    # KV cache in pages, no communicator needed (ops/paged.py)
+    P.token_logprobs(logits, tokens, top=20)                   # log probabilities of given tokens (ops/logprobs.py)
 
 With a GPU the calls go to the native communicator (symmetric heap + peer-memory
 kernels); without one they go to the gloo backend with the same semantics, which
@@ -21,15 +22,20 @@ import torch
 
 _BACKEND = None
 _PAGED = ("PagedKVCache", "PageStep", "OutOfPages", "page_tables", "paged_append", "paged_attention",
-          "paged_attention_workspace_bytes")
+          "paged_attention_workspace_bytes", "PageFork", "PageMoves", "PageGroups", "page_fork", "page_compact", "page_copy", "page_groups")
+_LOGPROBS = ("TokenLogprobs", "token_logprobs")
 
 
 def __getattr__(name):
-    # (the paged KV cache needs the extension, the collectives on the gloo backend do not)
-    if name not in _PAGED:
+    # (the paged KV cache and the log probabilities need the extension, the collectives on the gloo backend do not)
+    if name in _PAGED:
+        from . import paged
+        globals().update({n: getattr(paged, n) for n in _PAGED})
+    elif name in _LOGPROBS:
+        from . import logprobs
+        globals().update({n: getattr(logprobs, n) for n in _LOGPROBS})
+    else:
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
-    from . import paged
-    globals().update({n: getattr(paged, n) for n in _PAGED})
     return globals()[name]
 
 

@@ -8,8 +8,15 @@
         cache.append(i, qkv, step, heads, theta)            # q and k rotated in place, k and v into the pages
         o = cache.attend(i, qkv[:, :heads * 128].unflatten(1, (heads, 128)))      # a step of one token per row
 
+Several continuations of one prompt (`sharing=True`): the rows of a fork have their prompt's whole pages in common.
+
+    moves = cache.fork(source, target)                      # [forks] int32 rows: every target begins as its source is
+    groups = cache.groups()                                 # which rows have the same first pages, once a step
+    o = cache.attend(i, q, groups=groups)                   # positions that a group shares are read once for all its rows
+
 All state lives on the device and nothing here waits for it: the calls may be captured in a CUDA graph, which keeps counting.
-`page_tables`, `paged_append` and `paged_attention` are the same calls on a caller's own tensors.
+`page_tables`, `paged_append`, `paged_attention`, `page_fork`, `page_compact`, `page_copy` and `page_groups` are the same calls on a
+caller's own tensors.
 
 The reference has no KV cache: it serves the paged ones of vLLM and SGLang (README.md:20-33).
 """
@@ -30,6 +37,26 @@ class PageStep(NamedTuple):
     granted: torch.Tensor    # [rows] bool
 
 
+class PageFork(NamedTuple):
+    """What a fork leaves to be copied, and who was granted one."""
+    copy_from: torch.Tensor  # [forks] int32: pages that rows end inside; -1 behind the last
+    copy_to: torch.Tensor    # [forks] int32
+    granted: torch.Tensor    # [forks] bool
+
+
+class PageMoves(NamedTuple):
+    """Pages that moved, as `page_copy` takes them."""
+    copy_from: torch.Tensor  # [pages // 2] int32, -1 behind the last
+    copy_to: torch.Tensor
+
+
+class PageGroups(NamedTuple):
+    """Rows in groups of those that have the same first pages; a row by itself is a group too."""
+    order: torch.Tensor   # [rows] int32: the groups' rows one behind the other, groups by their lowest row, rows ascending
+    starts: torch.Tensor  # [rows + 1] int32: group g has order[starts[g]:starts[g + 1]]; `rows` behind the last group
+    shared: torch.Tensor  # [rows] int32: how many first positions a row has in common with its group, whole pages (0 by itself)
+
+
 class OutOfPages(RuntimeError):
     """Rows that were not granted a token (no page, or at their longest), and the tokens that the step gave all the same."""
 
@@ -39,7 +66,7 @@ class OutOfPages(RuntimeError):
 
 
 def page_tables(table, lengths, free, free_count, new, page_size: int, tokens: int, out: Optional[PageStep] = None,
-                max_len: Optional[int] = None) -> PageStep:
+                max_len: Optional[int] = None, refs=None) -> PageStep:
     """Lets new[r] tokens come to row r, or its last -new[r] leave, and moves the pages that follow from it.
 
     table [rows, pages of a row] int32, lengths [rows] int32: the sequences; free [pages] int32 with free_count [1] int32: a
@@ -52,8 +79,47 @@ def page_tables(table, lengths, free, free_count, new, page_size: int, tokens: i
     are pages for it and every row before it that passes these tests; one that is not keeps its length, and its slots are -1.  A
     row that gets no tokens is granted.
     At most 8192 rows.  `tokens` may exceed the sum of new (a captured step's fixed number).  Entries of a table row behind its
-    pages, and of free from free_count on, say nothing."""
-    return PageStep._make(ops.page_tables(table, lengths, free, free_count, new, page_size, tokens, out, max_len))
+    pages, and of free from free_count on, say nothing.
+
+    refs [pages] int32, updated too: how many rows have a page (`page_fork`).  A page is put on the stack when the last of its rows leaves
+    it; of several that leave it in one call the one that is highest by row, then by page of the row, gives it its place.  Rows leave
+    before others come.  A row whose first new token would lie on a page that another row has too is not granted (one that was cut back
+    into the pages that it shares: a fork of it can go on)."""
+    return PageStep._make(ops.page_tables(table, lengths, free, free_count, new, page_size, tokens, out, max_len, refs))
+
+
+def page_fork(table, lengths, free, free_count, refs, source, target, page_size: int) -> PageFork:
+    """Lets row target[i], which is empty, become a copy of row source[i]: source, target [forks] int32, the state as in `page_tables`.
+
+    Whole pages are shared: refs [pages] int32 counts the rows of every page, zero for those on the stack.  A page that the source ends
+    inside is copied to one from the stack, by `page_copy` of the lists that this returns (only real copies are on them).  Forks are
+    granted in order, as long as there are pages for those that need one; not granted are rows that the table does not have, targets
+    that are not empty, a row onto itself, and a target that an earlier fork of the call asked for.  Lengths are those before the call."""
+    return PageFork._make(ops.page_fork(table, lengths, free, free_count, refs, source, target, page_size))
+
+
+def page_compact(table, lengths, free, free_count, refs, page_size: int) -> PageMoves:
+    """Moves the pages in use (refs above zero) to the front of the pool: of U such pages the i-th from page U on goes to the i-th free one
+    below U; tables and refs follow, the stack has the pages from U on, U on top.  The contents move by `page_copy` of the lists that
+    this returns, before anything else reads or writes them.  State as in `page_fork`."""
+    return PageMoves._make(ops.page_compact(table, lengths, free, free_count, refs, page_size))
+
+
+def page_copy(pools, copy_from, copy_to) -> None:
+    """Copies page copy_from[i] to page copy_to[i] in every one of `pools`, [pages, page_size, kv_heads, dim] of one shape and strides (whole 16
+    bytes, any type), apart from each other.  copy_from, copy_to [copies] int32: a pair with a page that the pools do not have (-1) is left
+    out.  No page is written twice, or both read and written."""
+    ops.page_copy(list(pools), copy_from, copy_to)
+
+
+def page_groups(table, lengths, page_size: int) -> PageGroups:
+    """Finds the rows that have the same first pages, for `paged_attention(groups=)`: table and lengths as there.
+
+    Rows whose first page is the same one are a group, if it lies in front of their last position's page; what they share are the
+    pages that all of them have in common with the lowest of them, each in front of its last position's.  So with a text that all
+    rows begin with and others that only some go on with, the former is what counts.  At most 8192 rows.  The groups hold as long as
+    their rows only grow (and until others come to be)."""
+    return PageGroups._make(ops.page_groups(table, lengths, page_size))
 
 
 def paged_append(qkv, k, v, slots, positions, heads: int, theta: float, out=None, k_scale=None, v_scale=None, early: bool = False) -> None:
@@ -94,10 +160,11 @@ class PagedKVCache:
 
     rows: sequences at a time (a row whose length is 0 is free for the next one); max_len: positions that a row can have;
     pages: of the pool, by default as many as all rows need at their longest.  dtype: bf16, fp16 or e4m3, whose scales
-    (k_scale, v_scale [kv_heads] fp32, one for all layers, or a list of them) default to one."""
+    (k_scale, v_scale [kv_heads] fp32, one for all layers, or a list of them) default to one.  sharing: rows may have pages in common
+    (`fork`, `compact`), which are counted in `refs`."""
 
     def __init__(self, layers: int, rows: int, max_len: int, kv_heads: int, head_dim: int = 128, page_size: int = 16, pages: Optional[int] = None,
-                 dtype: torch.dtype = torch.bfloat16, k_scale=None, v_scale=None, device=None):
+                 dtype: torch.dtype = torch.bfloat16, k_scale=None, v_scale=None, device=None, sharing: bool = False):
         if min(layers, rows, max_len, kv_heads, head_dim, page_size) < 1 or (pages is not None and pages < 1):
             raise ValueError("PagedKVCache: layers, rows, max_len, kv_heads, head_dim, page_size and pages above zero")
         if rows > ops.PAGED_MAX_ROWS:
@@ -128,10 +195,32 @@ class PagedKVCache:
         self.lengths = torch.zeros(rows, dtype=torch.int32, device=self.device)
         self.free = torch.arange(self.pages - 1, -1, -1, dtype=torch.int32, device=self.device)  # page 0 on top
         self.free_count = torch.full((1,), self.pages, dtype=torch.int32, device=self.device)
+        self.refs = torch.zeros(self.pages, dtype=torch.int32, device=self.device) if sharing else None
+
+    def _shared(self):
+        if self.refs is None:
+            raise ValueError("PagedKVCache: rows have pages in common with sharing=True only")
+        return self.table, self.lengths, self.free, self.free_count, self.refs
 
     def advance(self, new: torch.Tensor, tokens: int, out: Optional[PageStep] = None) -> PageStep:
         """`page_tables` on this cache: new[r] tokens come to row r or its last -new[r] leave (-lengths[r]: the row is free)."""
-        return page_tables(self.table, self.lengths, self.free, self.free_count, new, self.page_size, tokens, out, self.max_len)
+        return page_tables(self.table, self.lengths, self.free, self.free_count, new, self.page_size, tokens, out, self.max_len, self.refs)
+
+    def fork(self, source: torch.Tensor, target: torch.Tensor) -> PageFork:
+        """`page_fork` on this cache, with the copies in all layers: the empty rows `target` begin as rows `source` are."""
+        fork = page_fork(*self._shared(), source, target, self.page_size)
+        page_copy(self.k + self.v, fork.copy_from, fork.copy_to)
+        return fork
+
+    def compact(self) -> PageMoves:
+        """`page_compact` on this cache, with the copies in all layers: the pages in use are the pool's first ones."""
+        moves = page_compact(*self._shared(), self.page_size)
+        page_copy(self.k + self.v, moves.copy_from, moves.copy_to)
+        return moves
+
+    def groups(self) -> PageGroups:
+        """`page_groups` of this cache's rows."""
+        return page_groups(self.table, self.lengths, self.page_size)
 
     def append(self, layer: int, qkv: torch.Tensor, step: PageStep, heads: int, theta: float, out: Optional[torch.Tensor] = None,
                early: bool = False) -> None:
@@ -148,11 +237,14 @@ class PagedKVCache:
 
     def snapshot(self):
         """Which pages and lengths the rows have, for `restore` (the pages' contents are not kept)."""
-        return tuple(t.clone() for t in (self.table, self.lengths, self.free, self.free_count))
+        return tuple(t.clone() for t in self._state())
 
     def restore(self, snapshot) -> None:
-        for t, old in zip((self.table, self.lengths, self.free, self.free_count), snapshot):
+        for t, old in zip(self._state(), snapshot):
             t.copy_(old)
+
+    def _state(self):
+        return (self.table, self.lengths, self.free, self.free_count) + (() if self.refs is None else (self.refs,))
 
     def rows_of(self, layer: int, row: int, length: int):
         """(k, v) [kv_heads, length, head_dim] of a row's first positions, e4m3 ones times their scales in fp32: a copy, for looking at."""

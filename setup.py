@@ -42,6 +42,8 @@ CUDA_SOURCES = [
     "csrc/paged_tables.cu",
     "csrc/paged_append.cu",
     "csrc/paged_attention.cu",
+    "csrc/paged_share.cu",
+    "csrc/logprobs.cu",
 ]
 CPP_SOURCES = [
     "csrc/torch_interface.cpp",
@@ -49,6 +51,7 @@ CPP_SOURCES = [
     "csrc/gemm_binding.cpp",
     "csrc/decode_binding.cpp",
     "csrc/paged_binding.cpp",
+    "csrc/logprobs_binding.cpp",
     "csrc/bootstrap.cpp",
     "csrc/symm_heap.cpp",
 ]

@@ -18,6 +18,8 @@
 namespace py = pybind11;
 using namespace penny;
 
+uint32_t* penny_gemm_error_word();  // gemm_binding.cpp
+
 namespace {
 using OptTensor = c10::optional<at::Tensor>;
 
@@ -403,17 +405,21 @@ void bind_paged(py::module_& m) {
        "paged_append");
   }, py::arg("qkv"), py::arg("k"), py::arg("v"), py::arg("slots"), py::arg("positions"), py::arg("heads"), py::arg("theta"),
      py::arg("out") = py::none(), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(), py::arg("early") = false);
-  m.def("paged_attention_workspace_bytes", [](int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_len, int64_t window) {
+  m.def("paged_attention_workspace_bytes", [](int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_len, int64_t window, bool groups) {
     need(rows >= 1 && kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && dim >= 1 && max_len >= 1 && window >= 0,
          "paged_attention_workspace_bytes: rows, heads and lengths");
     need(rows < (1 << 24) && heads < (1 << 20) && dim <= 256, "paged_attention_workspace_bytes: rows, heads and dim");
+    need(!groups || rows <= kPagedMaxRows, "paged_attention_workspace_bytes: more than PAGED_MAX_ROWS rows");
+    if (groups) return (int64_t)shared_attention_workspace_bytes((int)rows, (int)heads, (int)dim, sms_of(at::cuda::current_device()));
     return (int64_t)paged_attention_workspace_bytes((int)rows, (int)heads, (int)kv_heads, (int)dim, (int)std::min<int64_t>(max_len, paged::kMaxLen),
                                                     (int)std::min<int64_t>(window, 1ll << 30),
                                                     sms_of(at::cuda::current_device()));
-  }, py::arg("rows"), py::arg("heads"), py::arg("kv_heads"), py::arg("dim"), py::arg("max_len"), py::arg("window") = 0);
+  }, py::arg("rows"), py::arg("heads"), py::arg("kv_heads"), py::arg("dim"), py::arg("max_len"), py::arg("window") = 0,
+     py::arg("groups") = false);
   // q [rows, heads, dim], one token of every row, attends to the row's last `window` positions (0: all of them).
   m.def("paged_attention", [](at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor table, at::Tensor lengths, OptTensor out, OptTensor lse,
-                              c10::optional<double> scale, int64_t window, OptTensor k_scale, OptTensor v_scale, OptTensor workspace, bool early) {
+                              c10::optional<double> scale, int64_t window, OptTensor k_scale, OptTensor v_scale, OptTensor workspace, bool early,
+                              c10::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> groups) {
     const PagedType type = type_of(q, "paged_attention: bf16 or fp16 q"), cache = type_of(k, "paged_attention: bf16, fp16 or e4m3 caches");
     need(type != PAGED_E4M3, "paged_attention: bf16 or fp16 q");
     const PagedPool pool = pool_of(k, v, type, cache, k_scale, v_scale);
@@ -447,9 +453,15 @@ void bind_paged(py::module_& m) {
     if (lse.has_value())
       need(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->dim() == 2 && lse->size(0) == B && lse->size(1) == H, "paged_attention: lse [rows, heads] fp32");
     if (workspace.has_value()) need(workspace->is_contiguous() && aligned(*workspace), "paged_attention: 16-byte aligned contiguous workspace");
+    if (groups.has_value()) {
+      const auto& [order, starts, shared] = *groups;
+      need(B <= kPagedMaxRows, "paged_attention: groups of PAGED_MAX_ROWS rows at most");
+      need(ints(order, B) && ints(starts, B + 1) && ints(shared, B), "paged_attention: groups are (order [rows], starts [rows + 1], shared [rows]) int32");
+    }
     on_device(q, {&k, &v, &table, &lengths}, "paged_attention expects tensors on one CUDA device");
     for (const OptTensor* t : {&out, &lse, &k_scale, &v_scale, &workspace})
       if (t->has_value()) on_device(q, {&**t}, "paged_attention expects tensors on one CUDA device");
+    if (groups.has_value()) on_device(q, {&std::get<0>(*groups), &std::get<1>(*groups), &std::get<2>(*groups)}, "paged_attention expects tensors on one CUDA device");
     const at::cuda::OptionalCUDAGuard guard(q.device());
     if (!out.has_value()) out = at::detail::empty_cuda({B, H, pool.dim}, q.scalar_type(), q.device(), c10::nullopt);
     if (B == 0) return *out;
@@ -457,15 +469,21 @@ void bind_paged(py::module_& m) {
     const int win = (int)std::min<int64_t>(window, 1ll << 30);
     const int max_len = (int)std::min<int64_t>(table.size(1) * pool.page_size, paged::kMaxLen);
     need(B * (int64_t)paged::units_of(win > 0 && win < max_len ? win : max_len, 16) <= paged::kMaxUnits, "paged_attention: a table for over 2^34 positions");
-    const size_t bytes = paged_attention_workspace_bytes((int)B, (int)H, pool.heads, pool.dim, max_len, win, sms);
+    const size_t bytes = groups.has_value() ? shared_attention_workspace_bytes((int)B, (int)H, pool.dim, sms)
+                                            : paged_attention_workspace_bytes((int)B, (int)H, pool.heads, pool.dim, max_len, win, sms);
     if (workspace.has_value()) need(workspace->nbytes() >= bytes, "workspace too small (paged_attention_workspace_bytes)");
     else if (bytes > 0) workspace = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, q.device(), c10::nullopt);
     const PagedAttention a = {q.data_ptr(), q.stride(0), q.stride(1), out->data_ptr(), out->stride(0), out->stride(1),
                               lse.has_value() ? lse->data_ptr<float>() : nullptr, table.data_ptr<int>(), table.stride(0), lengths.data_ptr<int>(),
                               (int)B, (int)H, (int)table.size(1), win, scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)pool.dim), early};
+    if (groups.has_value()) {
+      const SharedGroups g = {std::get<0>(*groups).data_ptr<int>(), std::get<1>(*groups).data_ptr<int>(), std::get<2>(*groups).data_ptr<int>()};
+      ck(launch_shared_attention(a, type, pool, cache, g, workspace->data_ptr(), sms, penny_gemm_error_word(), cur()), "paged_attention");
+      return *out;
+    }
     ck(launch_paged_attention(a, type, pool, cache, workspace.has_value() ? workspace->data_ptr() : nullptr, sms, cur()), "paged_attention");
     return *out;
   }, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("table"), py::arg("lengths"), py::arg("out") = py::none(), py::arg("lse") = py::none(),
      py::arg("scale") = py::none(), py::arg("window") = 0, py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(),
-     py::arg("workspace") = py::none(), py::arg("early") = false);
+     py::arg("workspace") = py::none(), py::arg("early") = false, py::arg("groups") = py::none());
 }

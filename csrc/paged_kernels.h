@@ -6,6 +6,7 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <stddef.h>
+#include <stdint.h>
 
 namespace penny {
 
@@ -100,5 +101,13 @@ struct PagedAttention {
 size_t paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int dim, int max_len, int window, int sms);
 cudaError_t launch_paged_attention(const PagedAttention& a, PagedType type, const PagedPool& pool, PagedType cache, void* workspace,
                                    int sms, cudaStream_t stream);
+
+// The same for rows that share pages (csrc/paged_shared_attention.cu), groups as k_page_groups finds them; a.early is not looked at.
+struct SharedGroups {
+  const int *order, *starts, *shared;
+};
+size_t shared_attention_workspace_bytes(int rows, int heads, int dim, int sms);
+cudaError_t launch_shared_attention(const PagedAttention& a, PagedType type, const PagedPool& pool, PagedType cache, const SharedGroups& groups,
+                                    void* workspace, int sms, uint32_t* error_word, cudaStream_t stream);
 
 }  // namespace penny

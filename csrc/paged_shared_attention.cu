@@ -1,0 +1,808 @@
+// Attention of one new token per row over a paged KV cache whose rows share pages: positions that a group of rows have in common are
+// read once, as a product of all their query heads with the keys.
+//
+//   o[r, h] = sum_j softmax_j(scale q[r, h] . K_j) V_j = (sum_i e^(m_i - m) O_i) / (sum_i e^(m_i - m) l_i)
+//
+// with one part (m_i, l_i, O_i) or more from the shared positions of the row's group and one or more from its own.  (Where no
+// row shares anything csrc/paged_attention.cu is the kernel to use.)
+//
+//   * Up to 128 (row, query head) pairs of a KV head are the M side of tcgen05 products: S = Q K^T with 128 positions on the N side, P to
+//     tensor memory in S's place, O += P V with P as the operand in tensor memory.  Groups with more pairs give a CTA two such
+//     tiles, which take turns: the exponentials of one run under the products of the other.  A row's own positions are products
+//     whose other rows are empty; there the cache's stream is the bound, and the tiles of positions go to the two in turn.
+//   * A thread has a query's row of S: no exchange between threads for maxima and sums.
+//   * Keys and values are staged by cp.async, 16 bytes at a time through a list of 128 places, so that any page size and any strides will
+//     do; what lies outside is filled with zeros and masked, never read.  e4m3 pages are converted on the way to q's type, which is exact.
+//   * All items (a KV head of a group, or of a row) lie in a line that is cut into equal shares, a CTA to an SM
+//     (paged_shared_plan.h).  A warp walks the line and hands the pieces to the others; loads run ahead across pieces.  Pieces leave unnormalised
+//     fp32 outputs in a workspace, a second kernel joins them.  No counters: a workspace holds nothing between calls.
+//   * Weights count from a base that follows the maximum when a score is above it by more than kSlack; the accumulators are scaled then,
+//     which is seldom.  bf16 weights are rounded by up to 2^-8 of each; the output is divided by the sum of the rounded ones, so that a
+//     weight that outweighs the others is not off, and the logarithm is that of the others' sum.  fp16 weights stand 2^kShift above, against what fp16 loses under 2^-14.
+//
+// Every wait is bounded; one that ran out sets the error word that all tcgen05 kernels here share, and the CTA ends.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "gemm_sm100.cuh"
+#include "gemm_sm100.h"
+#include "kernel_setup.h"
+#include "paged_kernels.h"
+#include "paged_shared_plan.h"
+#include "paged_sums.cuh"
+#include "pdl.h"
+
+namespace penny {
+namespace {
+using namespace paged;
+using namespace sm100;
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kRing = 8;  // pieces between the warp that walks the line and the others
+constexpr uint32_t kErrWait = 0x5a;
+
+template <int D>
+struct Shape {
+  static constexpr int kStreams = D <= 128 ? 2 : 1;          // tiles of 128 queries at a time
+  static constexpr int kTile = D <= 128 ? 128 : 64;          // positions of a tile
+  static constexpr int kQueries = 128 * kStreams;
+  static constexpr int kSlot = kTile * D * 2;                // bytes of a tile's keys, or values
+  static constexpr int kSlots = D == 64 ? 8 : 4;             // keys and values in turn
+  static constexpr int kQ = 128 * D * 2;
+  static constexpr int kSmem = kStreams * kQ + kSlots * kSlot + 1024;
+  static constexpr int kSoftmaxWarps = 4 * kStreams, kMma = kSoftmaxWarps, kLoad = kMma + 1, kWalk = kLoad + 4, kThreads = (kWalk + 1) * 32;
+  // tensor memory: S (and P) of each stream, then O
+  static constexpr int kColsO = kStreams * kTile, kCols = kColsO + kStreams * D <= 256 ? 256 : 512;
+  static_assert(kColsO + kStreams * D <= 512 && kSmem <= 200 << 10, "");
+};
+
+struct Params {
+  PagedAttention a;
+  PagedPool pool;
+  PageDiv div;
+  const int *order, *starts, *shared;
+  int group, max_len, max_units, ctas;
+  uint32_t page_step, pos_step, step_bytes;
+  // workspace
+  int* line;         // [2 rows + 1]: first unit of every element: groups, then rows; all units
+  int2* place;       // [rows]: a row's group and its number in it
+  float* out;        // [4][rows][heads][D]: first pieces: of shared positions, of own ones, two halves each
+  float4* ml;        // [4][rows][heads]: base, sum of the weights as they were multiplied, sum of the weights
+  float* more;       // [ctas][2][128][D]: pieces that do not begin an item
+  float4* more_ml;
+  uint32_t* error;
+};
+
+struct Element {
+  int begin, end;     // positions
+  int queries, first; // (row, head) pairs of a KV head; the first row's place in order, or ~row
+  int row;            // whose table it is
+};
+template <int D>
+__device__ __forceinline__ Element element_of(const Params& p, int e) {
+  Element x = {0, 0, 0, 0, 0};
+  const int rows = p.a.rows;
+  if (e < rows) {
+    const int s0 = min(max(p.starts[e], 0), rows), n = min(max(p.starts[e + 1], 0), rows) - s0;
+    if (n < 2) return x;
+    x.first = s0;
+    x.row = p.order[s0];
+    if ((unsigned)x.row >= (unsigned)rows) return x;
+    x.queries = n * p.group;
+    x.end = min(max(p.shared[x.row], 0), p.max_len);
+    x.begin = p.a.window > 0 ? max(0, x.end + 1 - p.a.window) : 0;  // (its rows are longer than what they share)
+  } else {
+    x.row = e - rows;
+    x.first = ~x.row;
+    x.queries = p.group;
+    const Seen s = seen_of(p.a.lengths[x.row], p.max_len, p.a.window);
+    x.end = s.end;
+    x.begin = max(s.first, min(max(p.shared[x.row], 0), s.end));
+  }
+  return x;
+}
+template <int D>
+__device__ __forceinline__ int items_of(const Params& p, const Element& x) {
+  return p.pool.heads * query_tiles(x.queries, Shape<D>::kQueries);
+}
+template <int D>
+__device__ __forceinline__ uint32_t units_of(const Params& p, const Element& x) {
+  return (uint32_t)min((long long)items_of<D>(p, x) * item_units(tiles_of(x.end - x.begin, Shape<D>::kTile)), 0x7fffffffll);
+}
+
+// What a CTA has of an item, as the walking warp hands it on.
+struct Piece {
+  int tiles;       // 0: the end
+  int begin, end;  // first position, and behind the item's last
+  int row;         // whose table it is
+  int first;       // as in Element
+  int head;        // KV head
+  int query0, queries;
+  int whole;       // it begins the item
+  int stream;      // of its first tile, where tiles go to the streams in turn
+  bool pair;       // both streams take every tile
+};
+
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+      "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+      "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] B[smem], 16 of K.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void cp_async16(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack2(const __nv_bfloat16*, float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(const __half*, float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// two e4m3 values as two of T
+__device__ __forceinline__ uint32_t widen(const __half*, uint32_t x) {
+  uint32_t r;
+  asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l;}" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t widen(const __nv_bfloat16*, uint32_t x) {
+  const uint32_t h = widen((const __half*)nullptr, x);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return pack2((const __nv_bfloat16*)nullptr, f.x, f.y);
+}
+// where 16-byte chunk c of row r lies in an operand of `rows` rows: blocks of 64 columns, 128 bytes a row, swizzled
+__device__ __forceinline__ uint32_t chunk_at(int rows, int r, int c) {
+  return (uint32_t)((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+// The values as the B operand of P V, K (positions) along the rows: blocks of 64 columns lie kTile rows apart, 8 rows 1024 bytes.
+template <int kTile>
+__device__ __forceinline__ uint64_t value_desc(uint32_t at) {
+  uint64_t d = (uint64_t)((at & 0x3ffffu) >> 4);
+  d |= (uint64_t)(kTile * 128 >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+template <int D, typename T, bool kE4M3>
+__global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(const __grid_constant__ Params p) {
+  using L = Shape<D>;
+  constexpr int kTile = L::kTile, kSlots = L::kSlots, kStreams = L::kStreams;
+  constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
+  // exponents: the base is kShift under the maximum, and follows when a score is above that by more than kSlack
+  constexpr float kSlack = 8.f, kShift = kBf16 ? 0.f : 7.f;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t b_full[kSlots], b_free[kSlots], b_q[2], b_s[2], b_p[2], b_o[2], b_piece[kRing], b_taken[kRing];
+  __shared__ Piece s_piece[kRing];
+  __shared__ uint32_t s_place[kSlots / 2][kTile], s_there[kSlots][4], s_tmem;
+  __shared__ uint32_t s_part[1][32];
+  __shared__ int s_first[3];  // the element that the CTA's share begins in, how far behind the element's first unit, all units
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* const tiles = align_tiles(smem_raw);
+  const uint32_t q_at = smem_u32(tiles), kv_at = q_at + kStreams * L::kQ;
+  if (tid == 0) {
+    for (int i = 0; i < kSlots; ++i) mbar_init(b_full + i, 128), mbar_init(b_free + i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(b_q + i, 128), mbar_init(b_s + i, 1), mbar_init(b_p + i, 4), mbar_init(b_o + i, 1);
+    for (int i = 0; i < kRing; ++i) mbar_init(b_piece + i, 1), mbar_init(b_taken + i, L::kSoftmaxWarps + 5);
+    mbar_fence_init();
+    s_first[0] = -1;
+  }
+  if (warp == L::kMma) tmem_alloc(&s_tmem, L::kCols);
+  pdl_wait();
+  // ---- the line ----
+  const int elements = 2 * p.a.rows, per = (elements + L::kThreads - 1) / L::kThreads, e0 = min(elements, tid * per), e1 = min(elements, e0 + per);
+  const int cta = blockIdx.x;
+  {
+    uint32_t sum[1] = {0}, total[1];
+    for (int e = e0; e < e1; ++e) sum[0] = add(sum[0], units_of<D>(p, element_of<D>(p, e)));
+    block_sums(sum, total, s_part);
+    const bool sound = total[0] <= (uint32_t)p.max_units;  // (groups that overlap: nothing is done)
+    const int units = sound ? (int)total[0] : 0, share = units > 0 ? unit_share(units, p.ctas) : 1;
+    const long long begin = (long long)cta * share;
+    long long at = sum[0];
+    for (int e = e0; e < e1; ++e) {
+      const uint32_t n = units_of<D>(p, element_of<D>(p, e));
+      if (cta == 0) p.line[e] = sound ? (int)at : 0;
+      if (begin < units && begin >= at && begin < at + n) s_first[0] = e, s_first[1] = (int)(begin - at);
+      at += n;
+    }
+    if (tid == 0) s_first[2] = units;
+    if (cta == 0 && tid == 0) p.line[elements] = units;
+    for (int i = cta * L::kThreads + tid; i < p.a.rows; i += p.ctas * L::kThreads) {
+      const int row = p.order[i];
+      if ((unsigned)row >= (unsigned)p.a.rows) continue;
+      const int g = row_at(p.starts, p.a.rows, i);
+      p.place[row] = make_int2(g, i - p.starts[g]);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  const int units = s_first[2], share = units > 0 ? unit_share(units, p.ctas) : 1;
+  bool ok = s_first[0] >= 0;
+  // (by whole warps, which see one outcome)
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity)); };
+  int piece_no = 0;
+  auto take = [&](Piece& x) {  // the next piece; false at the end
+    if (!wait(b_piece + piece_no % kRing, (piece_no / kRing) & 1)) return false;
+    x = s_piece[piece_no % kRing];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(b_taken + piece_no % kRing);
+    ++piece_no;
+    return x.tiles > 0;
+  };
+  // tiles of a piece that a stream has, and the first of them
+  auto tiles_of_stream = [&](const Piece& x, int t) { return x.pair || kStreams == 1 ? x.tiles : (x.tiles + 1 - (t ^ x.stream)) / 2; };
+
+  if (!ok) {
+    // (nothing for this CTA)
+  } else if (warp < L::kSoftmaxWarps) {
+    // ================= a stream's softmax: a thread has a query =================
+    const int t = warp >> 2, lane_at = (warp & 3) * 32, me = lane_at + lane;
+    const uint32_t s_cols = tmem + t * kTile + ((uint32_t)lane_at << 16), o_cols = tmem + L::kColsO + t * D + ((uint32_t)lane_at << 16);
+    unsigned char* const q_tile = tiles + t * L::kQ;
+    int steps = 0, items = 0, tile0 = 0;
+    Piece x;
+    while (take(x)) {
+      const int n = tiles_of_stream(x, t), from = tile0;
+      tile0 += x.tiles;
+      const int query = x.query0 + (x.pair ? t * 128 : 0) + me;
+      const bool real = query < x.query0 + x.queries && (x.pair || me < x.queries);
+      if (n == 0) continue;
+      float factor = p.a.scale * kLog2e;
+      if (kE4M3) factor *= p.pool.k_scale[x.head];
+      const uint32_t flip = factor < 0 ? 0x80008000u : 0;  // (the maximum is that of the scores before the factor)
+      factor = fabsf(factor);
+      int row = 0, head = 0, lo = 0, hi = 0;
+      if (real) {
+        const int member = query / p.group;
+        head = x.head * p.group + query - member * p.group;
+        row = x.first < 0 ? ~x.first : p.order[x.first + member];
+        if ((unsigned)row < (unsigned)p.a.rows) {
+          const Seen s = seen_of(p.a.lengths[row], p.max_len, p.a.window);
+          lo = s.first, hi = s.end;
+        } else {
+          row = -1;
+        }
+      }
+      const bool there = real && row >= 0;
+      {
+        const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.a.q) + row * p.a.q_stride + head * p.a.q_head_stride);
+#pragma unroll
+        for (int c0 = 0; c0 < D / 8; c0 += 8) {
+          uint4 v[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] = there ? q[c0 + c] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            v[c].x ^= flip, v[c].y ^= flip, v[c].z ^= flip, v[c].w ^= flip;
+            *reinterpret_cast<uint4*>(q_tile + chunk_at(128, me, c0 + c)) = v[c];
+          }
+        }
+        fence_async_shared();
+        mbar_arrive(b_q + t);
+      }
+      const bool idle = !__any_sync(0xffffffffu, there);  // a warp without queries
+      float base = -INFINITY, sum = 0.f, sum_p = 0.f;    // base: minus infinity before there is a score
+      for (int i = 0; i < n; ++i) {
+        const int tile = x.pair || kStreams == 1 ? i : 2 * i + (t ^ x.stream), pos = x.begin + tile * kTile;
+        if (!wait(b_s + t, steps & 1)) break;
+        ++steps;
+        if (!idle) {
+          tc_fence_after_sync();
+          // positions of the tile that are there and that this query sees
+          uint32_t mask[kTile / 32], all = 0xffffffffu;
+          const uint32_t* const words = s_there[(from + tile) % kSlots];
+#pragma unroll
+          for (int w = 0; w < kTile / 32; ++w) {
+            const int a = min(max(lo - pos - w * 32, 0), 32), b = min(max(hi - pos - w * 32, 0), 32);  // [a, b)
+            const uint32_t below = b >= 32 ? 0xffffffffu : (1u << b) - 1, under = a >= 32 ? 0xffffffffu : (1u << a) - 1;
+            mask[w] = words[w] & below & ~under;
+            all &= mask[w];
+          }
+          const bool full = __all_sync(0xffffffffu, all == 0xffffffffu || !there);
+          float top = -INFINITY;
+          uint32_t s[32];
+#pragma unroll
+          for (int w = 0; w < kTile / 32; ++w) {
+            tmem_ld_32x32(s_cols + w * 32, s);
+            tmem_ld_wait();
+            if (!full) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) s[j] = (mask[w] >> j) & 1 ? s[j] : 0xff800000u;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(s[j]));
+          }
+          // (rounded as the scores are: what is between the largest and the base is exact however large they are)
+          const float most = top == -INFINITY ? top : __fmul_rn(top, factor);
+          float by = 1.f;
+          if (most > (base == -INFINITY ? -INFINITY : base + (kShift + kSlack))) {
+            const float next = __fsub_rn(most, kShift);
+            by = exp2_ftz(base - next);
+            base = next;
+          }
+          if (i > 0 && __any_sync(0xffffffffu, by != 1.f)) {
+            sum *= by;
+            sum_p *= by;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32(o_cols + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
+              tmem_st_32x32(o_cols + c, o);
+            }
+          }
+          const float from_base = base == -INFINITY ? 0.f : base;
+          float part[2] = {0.f, 0.f}, part_p[2] = {0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < kTile / 32; ++w) {
+            tmem_ld_32x32(s_cols + w * 32, s);
+            tmem_ld_wait();
+            uint32_t packed[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float a = exp2_ftz(__fsub_rn(__fmul_rn(__uint_as_float(s[2 * j]), factor), from_base));
+              float b = exp2_ftz(__fsub_rn(__fmul_rn(__uint_as_float(s[2 * j + 1]), factor), from_base));
+              if (!full) {
+                a = (mask[w] >> (2 * j)) & 1 ? a : 0.f;
+                b = (mask[w] >> (2 * j + 1)) & 1 ? b : 0.f;
+              }
+              packed[j] = pack2((const T*)nullptr, a, b);
+              part[0] += a;
+              part[1] += b;
+              if constexpr (kBf16) {
+                part_p[0] += __uint_as_float(packed[j] << 16);
+                part_p[1] += __uint_as_float(packed[j] & 0xffff0000u);
+              }
+            }
+            tmem_st_32x16(s_cols + w * 16, packed);
+          }
+          sum += part[0] + part[1];
+          sum_p += kBf16 ? part_p[0] + part_p[1] : part[0] + part[1];
+          tmem_st_wait();
+          tc_fence_before_sync();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_p + t);
+      }
+      if (!wait(b_o + t, items & 1)) break;
+      ++items;
+      tc_fence_after_sync();
+      if (!idle) {
+        const int half = x.pair ? (x.whole ? 0 : t) : t ^ x.stream;
+        const long long at = x.whole ? (((x.first < 0 ? 2 : 0) + half) * (long long)p.a.rows + row) * p.a.heads + head : (cta * 2ll + half) * 128 + me;
+        float4* const to = reinterpret_cast<float4*>((x.whole ? p.out : p.more) + at * D);
+        if (there) (x.whole ? p.ml : p.more_ml)[at] = make_float4(base, sum_p, sum, 0.f);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32(o_cols + c, o);
+          tmem_ld_wait();
+          if (there) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              to[c / 4 + j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+          }
+        }
+        tc_fence_before_sync();
+      }
+    }
+  } else if (warp == L::kMma) {
+    // ================= products, a step (a tile of positions of a stream) after another =================
+    const bool lead = elect_one();
+    constexpr uint32_t kType = kBf16 ? (1u << 7) | (1u << 10) : 0;
+    constexpr uint32_t kIdS = (1u << 4) | kType | ((uint32_t)(kTile >> 3) << 17) | (8u << 24);
+    constexpr uint32_t kIdO = (1u << 4) | kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);  // B: K along its rows
+    struct Step {
+      int stream, value;  // slot number of the values
+      bool first, last, frees;
+    } queue[2] = {};
+    int queued = 0, q_no[2] = {0, 0}, p_no[2] = {0, 0};
+    auto pop = [&]() {  // O += P V of the oldest step
+      const Step x = queue[0];
+      queue[0] = queue[1];
+      --queued;
+      if (!wait(b_p + x.stream, p_no[x.stream] & 1)) return;
+      ++p_no[x.stream];
+      const int slot = x.value % kSlots;
+      if (!wait(b_full + slot, (x.value / kSlots) & 1)) return;
+      tc_fence_after_sync();
+      if (lead) {
+        const uint64_t v = value_desc<kTile>(kv_at + slot * L::kSlot);
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          umma_ts(tmem + L::kColsO + x.stream * D, tmem + x.stream * kTile + k * 8, v + (uint64_t)(k * 16 * 128 >> 4), kIdO, !x.first || k > 0);
+        if (x.frees) umma_commit(b_free + slot);
+        if (x.last) umma_commit(b_o + x.stream);
+      }
+      __syncwarp();
+    };
+    int tile0 = 0;
+    Piece x;
+    while (take(x)) {
+      const int per_tile = x.pair ? 2 : 1;
+      for (int i = 0; i < x.tiles * per_tile && ok; ++i) {
+        const int tile = x.pair ? i >> 1 : i, t = x.pair ? i & 1 : kStreams == 1 ? 0 : (x.stream + i) & 1;
+        const int nth = x.pair || kStreams == 1 ? tile : i >> 1, n = tiles_of_stream(x, t);
+        while (ok && queued > 0 && (queued == 2 || queue[0].stream == t)) pop();
+        if (nth == 0) {
+          // (the queries come when the stream's last item is done, which takes its last product)
+          while (ok && queued > 0 && !__all_sync(0xffffffffu, mbar_try_wait(b_q + t, q_no[t] & 1))) pop();
+          if (!wait(b_q + t, q_no[t] & 1)) break;
+          ++q_no[t];
+        }
+        const int number = 2 * (tile0 + tile), slot = number % kSlots;
+        if (!wait(b_full + slot, (number / kSlots) & 1)) break;
+        tc_fence_after_sync();
+        if (lead) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem + t * kTile, make_smem_desc(q_at + t * L::kQ + (k >> 2) * 128 * 128 + (k & 3) * 32),
+                      make_smem_desc(kv_at + slot * L::kSlot + (k >> 2) * kTile * 128 + (k & 3) * 32), kIdS, k > 0);
+          if (!x.pair || t == 1) umma_commit(b_free + slot);
+          umma_commit(b_s + t);
+        }
+        __syncwarp();
+        queue[queued++] = {t, number + 1, nth == 0, nth + 1 == n, !x.pair || t == 1};
+      }
+      tile0 += x.tiles;
+    }
+    while (ok && queued > 0) pop();
+  } else if (warp < L::kWalk) {
+    // ================= keys and values to shared memory =================
+    const int me = tid - L::kLoad * 32;
+    constexpr int kSize = kE4M3 ? 1 : 2, kChunks = D * kSize / 16, kPer = kTile * kChunks / 128;  // 16-byte chunks of a position, of a thread
+    const int c = me % kChunks, r0 = me / kChunks;
+    int number = 0, told = 0;  // slots begun, and handed on
+    auto tell = [&](int upto) {
+      fence_async_shared();
+      for (; told < upto; ++told) mbar_arrive(b_full + told % kSlots);
+    };
+    auto room = [&]() {  // for slot `number`
+      if (number < kSlots) return ok;
+      uint64_t* const bar = b_free + number % kSlots;
+      const uint32_t parity = ((number / kSlots) & 1) ^ 1;
+      if (!kE4M3 && !mbar_try_wait(bar, parity)) {
+        cp_async_wait<0>();  // (whoever frees it may be waiting for what is under way)
+        tell(number);
+      }
+      return wait(bar, parity);
+    };
+    int tile_no = 0;
+    Piece x;
+    // (a warp whose wait ran out leaves at a barrier, with the others)
+    while (named_bar_all(1, 128, take(x))) {
+      const int* const table = p.a.table + x.row * p.a.table_stride;
+      const char* const src[2] = {reinterpret_cast<const char*>(p.pool.k) + x.head * p.pool.head_stride * kSize + c * 16,
+                                  reinterpret_cast<const char*>(p.pool.v) + x.head * p.pool.head_stride * kSize + c * 16};
+      int pos = x.begin + me;
+      int id = me < kTile && pos < x.end ? table[div_page(p.div, pos)] : -1;
+      for (int tile = 0; tile < x.tiles; ++tile, ++tile_no) {
+        if (me < kTile) {
+          const uint32_t at = step_of(id, p.pool.pages, pos, p.div, p.page_step, p.pos_step);
+          s_place[tile_no % (kSlots / 2)][me] = at;
+          const uint32_t there = __ballot_sync(0xffffffffu, at != kNoStep);
+          if (lane == 0) s_there[tile_no % kSlots][me / 32] = there;
+        }
+        pos += kTile;
+        id = me < kTile && pos < x.end && tile + 1 < x.tiles ? table[div_page(p.div, pos)] : -1;
+        if (!named_bar_all(1, 128, ok)) {
+          ok = false;
+          break;
+        }
+        const uint32_t* const places = s_place[tile_no % (kSlots / 2)];
+        if constexpr (kE4M3) {
+          uint4 v[2][kPer];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              const uint32_t at = places[r0 + i * (128 / kChunks)];
+              v[h][i] = at != kNoStep ? *reinterpret_cast<const uint4*>(src[h] + (unsigned long long)at * p.step_bytes) : make_uint4(0, 0, 0, 0);
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!room()) break;
+            unsigned char* const to = tiles + kStreams * L::kQ + (number % kSlots) * L::kSlot;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              const uint32_t w[4] = {v[h][i].x, v[h][i].y, v[h][i].z, v[h][i].w};
+              uint32_t y[8];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) y[2 * j] = widen((const T*)nullptr, w[j]), y[2 * j + 1] = widen((const T*)nullptr, w[j] >> 16);
+              const int r = r0 + i * (128 / kChunks);
+              *reinterpret_cast<uint4*>(to + chunk_at(kTile, r, 2 * c)) = make_uint4(y[0], y[1], y[2], y[3]);
+              *reinterpret_cast<uint4*>(to + chunk_at(kTile, r, 2 * c + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+            }
+            ++number;
+            tell(number);
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!room()) break;
+            const uint32_t to = kv_at + (number % kSlots) * L::kSlot;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              const int r = r0 + i * (128 / kChunks);
+              const uint32_t at = places[r];
+              const bool there = at != kNoStep;
+              cp_async16(to + chunk_at(kTile, r, c), src[h] + (there ? (unsigned long long)at * p.step_bytes : 0), there);
+            }
+            cp_async_commit();
+            ++number;
+            if (number >= kSlots - 1) {
+              cp_async_wait<kSlots - 2>();
+              tell(max(told, number - (kSlots - 2)));
+            }
+          }
+        }
+      }
+    }
+    if constexpr (!kE4M3) {
+      cp_async_wait<0>();
+      if (ok) tell(number);
+    }
+  } else {
+    // ================= the walk along the line =================
+    int e = s_first[0], off = s_first[1], no = 0, parity = 0;
+    long long at = (long long)cta * share;
+    const long long end = min((long long)units, at + share);
+    auto hand = [&](const Piece& x) {
+      if (no >= kRing && !wait(b_taken + no % kRing, ((no / kRing) & 1) ^ 1)) return;
+      if (lane == 0) {
+        s_piece[no % kRing] = x;
+        mbar_arrive(b_piece + no % kRing);
+      }
+      __syncwarp();
+      ++no;
+    };
+    while (ok && at < end && e < elements) {
+      // 32 elements at a time
+      const Element mine = e + lane < elements ? element_of<D>(p, e + lane) : Element{0, 0, 0, 0, 0};
+      uint32_t some = __ballot_sync(0xffffffffu, mine.end > mine.begin);
+      for (; some != 0 && at < end && ok; some &= some - 1) {
+        const int l = __ffs(some) - 1;
+        Element x;
+        x.begin = __shfl_sync(0xffffffffu, mine.begin, l);
+        x.end = __shfl_sync(0xffffffffu, mine.end, l);
+        x.queries = __shfl_sync(0xffffffffu, mine.queries, l);
+        x.first = __shfl_sync(0xffffffffu, mine.first, l);
+        x.row = __shfl_sync(0xffffffffu, mine.row, l);
+        const int tiles = tiles_of(x.end - x.begin, kTile), each = item_units(tiles), cuts = query_tiles(x.queries, L::kQueries);
+        const long long start = at - off;  // the element's first unit
+        int item = off / each;
+        off = 0;
+        for (; item < p.pool.heads * cuts && start + (long long)item * each < end && ok; ++item) {
+          const Tiles part = piece_of((int)(start + (long long)item * each), tiles, share, cta);
+          if (part.to > part.from) {
+            Piece y;
+            y.tiles = part.to - part.from;
+            y.begin = x.begin + part.from * kTile;
+            y.end = x.end;
+            y.row = x.row;
+            y.first = x.first;
+            y.head = item / cuts;
+            y.query0 = (item - y.head * cuts) * L::kQueries;
+            y.queries = min(L::kQueries, x.queries - y.query0);
+            y.whole = part.from == 0;
+            y.pair = y.queries > 128;
+            y.stream = y.pair || kStreams == 1 ? 0 : parity;
+            if (!y.pair) parity = (parity + y.tiles) & (kStreams - 1);
+            else parity = 0;
+            hand(y);
+          }
+        }
+        at = start + (long long)p.pool.heads * cuts * each;
+      }
+      e += 32;
+    }
+    Piece last = {};
+    hand(last);
+  }
+  if (!ok && s_first[0] >= 0 && lane == 0) atomicCAS(p.error, 0u, kErrWait);
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == L::kMma) tmem_dealloc(tmem, L::kCols);
+}
+
+// Joins the pieces of a row's heads: a warp takes a head at a time.
+constexpr int kJoinWarps = 4;
+template <int D, typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) k_shared_join(const __grid_constant__ Params p) {
+  using L = Shape<D>;
+  constexpr int kPer = D / 32;  // values of a lane
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = blockIdx.x, kh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int elements = 2 * p.a.rows, units = p.line[elements], share = units > 0 ? unit_share(units, p.ctas) : 1;
+  const int2 place = p.place[row];
+  const Element of[2] = {element_of<D>(p, min(max(place.x, 0), p.a.rows - 1)), element_of<D>(p, p.a.rows + row)};
+  const int line[2] = {p.line[min(max(place.x, 0), p.a.rows - 1)], p.line[p.a.rows + row]};
+  const float v_scale = p.pool.v_scale ? p.pool.v_scale[kh] : 1.f;
+  for (int g = warp; g < p.group; g += kJoinWarps) {
+    const int head = kh * p.group + g;
+    float top = -INFINITY, sum = 0.f, sum_p = 0.f, acc[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
+#pragma unroll 1
+    for (int kind = 0; kind < 2; ++kind) {
+      const Element x = of[kind];
+      const int tiles = units > 0 ? tiles_of(x.end - x.begin, L::kTile) : 0;
+      if (tiles == 0) continue;
+      const int query = kind == 0 ? place.y * p.group + g : g;
+      if ((unsigned)query >= (unsigned)x.queries) continue;
+      const int cuts = query_tiles(x.queries, L::kQueries), cut = query / L::kQueries, within = query - cut * L::kQueries;
+      const bool pair = min(L::kQueries, x.queries - cut * L::kQueries) > 128;
+      const int begin = line[kind] + (kh * cuts + cut) * item_units(tiles);
+      const int first = cta_of(begin, 0, share), pieces = cta_of(begin, tiles - 1, share) - first + 1;
+      // parts: two halves of a piece where its tiles went to both streams
+      for (int i0 = 0; i0 < 2 * pieces; i0 += 32) {
+        const int i = i0 + lane, piece = i >> 1, half = i & 1;
+        bool some = piece < pieces;
+        long long at = 0;
+        if (some) {
+          const Tiles t = piece_of(begin, tiles, share, first + piece);
+          some = half == 0 || (!pair && L::kStreams == 2 && t.to - t.from > 1);
+          const int stream = pair ? within >> 7 : half, lane_of = pair ? within & 127 : within;
+          at = piece == 0 ? ((2 * kind + half) * (long long)p.a.rows + row) * p.a.heads + head : ((first + piece) * 2ll + stream) * 128 + lane_of;
+        }
+        const float4 ml = some ? (piece == 0 ? p.ml : p.more_ml)[at] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        float most = ml.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float next = fmaxf(top, most), base = next == -INFINITY ? 0.f : next;
+        const float old = exp2_ftz(top - base), by = exp2_ftz(ml.x - base);
+        float l = by * ml.z, l_p = by * ml.y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o), l_p += __shfl_xor_sync(0xffffffffu, l_p, o);
+        sum = sum * old + l;
+        sum_p = sum_p * old + l_p;
+        top = next;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) acc[j] *= old;
+        const float* const from = (piece == 0 ? p.out : p.more) + at * D;
+        for (uint32_t who = __ballot_sync(0xffffffffu, some); who != 0; who &= who - 1) {
+          const int l = __ffs(who) - 1;
+          const float* const o = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), l)) + lane * kPer;
+          const float w = __shfl_sync(0xffffffffu, by, l);
+          if constexpr (kPer == 2) {
+            const float2 v = *reinterpret_cast<const float2*>(o);
+            acc[0] += w * v.x, acc[1] += w * v.y;
+          } else {
+#pragma unroll
+            for (int j = 0; j < kPer; j += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(o + j);
+              acc[j] += w * v.x, acc[j + 1] += w * v.y, acc[j + 2] += w * v.z, acc[j + 3] += w * v.w;
+            }
+          }
+        }
+      }
+    }
+    // (no positions: zeros, as what was added up is zero)
+    const float inv = top == -INFINITY ? 0.f * sum_p : v_scale / sum_p;
+    uint32_t* const out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.a.out) + row * p.a.out_stride + head * p.a.out_head_stride + lane * kPer);
+#pragma unroll
+    for (int j = 0; j < kPer; j += 2) out[j / 2] = pack2((const T*)nullptr, acc[j] * inv, acc[j + 1] * inv);
+    if (p.a.lse && lane == 0) p.a.lse[(long long)row * p.a.heads + head] = (top + log2f(sum)) * kLn2;
+  }
+}
+
+size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
+struct Workspace {
+  size_t line, place, out, ml, more, more_ml, all;
+  Workspace(size_t rows, size_t heads, size_t dim, size_t ctas) {
+    line = 0;
+    place = line + rounded((2 * rows + 1) * sizeof(int));
+    out = place + rounded(rows * sizeof(int2));
+    ml = out + rounded(4 * rows * heads * dim * sizeof(float));
+    more = ml + rounded(4 * rows * heads * sizeof(float4));
+    more_ml = more + rounded(ctas * 256 * dim * sizeof(float));
+    all = more_ml + rounded(ctas * 256 * sizeof(float4));
+  }
+};
+
+template <int D, typename T, bool kE4M3>
+cudaError_t launch(Params p, char* workspace, int sms, cudaStream_t stream) {
+  using L = Shape<D>;
+  const long long most = most_units(p.a.rows, p.pool.heads, p.group, p.max_len, L::kTile, L::kQueries);
+  if (most > kMaxSharedUnits) return cudaErrorInvalidValue;
+  p.max_units = (int)most;
+  p.ctas = (int)std::min<long long>(sms, (most + kLeastUnits - 1) / kLeastUnits);
+  const Workspace w(p.a.rows, p.a.heads, D, p.ctas);
+  p.line = reinterpret_cast<int*>(workspace + w.line);
+  p.place = reinterpret_cast<int2*>(workspace + w.place);
+  p.out = reinterpret_cast<float*>(workspace + w.out);
+  p.ml = reinterpret_cast<float4*>(workspace + w.ml);
+  p.more = reinterpret_cast<float*>(workspace + w.more);
+  p.more_ml = reinterpret_cast<float4*>(workspace + w.more_ml);
+  auto* kernel = k_shared_attention<D, T, kE4M3>;
+  cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(kernel), L::kSmem).rc;
+  if (rc != cudaSuccess) return rc;
+  rc = launch_kernel_ex(kernel, dim3(p.ctas), dim3(L::kThreads), (size_t)L::kSmem, stream, true, 1, p);
+  if (rc != cudaSuccess) return rc;
+  return launch_kernel_ex(k_shared_join<D, T>, dim3(p.a.rows, p.pool.heads), dim3(kJoinWarps * 32), 0, stream, true, 1, p);
+}
+
+}  // namespace
+
+size_t shared_attention_workspace_bytes(int rows, int heads, int dim, int sms) { return Workspace(rows, heads, dim, sms).all; }
+
+cudaError_t launch_shared_attention(const PagedAttention& a, PagedType type, const PagedPool& pool, PagedType cache, const SharedGroups& groups,
+                                    void* workspace, int sms, uint32_t* error_word, cudaStream_t stream) {
+  if (a.rows < 1 || a.rows > kPagedMaxRows || pool.heads < 1 || pool.heads > 65535 || a.heads % pool.heads != 0 || a.heads < pool.heads || type == PAGED_E4M3 ||
+      (cache != PAGED_E4M3 && cache != type))
+    return cudaErrorInvalidValue;
+  Params p = {};
+  p.a = a;
+  p.pool = pool;
+  p.div = page_div(pool.page_size);
+  p.order = groups.order;
+  p.starts = groups.starts;
+  p.shared = groups.shared;
+  p.group = a.heads / pool.heads;
+  const long long cap = (long long)a.width * pool.page_size;
+  p.max_len = (int)(cap < kMaxLen ? cap : kMaxLen);
+  const Steps st = steps_of(pool.pages, pool.page_size, pool.page_stride, pool.pos_stride, cache == PAGED_E4M3 ? 1 : 2);
+  if (st.bytes == 0) return cudaErrorInvalidValue;
+  p.page_step = st.page;
+  p.pos_step = st.pos;
+  p.step_bytes = st.bytes;
+  p.error = error_word;
+  char* const w = reinterpret_cast<char*>(workspace);
+#define PENNY_SHARED_TYPE(D)                                                                                                     \
+  (cache == PAGED_E4M3 ? (type == PAGED_BF16 ? launch<D, __nv_bfloat16, true>(p, w, sms, stream) : launch<D, __half, true>(p, w, sms, stream)) \
+                       : (type == PAGED_BF16 ? launch<D, __nv_bfloat16, false>(p, w, sms, stream) : launch<D, __half, false>(p, w, sms, stream)))
+  switch (pool.dim) {
+    case 64: return PENNY_SHARED_TYPE(64);
+    case 128: return PENNY_SHARED_TYPE(128);
+    case 256: return PENNY_SHARED_TYPE(256);
+    default: return cudaErrorInvalidValue;
+  }
+#undef PENNY_SHARED_TYPE
+}
+
+}  // namespace penny

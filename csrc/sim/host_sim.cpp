@@ -26,6 +26,7 @@
 #include "../gemm_tile_order.h"
 #include "../decode_attn_plan.h"
 #include "../paged_plan.h"
+#include "../paged_shared_plan.h"
 #include "../decode_gemm_plan.h"
 #include "../all_reduce_oneshot.cuh"
 #include "../all_reduce_ring.cuh"
@@ -414,6 +415,17 @@ int penny_paged_walk(const int* lengths, int rows, int max_len, int window, int 
     to[0] = w.row, to[1] = p.from, to[2] = p.to, to[3] = p.begins | p.ends << 1 | (w.first == w.end) << 2, to[4] = w.units - w.at;
   }
   return n;
+}
+// Attention over shared pages (paged_shared_plan.h).
+int penny_shared_item_units(int tiles) { return penny::paged::item_units(tiles); }
+int penny_shared_share(int units, int ctas) { return penny::paged::unit_share(units, ctas); }
+void penny_shared_piece(int begin, int tiles, int share, int cta, int* from_to) {
+  const penny::paged::Tiles t = penny::paged::piece_of(begin, tiles, share, cta);
+  from_to[0] = t.from, from_to[1] = t.to;
+}
+int penny_shared_cta_of(int begin, int tile, int share) { return penny::paged::cta_of(begin, tile, share); }
+long long penny_shared_most_units(long long rows, int kv_heads, int group, long long positions, int tile, int most) {
+  return penny::paged::most_units(rows, kv_heads, group, positions, tile, most);
 }
 // Tile -> (row block, column block) of the persistent GEMM kernels; pair_rank < 0
 // selects the single-CTA kernel, 0 / 1 the CTA of a pair.  Returns the number of

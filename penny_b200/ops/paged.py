@@ -133,7 +133,7 @@ def paged_append(qkv, k, v, slots, positions, heads: int, theta: float, out=None
 
 
 def paged_attention(q, k, v, table, lengths, out=None, lse=None, scale: Optional[float] = None, window: int = 0, k_scale=None, v_scale=None,
-                    workspace=None, early: bool = False) -> torch.Tensor:
+                    workspace=None, early: bool = False, groups: Optional[PageGroups] = None) -> torch.Tensor:
     """softmax(scale q K^T) V of one token per row: q [rows, heads, dim] (bf16 or fp16) over the last `window` (0: all) of
     lengths[r] positions on the row's pages; scale: 1 / sqrt(dim) by default.  Returns out, like q.
 
@@ -146,13 +146,18 @@ def paged_attention(q, k, v, table, lengths, out=None, lse=None, scale: Optional
     bytes with max_len = table.size(1) * page_size, for callers that must not allocate; its contents mean nothing between calls,
     but two calls that may run at the same time need one each.  early: for a step whose kernels overlap (this library's are launched with
     programmatic dependency): those that may still run when this one starts, back to the last launch without it, write of what
-    it reads only q and the keys and values of each row's last position; the other rows, lengths and table are then read before they end."""
-    return ops.paged_attention(q, k, v, table, lengths, out, lse, scale, window, k_scale, v_scale, workspace, early)
+    it reads only q and the keys and values of each row's last position; the other rows, lengths and table are then read before they end.
+
+    groups: `page_groups` of this table and these lengths, or of a time since when the rows of its groups have kept the pages that they
+    share: what a group shares is read once for all its rows, on tensor cores, instead of once for each.  The result is the same but for
+    the order of sums (and weights of an e4m3 cache have q's type).  At most 8192 rows; the workspace is that of groups=True.  A wait of the kernel that ran
+    out (4 s) leaves its rows undone and shows in `gemm_error`."""
+    return ops.paged_attention(q, k, v, table, lengths, out, lse, scale, window, k_scale, v_scale, workspace, early, groups)
 
 
-def paged_attention_workspace_bytes(rows: int, heads: int, kv_heads: int, dim: int, max_len: int, window: int = 0) -> int:
+def paged_attention_workspace_bytes(rows: int, heads: int, kv_heads: int, dim: int, max_len: int, window: int = 0, groups: bool = False) -> int:
     """Bytes of a workspace for `paged_attention` on the current device, for tables of max_len positions a row (0: none is needed)."""
-    return ops.paged_attention_workspace_bytes(rows, heads, kv_heads, dim, max_len, window)
+    return ops.paged_attention_workspace_bytes(rows, heads, kv_heads, dim, max_len, window, groups)
 
 
 class PagedKVCache:
@@ -229,11 +234,11 @@ class PagedKVCache:
                      early)
 
     def attend(self, layer: int, q: torch.Tensor, out=None, lse=None, scale: Optional[float] = None, window: int = 0, workspace=None,
-               early: bool = False) -> torch.Tensor:
+               early: bool = False, groups: Optional[PageGroups] = None) -> torch.Tensor:
         """`paged_attention` of q [rows, heads, head_dim] over this cache's `layer`, all positions of lengths (those of the
         step that `advance` made room for included: append before)."""
         return paged_attention(q, self.k[layer], self.v[layer], self.table, self.lengths, out, lse, scale, window, self.k_scale[layer],
-                               self.v_scale[layer], workspace, early)
+                               self.v_scale[layer], workspace, early, groups)
 
     def snapshot(self):
         """Which pages and lengths the rows have, for `restore` (the pages' contents are not kept)."""
@@ -260,8 +265,9 @@ class PagedKVCache:
             got.append((rows.float() * scale[:, None] if self.e4m3 else rows).transpose(0, 1).contiguous())
         return tuple(got)
 
-    def workspace(self, heads: int, window: int = 0) -> torch.Tensor:
-        """A workspace for `attend` with q of `heads` heads."""
+    def workspace(self, heads: int, window: int = 0, groups: bool = False) -> torch.Tensor:
+        """A workspace for `attend` with q of `heads` heads (and with groups)."""
         with torch.cuda.device(self.device):
-            n = ops.paged_attention_workspace_bytes(self.rows, heads, self.kv_heads, self.head_dim, self.table.shape[1] * self.page_size, window)
+            n = ops.paged_attention_workspace_bytes(self.rows, heads, self.kv_heads, self.head_dim, self.table.shape[1] * self.page_size, window,
+                                                    groups)
         return torch.empty(n, dtype=torch.uint8, device=self.device)

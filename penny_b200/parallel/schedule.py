@@ -208,3 +208,32 @@ def paged_walk(lengths, max_len: int, warps: int, warp: int, window: int = 0, ti
     assert got >= 0, "a walk longer than this function's arrays"
     rows = [parts[5 * i:5 * i + 5] for i in range(got)]
     return [(r, a, b, bool(f & 1), bool(f & 2), bool(f & 4), z) for r, a, b, f, z in rows], tiles[:num.value], share.value
+
+
+def shared_units(tiles: int) -> int:
+    """Units of an item of the attention over shared pages (csrc/paged_shared_plan.h)."""
+    return sim_lib().penny_shared_item_units(tiles)
+
+
+def shared_share(units: int, ctas: int) -> int:
+    """Units of a CTA (csrc/paged_shared_plan.h)."""
+    return sim_lib().penny_shared_share(units, ctas)
+
+
+def shared_piece(begin: int, tiles: int, share: int, cta: int):
+    """The tiles [from, to) that a CTA has of an item whose first unit is `begin` (csrc/paged_shared_plan.h)."""
+    at = (ctypes.c_int * 2)()
+    sim_lib().penny_shared_piece(begin, tiles, share, cta, at)
+    return at[0], at[1]
+
+
+def shared_cta_of(begin: int, tile: int, share: int) -> int:
+    """The CTA that has a tile of such an item (csrc/paged_shared_plan.h)."""
+    return sim_lib().penny_shared_cta_of(begin, tile, share)
+
+
+def shared_most_units(rows: int, kv_heads: int, group: int, positions: int, tile: int, most: int) -> int:
+    """Units of a batch at most (csrc/paged_shared_plan.h)."""
+    f = sim_lib().penny_shared_most_units
+    f.restype, f.argtypes = ctypes.c_longlong, [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
+    return f(rows, kv_heads, group, positions, tile, most)

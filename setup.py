@@ -43,6 +43,7 @@ CUDA_SOURCES = [
     "csrc/paged_append.cu",
     "csrc/paged_attention.cu",
     "csrc/paged_share.cu",
+    "csrc/paged_shared_attention.cu",
     "csrc/logprobs.cu",
 ]
 CPP_SOURCES = [

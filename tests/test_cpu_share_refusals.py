@@ -72,6 +72,21 @@ def test_groups(over, said):
         P.page_groups(**(dict(table=ints(3, 4), lengths=ints(3), page_size=16) | over))
 
 
+def _groups(order=3, starts=4, shared=3):
+    return P.PageGroups(ints(order), ints(starts), ints(shared))
+
+
+@pytest.mark.parametrize("over,said", [
+    (dict(groups=_groups(order=2)), "groups are"), (dict(groups=_groups(starts=3)), "groups are"), (dict(groups=_groups(shared=4)), "groups are"),
+    (dict(groups=(ints(3), ints(4).long(), ints(3))), "groups are"), (dict(groups=(ints(6)[::2], ints(4), ints(3))), "groups are"),
+    (dict(groups=_groups(8193, 8194, 8193), q=torch.zeros(8193, 8, 64, dtype=BF), table=ints(8193, 1), lengths=ints(8193)), "PAGED_MAX_ROWS"),
+    (dict(groups=_groups(), window=-1), "window"), (dict(groups=_groups()), "CUDA")])
+def test_attention_with_groups(over, said):
+    with pytest.raises(RuntimeError, match=said):
+        P.paged_attention(**(dict(q=torch.zeros(3, 8, 64, dtype=BF), k=torch.zeros(6, 16, 2, 64, dtype=BF), v=torch.zeros(6, 16, 2, 64, dtype=BF), table=ints(3, 4),
+                                  lengths=ints(3)) | over))
+
+
 def test_cache_without_sharing():
     c = P.PagedKVCache(2, 3, 40, 2, head_dim=64, page_size=16, device="cpu")
     for call in (lambda: c.fork(ints(1), ints(1)), c.compact):

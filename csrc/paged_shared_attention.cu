@@ -125,13 +125,6 @@ struct Piece {
   bool pair;       // both streams take every tile
 };
 
-__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-      "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
@@ -199,6 +192,55 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t at) {
   return d;
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r, x = *reinterpret_cast<unsigned long long*>(&a), y = *reinterpret_cast<unsigned long long*>(&b);
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r, x = *reinterpret_cast<unsigned long long*>(&a), y = *reinterpret_cast<unsigned long long*>(&b);
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// A thread's row of S: weights exp2(score * factor - base), rounded to T, in pairs; their sums, unrounded and rounded; returns the largest
+// exponent (minus infinity: nothing is there).  kFull: all positions are there.  A base of minus infinity counts as zero.
+template <typename T, int kTile, bool kFull>
+__device__ __forceinline__ float weights(uint32_t s_cols, const uint32_t (&mask)[kTile / 32], float factor, float base, uint32_t (&packed)[kTile / 2],
+                                         float (&sums)[2]) {
+  const float minus = base == -INFINITY ? 0.f : -base;
+  float top[2] = {-INFINITY, -INFINITY};
+  float2 sum = make_float2(0.f, 0.f), sum_p = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < kTile / 32; ++w) {
+    uint32_t s[32];
+    tmem_ld_32x32(s_cols + w * 32, s);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float2 y = mul2(make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), make_float2(factor, factor));
+      y = add2(y, make_float2(minus, minus));
+      if (!kFull) {
+        y.x = (mask[w] >> (2 * j)) & 1 ? y.x : -INFINITY;
+        y.y = (mask[w] >> (2 * j + 1)) & 1 ? y.y : -INFINITY;
+      }
+      top[j & 1] = max3(top[j & 1], y.x, y.y);
+      const float2 p = make_float2(exp2_ftz(y.x), exp2_ftz(y.y));
+      const uint32_t both = pack2((const T*)nullptr, p.x, p.y);
+      packed[w * 16 + j] = both;
+      sum = add2(sum, p);
+      if constexpr (__is_same(T, __nv_bfloat16)) sum_p = add2(sum_p, make_float2(__uint_as_float(both << 16), __uint_as_float(both & 0xffff0000u)));
+    }
+  }
+  sums[0] = sum.x + sum.y;
+  sums[1] = __is_same(T, __nv_bfloat16) ? sum_p.x + sum_p.y : sums[0];
+  return fmaxf(top[0], top[1]);
+}
+
 template <int D, typename T, bool kE4M3>
 __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(const __grid_constant__ Params p) {
   using L = Shape<D>;
@@ -213,7 +255,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
   __shared__ uint32_t s_part[1][32];
   __shared__ int s_first[3];  // the element that the CTA's share begins in, how far behind the element's first unit, all units
   pdl_launch_dependents();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   unsigned char* const tiles = align_tiles(smem_raw);
   const uint32_t q_at = smem_u32(tiles), kv_at = q_at + kStreams * L::kQ;
   if (tid == 0) {
@@ -338,67 +380,39 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
             all &= mask[w];
           }
           const bool full = __all_sync(0xffffffffu, all == 0xffffffffu || !there);
-          float top = -INFINITY;
-          uint32_t s[32];
-#pragma unroll
-          for (int w = 0; w < kTile / 32; ++w) {
-            tmem_ld_32x32(s_cols + w * 32, s);
-            tmem_ld_wait();
-            if (!full) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) s[j] = (mask[w] >> j) & 1 ? s[j] : 0xff800000u;
+          // The weights against the base as it is, in registers; where a score is too far above it, they are taken again.  (The first
+          // tile has no base yet.)
+          uint32_t packed[kTile / 2];
+          float sums[2];
+          const float limit = base == -INFINITY ? -INFINITY : kShift + kSlack;
+          float top = full ? weights<T, kTile, true>(s_cols, mask, factor, base, packed, sums) : weights<T, kTile, false>(s_cols, mask, factor, base, packed, sums);
+          if (__any_sync(0xffffffffu, top > limit)) {
+            float by = 1.f;
+            if (top > limit) {
+              // (the exponents and the base move by the same amount, as rounded: the largest score's weight is right however large they are)
+              const float next = __fadd_rn(base == -INFINITY ? 0.f : base, __fsub_rn(top, kShift));
+              by = exp2_ftz(base - next);
+              base = next;
             }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(s[j]));
-          }
-          // (rounded as the scores are: what is between the largest and the base is exact however large they are)
-          const float most = top == -INFINITY ? top : __fmul_rn(top, factor);
-          float by = 1.f;
-          if (most > (base == -INFINITY ? -INFINITY : base + (kShift + kSlack))) {
-            const float next = __fsub_rn(most, kShift);
-            by = exp2_ftz(base - next);
-            base = next;
-          }
-          if (i > 0 && __any_sync(0xffffffffu, by != 1.f)) {
             sum *= by;
             sum_p *= by;
+            if (i > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld_32x32(o_cols + c, o);
-              tmem_ld_wait();
+              for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld_32x32(o_cols + c, o);
+                tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
-              tmem_st_32x32(o_cols + c, o);
-            }
-          }
-          const float from_base = base == -INFINITY ? 0.f : base;
-          float part[2] = {0.f, 0.f}, part_p[2] = {0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < kTile / 32; ++w) {
-            tmem_ld_32x32(s_cols + w * 32, s);
-            tmem_ld_wait();
-            uint32_t packed[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float a = exp2_ftz(__fsub_rn(__fmul_rn(__uint_as_float(s[2 * j]), factor), from_base));
-              float b = exp2_ftz(__fsub_rn(__fmul_rn(__uint_as_float(s[2 * j + 1]), factor), from_base));
-              if (!full) {
-                a = (mask[w] >> (2 * j)) & 1 ? a : 0.f;
-                b = (mask[w] >> (2 * j + 1)) & 1 ? b : 0.f;
-              }
-              packed[j] = pack2((const T*)nullptr, a, b);
-              part[0] += a;
-              part[1] += b;
-              if constexpr (kBf16) {
-                part_p[0] += __uint_as_float(packed[j] << 16);
-                part_p[1] += __uint_as_float(packed[j] & 0xffff0000u);
+                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
+                tmem_st_32x32(o_cols + c, o);
               }
             }
-            tmem_st_32x16(s_cols + w * 16, packed);
+            weights<T, kTile, false>(s_cols, mask, factor, base, packed, sums);
           }
-          sum += part[0] + part[1];
-          sum_p += kBf16 ? part_p[0] + part_p[1] : part[0] + part[1];
+          sum += sums[0];
+          sum_p += sums[1];
+#pragma unroll
+          for (int w = 0; w < kTile / 2; w += 32) tmem_st_32x32(s_cols + w, *reinterpret_cast<uint32_t(*)[32]>(packed + w));
           tmem_st_wait();
           tc_fence_before_sync();
         }
@@ -429,29 +443,35 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     }
   } else if (warp == L::kMma) {
     // ================= products, a step (a tile of positions of a stream) after another =================
-    const bool lead = elect_one();
+    // The whole warp walks along and elects a lane for the instructions alone; what they take is the same in all lanes and known to
+    // be (through a shuffle), else every operand of every one of them is fetched by itself (300 clocks for the product of a tile, so 60).
+    auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
     constexpr uint32_t kType = kBf16 ? (1u << 7) | (1u << 10) : 0;
     constexpr uint32_t kIdS = (1u << 4) | kType | ((uint32_t)(kTile >> 3) << 17) | (8u << 24);
     constexpr uint32_t kIdO = (1u << 4) | kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);  // B: K along its rows
+    const uint32_t cols = (uint32_t)same((int)tmem);
+    const uint64_t q_desc = make_smem_desc((uint32_t)same((int)q_at)), k_desc = make_smem_desc((uint32_t)same((int)kv_at)),
+                   v_desc = value_desc<kTile>((uint32_t)same((int)kv_at));
+    const uint32_t q_hi = (uint32_t)(q_desc >> 32), q_lo = (uint32_t)q_desc, k_lo = (uint32_t)k_desc, v_hi = (uint32_t)(v_desc >> 32), v_lo = (uint32_t)v_desc;
+    // the steps whose scores are asked for, and whose weights are not yet multiplied: stream, slot number of the values, what it is
     struct Step {
-      int stream, value;  // slot number of the values
+      int stream, value;
       bool first, last, frees;
-    } queue[2] = {};
-    int queued = 0, q_no[2] = {0, 0}, p_no[2] = {0, 0};
+    } old = {}, next = {};
+    int queued = 0, q_no = 0, p_no = 0;  // (q_no, p_no: a bit for each stream's parity)
     auto pop = [&]() {  // O += P V of the oldest step
-      const Step x = queue[0];
-      queue[0] = queue[1];
+      const Step x = old;
+      old = next;
       --queued;
-      if (!wait(b_p + x.stream, p_no[x.stream] & 1)) return;
-      ++p_no[x.stream];
+      if (!wait(b_p + x.stream, (p_no >> x.stream) & 1)) return;
+      p_no ^= 1 << x.stream;
       const int slot = x.value % kSlots;
       if (!wait(b_full + slot, (x.value / kSlots) & 1)) return;
       tc_fence_after_sync();
-      if (lead) {
-        const uint64_t v = value_desc<kTile>(kv_at + slot * L::kSlot);
+      const uint32_t d = cols + L::kColsO + x.stream * D, a = cols + x.stream * kTile, v = v_lo + slot * (L::kSlot >> 4);
+      if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          umma_ts(tmem + L::kColsO + x.stream * D, tmem + x.stream * kTile + k * 8, v + (uint64_t)(k * 16 * 128 >> 4), kIdO, !x.first || k > 0);
+        for (int k = 0; k < kTile / 16; ++k) umma_ts(d, a + k * 8, make_desc(v_hi, v + (k * 16 * 128 >> 4)), kIdO, !x.first || k > 0);
         if (x.frees) umma_commit(b_free + slot);
         if (x.last) umma_commit(b_o + x.stream);
       }
@@ -460,32 +480,36 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     int tile0 = 0;
     Piece x;
     while (take(x)) {
-      const int per_tile = x.pair ? 2 : 1;
-      for (int i = 0; i < x.tiles * per_tile && ok; ++i) {
-        const int tile = x.pair ? i >> 1 : i, t = x.pair ? i & 1 : kStreams == 1 ? 0 : (x.stream + i) & 1;
-        const int nth = x.pair || kStreams == 1 ? tile : i >> 1, n = tiles_of_stream(x, t);
-        while (ok && queued > 0 && (queued == 2 || queue[0].stream == t)) pop();
+      const int tiles_here = same(x.tiles), pair = same(x.pair), stream0 = same(x.stream);
+      for (int i = 0; i < (pair ? 2 * tiles_here : tiles_here) && ok; ++i) {
+        const int tile = pair ? i >> 1 : i, t = pair ? i & 1 : kStreams == 1 ? 0 : (stream0 + i) & 1;
+        const int nth = pair || kStreams == 1 ? tile : i >> 1;
+        const int n = pair || kStreams == 1 ? tiles_here : (tiles_here + 1 - (t ^ stream0)) / 2;
+        while (ok && queued > 0 && (queued == 2 || old.stream == t)) pop();
         if (nth == 0) {
           // (the queries come when the stream's last item is done, which takes its last product)
-          while (ok && queued > 0 && !__all_sync(0xffffffffu, mbar_try_wait(b_q + t, q_no[t] & 1))) pop();
-          if (!wait(b_q + t, q_no[t] & 1)) break;
-          ++q_no[t];
+          while (ok && queued > 0 && !__all_sync(0xffffffffu, mbar_try_wait(b_q + t, (q_no >> t) & 1))) pop();
+          if (!wait(b_q + t, (q_no >> t) & 1)) break;
+          q_no ^= 1 << t;
         }
         const int number = 2 * (tile0 + tile), slot = number % kSlots;
         if (!wait(b_full + slot, (number / kSlots) & 1)) break;
         tc_fence_after_sync();
-        if (lead) {
+        const bool frees = !pair || t == 1;
+        const uint32_t d = cols + t * kTile, q = q_lo + t * (L::kQ >> 4), k0 = k_lo + slot * (L::kSlot >> 4);
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem + t * kTile, make_smem_desc(q_at + t * L::kQ + (k >> 2) * 128 * 128 + (k & 3) * 32),
-                      make_smem_desc(kv_at + slot * L::kSlot + (k >> 2) * kTile * 128 + (k & 3) * 32), kIdS, k > 0);
-          if (!x.pair || t == 1) umma_commit(b_free + slot);
+            umma_bf16(d, make_desc(q_hi, q + ((k >> 2) * 128 * 128 + (k & 3) * 32 >> 4)), make_desc(q_hi, k0 + ((k >> 2) * kTile * 128 + (k & 3) * 32 >> 4)), kIdS,
+                      k > 0);
           umma_commit(b_s + t);
+          if (frees) umma_commit(b_free + slot);
         }
         __syncwarp();
-        queue[queued++] = {t, number + 1, nth == 0, nth + 1 == n, !x.pair || t == 1};
+        (queued == 0 ? old : next) = {t, number + 1, nth == 0, nth + 1 == n, frees};
+        ++queued;
       }
-      tile0 += x.tiles;
+      tile0 += tiles_here;
     }
     while (ok && queued > 0) pop();
   } else if (warp < L::kWalk) {

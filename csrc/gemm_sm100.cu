@@ -119,6 +119,25 @@ cudaError_t make_gate_up_map(CUtensorMap* map, const void* base, uint64_t blocks
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// A pool of pages [pages, page_size, heads, dim] of 16-bit values, strides in bytes; box = [box_rows positions x 64 values], 128-byte swizzle.
+cudaError_t make_page_map(CUtensorMap* map, const void* base, bool bf16, int dim, int page_size, int heads, int pages, long long pos_bytes,
+                          long long head_bytes, long long page_bytes, int box_rows) {
+  EncodeFn fn = encode_fn();
+  if (fn == nullptr) return cudaErrorNotSupported;
+  // (the stride of a single position, head or page says nothing)
+  const cuuint64_t any = (cuuint64_t)dim * 2;
+  cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)page_size, (cuuint64_t)heads, (cuuint64_t)pages};
+  cuuint64_t strides[3] = {page_size > 1 ? (cuuint64_t)pos_bytes : any, heads > 1 ? (cuuint64_t)head_bytes : any, pages > 1 ? (cuuint64_t)page_bytes : any};
+  for (cuuint64_t n : strides)
+    if (n == 0 || n % 16 != 0) return cudaErrorInvalidValue;
+  cuuint32_t box[4] = {(cuuint32_t)kBlockK, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // Plain GEMM: C row-major in this GPU's memory, nothing to wait for.
 struct StoreLocal : PolicyBase {
   __nv_bfloat16* c;

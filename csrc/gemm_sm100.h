@@ -17,6 +17,11 @@ cudaError_t make_tile_map(CUtensorMap* map, const void* base, uint64_t rows, uin
 cudaError_t make_gate_up_map(CUtensorMap* map, const void* base, uint64_t blocks, uint64_t rows, uint64_t cols,
                              uint64_t row_stride_elems, uint32_t box_blocks, uint32_t box_rows);
 
+// A pool of pages [pages, page_size, heads, dim] of 16-bit values (csrc/paged_kernels.h), strides in bytes: a box is 64 values of box_rows
+// positions of a page and head.  An error where a TMA tensor cannot have those strides.
+cudaError_t make_page_map(CUtensorMap* map, const void* base, bool bf16, int dim, int page_size, int heads, int pages, long long pos_bytes,
+                          long long head_bytes, long long page_bytes, int box_rows);
+
 // C[M, N] = A[M, K] * B[N, K]^T, bf16, row-major with leading dimensions lda /
 // ldb / ldc (elements).  K, lda, ldb multiples of 8.  block_n: 0 (choose), 128, 192 or
 // 256 (one CTA per 128 x block_n tile), or 512 = 256 x 256 tiles computed by CTA

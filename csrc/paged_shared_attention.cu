@@ -52,7 +52,10 @@ struct Shape {
   static constexpr int kSlots = D == 64 ? 8 : 4;             // keys and values in turn
   static constexpr int kQ = 128 * D * 2;
   static constexpr int kSmem = kStreams * kQ + kSlots * kSlot + 1024;
-  static constexpr int kSoftmaxWarps = 4 * kStreams, kMma = kSoftmaxWarps, kLoad = kMma + 1, kWalk = kLoad + 4, kThreads = (kWalk + 1) * 32;
+  static constexpr int kSoftmaxWarps = 4 * kStreams, kMma = kSoftmaxWarps, kLoad = kMma + 1, kWalk = kLoad + 4;
+  // whole warpgroups; those of two streams' softmax take registers from the others
+  static constexpr int kThreads = (kWalk + 4) / 4 * 4 * 32, kMoreRegs = kStreams == 2 ? 160 : 0, kFewerRegs = 96;
+  static_assert(kStreams == 1 || (kThreads == 512 && kMoreRegs * 256 + kFewerRegs * 256 <= 65536), "registers");
   // tensor memory: S (and P) of each stream, then O
   static constexpr int kColsO = kStreams * kTile, kCols = kColsO + kStreams * D <= 256 ? 256 : 512;
   static_assert(kColsO + kStreams * D <= 512 && kSmem <= 200 << 10, "");
@@ -64,6 +67,7 @@ struct Params {
   PageDiv div;
   const int *order, *starts, *shared;
   int group, max_len, max_units, ctas;
+  int box;                // positions of a TMA box, of which pages are whole multiples; 0: no TMA
   uint32_t page_step, pos_step, step_bytes;
   // workspace
   int* line;         // [2 rows + 1]: first unit of every element: groups, then rows; all units
@@ -76,13 +80,14 @@ struct Params {
 };
 
 struct Element {
-  int begin, end;     // positions
+  int begin, end;     // positions; begin at the start of a box, what is in front of `low` is not seen
+  int low;
   int queries, first; // (row, head) pairs of a KV head; the first row's place in order, or ~row
   int row;            // whose table it is
 };
 template <int D>
 __device__ __forceinline__ Element element_of(const Params& p, int e) {
-  Element x = {0, 0, 0, 0, 0};
+  Element x = {};
   const int rows = p.a.rows;
   if (e < rows) {
     const int s0 = min(max(p.starts[e], 0), rows), n = min(max(p.starts[e + 1], 0), rows) - s0;
@@ -92,15 +97,16 @@ __device__ __forceinline__ Element element_of(const Params& p, int e) {
     if ((unsigned)x.row >= (unsigned)rows) return x;
     x.queries = n * p.group;
     x.end = min(max(p.shared[x.row], 0), p.max_len);
-    x.begin = p.a.window > 0 ? max(0, x.end + 1 - p.a.window) : 0;  // (its rows are longer than what they share)
+    x.low = p.a.window > 0 ? max(0, x.end + 1 - p.a.window) : 0;  // (its rows are longer than what they share)
   } else {
     x.row = e - rows;
     x.first = ~x.row;
     x.queries = p.group;
     const Seen s = seen_of(p.a.lengths[x.row], p.max_len, p.a.window);
     x.end = s.end;
-    x.begin = max(s.first, min(max(p.shared[x.row], 0), s.end));
+    x.low = max(s.first, min(max(p.shared[x.row], 0), s.end));
   }
+  x.begin = p.box > 0 && x.low < x.end ? x.low & -p.box : x.low;
   return x;
 }
 template <int D>
@@ -116,6 +122,7 @@ __device__ __forceinline__ uint32_t units_of(const Params& p, const Element& x) 
 struct Piece {
   int tiles;       // 0: the end
   int begin, end;  // first position, and behind the item's last
+  int low;         // as in Element
   int row;         // whose table it is
   int first;       // as in Element
   int head;        // KV head
@@ -207,6 +214,29 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// Waits for what tcgen05.ld has under way; the registers are the loads' from here on.
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                 "+r"(r[31])::"memory");
+}
+// The largest score of a thread's row of S of those that are there.
+template <int kTile>
+__device__ __forceinline__ float largest(uint32_t s_cols, const uint32_t (&mask)[kTile / 32]) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kTile / 32; ++w) {
+    uint32_t s[32];
+    tmem_ld_32x32(s_cols + w * 32, s);
+    tmem_ld_done(s);
+#pragma unroll
+    for (int j = 0; j < 32; j += 2)
+      top = max3(top, (mask[w] >> j) & 1 ? __uint_as_float(s[j]) : -INFINITY, (mask[w] >> (j + 1)) & 1 ? __uint_as_float(s[j + 1]) : -INFINITY);
+  }
+  return top;
+}
 // A thread's row of S: weights exp2(score * factor - base), rounded to T, in pairs; their sums, unrounded and rounded; returns the largest
 // exponent (minus infinity: nothing is there).  kFull: all positions are there.  A base of minus infinity counts as zero.
 template <typename T, int kTile, bool kFull>
@@ -214,15 +244,16 @@ __device__ __forceinline__ float weights(uint32_t s_cols, const uint32_t (&mask)
                                          float (&sums)[2]) {
   const float minus = base == -INFINITY ? 0.f : -base;
   float top[2] = {-INFINITY, -INFINITY};
-  float2 sum = make_float2(0.f, 0.f), sum_p = make_float2(0.f, 0.f);
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, sum_p[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  uint32_t s[2][32];
+  tmem_ld_32x32(s_cols, s[0]);
 #pragma unroll
   for (int w = 0; w < kTile / 32; ++w) {
-    uint32_t s[32];
-    tmem_ld_32x32(s_cols + w * 32, s);
-    tmem_ld_wait();
+    tmem_ld_done(s[w & 1]);
+    if (w + 1 < kTile / 32) tmem_ld_32x32(s_cols + (w + 1) * 32, s[(w + 1) & 1]);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      float2 y = mul2(make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), make_float2(factor, factor));
+      float2 y = mul2(make_float2(__uint_as_float(s[w & 1][2 * j]), __uint_as_float(s[w & 1][2 * j + 1])), make_float2(factor, factor));
       y = add2(y, make_float2(minus, minus));
       if (!kFull) {
         y.x = (mask[w] >> (2 * j)) & 1 ? y.x : -INFINITY;
@@ -232,17 +263,30 @@ __device__ __forceinline__ float weights(uint32_t s_cols, const uint32_t (&mask)
       const float2 p = make_float2(exp2_ftz(y.x), exp2_ftz(y.y));
       const uint32_t both = pack2((const T*)nullptr, p.x, p.y);
       packed[w * 16 + j] = both;
-      sum = add2(sum, p);
-      if constexpr (__is_same(T, __nv_bfloat16)) sum_p = add2(sum_p, make_float2(__uint_as_float(both << 16), __uint_as_float(both & 0xffff0000u)));
+      sum[j & 1] = add2(sum[j & 1], p);
+      if constexpr (__is_same(T, __nv_bfloat16))
+        sum_p[j & 1] = add2(sum_p[j & 1], make_float2(__uint_as_float(both << 16), __uint_as_float(both & 0xffff0000u)));
     }
   }
-  sums[0] = sum.x + sum.y;
-  sums[1] = __is_same(T, __nv_bfloat16) ? sum_p.x + sum_p.y : sums[0];
+  sums[0] = sum[0].x + sum[0].y + (sum[1].x + sum[1].y);
+  sums[1] = __is_same(T, __nv_bfloat16) ? sum_p[0].x + sum_p[0].y + (sum_p[1].x + sum_p[1].y) : sums[0];
   return fmaxf(top[0], top[1]);
+}
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 template <int D, typename T, bool kE4M3>
-__global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap k_map,
+                                                                               const __grid_constant__ CUtensorMap v_map) {
   using L = Shape<D>;
   constexpr int kTile = L::kTile, kSlots = L::kSlots, kStreams = L::kStreams;
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
@@ -264,6 +308,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     for (int i = 0; i < kRing; ++i) mbar_init(b_piece + i, 1), mbar_init(b_taken + i, L::kSoftmaxWarps + 5);
     mbar_fence_init();
     s_first[0] = -1;
+    if (p.box > 0) tma_prefetch_desc(&k_map), tma_prefetch_desc(&v_map);
   }
   if (warp == L::kMma) tmem_alloc(&s_tmem, L::kCols);
   pdl_wait();
@@ -317,41 +362,45 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     // (nothing for this CTA)
   } else if (warp < L::kSoftmaxWarps) {
     // ================= a stream's softmax: a thread has a query =================
+    if constexpr (L::kMoreRegs > 0) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kMoreRegs > 0 ? L::kMoreRegs : 128));
     const int t = warp >> 2, lane_at = (warp & 3) * 32, me = lane_at + lane;
     const uint32_t s_cols = tmem + t * kTile + ((uint32_t)lane_at << 16), o_cols = tmem + L::kColsO + t * D + ((uint32_t)lane_at << 16);
     unsigned char* const q_tile = tiles + t * L::kQ;
-    int steps = 0, items = 0, tile0 = 0;
-    Piece x;
-    while (take(x)) {
-      const int n = tiles_of_stream(x, t), from = tile0;
-      tile0 += x.tiles;
-      const int query = x.query0 + (x.pair ? t * 128 : 0) + me;
-      const bool real = query < x.query0 + x.queries && (x.pair || me < x.queries);
-      if (n == 0) continue;
-      float factor = p.a.scale * kLog2e;
-      if (kE4M3) factor *= p.pool.k_scale[x.head];
-      const uint32_t flip = factor < 0 ? 0x80008000u : 0;  // (the maximum is that of the scores before the factor)
-      factor = fabsf(factor);
-      int row = 0, head = 0, lo = 0, hi = 0;
-      if (real) {
-        const int member = query / p.group;
-        head = x.head * p.group + query - member * p.group;
-        row = x.first < 0 ? ~x.first : p.order[x.first + member];
-        if ((unsigned)row < (unsigned)p.a.rows) {
-          const Seen s = seen_of(p.a.lengths[row], p.max_len, p.a.window);
-          lo = s.first, hi = s.end;
-        } else {
-          row = -1;
+    int tile0 = 0;
+    struct Work {
+      int begin, n, first_tile, tile_no;  // the piece's first position, tiles of this stream, its first one, their number among all of the CTA
+      int lo, hi;                         // positions that the query sees
+      long long to;                       // where its output goes
+      float factor;
+      bool there, idle, whole, pair;
+    };
+    // The next piece that this stream has tiles of: its queries to shared memory, which the products of the one before are done with.
+    auto begin = [&](Work& y) {
+      Piece x;
+      while (take(x)) {
+        y.tile_no = tile0;
+        tile0 += x.tiles;
+        y.n = tiles_of_stream(x, t);
+        if (y.n == 0) continue;
+        const int query = x.query0 + (x.pair ? t * 128 : 0) + me, member = query / p.group, head = x.head * p.group + query - member * p.group;
+        y.there = query < x.query0 + x.queries && (x.pair || me < x.queries);
+        int row = 0;
+        if (y.there) {
+          row = x.first < 0 ? ~x.first : p.order[x.first + member];
+          y.there = (unsigned)row < (unsigned)p.a.rows;
         }
-      }
-      const bool there = real && row >= 0;
-      {
+        y.factor = p.a.scale * kLog2e;
+        if (kE4M3) y.factor *= p.pool.k_scale[x.head];
+        const uint32_t flip = y.factor < 0 ? 0x80008000u : 0;  // (the maximum is that of the scores before the factor)
+        y.factor = fabsf(y.factor);
         const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.a.q) + row * p.a.q_stride + head * p.a.q_head_stride);
+        Seen seen = {0, 0};
+        if (y.there) seen = seen_of(p.a.lengths[row], p.max_len, p.a.window);
 #pragma unroll
         for (int c0 = 0; c0 < D / 8; c0 += 8) {
           uint4 v[8];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) v[c] = there ? q[c0 + c] : make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < 8; ++c) v[c] = y.there ? q[c0 + c] : make_uint4(0, 0, 0, 0);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             v[c].x ^= flip, v[c].y ^= flip, v[c].z ^= flip, v[c].w ^= flip;
@@ -360,37 +409,60 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         }
         fence_async_shared();
         mbar_arrive(b_q + t);
+        y.lo = seen.first, y.hi = seen.end;
+        y.begin = x.begin;
+        y.first_tile = x.pair || kStreams == 1 ? 0 : t ^ x.stream;
+        const int half = x.pair ? (x.whole ? 0 : t) : t ^ x.stream;
+        y.to = x.whole ? (((x.first < 0 ? 2 : 0) + half) * (long long)p.a.rows + row) * p.a.heads + head : (cta * 2ll + half) * 128 + me;
+        y.idle = !__any_sync(0xffffffffu, y.there);  // a warp without queries
+        y.whole = x.whole;
+        y.pair = x.pair;
+        return true;
       }
-      const bool idle = !__any_sync(0xffffffffu, there);  // a warp without queries
+      return false;
+    };
+    uint32_t s_parity = 0, o_parity = 0;
+    Work x;
+    bool more = begin(x);
+    while (more) {
       float base = -INFINITY, sum = 0.f, sum_p = 0.f;    // base: minus infinity before there is a score
-      for (int i = 0; i < n; ++i) {
-        const int tile = x.pair || kStreams == 1 ? i : 2 * i + (t ^ x.stream), pos = x.begin + tile * kTile;
-        if (!wait(b_s + t, steps & 1)) break;
-        ++steps;
-        if (!idle) {
+      for (int i = 0; i < x.n; ++i) {
+        const int tile = x.pair || kStreams == 1 ? i : 2 * i + x.first_tile, pos = x.begin + tile * kTile;
+        if (!wait(b_s + t, s_parity)) break;
+        s_parity ^= 1;
+        if (!x.idle) {
           tc_fence_after_sync();
           // positions of the tile that are there and that this query sees
-          uint32_t mask[kTile / 32], all = 0xffffffffu;
-          const uint32_t* const words = s_there[(from + tile) % kSlots];
+          uint32_t mask[kTile / 32];
+          const uint32_t* const words = s_there[(x.tile_no + tile) % kSlots];
+          uint32_t all = 0xffffffffu;
 #pragma unroll
-          for (int w = 0; w < kTile / 32; ++w) {
-            const int a = min(max(lo - pos - w * 32, 0), 32), b = min(max(hi - pos - w * 32, 0), 32);  // [a, b)
-            const uint32_t below = b >= 32 ? 0xffffffffu : (1u << b) - 1, under = a >= 32 ? 0xffffffffu : (1u << a) - 1;
-            mask[w] = words[w] & below & ~under;
-            all &= mask[w];
+          for (int w = 0; w < kTile / 32; ++w) all &= mask[w] = words[w];
+          const bool full = all == 0xffffffffu && __all_sync(0xffffffffu, !x.there || (pos >= x.lo && pos + kTile <= x.hi));
+          if (!full) {
+#pragma unroll
+            for (int w = 0; w < kTile / 32; ++w) {
+              const int a = min(max(x.lo - pos - w * 32, 0), 32), b = min(max(x.hi - pos - w * 32, 0), 32);  // [a, b)
+              mask[w] &= (b >= 32 ? 0xffffffffu : (1u << b) - 1) & ~(a >= 32 ? 0xffffffffu : (1u << a) - 1);
+            }
           }
-          const bool full = __all_sync(0xffffffffu, all == 0xffffffffu || !there);
-          // The weights against the base as it is, in registers; where a score is too far above it, they are taken again.  (The first
-          // tile has no base yet.)
+          if (i == 0) {
+            const float top = largest<kTile>(s_cols, mask);
+            if (top > -INFINITY) base = __fsub_rn(__fmul_rn(top, x.factor), kShift);
+          }
+          // The weights against the base as it is, in registers; where a score is too far above it, they are taken again.
           uint32_t packed[kTile / 2];
           float sums[2];
-          const float limit = base == -INFINITY ? -INFINITY : kShift + kSlack;
-          float top = full ? weights<T, kTile, true>(s_cols, mask, factor, base, packed, sums) : weights<T, kTile, false>(s_cols, mask, factor, base, packed, sums);
-          if (__any_sync(0xffffffffu, top > limit)) {
+          for (int again = 0; again < 2; ++again) {
+            const float top = full ? weights<T, kTile, true>(s_cols, mask, x.factor, base, packed, sums)
+                                   : weights<T, kTile, false>(s_cols, mask, x.factor, base, packed, sums);
+            const bool above = top > (base == -INFINITY ? -INFINITY : kShift + kSlack);
+            if (again != 0 || !__any_sync(0xffffffffu, above)) break;
+            // (from the score itself and not from the exponent: the largest one's weight is right however large the scores are)
+            const float most = largest<kTile>(s_cols, mask);
             float by = 1.f;
-            if (top > limit) {
-              // (the exponents and the base move by the same amount, as rounded: the largest score's weight is right however large they are)
-              const float next = __fadd_rn(base == -INFINITY ? 0.f : base, __fsub_rn(top, kShift));
+            if (above) {
+              const float next = __fsub_rn(__fmul_rn(most, x.factor), kShift);
               by = exp2_ftz(base - next);
               base = next;
             }
@@ -401,13 +473,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
               for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
                 tmem_ld_32x32(o_cols + c, o);
-                tmem_ld_wait();
+                tmem_ld_done(o);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
                 tmem_st_32x32(o_cols + c, o);
               }
             }
-            weights<T, kTile, false>(s_cols, mask, factor, base, packed, sums);
           }
           sum += sums[0];
           sum_p += sums[1];
@@ -419,20 +490,20 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         __syncwarp();
         if (lane == 0) mbar_arrive(b_p + t);
       }
-      if (!wait(b_o + t, items & 1)) break;
-      ++items;
+      Work y;
+      more = ok && begin(y);  // (its queries before this one's output: its scores come meanwhile)
+      if (!wait(b_o + t, o_parity)) break;
+      o_parity ^= 1;
       tc_fence_after_sync();
-      if (!idle) {
-        const int half = x.pair ? (x.whole ? 0 : t) : t ^ x.stream;
-        const long long at = x.whole ? (((x.first < 0 ? 2 : 0) + half) * (long long)p.a.rows + row) * p.a.heads + head : (cta * 2ll + half) * 128 + me;
-        float4* const to = reinterpret_cast<float4*>((x.whole ? p.out : p.more) + at * D);
-        if (there) (x.whole ? p.ml : p.more_ml)[at] = make_float4(base, sum_p, sum, 0.f);
+      if (!x.idle) {
+        float4* const to = reinterpret_cast<float4*>((x.whole ? p.out : p.more) + x.to * D);
+        if (x.there) (x.whole ? p.ml : p.more_ml)[x.to] = make_float4(base, sum_p, sum, 0.f);
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
           tmem_ld_32x32(o_cols + c, o);
-          tmem_ld_wait();
-          if (there) {
+          tmem_ld_done(o);
+          if (x.there) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               to[c / 4 + j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
@@ -440,9 +511,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         }
         tc_fence_before_sync();
       }
+      x = y;
     }
   } else if (warp == L::kMma) {
     // ================= products, a step (a tile of positions of a stream) after another =================
+    if constexpr (L::kMoreRegs > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kFewerRegs));
     // The whole warp walks along and elects a lane for the instructions alone; what they take is the same in all lanes and known to
     // be (through a shuffle), else every operand of every one of them is fetched by itself (300 clocks for the product of a tile, so 60).
     auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
@@ -453,67 +526,88 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     const uint64_t q_desc = make_smem_desc((uint32_t)same((int)q_at)), k_desc = make_smem_desc((uint32_t)same((int)kv_at)),
                    v_desc = value_desc<kTile>((uint32_t)same((int)kv_at));
     const uint32_t q_hi = (uint32_t)(q_desc >> 32), q_lo = (uint32_t)q_desc, k_lo = (uint32_t)k_desc, v_hi = (uint32_t)(v_desc >> 32), v_lo = (uint32_t)v_desc;
-    // the steps whose scores are asked for, and whose weights are not yet multiplied: stream, slot number of the values, what it is
+    // What each stream has under way: a step whose scores are asked for and whose weights are not yet multiplied.  Whatever is ready goes
+    // next, so that neither stream waits for the other.
     struct Step {
-      int stream, value;
-      bool first, last, frees;
-    } old = {}, next = {};
-    int queued = 0, q_no = 0, p_no = 0;  // (q_no, p_no: a bit for each stream's parity)
-    auto pop = [&]() {  // O += P V of the oldest step
-      const Step x = old;
-      old = next;
-      --queued;
-      if (!wait(b_p + x.stream, (p_no >> x.stream) & 1)) return;
-      p_no ^= 1 << x.stream;
-      const int slot = x.value % kSlots;
-      if (!wait(b_full + slot, (x.value / kSlots) & 1)) return;
-      tc_fence_after_sync();
-      const uint32_t d = cols + L::kColsO + x.stream * D, a = cols + x.stream * kTile, v = v_lo + slot * (L::kSlot >> 4);
-      if (elect_one()) {
+      int value;  // slot number of the values
+      bool on, first, last, alone;
+    } step[2] = {};
+    int done[2] = {-1, -1};           // the values that each has last multiplied
+    uint32_t q_no = 0, p_no = 0;      // a bit for each stream's parity
+    auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar, parity)); };
+    auto full = [&](int number) { return ready(b_full + number % kSlots, (number / kSlots) & 1); };
+    int tile0 = 0, tiles_here = 0, pair = 0, stream0 = 0, i = 0, end = 0;  // the piece at work: steps done, and all of them
+    bool more = true;
+    uint32_t idle = 0;
+    unsigned long long since = 0;
+    while (ok && (more || i < end || step[0].on || step[1].on)) {
+      bool moved = false;
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k) umma_ts(d, a + k * 8, make_desc(v_hi, v + (k * 16 * 128 >> 4)), kIdO, !x.first || k > 0);
-        if (x.frees) umma_commit(b_free + slot);
-        if (x.last) umma_commit(b_o + x.stream);
+      for (int t = 0; t < kStreams; ++t) {  // O += P V
+        Step& x = step[t];
+        if (!x.on || !ready(b_p + t, (p_no >> t) & 1) || !full(x.value)) continue;
+        tc_fence_after_sync();
+        const int slot = x.value % kSlots;
+        const bool frees = x.alone || done[t ^ 1] >= x.value;  // (the second of two)
+        done[t] = x.value;
+        const uint32_t d = cols + L::kColsO + t * D, a = cols + t * kTile, v = v_lo + slot * (L::kSlot >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k) umma_ts(d, a + k * 8, make_desc(v_hi, v + (k * 16 * 128 >> 4)), kIdO, !x.first || k > 0);
+          if (frees) umma_commit(b_free + slot);
+          if (x.last) umma_commit(b_o + t);
+        }
+        __syncwarp();
+        p_no ^= 1u << t;
+        x.on = false;
+        moved = true;
       }
-      __syncwarp();
-    };
-    int tile0 = 0;
-    Piece x;
-    while (take(x)) {
-      const int tiles_here = same(x.tiles), pair = same(x.pair), stream0 = same(x.stream);
-      for (int i = 0; i < (pair ? 2 * tiles_here : tiles_here) && ok; ++i) {
+      if (i == end && more && ready(b_piece + piece_no % kRing, (piece_no / kRing) & 1)) {
+        tile0 += tiles_here;
+        Piece x;
+        more = take(x);
+        tiles_here = same(x.tiles), pair = same(x.pair), stream0 = same(x.stream);
+        i = 0;
+        end = pair ? 2 * tiles_here : tiles_here;
+        moved = true;
+      }
+      if (i < end) {  // S = Q K^T
         const int tile = pair ? i >> 1 : i, t = pair ? i & 1 : kStreams == 1 ? 0 : (stream0 + i) & 1;
         const int nth = pair || kStreams == 1 ? tile : i >> 1;
         const int n = pair || kStreams == 1 ? tiles_here : (tiles_here + 1 - (t ^ stream0)) / 2;
-        while (ok && queued > 0 && (queued == 2 || old.stream == t)) pop();
-        if (nth == 0) {
-          // (the queries come when the stream's last item is done, which takes its last product)
-          while (ok && queued > 0 && !__all_sync(0xffffffffu, mbar_try_wait(b_q + t, (q_no >> t) & 1))) pop();
-          if (!wait(b_q + t, (q_no >> t) & 1)) break;
-          q_no ^= 1 << t;
-        }
         const int number = 2 * (tile0 + tile), slot = number % kSlots;
-        if (!wait(b_full + slot, (number / kSlots) & 1)) break;
-        tc_fence_after_sync();
-        const bool frees = !pair || t == 1;
-        const uint32_t d = cols + t * kTile, q = q_lo + t * (L::kQ >> 4), k0 = k_lo + slot * (L::kSlot >> 4);
-        if (elect_one()) {
+        if (!(t == 0 ? step[0].on : step[1].on) && (nth > 0 || ready(b_q + t, (q_no >> t) & 1)) && full(number)) {
+          tc_fence_after_sync();
+          const bool frees = !pair || t == 1;
+          const uint32_t d = cols + t * kTile, q = q_lo + t * (L::kQ >> 4), k0 = k_lo + slot * (L::kSlot >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_bf16(d, make_desc(q_hi, q + ((k >> 2) * 128 * 128 + (k & 3) * 32 >> 4)), make_desc(q_hi, k0 + ((k >> 2) * kTile * 128 + (k & 3) * 32 >> 4)), kIdS,
-                      k > 0);
-          umma_commit(b_s + t);
-          if (frees) umma_commit(b_free + slot);
+            for (int k = 0; k < D / 16; ++k)
+              umma_bf16(d, make_desc(q_hi, q + ((k >> 2) * 128 * 128 + (k & 3) * 32 >> 4)),
+                        make_desc(q_hi, k0 + ((k >> 2) * kTile * 128 + (k & 3) * 32 >> 4)), kIdS, k > 0);
+            umma_commit(b_s + t);
+            if (frees) umma_commit(b_free + slot);
+          }
+          __syncwarp();
+          if (nth == 0) q_no ^= 1u << t;
+          const Step x = {number + 1, true, nth == 0, nth + 1 == n, !pair};
+          if (t == 0) step[0] = x;
+          else step[1] = x;
+          ++i;
+          moved = true;
         }
-        __syncwarp();
-        (queued == 0 ? old : next) = {t, number + 1, nth == 0, nth + 1 == n, frees};
-        ++queued;
       }
-      tile0 += tiles_here;
+      if (moved) {
+        idle = 0;
+      } else if ((++idle & 1023u) == 0) {  // (bounded, as every wait is)
+        const unsigned long long now = (unsigned long long)__shfl_sync(0xffffffffu, gtime_ns(), 0);
+        if (idle == 1024) since = now;
+        else if (now - since > kWaitNs) ok = false;
+      }
     }
-    while (ok && queued > 0) pop();
   } else if (warp < L::kWalk) {
     // ================= keys and values to shared memory =================
+    if constexpr (L::kMoreRegs > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kFewerRegs));
     const int me = tid - L::kLoad * 32;
     constexpr int kSize = kE4M3 ? 1 : 2, kChunks = D * kSize / 16, kPer = kTile * kChunks / 128;  // 16-byte chunks of a position, of a thread
     const int c = me % kChunks, r0 = me / kChunks;
@@ -543,13 +637,44 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
       int id = me < kTile && pos < x.end ? table[div_page(p.div, pos)] : -1;
       for (int tile = 0; tile < x.tiles; ++tile, ++tile_no) {
         if (me < kTile) {
-          const uint32_t at = step_of(id, p.pool.pages, pos, p.div, p.page_step, p.pos_step);
+          const uint32_t at = pos >= x.low ? step_of(id, p.pool.pages, pos, p.div, p.page_step, p.pos_step) : kNoStep;
           s_place[tile_no % (kSlots / 2)][me] = at;
           const uint32_t there = __ballot_sync(0xffffffffu, at != kNoStep);
           if (lane == 0) s_there[tile_no % kSlots][me / 32] = there;
         }
+        const int now = id, at0 = pos - me;
         pos += kTile;
         id = me < kTile && pos < x.end && tile + 1 < x.tiles ? table[div_page(p.div, pos)] : -1;
+        if (!kE4M3 && p.box > 0 && at0 >= x.low && at0 + kTile <= x.end) {
+          // a whole tile of whole boxes: each warp asks for its 32 positions (a page that is none is out of the tensor, which gives zeros)
+          if (told < number) {
+            cp_async_wait<0>();
+            tell(number);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!room()) continue;
+            uint64_t* const bar = b_full + number % kSlots;
+            unsigned char* const to = tiles + kStreams * L::kQ + (number % kSlots) * L::kSlot + (me & -32) * 128;
+            if (me < kTile) {
+              if (lane == 0) mbar_expect_tx(bar, 32 * D * 2);
+              else mbar_arrive(bar);
+              for (int b = 0; b < 32; b += p.box) {
+                const int page = __shfl_sync(0xffffffffu, now, b), y = __shfl_sync(0xffffffffu, at0 + me, b), in = y - div_page(p.div, y) * p.pool.page_size;
+                const int z = (unsigned)page < (unsigned)p.pool.pages ? page : p.pool.pages, head = __shfl_sync(0xffffffffu, x.head, 0);
+                if (elect_one()) {
+#pragma unroll
+                  for (int c = 0; c < D / 64; ++c) tma_load_4d(to + c * kTile * 128 + b * 128, h == 0 ? &k_map : &v_map, bar, c * 64, in, head, z);
+                }
+                __syncwarp();
+              }
+            } else {
+              mbar_arrive(bar);
+            }
+            told = ++number;
+          }
+          continue;
+        }
         if (!named_bar_all(1, 128, ok)) {
           ok = false;
           break;
@@ -608,8 +733,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
       cp_async_wait<0>();
       if (ok) tell(number);
     }
+  } else if (warp > L::kWalk) {
+    if constexpr (L::kMoreRegs > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kFewerRegs));
   } else {
     // ================= the walk along the line =================
+    if constexpr (L::kMoreRegs > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kFewerRegs));
     int e = s_first[0], off = s_first[1], no = 0, parity = 0;
     long long at = (long long)cta * share;
     const long long end = min((long long)units, at + share);
@@ -624,13 +752,14 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     };
     while (ok && at < end && e < elements) {
       // 32 elements at a time
-      const Element mine = e + lane < elements ? element_of<D>(p, e + lane) : Element{0, 0, 0, 0, 0};
+      const Element mine = e + lane < elements ? element_of<D>(p, e + lane) : Element{};
       uint32_t some = __ballot_sync(0xffffffffu, mine.end > mine.begin);
       for (; some != 0 && at < end && ok; some &= some - 1) {
         const int l = __ffs(some) - 1;
         Element x;
         x.begin = __shfl_sync(0xffffffffu, mine.begin, l);
         x.end = __shfl_sync(0xffffffffu, mine.end, l);
+        x.low = __shfl_sync(0xffffffffu, mine.low, l);
         x.queries = __shfl_sync(0xffffffffu, mine.queries, l);
         x.first = __shfl_sync(0xffffffffu, mine.first, l);
         x.row = __shfl_sync(0xffffffffu, mine.row, l);
@@ -645,6 +774,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
             y.tiles = part.to - part.from;
             y.begin = x.begin + part.from * kTile;
             y.end = x.end;
+            y.low = x.low;
             y.row = x.row;
             y.first = x.first;
             y.head = item / cuts;
@@ -786,7 +916,19 @@ cudaError_t launch(Params p, char* workspace, int sms, cudaStream_t stream) {
   auto* kernel = k_shared_attention<D, T, kE4M3>;
   cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(kernel), L::kSmem).rc;
   if (rc != cudaSuccess) return rc;
-  rc = launch_kernel_ex(kernel, dim3(p.ctas), dim3(L::kThreads), (size_t)L::kSmem, stream, true, 1, p);
+  // TMA boxes of whole pages or parts of one, of 8 to 32 positions (so many divide a page); pools that no tensor map can have, and
+  // 8-bit ones, which are converted on the way, go by cp.async
+  CUtensorMap k_map = {}, v_map = {};
+  p.box = 32;
+  while (p.box > 1 && p.pool.page_size % p.box != 0) p.box /= 2;
+  const PagedPool& pool = p.pool;
+  const bool bf16 = __is_same(T, __nv_bfloat16);
+  auto map = [&](CUtensorMap* m, const void* base) {
+    return make_page_map(m, base, bf16, D, pool.page_size, pool.heads, pool.pages, pool.pos_stride * 2, pool.head_stride * 2, pool.page_stride * 2, p.box) ==
+           cudaSuccess;
+  };
+  if (kE4M3 || p.box < 8 || !map(&k_map, pool.k) || !map(&v_map, pool.v)) p.box = 0;
+  rc = launch_kernel_ex(kernel, dim3(p.ctas), dim3(L::kThreads), (size_t)L::kSmem, stream, true, 1, p, k_map, v_map);
   if (rc != cudaSuccess) return rc;
   return launch_kernel_ex(k_shared_join<D, T>, dim3(p.a.rows, p.pool.heads), dim3(kJoinWarps * 32), 0, stream, true, 1, p);
 }

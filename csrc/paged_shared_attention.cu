@@ -16,9 +16,10 @@
 //   * All items (a KV head of a group, or of a row) lie in a line that is cut into equal shares, a CTA to an SM
 //     (paged_shared_plan.h).  A warp walks the line and hands the pieces to the others; loads run ahead across pieces.  Pieces leave unnormalised
 //     fp32 outputs in a workspace, a second kernel joins them.  No counters: a workspace holds nothing between calls.
-//   * Weights count from a base that follows the maximum when a score is above it by more than kSlack; the accumulators are scaled then,
-//     which is seldom.  bf16 weights are rounded by up to 2^-8 of each; the output is divided by the sum of the rounded ones, so that a
-//     weight that outweighs the others is not off, and the logarithm is that of the others' sum.  fp16 weights stand 2^kShift above, against what fp16 loses under 2^-14.
+//   * Weights count from a base that is the largest score of the first tile; it follows, and the accumulators are scaled, when the weights
+//     of a tile add up to more than 2^40 (fp16 weights, which stand 2^7 above it against what fp16 loses under 2^-14: 2^15), which is seldom.
+//     Weights are rounded to their type by up to half a step of each, their sum is not; an output is then off by what the
+//     roundings of many weights leave, about one of its own.
 //
 // Every wait is bounded; one that ran out sets the error word that all tcgen05 kernels here share, and the CTA ends.
 #include <cuda_bf16.h>
@@ -73,9 +74,9 @@ struct Params {
   int* line;         // [2 rows + 1]: first unit of every element: groups, then rows; all units
   int2* place;       // [rows]: a row's group and its number in it
   float* out;        // [4][rows][heads][D]: first pieces: of shared positions, of own ones, two halves each
-  float4* ml;        // [4][rows][heads]: base, sum of the weights as they were multiplied, sum of the weights
+  float2* ml;        // [4][rows][heads]: base, sum of the weights
   float* more;       // [ctas][2][128][D]: pieces that do not begin an item
-  float4* more_ml;
+  float2* more_ml;
   uint32_t* error;
 };
 
@@ -237,14 +238,12 @@ __device__ __forceinline__ float largest(uint32_t s_cols, const uint32_t (&mask)
   }
   return top;
 }
-// A thread's row of S: weights exp2(score * factor - base), rounded to T, in pairs; their sums, unrounded and rounded; returns the largest
-// exponent (minus infinity: nothing is there).  kFull: all positions are there.  A base of minus infinity counts as zero.
+// A thread's row of S: weights exp2(score * factor - base), rounded to T, in pairs; returns their sum, unrounded.  kFull: all positions are
+// there.  (The multiplication by itself and then the difference: a score that is the base's has weight one however large it is.)
 template <typename T, int kTile, bool kFull>
-__device__ __forceinline__ float weights(uint32_t s_cols, const uint32_t (&mask)[kTile / 32], float factor, float base, uint32_t (&packed)[kTile / 2],
-                                         float (&sums)[2]) {
-  const float minus = base == -INFINITY ? 0.f : -base;
-  float top[2] = {-INFINITY, -INFINITY};
-  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, sum_p[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+__device__ __forceinline__ float weights(uint32_t s_cols, const uint32_t (&mask)[kTile / 32], float factor, float base, uint32_t (&packed)[kTile / 2]) {
+  const float2 by = make_float2(factor, factor), minus = make_float2(-base, -base);
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   uint32_t s[2][32];
   tmem_ld_32x32(s_cols, s[0]);
 #pragma unroll
@@ -253,24 +252,17 @@ __device__ __forceinline__ float weights(uint32_t s_cols, const uint32_t (&mask)
     if (w + 1 < kTile / 32) tmem_ld_32x32(s_cols + (w + 1) * 32, s[(w + 1) & 1]);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      float2 y = mul2(make_float2(__uint_as_float(s[w & 1][2 * j]), __uint_as_float(s[w & 1][2 * j + 1])), make_float2(factor, factor));
-      y = add2(y, make_float2(minus, minus));
+      const float2 y = add2(mul2(make_float2(__uint_as_float(s[w & 1][2 * j]), __uint_as_float(s[w & 1][2 * j + 1])), by), minus);
+      float2 p = make_float2(exp2_ftz(y.x), exp2_ftz(y.y));
       if (!kFull) {
-        y.x = (mask[w] >> (2 * j)) & 1 ? y.x : -INFINITY;
-        y.y = (mask[w] >> (2 * j + 1)) & 1 ? y.y : -INFINITY;
+        p.x = (mask[w] >> (2 * j)) & 1 ? p.x : 0.f;
+        p.y = (mask[w] >> (2 * j + 1)) & 1 ? p.y : 0.f;
       }
-      top[j & 1] = max3(top[j & 1], y.x, y.y);
-      const float2 p = make_float2(exp2_ftz(y.x), exp2_ftz(y.y));
-      const uint32_t both = pack2((const T*)nullptr, p.x, p.y);
-      packed[w * 16 + j] = both;
+      packed[w * 16 + j] = pack2((const T*)nullptr, p.x, p.y);
       sum[j & 1] = add2(sum[j & 1], p);
-      if constexpr (__is_same(T, __nv_bfloat16))
-        sum_p[j & 1] = add2(sum_p[j & 1], make_float2(__uint_as_float(both << 16), __uint_as_float(both & 0xffff0000u)));
     }
   }
-  sums[0] = sum[0].x + sum[0].y + (sum[1].x + sum[1].y);
-  sums[1] = __is_same(T, __nv_bfloat16) ? sum_p[0].x + sum_p[0].y + (sum_p[1].x + sum_p[1].y) : sums[0];
-  return fmaxf(top[0], top[1]);
+  return sum[0].x + sum[0].y + (sum[1].x + sum[1].y);
 }
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -290,12 +282,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
   using L = Shape<D>;
   constexpr int kTile = L::kTile, kSlots = L::kSlots, kStreams = L::kStreams;
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
-  // exponents: the base is kShift under the maximum, and follows when a score is above that by more than kSlack
-  constexpr float kSlack = 8.f, kShift = kBf16 ? 0.f : 7.f;
+  // The base is kShift under the largest score of the first tile that has any, and of a later one in which the weights' sum is above kLimit.
+  constexpr float kShift = kBf16 ? 0.f : 7.f, kLimit = kBf16 ? 0x1p40f : 0x1p15f;
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t b_full[kSlots], b_free[kSlots], b_q[2], b_s[2], b_p[2], b_o[2], b_piece[kRing], b_taken[kRing];
   __shared__ Piece s_piece[kRing];
-  __shared__ uint32_t s_place[kSlots / 2][kTile], s_there[kSlots][4], s_tmem;
+  __shared__ uint32_t s_place[kSlots / 2][kTile], s_tmem;
+  __shared__ __align__(16) uint32_t s_there[kSlots][4];
   __shared__ uint32_t s_part[1][32];
   __shared__ int s_first[3];  // the element that the CTA's share begins in, how far behind the element's first unit, all units
   pdl_launch_dependents();
@@ -425,7 +418,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     Work x;
     bool more = begin(x);
     while (more) {
-      float base = -INFINITY, sum = 0.f, sum_p = 0.f;    // base: minus infinity before there is a score
+      float base = -INFINITY, sum = 0.f;    // base: minus infinity before there is a score
       for (int i = 0; i < x.n; ++i) {
         const int tile = x.pair || kStreams == 1 ? i : 2 * i + x.first_tile, pos = x.begin + tile * kTile;
         if (!wait(b_s + t, s_parity)) break;
@@ -446,42 +439,39 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
               mask[w] &= (b >= 32 ? 0xffffffffu : (1u << b) - 1) & ~(a >= 32 ? 0xffffffffu : (1u << a) - 1);
             }
           }
-          if (i == 0) {
-            const float top = largest<kTile>(s_cols, mask);
-            if (top > -INFINITY) base = __fsub_rn(__fmul_rn(top, x.factor), kShift);
-          }
-          // The weights against the base as it is, in registers; where a score is too far above it, they are taken again.
+          // The weights against the base as it is, in registers; where there is none yet, or their sum says that it lies too low, against one
+          // from the tile's largest score.
           uint32_t packed[kTile / 2];
-          float sums[2];
+          float of_tile = 0.f;
+          bool low = x.there && base == -INFINITY;
           for (int again = 0; again < 2; ++again) {
-            const float top = full ? weights<T, kTile, true>(s_cols, mask, x.factor, base, packed, sums)
-                                   : weights<T, kTile, false>(s_cols, mask, x.factor, base, packed, sums);
-            const bool above = top > (base == -INFINITY ? -INFINITY : kShift + kSlack);
-            if (again != 0 || !__any_sync(0xffffffffu, above)) break;
-            // (from the score itself and not from the exponent: the largest one's weight is right however large the scores are)
-            const float most = largest<kTile>(s_cols, mask);
-            float by = 1.f;
-            if (above) {
-              const float next = __fsub_rn(__fmul_rn(most, x.factor), kShift);
-              by = exp2_ftz(base - next);
-              base = next;
-            }
-            sum *= by;
-            sum_p *= by;
-            if (i > 0) {
+            if (__any_sync(0xffffffffu, low)) {
+              const float top = largest<kTile>(s_cols, mask);
+              float by = 1.f;
+              if (low && top > -INFINITY) {
+                const float next = __fsub_rn(__fmul_rn(top, x.factor), kShift);
+                by = exp2_ftz(base - next);
+                base = next;
+              }
+              sum *= by;
+              if (i > 0) {
 #pragma unroll 1
-              for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_ld_32x32(o_cols + c, o);
-                tmem_ld_done(o);
+                for (int c = 0; c < D; c += 32) {
+                  uint32_t o[32];
+                  tmem_ld_32x32(o_cols + c, o);
+                  tmem_ld_done(o);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
-                tmem_st_32x32(o_cols + c, o);
+                  for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
+                  tmem_st_32x32(o_cols + c, o);
+                }
               }
             }
+            const float from = base == -INFINITY ? 0.f : base;
+            of_tile = full ? weights<T, kTile, true>(s_cols, mask, x.factor, from, packed) : weights<T, kTile, false>(s_cols, mask, x.factor, from, packed);
+            low = of_tile > kLimit;
+            if (!__any_sync(0xffffffffu, low)) break;
           }
-          sum += sums[0];
-          sum_p += sums[1];
+          sum += of_tile;
 #pragma unroll
           for (int w = 0; w < kTile / 2; w += 32) tmem_st_32x32(s_cols + w, *reinterpret_cast<uint32_t(*)[32]>(packed + w));
           tmem_st_wait();
@@ -497,7 +487,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
       tc_fence_after_sync();
       if (!x.idle) {
         float4* const to = reinterpret_cast<float4*>((x.whole ? p.out : p.more) + x.to * D);
-        if (x.there) (x.whole ? p.ml : p.more_ml)[x.to] = make_float4(base, sum_p, sum, 0.f);
+        if (x.there) (x.whole ? p.ml : p.more_ml)[x.to] = make_float2(base, sum);
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
@@ -540,6 +530,33 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     bool more = true;
     uint32_t idle = 0;
     unsigned long long since = 0;
+    // S = Q K^T of the next step, if its stream is free and its operands are there
+    auto scores = [&]() {
+      if (i >= end) return false;
+      const int tile = pair ? i >> 1 : i, t = pair ? i & 1 : kStreams == 1 ? 0 : (stream0 + i) & 1;
+      const int nth = pair || kStreams == 1 ? tile : i >> 1;
+      const int n = pair || kStreams == 1 ? tiles_here : (tiles_here + 1 - (t ^ stream0)) / 2;
+      const int number = 2 * (tile0 + tile), slot = number % kSlots;
+      if ((t == 0 ? step[0].on : step[1].on) || (nth == 0 && !ready(b_q + t, (q_no >> t) & 1)) || !full(number)) return false;
+      tc_fence_after_sync();
+      const bool frees = !pair || t == 1;
+      const uint32_t d = cols + t * kTile, q = q_lo + t * (L::kQ >> 4), k0 = k_lo + slot * (L::kSlot >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_bf16(d, make_desc(q_hi, q + ((k >> 2) * 128 * 128 + (k & 3) * 32 >> 4)), make_desc(q_hi, k0 + ((k >> 2) * kTile * 128 + (k & 3) * 32 >> 4)),
+                    kIdS, k > 0);
+        umma_commit(b_s + t);
+        if (frees) umma_commit(b_free + slot);
+      }
+      __syncwarp();
+      if (nth == 0) q_no ^= 1u << t;
+      const Step x = {number + 1, true, nth == 0, nth + 1 == n, !pair};
+      if (t == 0) step[0] = x;
+      else step[1] = x;
+      ++i;
+      return true;
+    };
     while (ok && (more || i < end || step[0].on || step[1].on)) {
       bool moved = false;
 #pragma unroll
@@ -561,6 +578,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         p_no ^= 1u << t;
         x.on = false;
         moved = true;
+        scores();  // (most often this stream's, which waited for that)
       }
       if (i == end && more && ready(b_piece + piece_no % kRing, (piece_no / kRing) & 1)) {
         tile0 += tiles_here;
@@ -571,32 +589,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         end = pair ? 2 * tiles_here : tiles_here;
         moved = true;
       }
-      if (i < end) {  // S = Q K^T
-        const int tile = pair ? i >> 1 : i, t = pair ? i & 1 : kStreams == 1 ? 0 : (stream0 + i) & 1;
-        const int nth = pair || kStreams == 1 ? tile : i >> 1;
-        const int n = pair || kStreams == 1 ? tiles_here : (tiles_here + 1 - (t ^ stream0)) / 2;
-        const int number = 2 * (tile0 + tile), slot = number % kSlots;
-        if (!(t == 0 ? step[0].on : step[1].on) && (nth > 0 || ready(b_q + t, (q_no >> t) & 1)) && full(number)) {
-          tc_fence_after_sync();
-          const bool frees = !pair || t == 1;
-          const uint32_t d = cols + t * kTile, q = q_lo + t * (L::kQ >> 4), k0 = k_lo + slot * (L::kSlot >> 4);
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              umma_bf16(d, make_desc(q_hi, q + ((k >> 2) * 128 * 128 + (k & 3) * 32 >> 4)),
-                        make_desc(q_hi, k0 + ((k >> 2) * kTile * 128 + (k & 3) * 32 >> 4)), kIdS, k > 0);
-            umma_commit(b_s + t);
-            if (frees) umma_commit(b_free + slot);
-          }
-          __syncwarp();
-          if (nth == 0) q_no ^= 1u << t;
-          const Step x = {number + 1, true, nth == 0, nth + 1 == n, !pair};
-          if (t == 0) step[0] = x;
-          else step[1] = x;
-          ++i;
-          moved = true;
-        }
-      }
+      moved |= scores();
       if (moved) {
         idle = 0;
       } else if ((++idle & 1023u) == 0) {  // (bounded, as every wait is)
@@ -819,7 +812,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_shared_join(const __grid_co
   const float v_scale = p.pool.v_scale ? p.pool.v_scale[kh] : 1.f;
   for (int g = warp; g < p.group; g += kJoinWarps) {
     const int head = kh * p.group + g;
-    float top = -INFINITY, sum = 0.f, sum_p = 0.f, acc[kPer];
+    float top = -INFINITY, sum = 0.f, acc[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
 #pragma unroll 1
@@ -844,17 +837,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_shared_join(const __grid_co
           const int stream = pair ? within >> 7 : half, lane_of = pair ? within & 127 : within;
           at = piece == 0 ? ((2 * kind + half) * (long long)p.a.rows + row) * p.a.heads + head : ((first + piece) * 2ll + stream) * 128 + lane_of;
         }
-        const float4 ml = some ? (piece == 0 ? p.ml : p.more_ml)[at] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        const float2 ml = some ? (piece == 0 ? p.ml : p.more_ml)[at] : make_float2(-INFINITY, 0.f);
         float most = ml.x;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
         const float next = fmaxf(top, most), base = next == -INFINITY ? 0.f : next;
         const float old = exp2_ftz(top - base), by = exp2_ftz(ml.x - base);
-        float l = by * ml.z, l_p = by * ml.y;
+        float l = by * ml.y;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o), l_p += __shfl_xor_sync(0xffffffffu, l_p, o);
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         sum = sum * old + l;
-        sum_p = sum_p * old + l_p;
         top = next;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) acc[j] *= old;
@@ -877,7 +869,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_shared_join(const __grid_co
       }
     }
     // (no positions: zeros, as what was added up is zero)
-    const float inv = top == -INFINITY ? 0.f * sum_p : v_scale / sum_p;
+    const float inv = top == -INFINITY ? 0.f * sum : v_scale / sum;
     uint32_t* const out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.a.out) + row * p.a.out_stride + head * p.a.out_head_stride + lane * kPer);
 #pragma unroll
     for (int j = 0; j < kPer; j += 2) out[j / 2] = pack2((const T*)nullptr, acc[j] * inv, acc[j + 1] * inv);
@@ -893,9 +885,9 @@ struct Workspace {
     place = line + rounded((2 * rows + 1) * sizeof(int));
     out = place + rounded(rows * sizeof(int2));
     ml = out + rounded(4 * rows * heads * dim * sizeof(float));
-    more = ml + rounded(4 * rows * heads * sizeof(float4));
+    more = ml + rounded(4 * rows * heads * sizeof(float2));
     more_ml = more + rounded(ctas * 256 * dim * sizeof(float));
-    all = more_ml + rounded(ctas * 256 * sizeof(float4));
+    all = more_ml + rounded(ctas * 256 * sizeof(float2));
   }
 };
 
@@ -910,9 +902,9 @@ cudaError_t launch(Params p, char* workspace, int sms, cudaStream_t stream) {
   p.line = reinterpret_cast<int*>(workspace + w.line);
   p.place = reinterpret_cast<int2*>(workspace + w.place);
   p.out = reinterpret_cast<float*>(workspace + w.out);
-  p.ml = reinterpret_cast<float4*>(workspace + w.ml);
+  p.ml = reinterpret_cast<float2*>(workspace + w.ml);
   p.more = reinterpret_cast<float*>(workspace + w.more);
-  p.more_ml = reinterpret_cast<float4*>(workspace + w.more_ml);
+  p.more_ml = reinterpret_cast<float2*>(workspace + w.more_ml);
   auto* kernel = k_shared_attention<D, T, kE4M3>;
   cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(kernel), L::kSmem).rc;
   if (rc != cudaSuccess) return rc;

@@ -16,8 +16,8 @@
 //   * All items (a KV head of a group, or of a row) lie in a line that is cut into equal shares, a CTA to an SM
 //     (paged_shared_plan.h).  A warp walks the line and hands the pieces to the others; loads run ahead across pieces.  Pieces leave unnormalised
 //     fp32 outputs in a workspace, a second kernel joins them.  No counters: a workspace holds nothing between calls.
-//   * Weights count from a base that is the largest score of the first tile; it follows, and the accumulators are scaled, when the weights
-//     of a tile add up to more than 2^40 (fp16 weights, which stand 2^7 above it against what fp16 loses under 2^-14: 2^15), which is seldom.
+//   * Weights count from a base that is the largest score of the first 64 positions; it follows, and the accumulators are scaled, when the
+//     weights of 64 positions add up to more than 2^40 (fp16 weights, which stand 2^7 above it against what fp16 loses under 2^-14: 2^15), which is seldom.
 //     Weights are rounded to their type by up to half a step of each, their sum is not; an output is then off by what the
 //     roundings of many weights leave, about one of its own.
 //
@@ -53,10 +53,13 @@ struct Shape {
   static constexpr int kSlots = D == 64 ? 8 : 4;             // keys and values in turn
   static constexpr int kQ = 128 * D * 2;
   static constexpr int kSmem = kStreams * kQ + kSlots * kSlot + 1024;
-  static constexpr int kSoftmaxWarps = 4 * kStreams, kMma = kSoftmaxWarps, kLoad = kMma + 1, kWalk = kLoad + 4;
-  // whole warpgroups; those of two streams' softmax take registers from the others
-  static constexpr int kThreads = (kWalk + 4) / 4 * 4 * 32, kMoreRegs = kStreams == 2 ? 160 : 0, kFewerRegs = 96;
-  static_assert(kStreams == 1 || (kThreads == 512 && kMoreRegs * 256 + kFewerRegs * 256 <= 65536), "registers");
+  static constexpr int kSoftmaxWarps = 4 * kStreams, kLoad = kSoftmaxWarps, kWalk = kLoad + 4, kMma = kWalk + 3;
+  // (the issuer, which polls, is not on the scheduler of each stream's first warp, which has the queries of a single row)
+  static constexpr int kThreads = (kMma + 1) * 32;
+  // registers: whole warpgroups; those of two streams' softmax take some from the others.  (What spills is read back through an L1 of
+  // 20 KB that all loads go through: a tile of one row took 4000 to 9000 clocks in place of 2500.)
+  static constexpr int kMoreRegs = kStreams == 2 ? 160 : 0, kFewerRegs = 96;
+  static_assert(kThreads % 128 == 0 && (kStreams == 1 || (kThreads == 512 && kMoreRegs * 256 + kFewerRegs * 256 <= 65536)), "warpgroups");
   // tensor memory: S (and P) of each stream, then O
   static constexpr int kColsO = kStreams * kTile, kCols = kColsO + kStreams * D <= 256 ? 256 : 512;
   static_assert(kColsO + kStreams * D <= 512 && kSmem <= 200 << 10, "");
@@ -223,46 +226,50 @@ __device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[32]) {
                  "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
                  "+r"(r[31])::"memory");
 }
-// The largest score of a thread's row of S of those that are there.
-template <int kTile>
-__device__ __forceinline__ float largest(uint32_t s_cols, const uint32_t (&mask)[kTile / 32]) {
+// The largest score of 32 positions of a thread's row of S, of those that are there.
+__device__ __forceinline__ float largest(uint32_t s_cols, uint32_t mask) {
   float top = -INFINITY;
+  uint32_t s[32];
+  tmem_ld_32x32(s_cols, s);
+  tmem_ld_done(s);
 #pragma unroll
-  for (int w = 0; w < kTile / 32; ++w) {
-    uint32_t s[32];
-    tmem_ld_32x32(s_cols + w * 32, s);
-    tmem_ld_done(s);
-#pragma unroll
-    for (int j = 0; j < 32; j += 2)
-      top = max3(top, (mask[w] >> j) & 1 ? __uint_as_float(s[j]) : -INFINITY, (mask[w] >> (j + 1)) & 1 ? __uint_as_float(s[j + 1]) : -INFINITY);
-  }
+  for (int j = 0; j < 32; j += 2)
+    top = max3(top, (mask >> j) & 1 ? __uint_as_float(s[j]) : -INFINITY, (mask >> (j + 1)) & 1 ? __uint_as_float(s[j + 1]) : -INFINITY);
   return top;
 }
-// A thread's row of S: weights exp2(score * factor - base), rounded to T, in pairs; returns their sum, unrounded.  kFull: all positions are
-// there.  (The multiplication by itself and then the difference: a score that is the base's has weight one however large it is.)
-template <typename T, int kTile, bool kFull>
-__device__ __forceinline__ float weights(uint32_t s_cols, const uint32_t (&mask)[kTile / 32], float factor, float base, uint32_t (&packed)[kTile / 2]) {
+// 64 positions of a thread's row of S: weights exp2(score * factor - base), rounded to T, in pairs; returns their sum, unrounded.  kFull: all
+// positions are there.  (The multiplication by itself and then the difference: a score that is the base's has weight one however large it is.)
+template <typename T, bool kFull>
+__device__ __forceinline__ float weights(uint32_t s_cols, uint32_t mask0, uint32_t mask1, float factor, float base, uint32_t (&packed)[32]) {
   const float2 by = make_float2(factor, factor), minus = make_float2(-base, -base);
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   uint32_t s[2][32];
   tmem_ld_32x32(s_cols, s[0]);
+  tmem_ld_32x32(s_cols + 32, s[1]);
 #pragma unroll
-  for (int w = 0; w < kTile / 32; ++w) {
-    tmem_ld_done(s[w & 1]);
-    if (w + 1 < kTile / 32) tmem_ld_32x32(s_cols + (w + 1) * 32, s[(w + 1) & 1]);
+  for (int w = 0; w < 2; ++w) {
+    tmem_ld_done(s[w]);
+    const uint32_t mask = w == 0 ? mask0 : mask1;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const float2 y = add2(mul2(make_float2(__uint_as_float(s[w & 1][2 * j]), __uint_as_float(s[w & 1][2 * j + 1])), by), minus);
+      const float2 y = add2(mul2(make_float2(__uint_as_float(s[w][2 * j]), __uint_as_float(s[w][2 * j + 1])), by), minus);
       float2 p = make_float2(exp2_ftz(y.x), exp2_ftz(y.y));
       if (!kFull) {
-        p.x = (mask[w] >> (2 * j)) & 1 ? p.x : 0.f;
-        p.y = (mask[w] >> (2 * j + 1)) & 1 ? p.y : 0.f;
+        p.x = (mask >> (2 * j)) & 1 ? p.x : 0.f;
+        p.y = (mask >> (2 * j + 1)) & 1 ? p.y : 0.f;
       }
       packed[w * 16 + j] = pack2((const T*)nullptr, p.x, p.y);
       sum[j & 1] = add2(sum[j & 1], p);
     }
   }
   return sum[0].x + sum[0].y + (sum[1].x + sum[1].y);
+}
+__device__ __forceinline__ uint32_t times(const __nv_bfloat16*, uint32_t both, float by) {
+  return pack2((const __nv_bfloat16*)nullptr, __uint_as_float(both << 16) * by, __uint_as_float(both & 0xffff0000u) * by);
+}
+__device__ __forceinline__ uint32_t times(const __half*, uint32_t both, float by) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&both));
+  return pack2((const __half*)nullptr, f.x * by, f.y * by);
 }
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -282,7 +289,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
   using L = Shape<D>;
   constexpr int kTile = L::kTile, kSlots = L::kSlots, kStreams = L::kStreams;
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
-  // The base is kShift under the largest score of the first tile that has any, and of a later one in which the weights' sum is above kLimit.
+  // The base is kShift under the largest score of the first 64 positions that have any, and of later ones whose weights add up to over kLimit.
   constexpr float kShift = kBf16 ? 0.f : 7.f, kLimit = kBf16 ? 0x1p40f : 0x1p15f;
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t b_full[kSlots], b_free[kSlots], b_q[2], b_s[2], b_p[2], b_o[2], b_piece[kRing], b_taken[kRing];
@@ -421,59 +428,68 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
       float base = -INFINITY, sum = 0.f;    // base: minus infinity before there is a score
       for (int i = 0; i < x.n; ++i) {
         const int tile = x.pair || kStreams == 1 ? i : 2 * i + x.first_tile, pos = x.begin + tile * kTile;
+        const bool inside = __all_sync(0xffffffffu, !x.there || (pos >= x.lo && pos + kTile <= x.hi));  // every query sees all of the tile
         if (!wait(b_s + t, s_parity)) break;
         s_parity ^= 1;
         if (!x.idle) {
           tc_fence_after_sync();
-          // positions of the tile that are there and that this query sees
-          uint32_t mask[kTile / 32];
+          // positions of the tile that are there (and that this query sees)
           const uint32_t* const words = s_there[(x.tile_no + tile) % kSlots];
           uint32_t all = 0xffffffffu;
 #pragma unroll
-          for (int w = 0; w < kTile / 32; ++w) all &= mask[w] = words[w];
-          const bool full = all == 0xffffffffu && __all_sync(0xffffffffu, !x.there || (pos >= x.lo && pos + kTile <= x.hi));
-          if (!full) {
-#pragma unroll
-            for (int w = 0; w < kTile / 32; ++w) {
-              const int a = min(max(x.lo - pos - w * 32, 0), 32), b = min(max(x.hi - pos - w * 32, 0), 32);  // [a, b)
-              mask[w] &= (b >= 32 ? 0xffffffffu : (1u << b) - 1) & ~(a >= 32 ? 0xffffffffu : (1u << a) - 1);
-            }
-          }
-          // The weights against the base as it is, in registers; where there is none yet, or their sum says that it lies too low, against one
-          // from the tile's largest score.
-          uint32_t packed[kTile / 2];
-          float of_tile = 0.f;
-          bool low = x.there && base == -INFINITY;
-          for (int again = 0; again < 2; ++again) {
-            if (__any_sync(0xffffffffu, low)) {
-              const float top = largest<kTile>(s_cols, mask);
-              float by = 1.f;
-              if (low && top > -INFINITY) {
-                const float next = __fsub_rn(__fmul_rn(top, x.factor), kShift);
-                by = exp2_ftz(base - next);
-                base = next;
-              }
-              sum *= by;
-              if (i > 0) {
+          for (int w = 0; w < kTile / 32; ++w) all &= words[w];
+          const bool full = inside && all == 0xffffffffu;
+          auto seen = [&](int w) {
+            const int a = min(max(x.lo - pos - w * 32, 0), 32), b = min(max(x.hi - pos - w * 32, 0), 32);  // [a, b)
+            return words[w] & (b >= 32 ? 0xffffffffu : (1u << b) - 1) & ~(a >= 32 ? 0xffffffffu : (1u << a) - 1);
+          };
+          // 64 positions at a time (straight code for more is more than the instruction caches hold): their weights against the base as it
+          // is, in registers; where there is none yet, or their sum says that it lies too low, against one from their largest score.
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                  uint32_t o[32];
-                  tmem_ld_32x32(o_cols + c, o);
-                  tmem_ld_done(o);
+          for (int h = 0; h < kTile / 64; ++h) {
+            const uint32_t from_cols = s_cols + h * 64;
+            const uint32_t mask0 = full ? 0xffffffffu : seen(2 * h), mask1 = full ? 0xffffffffu : seen(2 * h + 1);
+            uint32_t packed[32];
+            float of_half = 0.f;
+            bool low = x.there && base == -INFINITY;
+#pragma unroll 1
+            for (int again = 0; again < 2; ++again) {
+              if (__any_sync(0xffffffffu, low)) {
+                const float top = fmaxf(largest(from_cols, mask0), largest(from_cols + 32, mask1));
+                float by = 1.f;
+                if (low && top > -INFINITY) {
+                  const float next = __fsub_rn(__fmul_rn(top, x.factor), kShift);
+                  by = exp2_ftz(base - next);
+                  base = next;
+                }
+                sum *= by;
+                if (h > 0 && __any_sync(0xffffffffu, by != 1.f)) {  // the weights in front of these
+                  tmem_ld_32x32(s_cols, packed);
+                  tmem_ld_done(packed);
 #pragma unroll
-                  for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
-                  tmem_st_32x32(o_cols + c, o);
+                  for (int j = 0; j < 32; ++j) packed[j] = times((const T*)nullptr, packed[j], by);
+                  tmem_st_32x32(s_cols, packed);
+                }
+                if (i > 0 && __any_sync(0xffffffffu, by != 1.f)) {
+#pragma unroll 1
+                  for (int c = 0; c < D; c += 32) {
+                    tmem_ld_32x32(o_cols + c, packed);
+                    tmem_ld_done(packed);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) packed[j] = __float_as_uint(__uint_as_float(packed[j]) * by);
+                    tmem_st_32x32(o_cols + c, packed);
+                  }
                 }
               }
+              const float from = base == -INFINITY ? 0.f : base;
+              of_half = full ? weights<T, true>(from_cols, mask0, mask1, x.factor, from, packed)
+                             : weights<T, false>(from_cols, mask0, mask1, x.factor, from, packed);
+              low = of_half > kLimit;
+              if (!__any_sync(0xffffffffu, low)) break;
             }
-            const float from = base == -INFINITY ? 0.f : base;
-            of_tile = full ? weights<T, kTile, true>(s_cols, mask, x.factor, from, packed) : weights<T, kTile, false>(s_cols, mask, x.factor, from, packed);
-            low = of_tile > kLimit;
-            if (!__any_sync(0xffffffffu, low)) break;
+            sum += of_half;
+            tmem_st_32x32(s_cols + h * 32, packed);
           }
-          sum += of_tile;
-#pragma unroll
-          for (int w = 0; w < kTile / 2; w += 32) tmem_st_32x32(s_cols + w, *reinterpret_cast<uint32_t(*)[32]>(packed + w));
           tmem_st_wait();
           tc_fence_before_sync();
         }
@@ -592,7 +608,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
       moved |= scores();
       if (moved) {
         idle = 0;
-      } else if ((++idle & 1023u) == 0) {  // (bounded, as every wait is)
+        continue;
+      }
+      __nanosleep(20);  // (leaves the scheduler to the softmax)
+      if ((++idle & 1023u) == 0) {  // (bounded, as every wait is)
         const unsigned long long now = (unsigned long long)__shfl_sync(0xffffffffu, gtime_ns(), 0);
         if (idle == 1024) since = now;
         else if (now - since > kWaitNs) ok = false;
@@ -727,6 +746,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
       if (ok) tell(number);
     }
   } else if (warp > L::kWalk) {
+    // (completes a warpgroup)
     if constexpr (L::kMoreRegs > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kFewerRegs));
   } else {
     // ================= the walk along the line =================

@@ -11,8 +11,10 @@
 //     tiles, which take turns: the exponentials of one run under the products of the other.  A row's own positions are products
 //     whose other rows are empty; there the cache's stream is the bound, and the tiles of positions go to the two in turn.
 //   * A thread has a query's row of S: no exchange between threads for maxima and sums.
-//   * Keys and values are staged by cp.async, 16 bytes at a time through a list of 128 places, so that any page size and any strides will
-//     do; what lies outside is filled with zeros and masked, never read.  e4m3 pages are converted on the way to q's type, which is exact.
+//   * Keys and values are staged by TMA, boxes of 8 to 32 positions of a page; a warp zeroes what values of a tile lie behind its ends (stale
+//     rows may hold NaN).  Pages of no multiple of 8 positions come by cp.async, 16 bytes at a time through a list of places, which
+//     any page size and strides will do for; e4m3 pages are converted on the way to q's type, which is exact.  (By cp.async the ends of rows
+//     held up the exponentials, which take the same way out of a scheduler: a tile of four queries 7000 clocks for 3500.)
 //   * All items (a KV head of a group, or of a row) lie in a line that is cut into equal shares, a CTA to an SM
 //     (paged_shared_plan.h).  A warp walks the line and hands the pieces to the others; loads run ahead across pieces.  Pieces leave unnormalised
 //     fp32 outputs in a workspace, a second kernel joins them.  No counters: a workspace holds nothing between calls.
@@ -53,7 +55,7 @@ struct Shape {
   static constexpr int kSlots = D == 64 ? 8 : 4;             // keys and values in turn
   static constexpr int kQ = 128 * D * 2;
   static constexpr int kSmem = kStreams * kQ + kSlots * kSlot + 1024;
-  static constexpr int kSoftmaxWarps = 4 * kStreams, kLoad = kSoftmaxWarps, kWalk = kLoad + 4, kMma = kWalk + 3;
+  static constexpr int kSoftmaxWarps = 4 * kStreams, kLoad = kSoftmaxWarps, kWalk = kLoad + 4, kEnds = kWalk + 1, kMma = kWalk + 3;
   // (the issuer, which polls, is not on the scheduler of each stream's first warp, which has the queries of a single row)
   static constexpr int kThreads = (kMma + 1) * 32;
   // registers: whole warpgroups; those of two streams' softmax take some from the others.  (What spills is read back through an L1 of
@@ -283,6 +285,33 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+// Bounded by tries alone, each of which the hardware holds for a while: less code, of which all roles' has to stay in the instruction caches.
+__device__ __forceinline__ bool wait_some(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kSpinLimit; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+// Columns of a thread's row times `by`: fp32 values, or pairs of T.
+template <typename T>
+__device__ __forceinline__ void scale_columns(uint32_t cols, int n, float by, bool pairs) {
+#pragma unroll 1
+  for (int c = 0; c < n; c += 32) {
+    uint32_t v[32];
+    tmem_ld_32x32(cols + c, v);
+    tmem_ld_done(v);
+    if (pairs) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = times((const T*)nullptr, v[j], by);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * by);
+    }
+    tmem_st_32x32(cols + c, v);
+  }
+  tmem_st_wait();
+}
+
 template <int D, typename T, bool kE4M3>
 __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap k_map,
                                                                                const __grid_constant__ CUtensorMap v_map) {
@@ -292,7 +321,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
   // The base is kShift under the largest score of the first 64 positions that have any, and of later ones whose weights add up to over kLimit.
   constexpr float kShift = kBf16 ? 0.f : 7.f, kLimit = kBf16 ? 0x1p40f : 0x1p15f;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t b_full[kSlots], b_free[kSlots], b_q[2], b_s[2], b_p[2], b_o[2], b_piece[kRing], b_taken[kRing];
+  __shared__ uint64_t b_full[kSlots], b_free[kSlots], b_landed[kSlots], b_q[2], b_s[2], b_p[2], b_o[2], b_piece[kRing], b_taken[kRing];
   __shared__ Piece s_piece[kRing];
   __shared__ uint32_t s_place[kSlots / 2][kTile], s_tmem;
   __shared__ __align__(16) uint32_t s_there[kSlots][4];
@@ -303,9 +332,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
   unsigned char* const tiles = align_tiles(smem_raw);
   const uint32_t q_at = smem_u32(tiles), kv_at = q_at + kStreams * L::kQ;
   if (tid == 0) {
-    for (int i = 0; i < kSlots; ++i) mbar_init(b_full + i, 128), mbar_init(b_free + i, 1);
+    for (int i = 0; i < kSlots; ++i) mbar_init(b_full + i, 128), mbar_init(b_free + i, 1), mbar_init(b_landed + i, 128);
     for (int i = 0; i < 2; ++i) mbar_init(b_q + i, 128), mbar_init(b_s + i, 1), mbar_init(b_p + i, 4), mbar_init(b_o + i, 1);
-    for (int i = 0; i < kRing; ++i) mbar_init(b_piece + i, 1), mbar_init(b_taken + i, L::kSoftmaxWarps + 5);
+    for (int i = 0; i < kRing; ++i) mbar_init(b_piece + i, 1), mbar_init(b_taken + i, L::kSoftmaxWarps + 6);
     mbar_fence_init();
     s_first[0] = -1;
     if (p.box > 0) tma_prefetch_desc(&k_map), tma_prefetch_desc(&v_map);
@@ -345,7 +374,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
   const int units = s_first[2], share = units > 0 ? unit_share(units, p.ctas) : 1;
   bool ok = s_first[0] >= 0;
   // (by whole warps, which see one outcome)
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity)); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return ok = __all_sync(0xffffffffu, ok && wait_some(bar, parity));
+  };
   int piece_no = 0;
   auto take = [&](Piece& x) {  // the next piece; false at the end
     if (!wait(b_piece + piece_no % kRing, (piece_no / kRing) & 1)) return false;
@@ -422,10 +453,37 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
       return false;
     };
     uint32_t s_parity = 0, o_parity = 0;
-    Work x;
-    bool more = begin(x);
-    while (more) {
-      float base = -INFINITY, sum = 0.f;    // base: minus infinity before there is a score
+    Work x = {};
+    float base = -INFINITY, sum = 0.f;  // base: minus infinity before there is a score
+    bool first = true;
+    while (true) {
+      Work y;
+      const bool more = ok && begin(y);  // (the next queries before this piece's output: their scores come meanwhile)
+      if (!first) {
+        if (!wait(b_o + t, o_parity)) break;
+        o_parity ^= 1;
+        tc_fence_after_sync();
+        if (!x.idle) {
+          float4* const to = reinterpret_cast<float4*>((x.whole ? p.out : p.more) + x.to * D);
+          if (x.there) (x.whole ? p.ml : p.more_ml)[x.to] = make_float2(base, sum);
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(o_cols + c, o);
+            tmem_ld_done(o);
+            if (x.there) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                to[c / 4 + j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+            }
+          }
+          tc_fence_before_sync();
+        }
+      }
+      if (!more) break;
+      x = y;
+      first = false;
+      base = -INFINITY, sum = 0.f;
       for (int i = 0; i < x.n; ++i) {
         const int tile = x.pair || kStreams == 1 ? i : 2 * i + x.first_tile, pos = x.begin + tile * kTile;
         const bool inside = __all_sync(0xffffffffu, !x.there || (pos >= x.lo && pos + kTile <= x.hi));  // every query sees all of the tile
@@ -455,7 +513,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
 #pragma unroll 1
             for (int again = 0; again < 2; ++again) {
               if (__any_sync(0xffffffffu, low)) {
-                const float top = fmaxf(largest(from_cols, mask0), largest(from_cols + 32, mask1));
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int w = 0; w < 2; ++w) top = fmaxf(top, largest(from_cols + 32 * w, w == 0 ? mask0 : mask1));
                 float by = 1.f;
                 if (low && top > -INFINITY) {
                   const float next = __fsub_rn(__fmul_rn(top, x.factor), kShift);
@@ -463,22 +523,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
                   base = next;
                 }
                 sum *= by;
-                if (h > 0 && __any_sync(0xffffffffu, by != 1.f)) {  // the weights in front of these
-                  tmem_ld_32x32(s_cols, packed);
-                  tmem_ld_done(packed);
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) packed[j] = times((const T*)nullptr, packed[j], by);
-                  tmem_st_32x32(s_cols, packed);
-                }
-                if (i > 0 && __any_sync(0xffffffffu, by != 1.f)) {
-#pragma unroll 1
-                  for (int c = 0; c < D; c += 32) {
-                    tmem_ld_32x32(o_cols + c, packed);
-                    tmem_ld_done(packed);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) packed[j] = __float_as_uint(__uint_as_float(packed[j]) * by);
-                    tmem_st_32x32(o_cols + c, packed);
-                  }
+                if (__any_sync(0xffffffffu, by != 1.f)) {
+                  if (h > 0) scale_columns<T>(s_cols, 32, by, true);  // the weights in front of these
+                  if (i > 0) scale_columns<T>(o_cols, D, by, false);
                 }
               }
               const float from = base == -INFINITY ? 0.f : base;
@@ -496,28 +543,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         __syncwarp();
         if (lane == 0) mbar_arrive(b_p + t);
       }
-      Work y;
-      more = ok && begin(y);  // (its queries before this one's output: its scores come meanwhile)
-      if (!wait(b_o + t, o_parity)) break;
-      o_parity ^= 1;
-      tc_fence_after_sync();
-      if (!x.idle) {
-        float4* const to = reinterpret_cast<float4*>((x.whole ? p.out : p.more) + x.to * D);
-        if (x.there) (x.whole ? p.ml : p.more_ml)[x.to] = make_float2(base, sum);
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld_32x32(o_cols + c, o);
-          tmem_ld_done(o);
-          if (x.there) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              to[c / 4 + j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
-          }
-        }
-        tc_fence_before_sync();
-      }
-      x = y;
     }
   } else if (warp == L::kMma) {
     // ================= products, a step (a tile of positions of a stream) after another =================
@@ -575,26 +600,27 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     };
     while (ok && (more || i < end || step[0].on || step[1].on)) {
       bool moved = false;
+#pragma unroll 1
+      for (int t = 0; t < kStreams; ++t) {  // O += P V, and the scores that most often waited for that
+        const Step x = t == 0 ? step[0] : step[1];
+        if (x.on && ready(b_p + t, (p_no >> t) & 1) && full(x.value)) {
+          tc_fence_after_sync();
+          const int slot = x.value % kSlots;
+          const bool frees = x.alone || (t == 0 ? done[1] : done[0]) >= x.value;  // (the second of two)
+          const uint32_t d = cols + L::kColsO + t * D, a = cols + t * kTile, v = v_lo + slot * (L::kSlot >> 4);
+          if (elect_one()) {
 #pragma unroll
-      for (int t = 0; t < kStreams; ++t) {  // O += P V
-        Step& x = step[t];
-        if (!x.on || !ready(b_p + t, (p_no >> t) & 1) || !full(x.value)) continue;
-        tc_fence_after_sync();
-        const int slot = x.value % kSlots;
-        const bool frees = x.alone || done[t ^ 1] >= x.value;  // (the second of two)
-        done[t] = x.value;
-        const uint32_t d = cols + L::kColsO + t * D, a = cols + t * kTile, v = v_lo + slot * (L::kSlot >> 4);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k) umma_ts(d, a + k * 8, make_desc(v_hi, v + (k * 16 * 128 >> 4)), kIdO, !x.first || k > 0);
-          if (frees) umma_commit(b_free + slot);
-          if (x.last) umma_commit(b_o + t);
+            for (int k = 0; k < kTile / 16; ++k) umma_ts(d, a + k * 8, make_desc(v_hi, v + (k * 16 * 128 >> 4)), kIdO, !x.first || k > 0);
+            if (frees) umma_commit(b_free + slot);
+            if (x.last) umma_commit(b_o + t);
+          }
+          __syncwarp();
+          p_no ^= 1u << t;
+          if (t == 0) step[0].on = false, done[0] = x.value;
+          else step[1].on = false, done[1] = x.value;
+          moved = true;
         }
-        __syncwarp();
-        p_no ^= 1u << t;
-        x.on = false;
-        moved = true;
-        scores();  // (most often this stream's, which waited for that)
+        moved |= scores();
       }
       if (i == end && more && ready(b_piece + piece_no % kRing, (piece_no / kRing) & 1)) {
         tile0 += tiles_here;
@@ -605,7 +631,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         end = pair ? 2 * tiles_here : tiles_here;
         moved = true;
       }
-      moved |= scores();
       if (moved) {
         idle = 0;
         continue;
@@ -657,31 +682,27 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         const int now = id, at0 = pos - me;
         pos += kTile;
         id = me < kTile && pos < x.end && tile + 1 < x.tiles ? table[div_page(p.div, pos)] : -1;
-        if (!kE4M3 && p.box > 0 && at0 >= x.low && at0 + kTile <= x.end) {
-          // a whole tile of whole boxes: each warp asks for its 32 positions (a page that is none is out of the tensor, which gives zeros)
-          if (told < number) {
-            cp_async_wait<0>();
-            tell(number);
-          }
+        if (!kE4M3 && p.box > 0) {
+          // boxes of positions that are seen: each warp asks for those of its 32 (a page that is none is out of the tensor, which gives zeros)
+          const int from = max(x.low - at0, 0), to = min(x.end - at0, kTile), w0 = me & -32;
+          const int box0 = max(from - w0, 0) & -p.box, box1 = min(to - w0, 32);
+          const bool part = from > 0 || to < kTile;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (!room()) continue;
-            uint64_t* const bar = b_full + number % kSlots;
-            unsigned char* const to = tiles + kStreams * L::kQ + (number % kSlots) * L::kSlot + (me & -32) * 128;
-            if (me < kTile) {
-              if (lane == 0) mbar_expect_tx(bar, 32 * D * 2);
-              else mbar_arrive(bar);
-              for (int b = 0; b < 32; b += p.box) {
-                const int page = __shfl_sync(0xffffffffu, now, b), y = __shfl_sync(0xffffffffu, at0 + me, b), in = y - div_page(p.div, y) * p.pool.page_size;
-                const int z = (unsigned)page < (unsigned)p.pool.pages ? page : p.pool.pages, head = __shfl_sync(0xffffffffu, x.head, 0);
-                if (elect_one()) {
+            // (of a tile that is not whole the values behind its ends are zeroed by another warp, which hands it on)
+            uint64_t* const bar = (part && h == 1 ? b_landed : b_full) + number % kSlots;
+            unsigned char* const at = tiles + kStreams * L::kQ + (number % kSlots) * L::kSlot + w0 * 128;
+            if (lane == 0 && box1 > box0) mbar_expect_tx(bar, ((box1 - box0 + p.box - 1) & -p.box) * D * 2);
+            else mbar_arrive(bar);
+            for (int b = box0; b < box1; b += p.box) {
+              const int page = __shfl_sync(0xffffffffu, now, b), y = __shfl_sync(0xffffffffu, at0 + me, b), in = y - div_page(p.div, y) * p.pool.page_size;
+              const int z = (unsigned)page < (unsigned)p.pool.pages ? page : p.pool.pages, head = __shfl_sync(0xffffffffu, x.head, 0);
+              if (elect_one()) {
 #pragma unroll
-                  for (int c = 0; c < D / 64; ++c) tma_load_4d(to + c * kTile * 128 + b * 128, h == 0 ? &k_map : &v_map, bar, c * 64, in, head, z);
-                }
-                __syncwarp();
+                for (int c = 0; c < D / 64; ++c) tma_load_4d(at + c * kTile * 128 + b * 128, h == 0 ? &k_map : &v_map, bar, c * 64, in, head, z);
               }
-            } else {
-              mbar_arrive(bar);
+              __syncwarp();
             }
             told = ++number;
           }
@@ -744,6 +765,31 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     if constexpr (!kE4M3) {
       cp_async_wait<0>();
       if (ok) tell(number);
+    }
+  } else if (warp == L::kEnds) {
+    // ================= values of tiles that are not whole: zeros behind their ends =================
+    if constexpr (L::kMoreRegs > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kFewerRegs));
+    uint32_t landed = 0;  // a bit for each slot's parity
+    int tile_no = 0;
+    Piece x;
+    while (take(x)) {
+      if (!kE4M3 && p.box > 0) {
+        for (int tile = 0; tile < x.tiles && ok; ++tile) {
+          const int at0 = x.begin + tile * kTile, from = max(x.low - at0, 0), to = min(x.end - at0, kTile);
+          if (from == 0 && to == kTile) continue;
+          const int slot = (2 * (tile_no + tile) + 1) % kSlots;
+          if (!wait(b_landed + slot, (landed >> slot) & 1)) break;
+          landed ^= 1u << slot;
+          unsigned char* const values = tiles + kStreams * L::kQ + slot * L::kSlot;
+          for (int i = lane; i < kTile * (D / 8); i += 32) {
+            const int r = i / (D / 8);
+            if (r < from || r >= to) *reinterpret_cast<uint4*>(values + chunk_at(kTile, r, i % (D / 8))) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async_shared();
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 4;" ::"r"(smem_u32(b_full + slot)) : "memory");
+        }
+      }
+      tile_no += x.tiles;
     }
   } else if (warp > L::kWalk) {
     // (completes a warpgroup)

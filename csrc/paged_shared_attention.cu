@@ -312,12 +312,14 @@ __device__ __forceinline__ void scale_columns(uint32_t cols, int n, float by, bo
   tmem_st_wait();
 }
 
-template <int D, typename T, bool kE4M3>
+// How keys and values come to shared memory.
+enum Stage { STAGE_TMA, STAGE_COPY, STAGE_E4M3 };
+template <int D, typename T, Stage kStage>
 __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap k_map,
                                                                                const __grid_constant__ CUtensorMap v_map) {
   using L = Shape<D>;
   constexpr int kTile = L::kTile, kSlots = L::kSlots, kStreams = L::kStreams;
-  constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
+  constexpr bool kBf16 = __is_same(T, __nv_bfloat16), kTma = kStage == STAGE_TMA, kE4M3 = kStage == STAGE_E4M3;
   // The base is kShift under the largest score of the first 64 positions that have any, and of later ones whose weights add up to over kLimit.
   constexpr float kShift = kBf16 ? 0.f : 7.f, kLimit = kBf16 ? 0x1p40f : 0x1p15f;
   extern __shared__ unsigned char smem_raw[];
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     for (int i = 0; i < kRing; ++i) mbar_init(b_piece + i, 1), mbar_init(b_taken + i, L::kSoftmaxWarps + 6);
     mbar_fence_init();
     s_first[0] = -1;
-    if (p.box > 0) tma_prefetch_desc(&k_map), tma_prefetch_desc(&v_map);
+    if (kTma) tma_prefetch_desc(&k_map), tma_prefetch_desc(&v_map);
   }
   if (warp == L::kMma) tmem_alloc(&s_tmem, L::kCols);
   pdl_wait();
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.a.q) + row * p.a.q_stride + head * p.a.q_head_stride);
         Seen seen = {0, 0};
         if (y.there) seen = seen_of(p.a.lengths[row], p.max_len, p.a.window);
-#pragma unroll
+#pragma unroll 1
         for (int c0 = 0; c0 < D / 8; c0 += 8) {
           uint4 v[8];
 #pragma unroll
@@ -657,7 +659,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
       if (number < kSlots) return ok;
       uint64_t* const bar = b_free + number % kSlots;
       const uint32_t parity = ((number / kSlots) & 1) ^ 1;
-      if (!kE4M3 && !mbar_try_wait(bar, parity)) {
+      if (kStage == STAGE_COPY && !mbar_try_wait(bar, parity)) {
         cp_async_wait<0>();  // (whoever frees it may be waiting for what is under way)
         tell(number);
       }
@@ -675,14 +677,14 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
       for (int tile = 0; tile < x.tiles; ++tile, ++tile_no) {
         if (me < kTile) {
           const uint32_t at = pos >= x.low ? step_of(id, p.pool.pages, pos, p.div, p.page_step, p.pos_step) : kNoStep;
-          s_place[tile_no % (kSlots / 2)][me] = at;
+          if constexpr (!kTma) s_place[tile_no % (kSlots / 2)][me] = at;
           const uint32_t there = __ballot_sync(0xffffffffu, at != kNoStep);
           if (lane == 0) s_there[tile_no % kSlots][me / 32] = there;
         }
         const int now = id, at0 = pos - me;
         pos += kTile;
         id = me < kTile && pos < x.end && tile + 1 < x.tiles ? table[div_page(p.div, pos)] : -1;
-        if (!kE4M3 && p.box > 0) {
+        if constexpr (kTma) {
           // boxes of positions that are seen: each warp asks for those of its 32 (a page that is none is out of the tensor, which gives zeros)
           const int from = max(x.low - at0, 0), to = min(x.end - at0, kTile), w0 = me & -32;
           const int box0 = max(from - w0, 0) & -p.box, box1 = min(to - w0, 32);
@@ -707,7 +709,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
             told = ++number;
           }
           continue;
-        }
+        } else {
         if (!named_bar_all(1, 128, ok)) {
           ok = false;
           break;
@@ -760,9 +762,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
             }
           }
         }
+        }
       }
     }
-    if constexpr (!kE4M3) {
+    if constexpr (kStage == STAGE_COPY) {
       cp_async_wait<0>();
       if (ok) tell(number);
     }
@@ -773,7 +776,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     int tile_no = 0;
     Piece x;
     while (take(x)) {
-      if (!kE4M3 && p.box > 0) {
+      if constexpr (kTma) {
         for (int tile = 0; tile < x.tiles && ok; ++tile) {
           const int at0 = x.begin + tile * kTile, from = max(x.low - at0, 0), to = min(x.end - at0, kTile);
           if (from == 0 && to == kTile) continue;
@@ -971,9 +974,6 @@ cudaError_t launch(Params p, char* workspace, int sms, cudaStream_t stream) {
   p.ml = reinterpret_cast<float2*>(workspace + w.ml);
   p.more = reinterpret_cast<float*>(workspace + w.more);
   p.more_ml = reinterpret_cast<float2*>(workspace + w.more_ml);
-  auto* kernel = k_shared_attention<D, T, kE4M3>;
-  cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(kernel), L::kSmem).rc;
-  if (rc != cudaSuccess) return rc;
   // TMA boxes of whole pages or parts of one, of 8 to 32 positions (so many divide a page); pools that no tensor map can have, and
   // 8-bit ones, which are converted on the way, go by cp.async
   CUtensorMap k_map = {}, v_map = {};
@@ -986,6 +986,10 @@ cudaError_t launch(Params p, char* workspace, int sms, cudaStream_t stream) {
            cudaSuccess;
   };
   if (kE4M3 || p.box < 8 || !map(&k_map, pool.k) || !map(&v_map, pool.v)) p.box = 0;
+  auto* kernel = k_shared_attention<D, T, kE4M3 ? STAGE_E4M3 : STAGE_COPY>;
+  if constexpr (!kE4M3) kernel = p.box > 0 ? k_shared_attention<D, T, STAGE_TMA> : kernel;
+  cudaError_t rc = kernel_setup(reinterpret_cast<const void*>(kernel), L::kSmem).rc;
+  if (rc != cudaSuccess) return rc;
   rc = launch_kernel_ex(kernel, dim3(p.ctas), dim3(L::kThreads), (size_t)L::kSmem, stream, true, 1, p, k_map, v_map);
   if (rc != cudaSuccess) return rc;
   return launch_kernel_ex(k_shared_join<D, T>, dim3(p.a.rows, p.pool.heads), dim3(kJoinWarps * 32), 0, stream, true, 1, p);

@@ -121,7 +121,7 @@ __device__ __forceinline__ int items_of(const Params& p, const Element& x) {
 }
 template <int D>
 __device__ __forceinline__ uint32_t units_of(const Params& p, const Element& x) {
-  return (uint32_t)min((long long)items_of<D>(p, x) * item_units(tiles_of(x.end - x.begin, Shape<D>::kTile)), 0x7fffffffll);
+  return (uint32_t)min((long long)items_of<D>(p, x) * item_units(tiles_of(x.end - x.begin, Shape<D>::kTile), pair_of(x.queries, Shape<D>::kQueries)), 0x7fffffffll);
 }
 
 // What a CTA has of an item, as the walking warp hands it on.
@@ -825,12 +825,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         x.queries = __shfl_sync(0xffffffffu, mine.queries, l);
         x.first = __shfl_sync(0xffffffffu, mine.first, l);
         x.row = __shfl_sync(0xffffffffu, mine.row, l);
-        const int tiles = tiles_of(x.end - x.begin, kTile), each = item_units(tiles), cuts = query_tiles(x.queries, L::kQueries);
+        const bool two = pair_of(x.queries, L::kQueries);
+        const int tiles = tiles_of(x.end - x.begin, kTile), each = item_units(tiles, two), cuts = query_tiles(x.queries, L::kQueries);
         const long long start = at - off;  // the element's first unit
         int item = off / each;
         off = 0;
         for (; item < p.pool.heads * cuts && start + (long long)item * each < end && ok; ++item) {
-          const Tiles part = piece_of((int)(start + (long long)item * each), tiles, share, cta);
+          const Tiles part = piece_of((int)(start + (long long)item * each), tiles, two, share, cta);
           if (part.to > part.from) {
             Piece y;
             y.tiles = part.to - part.from;
@@ -893,15 +894,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_shared_join(const __grid_co
       if ((unsigned)query >= (unsigned)x.queries) continue;
       const int cuts = query_tiles(x.queries, L::kQueries), cut = query / L::kQueries, within = query - cut * L::kQueries;
       const bool pair = min(L::kQueries, x.queries - cut * L::kQueries) > 128;
-      const int begin = line[kind] + (kh * cuts + cut) * item_units(tiles);
-      const int first = cta_of(begin, 0, share), pieces = cta_of(begin, tiles - 1, share) - first + 1;
+      const bool two = pair_of(x.queries, L::kQueries);
+      const int begin = line[kind] + (kh * cuts + cut) * item_units(tiles, two);
+      const int first = cta_of(begin, 0, two, share), pieces = cta_of(begin, tiles - 1, two, share) - first + 1;
       // parts: two halves of a piece where its tiles went to both streams
       for (int i0 = 0; i0 < 2 * pieces; i0 += 32) {
         const int i = i0 + lane, piece = i >> 1, half = i & 1;
         bool some = piece < pieces;
         long long at = 0;
         if (some) {
-          const Tiles t = piece_of(begin, tiles, share, first + piece);
+          const Tiles t = piece_of(begin, tiles, two, share, first + piece);
           some = half == 0 || (!pair && L::kStreams == 2 && t.to - t.from > 1);
           const int stream = pair ? within >> 7 : half, lane_of = pair ? within & 127 : within;
           at = piece == 0 ? ((2 * kind + half) * (long long)p.a.rows + row) * p.a.heads + head : ((first + piece) * 2ll + stream) * 128 + lane_of;

@@ -417,13 +417,13 @@ int penny_paged_walk(const int* lengths, int rows, int max_len, int window, int 
   return n;
 }
 // Attention over shared pages (paged_shared_plan.h).
-int penny_shared_item_units(int tiles) { return penny::paged::item_units(tiles); }
+int penny_shared_item_units(int tiles, int pair) { return penny::paged::item_units(tiles, pair != 0); }
 int penny_shared_share(int units, int ctas) { return penny::paged::unit_share(units, ctas); }
-void penny_shared_piece(int begin, int tiles, int share, int cta, int* from_to) {
-  const penny::paged::Tiles t = penny::paged::piece_of(begin, tiles, share, cta);
+void penny_shared_piece(int begin, int tiles, int pair, int share, int cta, int* from_to) {
+  const penny::paged::Tiles t = penny::paged::piece_of(begin, tiles, pair != 0, share, cta);
   from_to[0] = t.from, from_to[1] = t.to;
 }
-int penny_shared_cta_of(int begin, int tile, int share) { return penny::paged::cta_of(begin, tile, share); }
+int penny_shared_cta_of(int begin, int tile, int pair, int share) { return penny::paged::cta_of(begin, tile, pair != 0, share); }
 long long penny_shared_most_units(long long rows, int kv_heads, int group, long long positions, int tile, int most) {
   return penny::paged::most_units(rows, kv_heads, group, positions, tile, most);
 }

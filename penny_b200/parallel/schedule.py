@@ -210,9 +210,9 @@ def paged_walk(lengths, max_len: int, warps: int, warp: int, window: int = 0, ti
     return [(r, a, b, bool(f & 1), bool(f & 2), bool(f & 4), z) for r, a, b, f, z in rows], tiles[:num.value], share.value
 
 
-def shared_units(tiles: int) -> int:
+def shared_units(tiles: int, pair: bool) -> int:
     """Units of an item of the attention over shared pages (csrc/paged_shared_plan.h)."""
-    return sim_lib().penny_shared_item_units(tiles)
+    return sim_lib().penny_shared_item_units(tiles, pair)
 
 
 def shared_share(units: int, ctas: int) -> int:
@@ -220,16 +220,16 @@ def shared_share(units: int, ctas: int) -> int:
     return sim_lib().penny_shared_share(units, ctas)
 
 
-def shared_piece(begin: int, tiles: int, share: int, cta: int):
+def shared_piece(begin: int, tiles: int, pair: bool, share: int, cta: int):
     """The tiles [from, to) that a CTA has of an item whose first unit is `begin` (csrc/paged_shared_plan.h)."""
     at = (ctypes.c_int * 2)()
-    sim_lib().penny_shared_piece(begin, tiles, share, cta, at)
+    sim_lib().penny_shared_piece(begin, tiles, pair, share, cta, at)
     return at[0], at[1]
 
 
-def shared_cta_of(begin: int, tile: int, share: int) -> int:
+def shared_cta_of(begin: int, tile: int, pair: bool, share: int) -> int:
     """The CTA that has a tile of such an item (csrc/paged_shared_plan.h)."""
-    return sim_lib().penny_shared_cta_of(begin, tile, share)
+    return sim_lib().penny_shared_cta_of(begin, tile, pair, share)
 
 
 def shared_most_units(rows: int, kv_heads: int, group: int, positions: int, tile: int, most: int) -> int:

@@ -402,7 +402,7 @@ cudaError_t launch_page_fork(const PageFork& a, cudaStream_t stream) {
   if (a.rows < 1 || a.rows > kPagedMaxRows || a.forks < 0 || a.forks > kPagedMaxRows || a.width < 1 || a.page_size < 1 || a.pages < 1)
     return cudaErrorInvalidValue;
   if (a.forks == 0) return cudaSuccess;
-  return launch_cluster(k_page_fork, (size_t)kPagedMaxRows * 16, (size_t)(a.rows + 3 * a.forks) * 4, (long long)a.forks * a.width > 16384, stream, a,
+  return launch_cluster(k_page_fork, (size_t)kPagedMaxRows * 16, (size_t)(a.rows + 3 * a.forks) * 4, (long long)a.forks * a.width > 2048, stream, a,
                         page_div(a.page_size));
 }
 

@@ -50,7 +50,7 @@ __device__ __forceinline__ void put(int* to, int r0, int rows, const int (&v)[kP
 // many are on it now.  s_old, s_gone: per row its length and the number of its first reference among all `total` that leave.  Called by
 // all threads of the cluster.
 __device__ __noinline__ int leave_shared(const PageTables& a, const PageDiv& div, int cluster, int count, const int* s_old, const int* s_gone, int total) {
-  __shared__ int s_warp[32], s_run;
+  __shared__ int s_warp[32], s_counts[16];
   const int tid = threadIdx.x, rank = blockIdx.x, threads = cluster * blockDim.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   auto page_of = [&](int k) {  // -1: none of the pool's
     const int r = row_at(s_gone, a.rows, k), left = pages_of(div, (int)max(0ll, (long long)s_old[r] + a.news[r]));
@@ -71,31 +71,44 @@ __device__ __noinline__ int leave_shared(const PageTables& a, const PageDiv& div
     if (page >= 0 && __ldcg(a.refs + page) <= 0) atomicMin(a.refs + page, -1 - k);
   }
   barrier();
-  if (rank == 0) {  // numbers in descending order onto the stack
-    if (tid == 0) s_run = count;
-    __syncthreads();
-    for (int top = total; top > 0; top -= (int)blockDim.x) {
-      const int k = top - 1 - tid, page = k >= 0 ? page_of(k) : -1;
-      const bool mine = page >= 0 && __ldcg(a.refs + page) == -1 - k;
-      const uint32_t who = __ballot_sync(0xffffffffu, mine);
-      if (lane == 0) s_warp[warp] = __popc(who);
-      __syncthreads();
-      int before = s_run, all = 0;
-      for (int w = 0; w < warps; ++w) {
-        before += w < warp ? s_warp[w] : 0;
-        all += s_warp[w];
-      }
-      const int at = before + __popc(who & ((1u << lane) - 1));
-      if (mine) {
-        if (at < a.pages) a.free_pages[at] = page;
-        a.refs[page] = 0;
-      }
-      __syncthreads();
-      if (tid == 0) s_run = min(a.pages, s_run + all);
-      __syncthreads();
-    }
-    if (tid == 0) *a.free_count = s_run;
+  // numbers in descending order onto the stack: each CTA has a piece of them, counts those that stand for a page and learns of the others'
+  const int chunk = (total - 1) / cluster + 1, end = max(0, total - rank * chunk), begin = max(0, end - chunk);
+  auto stands = [&](int k) {
+    const int page = k >= begin ? page_of(k) : -1;
+    return page >= 0 && __ldcg(a.refs + page) == -1 - k ? page : -1;
+  };
+  int mine = 0;
+  for (int k = end - 1 - tid; k >= begin; k -= (int)blockDim.x) mine += stands(k) >= 0;
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if (lane == 0) s_warp[warp] = mine;
+  __syncthreads();
+  mine = __reduce_add_sync(0xffffffffu, lane < warps ? s_warp[lane] : 0);
+  if (tid < cluster) {
+    uint32_t to;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(s_counts + rank)), "r"(tid));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(mine) : "memory");
   }
+  barrier();
+  int run = count, all = 0;
+  for (int c = 0; c < cluster; ++c) {
+    run += c < rank ? s_counts[c] : 0;
+    all += s_counts[c];
+  }
+  for (int top = end; top > begin; top -= (int)blockDim.x) {
+    const int k = top - 1 - tid, page = stands(k);
+    const uint32_t who = __ballot_sync(0xffffffffu, page >= 0);
+    if (lane == 0) s_warp[warp] = __popc(who);
+    __syncthreads();
+    const int here = lane < warps ? s_warp[lane] : 0;
+    const int at = run + __reduce_add_sync(0xffffffffu, lane < warp ? here : 0) + __popc(who & ((1u << lane) - 1));
+    if (page >= 0) {
+      if (at < a.pages) a.free_pages[at] = page;
+      a.refs[page] = 0;
+    }
+    run += __reduce_add_sync(0xffffffffu, here);
+    __syncthreads();
+  }
+  if (rank == 0 && tid == 0) *a.free_count = min(a.pages, count + all);
   barrier();
   return __ldcg(a.free_count);
 }
@@ -281,7 +294,10 @@ cudaError_t launch_page_tables(const PageTables& a, cudaStream_t stream) {
   const size_t smem = (size_t)(a.rows + 3) / 4 * 16 * sizeof(int);
   // One CTA for a decode step; a cluster for many rows or tokens.  There and back, on the device: 64 rows of one token 5.6 us; 1000 rows
   // with 3060 tokens 9.1, in one CTA 10.2; 4000 rows with 42,209 tokens in 5342 pages 16.1, of eight CTAs instead of sixteen 3 more.
-  const int threads = a.rows <= 256 && a.tokens <= 1024 ? 256 : 1024, big = a.tokens > 2048 || a.rows > 1024;
+  // (Counted pages may leave by the table's size in a call: 64 rows of 62 pages each, forked and gone again, 50 us in one CTA of 256 threads,
+  // so 17.)
+  const bool leaves = a.refs != nullptr && (long long)a.rows * a.width > 2048;
+  const int threads = a.rows <= 256 && a.tokens <= 1024 && !leaves ? 256 : 1024, big = a.tokens > 2048 || a.rows > 1024 || leaves;
   const int per = (a.rows + threads - 1) / threads;
 #define PENNY_PAGE_TABLES(N, R)                                                                                                        \
   do {                                                                                                                                \

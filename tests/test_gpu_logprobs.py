@@ -101,6 +101,30 @@ def test_masked_and_far_logits():
             assert P.token_logprobs(y[:1], torch.tensor([bad], device="cuda")).logprobs.isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_masks_of_the_lowest_value(dtype):
+    """Tokens that are masked by the type's lowest number and not by minus infinity; rows of nothing else, and of its opposite."""
+    for vocab in (5000, 128256):
+        x = (torch.randn(6, vocab, device="cuda") * 3).to(dtype)
+        lowest, highest = torch.finfo(dtype).min, torch.finfo(dtype).max
+        x[0, torch.rand(vocab, device="cuda") < 0.9] = lowest
+        x[1, 1:] = lowest
+        x[2] = lowest
+        x[3, 7] = highest
+        x[4] = highest
+        x[5, ::2] = lowest
+        x[5, 1::4] = highest
+        got = P.token_logprobs(x, torch.tensor([0, 0, 9, 7, 8, 1], device="cuda"), 5)
+        want = _want(x, torch.tensor([0, 0, 9, 7, 8, 1], device="cuda"), 5)
+        assert torch.equal(got.top_ids, want[3])
+        flat = math.log(vocab)
+        assert abs(got.entropy[2] - flat) < 1e-4 and abs(got.entropy[4] - flat) < 1e-4 and abs(got.logprobs[2] + flat) < 1e-4 and abs(got.logprobs[4] + flat) < 1e-4
+        assert got.logprobs[1] == 0 and got.logprobs[3] == 0 and got.entropy[1] == 0 and got.entropy[3] == 0
+        for a, b in zip(got[:3], want[:3]):
+            far = b.abs() > 1e4  # (numbers of the type's size: as fp32 has them)
+            assert ((a.double() - b).abs()[~far] < 1e-4).all() and (((a.double() - b) / b).abs()[far] < 2.0 ** -20).all() and not a.isnan().any()
+
+
 def test_no_rows_graph_and_stream():
     assert [t.shape for t in P.token_logprobs(torch.zeros(0, 50, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda"), 3)] == [(0,), (0,), (0, 3), (0, 3)]
     x, tokens = torch.randn(5, 128256, device="cuda"), torch.arange(5, device="cuda")

@@ -60,7 +60,7 @@ struct Shape {
   static constexpr int kThreads = (kMma + 1) * 32;
   // registers: whole warpgroups; those of two streams' softmax take some from the others.  (What spills is read back through an L1 of
   // 20 KB that all loads go through: a tile of one row took 4000 to 9000 clocks in place of 2500.)
-  static constexpr int kMoreRegs = kStreams == 2 ? 160 : 0, kFewerRegs = 96;
+  static constexpr int kMoreRegs = kStreams == 2 ? 144 : 0, kFewerRegs = 112;
   static_assert(kThreads % 128 == 0 && (kStreams == 1 || (kThreads == 512 && kMoreRegs * 256 + kFewerRegs * 256 <= 65536)), "warpgroups");
   // tensor memory: S (and P) of each stream, then O
   static constexpr int kColsO = kStreams * kTile, kCols = kColsO + kStreams * D <= 256 ? 256 : 512;
@@ -667,6 +667,70 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     };
     int tile_no = 0;
     Piece x;
+    if constexpr (kE4M3) {
+      // A tile's keys and values lie in registers while they are on their way: those of the next one are asked for where this one's have
+      // been converted and stored.
+      int tile = -1, pos = 0, id = -1;
+      x.tiles = 0;
+      const char *k_src = nullptr, *v_src = nullptr;
+      const uint32_t* places = nullptr;
+      auto advance = [&]() {  // the next tile's places; false at the end (a warp whose wait ran out leaves at a barrier, with the others)
+        if (++tile >= x.tiles) {
+          if (!named_bar_all(1, 128, take(x))) return false;
+          tile = 0;
+          k_src = reinterpret_cast<const char*>(p.pool.k) + x.head * p.pool.head_stride + c * 16;
+          v_src = reinterpret_cast<const char*>(p.pool.v) + x.head * p.pool.head_stride + c * 16;
+          pos = x.begin + me;
+          id = me < kTile && pos < x.end ? p.a.table[x.row * p.a.table_stride + div_page(p.div, pos)] : -1;
+        }
+        if (me < kTile) {
+          const uint32_t at = step_of(id, p.pool.pages, pos, p.div, p.page_step, p.pos_step);
+          s_place[tile_no % (kSlots / 2)][me] = at;
+          const uint32_t there = __ballot_sync(0xffffffffu, at != kNoStep);
+          if (lane == 0) s_there[tile_no % kSlots][me / 32] = there;
+        }
+        pos += kTile;
+        id = me < kTile && pos < x.end && tile + 1 < x.tiles ? p.a.table[x.row * p.a.table_stride + div_page(p.div, pos)] : -1;
+        if (!named_bar_all(1, 128, ok)) return false;
+        places = s_place[tile_no % (kSlots / 2)];
+        ++tile_no;
+        return true;
+      };
+      uint4 v[2][kPer];
+      auto load = [&](uint4 (&to)[kPer], const char* src) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const uint32_t at = places[r0 + i * (128 / kChunks)];
+          to[i] = at != kNoStep ? *reinterpret_cast<const uint4*>(src + (unsigned long long)at * p.step_bytes) : make_uint4(0, 0, 0, 0);
+        }
+      };
+      auto store = [&](const uint4 (&from)[kPer]) {
+        if (!room()) return;
+        unsigned char* const to = tiles + kStreams * L::kQ + (number % kSlots) * L::kSlot;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const uint32_t w[4] = {from[i].x, from[i].y, from[i].z, from[i].w};
+          uint32_t y[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[2 * j] = widen((const T*)nullptr, w[j]), y[2 * j + 1] = widen((const T*)nullptr, w[j] >> 16);
+          const int r = r0 + i * (128 / kChunks);
+          *reinterpret_cast<uint4*>(to + chunk_at(kTile, r, 2 * c)) = make_uint4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<uint4*>(to + chunk_at(kTile, r, 2 * c + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+        }
+        ++number;
+        tell(number);
+      };
+      bool some = advance();
+      if (some) load(v[0], k_src), load(v[1], v_src);
+      while (some) {
+        const bool more = advance();
+        store(v[0]);
+        if (more) load(v[0], k_src);
+        store(v[1]);
+        if (more) load(v[1], v_src);
+        some = more;
+      }
+    } else {
     // (a warp whose wait ran out leaves at a barrier, with the others)
     while (named_bar_all(1, 128, take(x))) {
       const int* const table = p.a.table + x.row * p.a.table_stride;
@@ -715,34 +779,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
           break;
         }
         const uint32_t* const places = s_place[tile_no % (kSlots / 2)];
-        if constexpr (kE4M3) {
-          uint4 v[2][kPer];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              const uint32_t at = places[r0 + i * (128 / kChunks)];
-              v[h][i] = at != kNoStep ? *reinterpret_cast<const uint4*>(src[h] + (unsigned long long)at * p.step_bytes) : make_uint4(0, 0, 0, 0);
-            }
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!room()) break;
-            unsigned char* const to = tiles + kStreams * L::kQ + (number % kSlots) * L::kSlot;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              const uint32_t w[4] = {v[h][i].x, v[h][i].y, v[h][i].z, v[h][i].w};
-              uint32_t y[8];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) y[2 * j] = widen((const T*)nullptr, w[j]), y[2 * j + 1] = widen((const T*)nullptr, w[j] >> 16);
-              const int r = r0 + i * (128 / kChunks);
-              *reinterpret_cast<uint4*>(to + chunk_at(kTile, r, 2 * c)) = make_uint4(y[0], y[1], y[2], y[3]);
-              *reinterpret_cast<uint4*>(to + chunk_at(kTile, r, 2 * c + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
-            }
-            ++number;
-            tell(number);
-          }
-        } else {
+        {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (!room()) break;
@@ -764,6 +801,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         }
         }
       }
+    }
     }
     if constexpr (kStage == STAGE_COPY) {
       cp_async_wait<0>();

@@ -13,8 +13,8 @@
 //   * A thread has a query's row of S: no exchange between threads for maxima and sums.
 //   * Keys and values are staged by TMA, boxes of 8 to 32 positions of a page; a warp zeroes what values of a tile lie behind its ends (stale
 //     rows may hold NaN).  Pages of no multiple of 8 positions come by cp.async, 16 bytes at a time through a list of places, which
-//     any page size and strides will do for; e4m3 pages are converted on the way to q's type, which is exact.  (By cp.async the ends of rows
-//     held up the exponentials, which take the same way out of a scheduler: a tile of four queries 7000 clocks for 3500.)
+//     any page size and strides will do for.  e4m3 pages are converted on the way to fp16, which is exact, and bf16 queries meet them as fp16 times
+//     a power of two (four conversions for a pair of values in place of one were the bound: 91 us for 130 rows of nine prompts).
 //   * All items (a KV head of a group, or of a row) lie in a line that is cut into equal shares, a CTA to an SM
 //     (paged_shared_plan.h).  A warp walks the line and hands the pieces to the others; loads run ahead across pieces.  Pieces leave unnormalised
 //     fp32 outputs in a workspace, a second kernel joins them.  No counters: a workspace holds nothing between calls.
@@ -28,6 +28,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_sm100.cuh"
 #include "gemm_sm100.h"
@@ -179,16 +180,11 @@ __device__ __forceinline__ uint32_t pack2(const __half*, float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// two e4m3 values as two of T
-__device__ __forceinline__ uint32_t widen(const __half*, uint32_t x) {
+// two e4m3 values as fp16
+__device__ __forceinline__ uint32_t widen(uint32_t x) {
   uint32_t r;
   asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l;}" : "=r"(r) : "r"(x));
   return r;
-}
-__device__ __forceinline__ uint32_t widen(const __nv_bfloat16*, uint32_t x) {
-  const uint32_t h = widen((const __half*)nullptr, x);
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  return pack2((const __nv_bfloat16*)nullptr, f.x, f.y);
 }
 // where 16-byte chunk c of row r lies in an operand of `rows` rows: blocks of 64 columns, 128 bytes a row, swizzled
 __device__ __forceinline__ uint32_t chunk_at(int rows, int r, int c) {
@@ -314,11 +310,12 @@ __device__ __forceinline__ void scale_columns(uint32_t cols, int n, float by, bo
 
 // How keys and values come to shared memory.
 enum Stage { STAGE_TMA, STAGE_COPY, STAGE_E4M3 };
-template <int D, typename T, Stage kStage>
+template <int D, typename TQ, Stage kStage>
 __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap k_map,
                                                                                const __grid_constant__ CUtensorMap v_map) {
   using L = Shape<D>;
   constexpr int kTile = L::kTile, kSlots = L::kSlots, kStreams = L::kStreams;
+  using T = std::conditional_t<kStage == STAGE_E4M3, __half, TQ>;  // of the products
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16), kTma = kStage == STAGE_TMA, kE4M3 = kStage == STAGE_E4M3;
   // The base is kShift under the largest score of the first 64 positions that have any, and of later ones whose weights add up to over kLimit.
   constexpr float kShift = kBf16 ? 0.f : 7.f, kLimit = kBf16 ? 0x1p40f : 0x1p15f;
@@ -426,9 +423,25 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         if (kE4M3) y.factor *= p.pool.k_scale[x.head];
         const uint32_t flip = y.factor < 0 ? 0x80008000u : 0;  // (the maximum is that of the scores before the factor)
         y.factor = fabsf(y.factor);
-        const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.a.q) + row * p.a.q_stride + head * p.a.q_head_stride);
+        const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const TQ*>(p.a.q) + row * p.a.q_stride + head * p.a.q_head_stride);
         Seen seen = {0, 0};
         if (y.there) seen = seen_of(p.a.lengths[row], p.max_len, p.a.window);
+        float up = 1.f;
+        if constexpr (!__is_same(T, TQ)) {
+          // bf16 queries as fp16, times the power of two that brings a row's largest value to [2^15, 2^16) (values under 2^-29 of that keep
+          // 2^-40 of it); the factor takes it back
+          float top = 0.f;
+          if (y.there) {
+#pragma unroll 4
+            for (int c = 0; c < D / 8; ++c) {
+              const uint4 v = q[c];
+              for (uint32_t w : {v.x, v.y, v.z, v.w}) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
+            }
+          }
+          const int e = max((__float_as_int(top) >> 23) & 255, 16);
+          up = __int_as_float((269 - e) << 23);
+          y.factor *= __int_as_float((e - 15) << 23);
+        }
 #pragma unroll 1
         for (int c0 = 0; c0 < D / 8; c0 += 8) {
           uint4 v[8];
@@ -436,8 +449,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
           for (int c = 0; c < 8; ++c) v[c] = y.there ? q[c0 + c] : make_uint4(0, 0, 0, 0);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            v[c].x ^= flip, v[c].y ^= flip, v[c].z ^= flip, v[c].w ^= flip;
-            *reinterpret_cast<uint4*>(q_tile + chunk_at(128, me, c0 + c)) = v[c];
+            uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if constexpr (!__is_same(T, TQ)) w[j] = pack2((const T*)nullptr, __uint_as_float(w[j] << 16) * up, __uint_as_float(w[j] & 0xffff0000u) * up);
+              w[j] ^= flip;
+            }
+            *reinterpret_cast<uint4*>(q_tile + chunk_at(128, me, c0 + c)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
         fence_async_shared();
@@ -712,7 +730,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
           const uint32_t w[4] = {from[i].x, from[i].y, from[i].z, from[i].w};
           uint32_t y[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[2 * j] = widen((const T*)nullptr, w[j]), y[2 * j + 1] = widen((const T*)nullptr, w[j] >> 16);
+          for (int j = 0; j < 4; ++j) y[2 * j] = widen(w[j]), y[2 * j + 1] = widen(w[j] >> 16);
           const int r = r0 + i * (128 / kChunks);
           *reinterpret_cast<uint4*>(to + chunk_at(kTile, r, 2 * c)) = make_uint4(y[0], y[1], y[2], y[3]);
           *reinterpret_cast<uint4*>(to + chunk_at(kTile, r, 2 * c + 1)) = make_uint4(y[4], y[5], y[6], y[7]);

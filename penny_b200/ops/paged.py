@@ -150,7 +150,7 @@ def paged_attention(q, k, v, table, lengths, out=None, lse=None, scale: Optional
 
     groups: `page_groups` of this table and these lengths, or of a time since when the rows of its groups have kept the pages that they
     share: what a group shares is read once for all its rows, on tensor cores, instead of once for each.  The result is the same but for
-    the order of sums (and weights of an e4m3 cache have q's type).  At most 8192 rows; the workspace is that of groups=True.  A wait of the kernel that ran
+    the order of sums.  At most 8192 rows; the workspace is that of groups=True.  A wait of the kernel that ran
     out (4 s) leaves its rows undone and shows in `gemm_error`."""
     return ops.paged_attention(q, k, v, table, lengths, out, lse, scale, window, k_scale, v_scale, workspace, early, groups)
 

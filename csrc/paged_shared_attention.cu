@@ -186,6 +186,17 @@ __device__ __forceinline__ uint32_t widen(uint32_t x) {
   asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l;}" : "=r"(r) : "r"(x));
   return r;
 }
+// 16 bytes, or zeros without a look at them
+__device__ __forceinline__ uint4 load_or_zero(const void* from, bool there) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(from), "r"((int)there)
+      : "memory");
+  return v;
+}
 // where 16-byte chunk c of row r lies in an operand of `rows` rows: blocks of 64 columns, 128 bytes a row, swizzled
 __device__ __forceinline__ uint32_t chunk_at(int rows, int r, int c) {
   return (uint32_t)((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
@@ -322,7 +333,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t b_full[kSlots], b_free[kSlots], b_landed[kSlots], b_q[2], b_s[2], b_p[2], b_o[2], b_piece[kRing], b_taken[kRing];
   __shared__ Piece s_piece[kRing];
-  __shared__ uint32_t s_place[kSlots / 2][kTile], s_tmem;
+  __shared__ uint32_t s_tmem;
   __shared__ __align__(16) uint32_t s_there[kSlots][4];
   __shared__ uint32_t s_part[1][32];
   __shared__ int s_first[3];  // the element that the CTA's share begins in, how far behind the element's first unit, all units
@@ -666,8 +677,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
     // ================= keys and values to shared memory =================
     if constexpr (L::kMoreRegs > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kFewerRegs));
     const int me = tid - L::kLoad * 32;
-    constexpr int kSize = kE4M3 ? 1 : 2, kChunks = D * kSize / 16, kPer = kTile * kChunks / 128;  // 16-byte chunks of a position, of a thread
-    const int c = me % kChunks, r0 = me / kChunks;
+    // A warp has a quarter of a tile's positions, of which it finds the places by itself, a lane each; its lanes then take the chunks of 16 bytes
+    // of a position one behind the other.
+    constexpr int kRows = kTile / 4, kSize = kE4M3 ? 1 : 2, kChunks = D * kSize / 16, kPer = kRows * kChunks / 32, kStep = 32 / kChunks;
+    static_assert(kChunks <= 32, "a position to a pass at least");
+    const int row0 = (me >> 5) * kRows, c = lane % kChunks, r0 = lane / kChunks;
     int number = 0, told = 0;  // slots begun, and handed on
     auto tell = [&](int upto) {
       fence_async_shared();
@@ -683,44 +697,80 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
       }
       return wait(bar, parity);
     };
-    int tile_no = 0;
     Piece x;
-    if constexpr (kE4M3) {
+    x.tiles = 0;
+    int tile_no = -1, tile = -1, at0 = 0, now = -1, id = -1;  // now, id: the page of this lane's position in this tile and in the next
+    const char *k_src = nullptr, *v_src = nullptr;
+    uint32_t place = kNoStep;
+    // The next tile: where this lane's position lies, and which of the warp's are there; false at the end.
+    auto advance = [&]() {
+      auto page = [&](int pos) { return lane < kRows && pos < x.end ? p.a.table[x.row * p.a.table_stride + div_page(p.div, pos)] : -1; };
+      if (++tile >= x.tiles) {
+        if (!take(x)) return false;
+        tile = 0;
+        at0 = x.begin - kTile;
+        id = page(x.begin + row0 + lane);
+        k_src = reinterpret_cast<const char*>(p.pool.k) + x.head * p.pool.head_stride * kSize + c * 16;
+        v_src = reinterpret_cast<const char*>(p.pool.v) + x.head * p.pool.head_stride * kSize + c * 16;
+      }
+      ++tile_no;
+      at0 += kTile;
+      now = id;
+      const int pos = at0 + row0 + lane;
+      place = lane < kRows && pos >= x.low ? step_of(now, p.pool.pages, pos, p.div, p.page_step, p.pos_step) : kNoStep;
+      const uint32_t there = __ballot_sync(0xffffffffu, place != kNoStep);
+      if (lane == 0) {
+        if constexpr (kRows == 32) s_there[tile_no % kSlots][me >> 5] = there;
+        else reinterpret_cast<uint16_t*>(s_there[tile_no % kSlots])[me >> 5] = (uint16_t)there;
+      }
+      if (kE4M3 && place != kNoStep) {  // (to L2: the loads, for which there are registers a tile later, come from there)
+        const long long by = (long long)place * p.step_bytes + x.head * p.pool.head_stride;
+#pragma unroll
+        for (int i = 0; i < D; i += 128) {
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(p.pool.k) + by + i));
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(p.pool.v) + by + i));
+        }
+      }
+      id = tile + 1 < x.tiles ? page(pos + kTile) : -1;
+      return ok;
+    };
+    if constexpr (kTma) {
+      while (advance()) {
+        // boxes of positions that are seen: each warp asks for its own (a page that is none is out of the tensor, which gives zeros)
+        const int from = max(x.low - at0, 0), to = min(x.end - at0, kTile);
+        const int box0 = max(from - row0, 0) & -p.box, box1 = min(to - row0, kRows);
+        const bool part = from > 0 || to < kTile;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!room()) continue;
+          // (of a tile that is not whole the values behind its ends are zeroed by another warp, which hands it on)
+          uint64_t* const bar = (part && h == 1 ? b_landed : b_full) + number % kSlots;
+          unsigned char* const at = tiles + kStreams * L::kQ + (number % kSlots) * L::kSlot + row0 * 128;
+          if (lane == 0 && box1 > box0) mbar_expect_tx(bar, ((box1 - box0 + p.box - 1) & -p.box) * D * 2);
+          else mbar_arrive(bar);
+          for (int b = box0; b < box1; b += p.box) {
+            const int page = __shfl_sync(0xffffffffu, now, b), y = at0 + row0 + b, in = y - div_page(p.div, y) * p.pool.page_size;
+            const int z = (unsigned)page < (unsigned)p.pool.pages ? page : p.pool.pages, head = __shfl_sync(0xffffffffu, x.head, 0);
+            if (elect_one()) {
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c) tma_load_4d(at + c * kTile * 128 + b * 128, h == 0 ? &k_map : &v_map, bar, c * 64, in, head, z);
+            }
+            __syncwarp();
+          }
+          told = ++number;
+        }
+      }
+    } else if constexpr (kE4M3) {
       // A tile's keys and values lie in registers while they are on their way: those of the next one are asked for where this one's have
       // been converted and stored.
-      int tile = -1, pos = 0, id = -1;
-      x.tiles = 0;
-      const char *k_src = nullptr, *v_src = nullptr;
-      const uint32_t* places = nullptr;
-      auto advance = [&]() {  // the next tile's places; false at the end (a warp whose wait ran out leaves at a barrier, with the others)
-        if (++tile >= x.tiles) {
-          if (!named_bar_all(1, 128, take(x))) return false;
-          tile = 0;
-          k_src = reinterpret_cast<const char*>(p.pool.k) + x.head * p.pool.head_stride + c * 16;
-          v_src = reinterpret_cast<const char*>(p.pool.v) + x.head * p.pool.head_stride + c * 16;
-          pos = x.begin + me;
-          id = me < kTile && pos < x.end ? p.a.table[x.row * p.a.table_stride + div_page(p.div, pos)] : -1;
-        }
-        if (me < kTile) {
-          const uint32_t at = step_of(id, p.pool.pages, pos, p.div, p.page_step, p.pos_step);
-          s_place[tile_no % (kSlots / 2)][me] = at;
-          const uint32_t there = __ballot_sync(0xffffffffu, at != kNoStep);
-          if (lane == 0) s_there[tile_no % kSlots][me / 32] = there;
-        }
-        pos += kTile;
-        id = me < kTile && pos < x.end && tile + 1 < x.tiles ? p.a.table[x.row * p.a.table_stride + div_page(p.div, pos)] : -1;
-        if (!named_bar_all(1, 128, ok)) return false;
-        places = s_place[tile_no % (kSlots / 2)];
-        ++tile_no;
-        return true;
-      };
       uint4 v[2][kPer];
       auto load = [&](uint4 (&to)[kPer], const char* src) {
+        // (all places before the first load, and no branch around a load: with either between them they went one by one, 200 clocks each)
+        uint32_t at[kPer];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const uint32_t at = places[r0 + i * (128 / kChunks)];
-          to[i] = at != kNoStep ? *reinterpret_cast<const uint4*>(src + (unsigned long long)at * p.step_bytes) : make_uint4(0, 0, 0, 0);
-        }
+        for (int i = 0; i < kPer; ++i) at[i] = __shfl_sync(0xffffffffu, place, i * kStep + r0);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) to[i] = load_or_zero(src + (unsigned long long)(at[i] != kNoStep ? at[i] : 0) * p.step_bytes, at[i] != kNoStep);
       };
       auto store = [&](const uint4 (&from)[kPer]) {
         if (!room()) return;
@@ -731,7 +781,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
           uint32_t y[8];
 #pragma unroll
           for (int j = 0; j < 4; ++j) y[2 * j] = widen(w[j]), y[2 * j + 1] = widen(w[j] >> 16);
-          const int r = r0 + i * (128 / kChunks);
+          const int r = row0 + i * kStep + r0;
           *reinterpret_cast<uint4*>(to + chunk_at(kTile, r, 2 * c)) = make_uint4(y[0], y[1], y[2], y[3]);
           *reinterpret_cast<uint4*>(to + chunk_at(kTile, r, 2 * c + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
         }
@@ -749,79 +799,25 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
         some = more;
       }
     } else {
-    // (a warp whose wait ran out leaves at a barrier, with the others)
-    while (named_bar_all(1, 128, take(x))) {
-      const int* const table = p.a.table + x.row * p.a.table_stride;
-      const char* const src[2] = {reinterpret_cast<const char*>(p.pool.k) + x.head * p.pool.head_stride * kSize + c * 16,
-                                  reinterpret_cast<const char*>(p.pool.v) + x.head * p.pool.head_stride * kSize + c * 16};
-      int pos = x.begin + me;
-      int id = me < kTile && pos < x.end ? table[div_page(p.div, pos)] : -1;
-      for (int tile = 0; tile < x.tiles; ++tile, ++tile_no) {
-        if (me < kTile) {
-          const uint32_t at = pos >= x.low ? step_of(id, p.pool.pages, pos, p.div, p.page_step, p.pos_step) : kNoStep;
-          if constexpr (!kTma) s_place[tile_no % (kSlots / 2)][me] = at;
-          const uint32_t there = __ballot_sync(0xffffffffu, at != kNoStep);
-          if (lane == 0) s_there[tile_no % kSlots][me / 32] = there;
-        }
-        const int now = id, at0 = pos - me;
-        pos += kTile;
-        id = me < kTile && pos < x.end && tile + 1 < x.tiles ? table[div_page(p.div, pos)] : -1;
-        if constexpr (kTma) {
-          // boxes of positions that are seen: each warp asks for those of its 32 (a page that is none is out of the tensor, which gives zeros)
-          const int from = max(x.low - at0, 0), to = min(x.end - at0, kTile), w0 = me & -32;
-          const int box0 = max(from - w0, 0) & -p.box, box1 = min(to - w0, 32);
-          const bool part = from > 0 || to < kTile;
+      while (advance()) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!room()) continue;
-            // (of a tile that is not whole the values behind its ends are zeroed by another warp, which hands it on)
-            uint64_t* const bar = (part && h == 1 ? b_landed : b_full) + number % kSlots;
-            unsigned char* const at = tiles + kStreams * L::kQ + (number % kSlots) * L::kSlot + w0 * 128;
-            if (lane == 0 && box1 > box0) mbar_expect_tx(bar, ((box1 - box0 + p.box - 1) & -p.box) * D * 2);
-            else mbar_arrive(bar);
-            for (int b = box0; b < box1; b += p.box) {
-              const int page = __shfl_sync(0xffffffffu, now, b), y = __shfl_sync(0xffffffffu, at0 + me, b), in = y - div_page(p.div, y) * p.pool.page_size;
-              const int z = (unsigned)page < (unsigned)p.pool.pages ? page : p.pool.pages, head = __shfl_sync(0xffffffffu, x.head, 0);
-              if (elect_one()) {
+        for (int h = 0; h < 2; ++h) {
+          if (!room()) break;
+          const uint32_t to = kv_at + (number % kSlots) * L::kSlot;
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c) tma_load_4d(at + c * kTile * 128 + b * 128, h == 0 ? &k_map : &v_map, bar, c * 64, in, head, z);
-              }
-              __syncwarp();
-            }
-            told = ++number;
+          for (int i = 0; i < kPer; ++i) {
+            const uint32_t at = __shfl_sync(0xffffffffu, place, i * kStep + r0);
+            const bool there = at != kNoStep;
+            cp_async16(to + chunk_at(kTile, row0 + i * kStep + r0, c), (h == 0 ? k_src : v_src) + (there ? (unsigned long long)at * p.step_bytes : 0), there);
           }
-          continue;
-        } else {
-        if (!named_bar_all(1, 128, ok)) {
-          ok = false;
-          break;
-        }
-        const uint32_t* const places = s_place[tile_no % (kSlots / 2)];
-        {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!room()) break;
-            const uint32_t to = kv_at + (number % kSlots) * L::kSlot;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              const int r = r0 + i * (128 / kChunks);
-              const uint32_t at = places[r];
-              const bool there = at != kNoStep;
-              cp_async16(to + chunk_at(kTile, r, c), src[h] + (there ? (unsigned long long)at * p.step_bytes : 0), there);
-            }
-            cp_async_commit();
-            ++number;
-            if (number >= kSlots - 1) {
-              cp_async_wait<kSlots - 2>();
-              tell(max(told, number - (kSlots - 2)));
-            }
+          cp_async_commit();
+          ++number;
+          if (number >= kSlots - 1) {
+            cp_async_wait<kSlots - 2>();
+            tell(max(told, number - (kSlots - 2)));
           }
-        }
         }
       }
-    }
-    }
-    if constexpr (kStage == STAGE_COPY) {
       cp_async_wait<0>();
       if (ok) tell(number);
     }
@@ -1032,10 +1028,10 @@ cudaError_t launch(Params p, char* workspace, int sms, cudaStream_t stream) {
   p.ml = reinterpret_cast<float2*>(workspace + w.ml);
   p.more = reinterpret_cast<float*>(workspace + w.more);
   p.more_ml = reinterpret_cast<float2*>(workspace + w.more_ml);
-  // TMA boxes of whole pages or parts of one, of 8 to 32 positions (so many divide a page); pools that no tensor map can have, and
-  // 8-bit ones, which are converted on the way, go by cp.async
+  // TMA boxes of whole pages or parts of one, of 8 positions up to a warp's share of a tile (so many divide a page); pools that no tensor map
+  // can have, and 8-bit ones, which are converted on the way, go without
   CUtensorMap k_map = {}, v_map = {};
-  p.box = 32;
+  p.box = L::kTile / 4;
   while (p.box > 1 && p.pool.page_size % p.box != 0) p.box /= 2;
   const PagedPool& pool = p.pool;
   const bool bf16 = __is_same(T, __nv_bfloat16);

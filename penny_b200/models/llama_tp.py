@@ -83,13 +83,14 @@ class LlamaTPDecoder:
                  max_len: int = 2560, backend: str = "penny", proto: str = "auto", seed: int = 0,
                  use_graph: bool = True, full_init: bool = False, process_group=None, linears: str = "auto",
                  pdl: bool = True, page_size: int = 0, pages: Optional[int] = None, cache_dtype: Optional[torch.dtype] = None,
-                 cache_scales: Optional[tuple] = None):
+                 cache_scales: Optional[tuple] = None, sharing: bool = False):
         """page_size > 0: KV cache in pages of that many positions, `pages` of them (by default enough for max_batch sequences
         of max_len), of cache_dtype (bf16 or e4m3; cache_scales: its (k_scale, v_scale), as PagedKVCache takes them).  `positions` are
         that cache's lengths then; every step lets one token come to every
-        row.  A row for which there is no page is left out of a step, which raises OutOfPages when it has waited for the device."""
-        if page_size < 0 or (page_size == 0 and (pages is not None or cache_dtype is not None or cache_scales is not None)):
-            raise ValueError("pages, cache_dtype and cache_scales belong to a cache in pages: page_size above 0")
+        row.  A row for which there is no page is left out of a step, which raises OutOfPages when it has waited for the device.
+        sharing: rows may be forked (`fork`); a step finds the rows that have pages in common and reads those once."""
+        if page_size < 0 or (page_size == 0 and (pages is not None or cache_dtype is not None or cache_scales is not None or sharing)):
+            raise ValueError("pages, cache_dtype, cache_scales and sharing belong to a cache in pages: page_size above 0")
         if cache_dtype not in (None, torch.bfloat16, torch.float8_e4m3fn):
             raise ValueError("cache_dtype: bf16 or e4m3, beside a bf16 projection")
         assert cfg.heads % world == 0 and cfg.kv_heads % world == 0 and cfg.ffn % world == 0
@@ -192,7 +193,7 @@ class LlamaTPDecoder:
         self.paged: Optional[PagedKVCache] = None
         if page_size > 0:
             self.paged = PagedKVCache(cfg.layers, B, max_len, self.Hkv, D, page_size, pages, cache_dtype or dt, *(cache_scales or (None, None)),
-                                      device=self.dev)
+                                      device=self.dev, sharing=sharing)
             self.page_step = PageStep(torch.full((B,), -1, dtype=torch.int64, device=self.dev), torch.zeros(B, dtype=torch.int32, device=self.dev),
                                       torch.zeros(B + 1, dtype=torch.int32, device=self.dev), torch.ones(B, dtype=torch.bool, device=self.dev))
             self.one_each = torch.ones(B, dtype=torch.int32, device=self.dev)
@@ -201,7 +202,8 @@ class LlamaTPDecoder:
             # kernel counts on says nothing
             self.positions, self.counted = self.paged.lengths, self.positions
             self._host_served = torch.ones(B, dtype=torch.bool).pin_memory()
-            self.page_workspace = self.paged.workspace(self.Hq)
+            self.sharing, self.page_groups = sharing, None
+            self.page_workspace = self.paged.workspace(self.Hq, groups=sharing)
             self.kcache = self.vcache = []
         else:
             self.counted = self.positions
@@ -230,7 +232,7 @@ class LlamaTPDecoder:
         if self.fold:
             self.kernels_per_step = 5 * cfg.layers + 3
         if self.paged is not None:  # + page tables; append, attention and (where rows can be cut) join for the attention
-            self.kernels_per_step += 1 + cfg.layers * (2 if self.page_workspace.numel() else 1)
+            self.kernels_per_step += 1 + int(sharing) + cfg.layers * (2 if self.page_workspace.numel() else 1)
 
     @staticmethod
     def tiled_linears(cfg: LlamaConfig, batch: int) -> frozenset:
@@ -387,7 +389,7 @@ class LlamaTPDecoder:
         # (early: the tables are complete since the launch without programmatic dependency at the step's start)
         self.paged.append(li, self.qkv, self.page_step, self.Hq, theta, early=True)
         self.paged.attend(li, self.qkv[:, :self.Hq * self.cfg.head_dim].unflatten(1, heads), out=self.attn.unflatten(1, heads), scale=self.scale,
-                          workspace=self.page_workspace, early=True)
+                          workspace=self.page_workspace, early=True, groups=self.page_groups)
 
     def _layers_folded(self, tokens):
         """One rank: five launches per layer, q/k/v, gate/up and head on the tiled or on the decode GEMM (`tiled_linears`).  x
@@ -453,6 +455,8 @@ class LlamaTPDecoder:
     def _step_impl(self, warm_up: bool = False, separate: bool = False, host: bool = False):
         if self.paged is not None:
             self.paged.advance(self.one_each, self.B, out=self.page_step)
+            if self.sharing:
+                self.page_groups = self.paged.groups()
             torch.logical_and(self.served, self.page_step.granted, out=self.served)  # (and nothing behind it starts before the tables are done)
         if self.fold and not separate:
             self._layers_folded(self._host_in if host else self.tokens)
@@ -530,6 +534,39 @@ class LlamaTPDecoder:
         leave[rows] = -1
         self.paged.advance(leave.to(self.dev) * self.paged.lengths, 0)
         self.served[leave.to(self.dev) != 0] = True
+
+    def fork(self, source, target):
+        """Rows `target` of a cache in pages with sharing, which are empty, become copies of rows `source`: their sequences go on from the same
+        positions with the same next token, and the pages that are full are kept once.  (A row as it is after a step, or released, or never used.)
+        Raises OutOfPages, which has the rows, if some are not empty or have no page for the positions behind their last full one."""
+        if self.paged is None or not self.sharing:
+            raise ValueError("fork: a cache in pages with sharing=True has rows that share them")
+        source, target = list(source), list(target)
+        if len(source) != len(target) or any(not 0 <= r < self.B for r in source + target):
+            raise IndexError(f"fork: a source for every target, rows in [0, {self.B})")
+        a, b = (torch.tensor(v, dtype=torch.int32, device=self.dev) for v in (source, target))
+        granted = self.paged.fork(a, b).granted
+        a, b = a[granted].long(), b[granted].long()
+        for t in (self.tokens, self.next_tokens):
+            t[b] = t[a]
+        self.served[b] = self.served[a]
+        refused = [r for r, ok in zip(target, granted.tolist()) if not ok]
+        if refused:
+            raise OutOfPages(f"rows {refused[:8]} were not forked: not empty, or no page of {self.paged.pages}", refused, self.next_tokens.clone())
+
+    def logprobs(self, top: int = 0):
+        """`ops.token_logprobs` of the tokens that the last step chose (self.next_tokens), under the whole vocabulary's softmax."""
+        from ..ops.logprobs import token_logprobs
+        logits = self.logits
+        if self.world > 1:  # (the ranks' shards of the vocabulary side by side)
+            if self.backend == "nccl":
+                import torch.distributed as dist
+                every = torch.empty(self.world * self.B, self.V, dtype=logits.dtype, device=self.dev)
+                dist.all_gather_into_tensor(every, logits, group=self.pg)
+            else:
+                every = self.comm.all_gather(logits)
+            logits = every.view(self.world, self.B, self.V).transpose(0, 1).reshape(self.B, self.world * self.V)
+        return token_logprobs(logits, self.next_tokens, top)
 
     def step_device(self):
         """One decode step on the device buffers: self.tokens -> self.next_tokens."""

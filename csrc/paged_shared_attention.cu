@@ -19,7 +19,7 @@
 //     (paged_shared_plan.h).  A warp walks the line and hands the pieces to the others; loads run ahead across pieces.  Pieces leave unnormalised
 //     fp32 outputs in a workspace, a second kernel joins them.  No counters: a workspace holds nothing between calls.
 //   * Weights count from a base that is the largest score of the first 64 positions; it follows, and the accumulators are scaled, when the
-//     weights of 64 positions add up to more than 2^40 (fp16 weights, which stand 2^7 above it against what fp16 loses under 2^-14: 2^15), which is seldom.
+//     weights of 64 positions add up to more than 2^10 (fp16 weights, which stand 2^7 above it against what fp16 loses under 2^-14: 2^15), which is seldom.
 //     Weights are rounded to their type by up to half a step of each, their sum is not; an output is then off by what the
 //     roundings of many weights leave, about one of its own.
 //
@@ -92,6 +92,9 @@ struct Element {
   int queries, first; // (row, head) pairs of a KV head; the first row's place in order, or ~row
   int row;            // whose table it is
 };
+// A row takes what its group shares if it sees all of it; one whose window leaves some out, or that was cut back since, reads what it sees by itself.
+// (A weight of zero does not take a value that is not finite out of a product.)
+__device__ __forceinline__ bool takes_part(const Params& p, int row, const Seen& s) { return s.first == 0 && p.shared[row] <= s.end; }
 template <int D>
 __device__ __forceinline__ Element element_of(const Params& p, int e) {
   Element x = {};
@@ -104,14 +107,14 @@ __device__ __forceinline__ Element element_of(const Params& p, int e) {
     if ((unsigned)x.row >= (unsigned)rows) return x;
     x.queries = n * p.group;
     x.end = min(max(p.shared[x.row], 0), p.max_len);
-    x.low = p.a.window > 0 ? max(0, x.end + 1 - p.a.window) : 0;  // (its rows are longer than what they share)
+    if (p.a.window > 0 && x.end >= p.a.window) x.end = 0;  // (its rows are longer than what they share: none sees all of it)
   } else {
     x.row = e - rows;
     x.first = ~x.row;
     x.queries = p.group;
     const Seen s = seen_of(p.a.lengths[x.row], p.max_len, p.a.window);
     x.end = s.end;
-    x.low = max(s.first, min(max(p.shared[x.row], 0), s.end));
+    x.low = takes_part(p, x.row, s) ? max(p.shared[x.row], 0) : s.first;
   }
   x.begin = p.box > 0 && x.low < x.end ? x.low & -p.box : x.low;
   return x;
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
   using T = std::conditional_t<kStage == STAGE_E4M3, __half, TQ>;  // of the products
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16), kTma = kStage == STAGE_TMA, kE4M3 = kStage == STAGE_E4M3;
   // The base is kShift under the largest score of the first 64 positions that have any, and of later ones whose weights add up to over kLimit.
-  constexpr float kShift = kBf16 ? 0.f : 7.f, kLimit = kBf16 ? 0x1p40f : 0x1p15f;
+  constexpr float kShift = kBf16 ? 0.f : 7.f, kLimit = kBf16 ? 0x1p10f : 0x1p15f;
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t b_full[kSlots], b_free[kSlots], b_landed[kSlots], b_q[2], b_s[2], b_p[2], b_o[2], b_piece[kRing], b_taken[kRing];
   __shared__ Piece s_piece[kRing];
@@ -940,6 +943,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_shared_join(const __grid_co
 #pragma unroll 1
     for (int kind = 0; kind < 2; ++kind) {
       const Element x = of[kind];
+      if (kind == 0 && !takes_part(p, row, seen_of(p.a.lengths[row], p.max_len, p.a.window))) continue;
       const int tiles = units > 0 ? tiles_of(x.end - x.begin, L::kTile) : 0;
       if (tiles == 0) continue;
       const int query = kind == 0 ? place.y * p.group + g : g;

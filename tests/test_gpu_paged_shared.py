@@ -101,7 +101,7 @@ class Case:
         return out
 
 
-LAYOUTS = [(4, 1, 128), (32, 8, 128), (8, 2, 64), (20, 20, 64), (35, 7, 64), (28, 2, 128), (8, 1, 256), (64, 1, 64), (24, 2, 256)]
+LAYOUTS = [(4, 1, 128), (32, 8, 128), (8, 2, 64), (20, 20, 64), (35, 7, 64), (28, 2, 128), (8, 1, 256), (64, 1, 64), (24, 2, 256), (150, 1, 128), (300, 1, 64)]
 
 
 def test_one_group():
@@ -222,6 +222,39 @@ def test_infinities_and_nan():
             else:
                 assert torch.equal(got[r], base[r])
         case.k[page, 3, 0] = keep
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_values_that_are_not_finite(value):
+    """A shared position whose values are not finite: not in rows whose window leaves it out, nor in rows that end in front of it."""
+    case = Case([(0, 256, n) for n in (1, 30, 100, 300)] + [(None, 0, 40)], 4, 2, 128, 16, seed=4)
+    groups = case.groups()
+    call = lambda **more: P.paged_attention(case.q, case.k, case.v, case.table, case.lengths, groups=groups, **more)  # noqa: E731
+    inside = [r for r in range(5) if case.lengths[r] > 255]
+    page = int(case.table[inside[0], 1])  # positions 16 to 31
+    for window in (0, 250, 290, 400):
+        want = call(window=window)
+        keep = case.v[page, 4].clone()
+        case.v[page, 4] = value
+        got = call(window=window)
+        for r in range(5):
+            sees = r in inside and (window == 0 or int(case.lengths[r]) - window <= 20)
+            assert got[r].isfinite().all() != sees and (sees or torch.equal(got[r], want[r])), (window, r)
+        case.v[page, 4] = keep
+    lengths = case.lengths.clone()
+    case.lengths[inside[1]] = 20
+    want = call()
+    case.v[page, 4] = value
+    got = call()
+    assert torch.equal(got[inside[1]], want[inside[1]]) and not got[inside[0]].isfinite().any()
+    case.lengths = lengths
+
+
+def test_large_values():
+    """Values near the end of bf16's range, with weights that grow along the row."""
+    case = Case([(0, 256, n) for n in (1, 200)], 4, 2, 128, 16, seed=4)
+    case.v.mul_(1e34)
+    case.check()
 
 
 def test_strides_and_out():

@@ -14,6 +14,7 @@
 
 #include "paged_kernels.h"
 #include "paged_plan.h"
+#include "paged_shared_plan.h"
 
 namespace py = pybind11;
 using namespace penny;
@@ -410,10 +411,10 @@ void bind_paged(py::module_& m) {
          "paged_attention_workspace_bytes: rows, heads and lengths");
     need(rows < (1 << 24) && heads < (1 << 20) && dim <= 256, "paged_attention_workspace_bytes: rows, heads and dim");
     need(!groups || rows <= kPagedMaxRows, "paged_attention_workspace_bytes: more than PAGED_MAX_ROWS rows");
-    if (groups) return (int64_t)shared_attention_workspace_bytes((int)rows, (int)heads, (int)dim, sms_of(at::cuda::current_device()));
-    return (int64_t)paged_attention_workspace_bytes((int)rows, (int)heads, (int)kv_heads, (int)dim, (int)std::min<int64_t>(max_len, paged::kMaxLen),
+    const size_t shared = groups ? shared_attention_workspace_bytes((int)rows, (int)heads, (int)dim, sms_of(at::cuda::current_device())) : 0;
+    return (int64_t)std::max(shared, paged_attention_workspace_bytes((int)rows, (int)heads, (int)kv_heads, (int)dim, (int)std::min<int64_t>(max_len, paged::kMaxLen),
                                                     (int)std::min<int64_t>(window, 1ll << 30),
-                                                    sms_of(at::cuda::current_device()));
+                                                    sms_of(at::cuda::current_device())));
   }, py::arg("rows"), py::arg("heads"), py::arg("kv_heads"), py::arg("dim"), py::arg("max_len"), py::arg("window") = 0,
      py::arg("groups") = false);
   // q [rows, heads, dim], one token of every row, attends to the row's last `window` positions (0: all of them).
@@ -469,14 +470,15 @@ void bind_paged(py::module_& m) {
     const int win = (int)std::min<int64_t>(window, 1ll << 30);
     const int max_len = (int)std::min<int64_t>(table.size(1) * pool.page_size, paged::kMaxLen);
     need(B * (int64_t)paged::units_of(win > 0 && win < max_len ? win : max_len, 16) <= paged::kMaxUnits, "paged_attention: a table for over 2^34 positions");
-    const size_t bytes = groups.has_value() ? shared_attention_workspace_bytes((int)B, (int)H, pool.dim, sms)
-                                            : paged_attention_workspace_bytes((int)B, (int)H, pool.heads, pool.dim, max_len, win, sms);
+    const bool shared = groups.has_value() && paged::shared_pays(B, win > 0 && win < max_len ? win : max_len, pool.heads, pool.dim, (int)k.element_size());
+    const size_t bytes = shared ? shared_attention_workspace_bytes((int)B, (int)H, pool.dim, sms)
+                                : paged_attention_workspace_bytes((int)B, (int)H, pool.heads, pool.dim, max_len, win, sms);
     if (workspace.has_value()) need(workspace->nbytes() >= bytes, "workspace too small (paged_attention_workspace_bytes)");
     else if (bytes > 0) workspace = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, q.device(), c10::nullopt);
     const PagedAttention a = {q.data_ptr(), q.stride(0), q.stride(1), out->data_ptr(), out->stride(0), out->stride(1),
                               lse.has_value() ? lse->data_ptr<float>() : nullptr, table.data_ptr<int>(), table.stride(0), lengths.data_ptr<int>(),
                               (int)B, (int)H, (int)table.size(1), win, scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)pool.dim), early};
-    if (groups.has_value()) {
+    if (shared) {
       const SharedGroups g = {std::get<0>(*groups).data_ptr<int>(), std::get<1>(*groups).data_ptr<int>(), std::get<2>(*groups).data_ptr<int>()};
       ck(launch_shared_attention(a, type, pool, cache, g, workspace->data_ptr(), sms, penny_gemm_error_word(), cur()), "paged_attention");
       return *out;

@@ -32,6 +32,13 @@ PENNY_ATTN_HD Tiles piece_of(int begin, int tiles, bool pair, int share, int cta
   return {first_tile(from, tiles, pair), first_tile(from + share, tiles, pair)};
 }
 PENNY_ATTN_HD int cta_of(int begin, int tile, bool pair, int share) { return (begin + kItemStart + tile * (pair ? kPairUnits : kTileUnits)) / share; }
+// Whether a batch whose rows can see `positions` each is worth the shared kernel's tiles.  The one that reads every row by itself finds what they
+// share in L2, and needs no time to start tensor cores: us with / without, of bytes for all rows, 32 of 8 heads of 128: 138 MB 25 / 20, 167 30 /
+// 22, 543 36 / 49, 554 38 / 51, 2174 48 / 165; e4m3 272 MB 41 / 39 and 44 / 41, 1087 55 / 131; 20 of 20 of 64, fp16: 170 MB 29 / 24, 173 21 / 25, 209 30 / 28,
+// 679 31 / 71; 4 of 1: 272 MB 51 / 30.  (The lengths are on the device; a table's width says what they can be.)
+inline bool shared_pays(long long rows, long long positions, int kv_heads, int dim, int value_bytes) {
+  return rows * positions * kv_heads * dim * 2 * value_bytes > 256ll << 20;
+}
 // (row, query head) pairs of an item, and of how many items: of `queries` pairs, `most` to an item
 PENNY_ATTN_HD int query_tiles(int queries, int most) { return (queries + most - 1) / most; }
 // The items of an element are alike but for its last queries of each head, which may be fewer; they count as the others do.

@@ -149,8 +149,9 @@ def paged_attention(q, k, v, table, lengths, out=None, lse=None, scale: Optional
     it reads only q and the keys and values of each row's last position; the other rows, lengths and table are then read before they end.
 
     groups: `page_groups` of this table and these lengths, or of a time since when the rows of its groups have kept the pages that they
-    share: what a group shares is read once for all its rows, on tensor cores, instead of once for each.  The result is the same but for
-    the order of sums.  At most 8192 rows; the workspace is that of groups=True.  A wait of the kernel that ran
+    share: what a group shares is read once for all its rows, on tensor cores, instead of once for each, where the rows can see over 256 MB of keys
+    and values together by the table's width (under that, reading each row by itself takes less time).  The result is the same but for the
+    order of sums.  At most 8192 rows; the workspace is that of groups=True.  A wait of the kernel that ran
     out (4 s) leaves its rows undone and shows in `gemm_error`."""
     return ops.paged_attention(q, k, v, table, lengths, out, lse, scale, window, k_scale, v_scale, workspace, early, groups)
 

@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 
 def _model(**more):
-    return LlamaTPDecoder(LlamaConfig.tiny(), max_batch=8, max_len=400, page_size=16, full_init=True, **more)
+    return LlamaTPDecoder(LlamaConfig.tiny(), max_batch=8, page_size=16, full_init=True, **(dict(max_len=80000, pages=400) | more))
 
 
 def _prompts(model, lengths):

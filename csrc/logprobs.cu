@@ -14,8 +14,8 @@
 //
 // Few rows: a row's cluster has up to eight CTAs, whose sums and lists meet in the first one's shared memory.
 //
-// Bound by memory where rows are many (a value takes about six instructions and one exponential, three quarters of what an SM can do
-// in the time), by latency where they are few.
+// Many rows are bound by instructions and exponentials, near the copy rate: 2047 rows of 128256 in bf16 101 us (5.2 TB/s), with the 20 likeliest
+// 145; 1000 in fp32 87 (5.9 TB/s).  Few by latency: 64 rows 8.6 us, with the 20 likeliest 13.5; one 4.8.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>

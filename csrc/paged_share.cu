@@ -15,7 +15,8 @@
 //                   rows.
 //
 // All but the copy are latency: a few reads one after another, prefix sums, barriers.  One CTA for a small state, a cluster of up
-// to sixteen for a large one.
+// to sixteen for a large one: 64 forks of 62 pages each and their leaving 17 us (fork 8 of 12 pages 5), 600 pages moved together 5.5 (and 78 for 143
+// copies in 48 pools, 5.6 TB/s), groups of 64 rows 7.4, of 4000 25.
 #include "kernel_setup.h"
 #include "paged_kernels.h"
 #include "paged_plan.h"
@@ -215,13 +216,14 @@ __global__ void __launch_bounds__(kThreads) k_page_compact(const PageCompact a, 
   if (me == 0) *a.free_count = a.pages - used;
 }
 
-// A CTA takes pieces of pages, (copy, pool, piece) in a line, the pools of a copy one behind the other.
-constexpr int kCopyThreads = 256, kAhead = 8, kPiece = kCopyThreads * kAhead * 16;
-__global__ void __launch_bounds__(kCopyThreads) k_page_copy(const __grid_constant__ PageCopy a, int pieces) {
+// A CTA takes pieces of a page, or the same page of `group` pools where pages are small; (copy, pools, piece) in a line, the pools of a copy one
+// behind the other.  (A pool of small pages, one by one, 880 GB/s, so 4000.)
+constexpr int kCopyThreads = 256, kAhead = 8, kPiece = kCopyThreads * kAhead;  // vectors of 16 bytes
+__global__ void __launch_bounds__(kCopyThreads) k_page_copy(const __grid_constant__ PageCopy a, int pieces, int group) {
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, vecs = a.run_bytes / 16, total = a.outer * a.inner * vecs;  // of a page
-  const long long each = (long long)a.pools * pieces, units = a.copies * each;
+  const long long each = (long long)((a.pools + group - 1) / group) * pieces, units = a.copies * each;
   for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const int copy = (int)(unit / each), rest = (int)(unit - copy * each);
     const int from = a.from[copy], to = a.to[copy];
@@ -229,26 +231,33 @@ __global__ void __launch_bounds__(kCopyThreads) k_page_copy(const __grid_constan
       unit += (each - 1 - rest) / gridDim.x * gridDim.x;
       continue;
     }
-    const int pool = rest / pieces, piece = rest - pool * pieces;
-    const char* const src = a.pool[pool] + from * a.page_bytes;
-    char* const dst = a.pool[pool] + to * a.page_bytes;
+    const int set = rest / pieces, first = (rest - set * pieces) * kPiece, pool0 = set * group;
+    const int count = group > 1 ? min(group, a.pools - pool0) * total : total;  // vectors of this unit's pools
+    const long long src = from * a.page_bytes, dst = to * a.page_bytes;
     uint4 v[kAhead];
-    auto at = [&](int u) {
-      const int i = piece * (kCopyThreads * kAhead) + u * kCopyThreads + tid;
-      if (i >= total) return -1ll;
+    auto at = [&](int u, char*& base) {  // where a vector lies in its page, -1 behind the last
+      int i = first + u * kCopyThreads + tid;
+      if (i >= count) return -1ll;
+      int pool = pool0;
+      if (group > 1) {
+        pool += i / total;
+        i %= total;
+      }
+      base = a.pool[pool];
       if (a.outer == 1 && a.inner == 1) return (long long)i * 16;
       const int run = i / vecs, o = run / a.inner;
       return o * a.outer_bytes + (run - o * a.inner) * a.inner_bytes + (long long)(i - run * vecs) * 16;
     };
+    char* base = nullptr;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const long long x = at(u);
-      if (x >= 0) v[u] = *reinterpret_cast<const uint4*>(src + x);
+      const long long x = at(u, base);
+      if (x >= 0) v[u] = *reinterpret_cast<const uint4*>(base + src + x);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const long long x = at(u);
-      if (x >= 0) *reinterpret_cast<uint4*>(dst + x) = v[u];
+      const long long x = at(u, base);
+      if (x >= 0) *reinterpret_cast<uint4*>(base + dst + x) = v[u];
     }
   }
 }
@@ -415,13 +424,13 @@ cudaError_t launch_page_copy(const PageCopy& a, int sms, cudaStream_t stream) {
   if (a.pools < 0 || a.pools > kPageCopyPools || a.copies < 0 || a.outer < 1 || a.inner < 1 || a.run_bytes < 16 || a.run_bytes % 16 != 0)
     return cudaErrorInvalidValue;
   if (a.pools == 0 || a.copies == 0) return cudaSuccess;
-  const long long bytes = (long long)a.outer * a.inner * a.run_bytes;
-  if (bytes / 16 > INT_MAX - kPiece) return cudaErrorInvalidValue;
-  const int pieces = (int)((bytes + kPiece - 1) / kPiece);
+  const long long total = (long long)a.outer * a.inner * (a.run_bytes / 16);
+  if (total > INT_MAX - kPiece) return cudaErrorInvalidValue;
+  const int pieces = (int)((total + kPiece - 1) / kPiece), group = pieces > 1 ? 1 : (int)std::min<long long>(a.pools, kPiece / total);
   if ((long long)a.pools * pieces > INT_MAX) return cudaErrorInvalidValue;
-  const long long units = (long long)a.copies * a.pools * pieces;
+  const long long units = (long long)a.copies * ((a.pools + group - 1) / group) * pieces;
   const int ctas = (int)std::min<long long>(units, 8ll * sms);
-  return launch_kernel_ex(k_page_copy, dim3((unsigned)ctas), dim3(kCopyThreads), 0, stream, true, 1, a, pieces);
+  return launch_kernel_ex(k_page_copy, dim3((unsigned)ctas), dim3(kCopyThreads), 0, stream, true, 1, a, pieces, group);
 }
 
 cudaError_t launch_page_groups(const PageGroups& a, cudaStream_t stream) {

@@ -299,12 +299,17 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Bounded by tries alone, each of which the hardware holds for a while: less code, of which all roles' has to stay in the instruction caches.
+// Bounded by the clock, as mbar_wait is, in less code (that of all roles has to stay in the instruction caches).
 __device__ __forceinline__ bool wait_some(uint64_t* bar, uint32_t parity) {
+  unsigned long long since = 0;
 #pragma unroll 1
-  for (uint32_t i = 0; i < kSpinLimit; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return false;
+  for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {
+    if ((i & 255u) != 0) continue;
+    const unsigned long long now = gtime_ns();
+    if (since == 0) since = now;
+    if (now - since > kWaitNs) return false;
+  }
+  return true;
 }
 // Columns of a thread's row times `by`: fp32 values, or pairs of T.
 template <typename T>

@@ -426,7 +426,10 @@ cudaError_t launch_page_copy(const PageCopy& a, int sms, cudaStream_t stream) {
   if (a.pools == 0 || a.copies == 0) return cudaSuccess;
   const long long total = (long long)a.outer * a.inner * (a.run_bytes / 16);
   if (total > INT_MAX - kPiece) return cudaErrorInvalidValue;
-  const int pieces = (int)((total + kPiece - 1) / kPiece), group = pieces > 1 ? 1 : (int)std::min<long long>(a.pools, kPiece / total);
+  const int pieces = (int)((total + kPiece - 1) / kPiece);
+  // (several pools only where there are CTAs for more than one round: 8 copies of 4 KB in 48 pools 2.2 us one by one, eight pools at a time 4.2)
+  const long long rounds = std::max<long long>(1, (long long)a.copies * a.pools / (8 * sms));
+  const int group = pieces > 1 ? 1 : (int)std::min({(long long)a.pools, kPiece / total, rounds});
   if ((long long)a.pools * pieces > INT_MAX) return cudaErrorInvalidValue;
   const long long units = (long long)a.copies * ((a.pools + group - 1) / group) * pieces;
   const int ctas = (int)std::min<long long>(units, 8ll * sms);

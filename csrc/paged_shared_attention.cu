@@ -25,7 +25,7 @@
 //
 // Bound by chains of waits, not by a pipe: a tile of 128 positions of two times 128 queries takes 4200 clocks, 2050 of softmax and 1600 of products
 // that wait for each other, in two streams; one of a row's own positions 2600.  64 rows of 4000 shared and 300 own positions, 32 of 8 heads of 128,
-// bf16, 54 us; 100 of 16000 and 500 97; 130 of nine prompts, e4m3, 85.
+// bf16, 55 us; 100 of 16000 and 500 97; 130 of nine prompts, e4m3, 89.
 //
 // Every wait is bounded; one that ran out sets the error word that all tcgen05 kernels here share, and the CTA ends.
 #include <cuda_bf16.h>

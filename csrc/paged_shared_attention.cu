@@ -567,7 +567,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) k_shared_attention(cons
                 }
                 sum *= by;
                 if (__any_sync(0xffffffffu, by != 1.f)) {
-                  if (h > 0) scale_columns<T>(s_cols, 32, by, true);  // the weights in front of these
+                  if (h > 0) {  // the weights in front of these, which have to be there (a wait for loads is none for stores)
+                    tmem_st_wait();
+                    scale_columns<T>(s_cols, 32, by, true);
+                  }
                   if (i > 0) scale_columns<T>(o_cols, D, by, false);
                 }
               }

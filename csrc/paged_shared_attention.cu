@@ -96,9 +96,6 @@ struct Element {
   int queries, first; // (row, head) pairs of a KV head; the first row's place in order, or ~row
   int row;            // whose table it is
 };
-// A row takes what its group shares if it sees all of it; one whose window leaves some out, or that was cut back since, reads what it sees by itself.
-// (A weight of zero does not take a value that is not finite out of a product.)
-__device__ __forceinline__ bool takes_part(const Params& p, int row, const Seen& s) { return s.first == 0 && p.shared[row] <= s.end; }
 template <int D>
 __device__ __forceinline__ Element element_of(const Params& p, int e) {
   Element x = {};
@@ -110,15 +107,14 @@ __device__ __forceinline__ Element element_of(const Params& p, int e) {
     x.row = p.order[s0];
     if ((unsigned)x.row >= (unsigned)rows) return x;
     x.queries = n * p.group;
-    x.end = min(max(p.shared[x.row], 0), p.max_len);
-    if (p.a.window > 0 && x.end >= p.a.window) x.end = 0;  // (its rows are longer than what they share: none sees all of it)
+    x.end = group_end(p.shared[x.row], p.max_len, p.a.window);
   } else {
     x.row = e - rows;
     x.first = ~x.row;
     x.queries = p.group;
     const Seen s = seen_of(p.a.lengths[x.row], p.max_len, p.a.window);
     x.end = s.end;
-    x.low = takes_part(p, x.row, s) ? max(p.shared[x.row], 0) : s.first;
+    x.low = takes_part(s, p.shared[x.row]) ? max(p.shared[x.row], 0) : s.first;
   }
   x.begin = p.box > 0 && x.low < x.end ? x.low & -p.box : x.low;
   return x;
@@ -955,7 +951,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_shared_join(const __grid_co
 #pragma unroll 1
     for (int kind = 0; kind < 2; ++kind) {
       const Element x = of[kind];
-      if (kind == 0 && !takes_part(p, row, seen_of(p.a.lengths[row], p.max_len, p.a.window))) continue;
+      if (kind == 0 && !takes_part(seen_of(p.a.lengths[row], p.max_len, p.a.window), p.shared[row])) continue;
       const int tiles = units > 0 ? tiles_of(x.end - x.begin, L::kTile) : 0;
       if (tiles == 0) continue;
       const int query = kind == 0 ? place.y * p.group + g : g;

@@ -39,6 +39,15 @@ PENNY_ATTN_HD int cta_of(int begin, int tile, bool pair, int share) { return (be
 inline bool shared_pays(long long rows, long long positions, int kv_heads, int dim, int value_bytes) {
   return rows * positions * kv_heads * dim * 2 * value_bytes > 256ll << 20;
 }
+// A row takes what its group shares, the group's first `shared` positions, if it sees all of it; one whose window leaves some out, or that was cut
+// back since, reads what it sees by itself.  (A weight of zero does not take a value that is not finite out of a product.)
+PENNY_ATTN_HD bool takes_part(const Seen& seen, int shared) { return seen.first == 0 && shared <= seen.end; }
+// What of `shared` positions is worth reading for a group: nothing where a row that has them all cannot see them all, else all that a table can
+// hold.  (Of a row that sees nothing else the window may end with them.)
+PENNY_ATTN_HD int group_end(int shared, int max_len, int window) {
+  const int end = attn::cached_rows(shared, max_len);
+  return window > 0 && end > window ? 0 : end;
+}
 // (row, query head) pairs of an item, and of how many items: of `queries` pairs, `most` to an item
 PENNY_ATTN_HD int query_tiles(int queries, int most) { return (queries + most - 1) / most; }
 // The items of an element are alike but for its last queries of each head, which may be fewer; they count as the others do.

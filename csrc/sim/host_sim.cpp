@@ -424,6 +424,13 @@ void penny_shared_piece(int begin, int tiles, int pair, int share, int cta, int*
   from_to[0] = t.from, from_to[1] = t.to;
 }
 int penny_shared_cta_of(int begin, int tile, int pair, int share) { return penny::paged::cta_of(begin, tile, pair != 0, share); }
+// The positions [from, to) that a row of `length` takes from its group (of which `shared` are in common) and by itself, for the two kinds of its elements.
+void penny_shared_row(int length, int shared, int max_len, int window, int* of_group, int* own) {
+  const penny::paged::Seen s = penny::paged::seen_of(length, max_len, window);
+  const bool part = penny::paged::takes_part(s, shared);
+  of_group[0] = 0, of_group[1] = part ? penny::paged::group_end(shared, max_len, window) : 0;
+  own[0] = part ? (shared > 0 ? shared : 0) : s.first, own[1] = s.end;
+}
 long long penny_shared_most_units(long long rows, int kv_heads, int group, long long positions, int tile, int most) {
   return penny::paged::most_units(rows, kv_heads, group, positions, tile, most);
 }

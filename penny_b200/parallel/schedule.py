@@ -232,6 +232,13 @@ def shared_cta_of(begin: int, tile: int, pair: bool, share: int) -> int:
     return sim_lib().penny_shared_cta_of(begin, tile, pair, share)
 
 
+def shared_row(length: int, shared: int, max_len: int, window: int = 0):
+    """The positions [from, to) that a row takes from its group, and those that it reads by itself (csrc/paged_shared_plan.h)."""
+    group, own = (ctypes.c_int * 2)(), (ctypes.c_int * 2)()
+    sim_lib().penny_shared_row(length, shared, max_len, window, group, own)
+    return tuple(group), tuple(own)
+
+
 def shared_most_units(rows: int, kv_heads: int, group: int, positions: int, tile: int, most: int) -> int:
     """Units of a batch at most (csrc/paged_shared_plan.h)."""
     f = sim_lib().penny_shared_most_units

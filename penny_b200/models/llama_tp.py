@@ -537,7 +537,7 @@ class LlamaTPDecoder:
 
     def fork(self, source, target):
         """Rows `target` of a cache in pages with sharing, which are empty, become copies of rows `source`: their sequences go on from the same
-        positions with the same next token, and the pages that are full are kept once.  (A row as it is after a step, or released, or never used.)
+        positions with the same next token and logits, and the pages that are full are kept once.  (A row as it is after a step, or released, or never used.)
         Raises OutOfPages, which has the rows, if some are not empty or have no page for the positions behind their last full one."""
         if self.paged is None or not self.sharing:
             raise ValueError("fork: a cache in pages with sharing=True has rows that share them")
@@ -547,9 +547,8 @@ class LlamaTPDecoder:
         a, b = (torch.tensor(v, dtype=torch.int32, device=self.dev) for v in (source, target))
         granted = self.paged.fork(a, b).granted
         a, b = a[granted].long(), b[granted].long()
-        for t in (self.tokens, self.next_tokens):
+        for t in (self.tokens, self.next_tokens, self.logits, self.served):
             t[b] = t[a]
-        self.served[b] = self.served[a]
         refused = [r for r, ok in zip(target, granted.tolist()) if not ok]
         if refused:
             raise OutOfPages(f"rows {refused[:8]} were not forked: not empty, or no page of {self.paged.pages}", refused, self.next_tokens.clone())

@@ -470,7 +470,8 @@ void bind_paged(py::module_& m) {
     const int win = (int)std::min<int64_t>(window, 1ll << 30);
     const int max_len = (int)std::min<int64_t>(table.size(1) * pool.page_size, paged::kMaxLen);
     need(B * (int64_t)paged::units_of(win > 0 && win < max_len ? win : max_len, 16) <= paged::kMaxUnits, "paged_attention: a table for over 2^34 positions");
-    const bool shared = groups.has_value() && paged::shared_pays(B, win > 0 && win < max_len ? win : max_len, pool.heads, pool.dim, (int)k.element_size());
+    const bool shared = groups.has_value() && paged::shared_pays(B, win > 0 && win < max_len ? win : max_len, pool.heads, pool.dim, (int)k.element_size()) &&
+                        paged::shared_fits(B, pool.heads, (int)(H / pool.heads), max_len, pool.dim);
     const size_t bytes = shared ? shared_attention_workspace_bytes((int)B, (int)H, pool.dim, sms)
                                 : paged_attention_workspace_bytes((int)B, (int)H, pool.heads, pool.dim, max_len, win, sms);
     if (workspace.has_value()) need(workspace->nbytes() >= bytes, "workspace too small (paged_attention_workspace_bytes)");

@@ -54,8 +54,8 @@ constexpr uint32_t kErrWait = 0x5a;
 template <int D>
 struct Shape {
   static constexpr int kStreams = D <= 128 ? 2 : 1;          // tiles of 128 queries at a time
-  static constexpr int kTile = D <= 128 ? 128 : 64;          // positions of a tile
-  static constexpr int kQueries = 128 * kStreams;
+  static constexpr int kTile = tile_positions(D), kQueries = tile_queries(D);
+  static_assert(kQueries == 128 * kStreams, "a tile of queries for each stream");
   static constexpr int kSlot = kTile * D * 2;                // bytes of a tile's keys, or values
   static constexpr int kSlots = D == 64 ? 8 : 4;             // keys and values in turn
   static constexpr int kQ = 128 * D * 2;
@@ -1030,7 +1030,6 @@ template <int D, typename T, bool kE4M3>
 cudaError_t launch(Params p, char* workspace, int sms, cudaStream_t stream) {
   using L = Shape<D>;
   const long long most = most_units(p.a.rows, p.pool.heads, p.group, p.max_len, L::kTile, L::kQueries);
-  if (most > kMaxSharedUnits) return cudaErrorInvalidValue;
   p.max_units = (int)most;
   p.ctas = (int)std::min<long long>(sms, (most + kLeastUnits - 1) / kLeastUnits);
   const Workspace w(p.a.rows, p.a.heads, D, p.ctas);
@@ -1070,6 +1069,9 @@ cudaError_t launch_shared_attention(const PagedAttention& a, PagedType type, con
   if (a.rows < 1 || a.rows > kPagedMaxRows || pool.heads < 1 || pool.heads > 65535 || a.heads % pool.heads != 0 || a.heads < pool.heads || type == PAGED_E4M3 ||
       (cache != PAGED_E4M3 && cache != type))
     return cudaErrorInvalidValue;
+  const long long cap = (long long)a.width * pool.page_size;
+  const int max_len = (int)(cap < kMaxLen ? cap : kMaxLen);
+  if (!shared_fits(a.rows, pool.heads, a.heads / pool.heads, max_len, pool.dim)) return cudaErrorInvalidValue;
   Params p = {};
   p.a = a;
   p.pool = pool;
@@ -1078,8 +1080,7 @@ cudaError_t launch_shared_attention(const PagedAttention& a, PagedType type, con
   p.starts = groups.starts;
   p.shared = groups.shared;
   p.group = a.heads / pool.heads;
-  const long long cap = (long long)a.width * pool.page_size;
-  p.max_len = (int)(cap < kMaxLen ? cap : kMaxLen);
+  p.max_len = max_len;
   const Steps st = steps_of(pool.pages, pool.page_size, pool.page_stride, pool.pos_stride, cache == PAGED_E4M3 ? 1 : 2);
   if (st.bytes == 0) return cudaErrorInvalidValue;
   p.page_step = st.page;

@@ -57,5 +57,14 @@ inline long long most_units(long long rows, int kv_heads, int group, long long p
   return 2 * rows * kv_heads * ((group + most - 1) / most) * (kItemStart + kPairUnits * ((positions + tile - 1) / tile));
 }
 
+// Tiles of a head size: positions, and (row, query head) pairs that an item takes at most (tensor memory and shared memory hold two tiles of 128
+// queries for heads of up to 128, one for 256).
+PENNY_ATTN_HD constexpr int tile_positions(int dim) { return dim <= 128 ? 128 : 64; }
+PENNY_ATTN_HD constexpr int tile_queries(int dim) { return dim <= 128 ? 256 : 128; }
+// Whether the line of a batch whose tables hold `positions` a row can be counted, and its heads be a grid's; others are read each row by itself.
+inline bool shared_fits(long long rows, int kv_heads, int group, long long positions, int dim) {
+  return kv_heads <= 65535 && most_units(rows, kv_heads, group, positions, tile_positions(dim), tile_queries(dim)) <= kMaxSharedUnits;
+}
+
 }  // namespace paged
 }  // namespace penny

@@ -434,6 +434,9 @@ void penny_shared_row(int length, int shared, int max_len, int window, int* of_g
 long long penny_shared_most_units(long long rows, int kv_heads, int group, long long positions, int tile, int most) {
   return penny::paged::most_units(rows, kv_heads, group, positions, tile, most);
 }
+int penny_shared_fits(long long rows, int kv_heads, int group, long long positions, int dim) {
+  return penny::paged::shared_fits(rows, kv_heads, group, positions, dim);
+}
 // Tile -> (row block, column block) of the persistent GEMM kernels; pair_rank < 0
 // selects the single-CTA kernel, 0 / 1 the CTA of a pair.  Returns the number of
 // tiles (pair tiles) of the grid.

@@ -244,3 +244,10 @@ def shared_most_units(rows: int, kv_heads: int, group: int, positions: int, tile
     f = sim_lib().penny_shared_most_units
     f.restype, f.argtypes = ctypes.c_longlong, [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
     return f(rows, kv_heads, group, positions, tile, most)
+
+
+def shared_fits(rows: int, kv_heads: int, group: int, positions: int, dim: int) -> bool:
+    """Whether the kernel for shared pages can take tables of so many positions a row (csrc/paged_shared_plan.h)."""
+    f = sim_lib().penny_shared_fits
+    f.restype, f.argtypes = ctypes.c_int, [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, ctypes.c_int]
+    return bool(f(rows, kv_heads, group, positions, dim))

@@ -17,3 +17,11 @@ def test_every_position_once(max_len):
         assert schedule.shared_row(n, n, 8192, n) == ((0, n), (n, n))
         assert schedule.shared_row(n + 1, n, 8192, n)[1] == (1, n + 1) and schedule.shared_row(n, n, 8192, n - 1)[1] == (1, n)
     assert schedule.shared_row(2 ** 31 - 1, 2 ** 31 - 1, max_len, 0) == ((0, 0), (0, max_len))
+
+
+def test_tables_that_the_line_cannot_hold():
+    for rows, heads, group, positions, dim in ((1024, 32, 1, 1 << 20, 128), (64, 8, 4, 8192, 128), (8192, 8, 4, 2 ** 31 - 65536, 64), (8192, 1, 200, 400, 256), (300, 2, 7, 1 << 17, 64)):
+        tile, most = (128, 256) if dim <= 128 else (64, 128)
+        assert schedule.shared_fits(rows, heads, group, positions, dim) == (schedule.shared_most_units(rows, heads, group, positions, tile, most) <= 1 << 30)
+    assert not schedule.shared_fits(1024, 32, 1, 1 << 20, 128) and schedule.shared_fits(1024, 32, 1, 1 << 19, 128)
+    assert not schedule.shared_fits(1, 65536, 1, 16, 64)  # (heads are a dimension of a grid)

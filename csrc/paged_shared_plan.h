@@ -33,11 +33,18 @@ PENNY_ATTN_HD Tiles piece_of(int begin, int tiles, bool pair, int share, int cta
 }
 PENNY_ATTN_HD int cta_of(int begin, int tile, bool pair, int share) { return (begin + kItemStart + tile * (pair ? kPairUnits : kTileUnits)) / share; }
 // Whether a batch whose rows can see `positions` each is worth the shared kernel's tiles.  The one that reads every row by itself finds what they
-// share in L2, and needs no time to start tensor cores: us with / without, of bytes for all rows, 32 of 8 heads of 128: 138 MB 25 / 20, 167 30 /
-// 22, 543 36 / 49, 554 38 / 51, 2174 48 / 165; e4m3 272 MB 41 / 39 and 44 / 41, 1087 55 / 131; 20 of 20 of 64, fp16: 170 MB 29 / 24, 173 21 / 25, 209 30 / 28,
-// 679 31 / 71; 4 of 1: 272 MB 51 / 30.  (The lengths are on the device; a table's width says what they can be.)
+// share in L2, and needs no time to start tensor cores.  What decides is how much the rows hold and share, which only the device knows;
+// by what they can hold, the shared kernel's time over the other's (16 / 64 / 200 rows full of positions, 94 % of them shared; `-`: not timed):
+//   heads                 275 MB             350                430                520                620                800                1100
+//   32 of 8 of 128 bf16   1.05 1.23 1.95     0.92 1.07 1.65     0.86 0.92 1.45     0.77 0.82 1.29     0.72 0.83 1.03     0.65 0.69 0.94     0.59 0.60 0.75
+//   the same e4m3         1.16 1.30 1.86     1.01 1.13 1.56     0.93 0.96 1.35     0.87 0.86 1.16     0.81 0.82 0.93     0.78 0.67 1.04     0.69 0.58 0.84
+//   4 of 1 of 128 bf16    2.39 1.29 1.22     2.06 1.15 1.08     1.81 1.04 0.99     1.62 0.97 0.86     -    0.85 0.84     -    0.73 0.68     -    0.62 0.58
+//   28 of 2 of 128 e4m3   2.46 1.77 1.39     1.91 1.51 1.14     1.78 1.40 1.10     1.63 1.25 0.97     -    1.11 0.89     -    1.01 0.82     -    0.81 0.69
+//   8 of 1 of 256 bf16    2.87 1.42 1.29     2.51 1.31 1.14     2.22 1.18 1.03     2.01 1.08 0.95     1.73 0.98 0.87     1.49 0.85 0.75     1.20 0.74 0.67
+//   20 of 20 of 64 fp16   0.82 0.92 -        0.77 0.79 2.23     0.68 0.69 1.77     0.65 0.59 1.58     0.58 0.51 1.33     0.54 0.56 1.07     0.50 0.45 0.81
+// With 80 % shared 0.8 to 1.4 at 1100 MB, with 30 % 1.1 to 3.1 at any size: a row's own positions take longer here, so such rows go without groups.
 inline bool shared_pays(long long rows, long long positions, int kv_heads, int dim, int value_bytes) {
-  return rows * positions * kv_heads * dim * 2 * value_bytes > 256ll << 20;
+  return rows * positions * kv_heads * dim * 2 * value_bytes > 512ll << 20;
 }
 // A row takes what its group shares, the group's first `shared` positions, if it sees all of it; one whose window leaves some out, or that was cut
 // back since, reads what it sees by itself.  (A weight of zero does not take a value that is not finite out of a product.)

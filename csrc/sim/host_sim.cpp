@@ -434,6 +434,9 @@ void penny_shared_row(int length, int shared, int max_len, int window, int* of_g
 long long penny_shared_most_units(long long rows, int kv_heads, int group, long long positions, int tile, int most) {
   return penny::paged::most_units(rows, kv_heads, group, positions, tile, most);
 }
+int penny_shared_pays(long long rows, long long positions, int kv_heads, int dim, int value_bytes) {
+  return penny::paged::shared_pays(rows, positions, kv_heads, dim, value_bytes);
+}
 int penny_shared_fits(long long rows, int kv_heads, int group, long long positions, int dim) {
   return penny::paged::shared_fits(rows, kv_heads, group, positions, dim);
 }

@@ -149,9 +149,13 @@ def paged_attention(q, k, v, table, lengths, out=None, lse=None, scale: Optional
     it reads only q and the keys and values of each row's last position; the other rows, lengths and table are then read before they end.
 
     groups: `page_groups` of this table and these lengths, or of a time since when the rows of its groups have kept the pages that they
-    share: what a group shares is read once for all its rows, on tensor cores, instead of once for each, where the rows can see over 256 MB of keys
-    and values together by the table's width (under that, reading each row by itself takes less time).  The result is the same but for the
-    order of sums.  At most 8192 rows; the workspace is that of groups=True.  A wait of the kernel that ran
+    share: what a group shares is read once for all its rows, on tensor cores, instead of once for each.  For rows that hardly differ: a row's own
+    positions take longer than without groups.  At 1 GB of keys and values (every row's counted) it takes 0.45 to 0.85 of the time without
+    groups where 94 % of the positions are shared, 0.8 to 1.2 (e4m3: 1.0 to 1.4) with 80 %, 1.1 to 3 with 30 %, and 1.3 where 64 rows of 2048 share nothing.
+    The kernel is chosen by the table's width alone: where rows cannot see over 512 MB together, or the tables are more than it can count, each
+    row is read by itself, and a table much wider than its rows (64 rows of 212 positions in one for 2560: 37 us, without groups 15) takes the longer
+    way.  At most 8192 rows; the workspace is that of groups=True.  Weights of 16-bit caches are rounded to q's type against a base that may lag behind the
+    maximum: a bf16 output is then 0.0023 of its norm from 64 bits, without groups 0.0019 (its own rounding is 0.0017).  A wait of the kernel that ran
     out (4 s) leaves its rows undone and shows in `gemm_error`."""
     return ops.paged_attention(q, k, v, table, lengths, out, lse, scale, window, k_scale, v_scale, workspace, early, groups)
 

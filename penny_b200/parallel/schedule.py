@@ -251,3 +251,10 @@ def shared_fits(rows: int, kv_heads: int, group: int, positions: int, dim: int) 
     f = sim_lib().penny_shared_fits
     f.restype, f.argtypes = ctypes.c_int, [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, ctypes.c_int]
     return bool(f(rows, kv_heads, group, positions, dim))
+
+
+def shared_pays(rows: int, positions: int, kv_heads: int, dim: int, value_bytes: int) -> bool:
+    """Whether rows that can see so many positions take the kernel for shared pages (csrc/paged_shared_plan.h)."""
+    f = sim_lib().penny_shared_pays
+    f.restype, f.argtypes = ctypes.c_int, [ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_int]
+    return bool(f(rows, positions, kv_heads, dim, value_bytes))

@@ -25,3 +25,12 @@ def test_tables_that_the_line_cannot_hold():
         assert schedule.shared_fits(rows, heads, group, positions, dim) == (schedule.shared_most_units(rows, heads, group, positions, tile, most) <= 1 << 30)
     assert not schedule.shared_fits(1024, 32, 1, 1 << 20, 128) and schedule.shared_fits(1024, 32, 1, 1 << 19, 128)
     assert not schedule.shared_fits(1, 65536, 1, 16, 64)  # (heads are a dimension of a grid)
+
+
+def test_what_is_read_each_row_by_itself():
+    """Sizes at which the kernel for shared pages was timed on both sides: us with / without."""
+    for rows, positions, kv_heads, dim, size, pays in ((64, 8292, 1, 128, 2, False),   # 50.5 / 30.2
+                                                       (16, 8292, 8, 128, 1, False), (64, 2112, 8, 128, 1, False), (64, 2548, 8, 128, 1, False),  # 64.7 / 47.5
+                                                       (16, 8292, 8, 128, 2, True), (64, 2112, 8, 128, 2, True), (64, 8292, 8, 128, 2, True),  # 48.1 / 164.9
+                                                       (64, 8292, 8, 128, 1, True), (16, 8292, 20, 64, 2, True), (4, 220, 1, 128, 2, False)):
+        assert schedule.shared_pays(rows, positions, kv_heads, dim, size) == pays, (rows, positions)

@@ -4,7 +4,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged_shared import BF, F8, HALF, Case
+from test_gpu_paged_shared import BF, F8, HALF
+from test_gpu_paged_shared_wide import Wide
 
 pytestmark = pytest.mark.gpu
 
@@ -14,7 +15,7 @@ pytestmark = pytest.mark.gpu
 def test_base_that_moves_behind_half_a_tile(cache, heads, kv_heads, dim):
     """In every tile of 128 positions the second half has a score so far above all in front of it that their weights are scaled; the values
     of the first half are larger, so that what was scaled counts beside what was not."""
-    case = Case([(0, 512, n) for n in (1, 100, 400)] + [(None, 0, 500)], heads, kv_heads, dim, 16, cache, seed=dim, spread=1.0)
+    case = Wide([(0, 512, n) for n in (1, 100, 400)] + [(None, 0, 500)], heads, kv_heads, dim, 16, cache, seed=dim, spread=1.0)
     g = torch.Generator(device="cuda").manual_seed(dim)
     unit = 0.02 if cache == F8 else 1.0
     if cache == F8:

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from test_gpu_paged_shared import BF, F8, HALF, Case
+from test_gpu_paged_shared import BF, F8, HALF
+from test_gpu_paged_shared_wide import Wide
 
 pytestmark = pytest.mark.gpu
 
@@ -11,7 +12,7 @@ pytestmark = pytest.mark.gpu
 def test_rows_that_end_with_what_they_share(heads, kv_heads, dim, shared, rows, cache):
     """Rows cut back to what they share, or near to it, under windows of about as many positions; others that are longer.  (So many that the
     kernel for shared pages is what runs.)"""
-    case = Case([(0, shared, 16 + 40 * (i % 30)) for i in range(rows)] + [(None, 0, 200)], heads, kv_heads, dim, 16, cache, seed=shared, spread=0.5)
+    case = Wide([(0, shared, 16 + 40 * (i % 30)) for i in range(rows)] + [(None, 0, 200)], heads, kv_heads, dim, 16, cache, seed=shared, spread=0.5)
     groups, full = case.groups(), case.lengths.clone()
     case.table = torch.cat([case.table, torch.full((len(full), 200), -1, device="cuda", dtype=torch.int32)], 1)
     kind = torch.arange(len(full), device="cuda") % 3

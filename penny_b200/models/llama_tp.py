@@ -553,19 +553,24 @@ class LlamaTPDecoder:
         if refused:
             raise OutOfPages(f"rows {refused[:8]} were not forked: not empty, or no page of {self.paged.pages}", refused, self.next_tokens.clone())
 
-    def logprobs(self, top: int = 0):
-        """`ops.token_logprobs` of the tokens that the last step chose (self.next_tokens), under the whole vocabulary's softmax."""
+    def logprobs(self, top: int = 0, tokens: Optional[torch.Tensor] = None):
+        """`ops.token_logprobs` under the last step's logits, of the whole vocabulary: of the tokens that the step chose (self.next_tokens), or of
+        those that the caller means to take next (tokens [batch] int64).  On several ranks all call it, each with the whole result."""
         from ..ops.logprobs import token_logprobs
+        if tokens is None:
+            tokens = self.next_tokens
+        elif tokens.dtype != torch.int64 or tokens.shape != (self.B,):
+            raise ValueError(f"logprobs: tokens [{self.B}] int64")
         logits = self.logits
         if self.world > 1:  # (the ranks' shards of the vocabulary side by side)
+            every = torch.empty(self.world * self.B, self.V, dtype=logits.dtype, device=self.dev)
             if self.backend == "nccl":
                 import torch.distributed as dist
-                every = torch.empty(self.world * self.B, self.V, dtype=logits.dtype, device=self.dev)
                 dist.all_gather_into_tensor(every, logits, group=self.pg)
             else:
-                every = self.comm.all_gather(logits)
+                self.comm.all_gather(logits, out=every)
             logits = every.view(self.world, self.B, self.V).transpose(0, 1).reshape(self.B, self.world * self.V)
-        return token_logprobs(logits, self.next_tokens, top)
+        return token_logprobs(logits, tokens.to(self.dev).contiguous(), top)
 
     def step_device(self):
         """One decode step on the device buffers: self.tokens -> self.next_tokens."""

@@ -413,25 +413,25 @@ __global__ void __launch_bounds__(kWarps * 32, kWarpsOfSm / kWarps) k_token_logp
 }
 
 template <typename T, bool kTop>
-cudaError_t launch(const TokenLogprobs& a, cudaStream_t stream) {
+cudaError_t launch(const TokenLogprobs& a, int sms, cudaStream_t stream) {
   // Many rows: a CTA of eight warps each, four to an SM, so that some read while others sort.  Few: sixteen warps and as many CTAs of a row
   // as the SMs hold, each with 4096 values at least (64 rows of 128256, top 20: 13 us, with eight warps 17).
-  const bool few = a.rows <= 3 * 148;
+  const bool few = a.rows <= 3 * sms;
   int cluster = 1;
-  while (few && cluster < kMaxCluster && a.rows * cluster * 2 <= 2 * 148 && a.vocab / (cluster * 2) >= 4096) cluster *= 2;
+  while (few && cluster < kMaxCluster && a.rows * cluster * 2 <= 2 * sms && a.vocab / (cluster * 2) >= 4096) cluster *= 2;
   return few ? launch_kernel_ex(k_token_logprobs<T, kTop, 16>, dim3((unsigned)(a.rows * cluster)), dim3(512), 0, stream, true, cluster, a, cluster)
              : launch_kernel_ex(k_token_logprobs<T, kTop, 8>, dim3((unsigned)a.rows), dim3(256), 0, stream, true, 1, a, 1);
 }
 
 }  // namespace
 
-cudaError_t launch_token_logprobs(const TokenLogprobs& a, LogitType type, cudaStream_t stream) {
+cudaError_t launch_token_logprobs(const TokenLogprobs& a, LogitType type, int sms, cudaStream_t stream) {
   if (a.rows < 0 || a.vocab < 1 || a.vocab > (1 << 30) || a.top < 0 || a.top > kLogprobsMaxTop || a.top > a.vocab) return cudaErrorInvalidValue;
   if (a.rows == 0) return cudaSuccess;
   switch (type) {
-    case LOGITS_BF16: return a.top > 0 ? launch<__nv_bfloat16, true>(a, stream) : launch<__nv_bfloat16, false>(a, stream);
-    case LOGITS_FP16: return a.top > 0 ? launch<__half, true>(a, stream) : launch<__half, false>(a, stream);
-    default: return a.top > 0 ? launch<float, true>(a, stream) : launch<float, false>(a, stream);
+    case LOGITS_BF16: return a.top > 0 ? launch<__nv_bfloat16, true>(a, sms, stream) : launch<__nv_bfloat16, false>(a, sms, stream);
+    case LOGITS_FP16: return a.top > 0 ? launch<__half, true>(a, sms, stream) : launch<__half, false>(a, sms, stream);
+    default: return a.top > 0 ? launch<float, true>(a, sms, stream) : launch<float, false>(a, sms, stream);
   }
 }
 

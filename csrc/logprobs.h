@@ -17,6 +17,6 @@ struct TokenLogprobs {
   long long* top_ids;
   int rows, vocab, top;
 };
-cudaError_t launch_token_logprobs(const TokenLogprobs& a, LogitType type, cudaStream_t stream);
+cudaError_t launch_token_logprobs(const TokenLogprobs& a, LogitType type, int sms, cudaStream_t stream);
 
 }  // namespace penny

@@ -34,8 +34,11 @@ void bind_logprobs(py::module_& m) {
     const at::Tensor top_ids = at::detail::empty_cuda({R, top}, at::kLong, logits.device(), c10::nullopt);
     const TokenLogprobs a = {logits.data_ptr(), logits.stride(0), (const long long*)tokens.data_ptr<int64_t>(), both.data_ptr<float>(),
                              both.data_ptr<float>() + R, top_logprobs.data_ptr<float>(), (long long*)top_ids.data_ptr<int64_t>(), (int)R, (int)V, (int)top};
-    const cudaError_t rc = launch_token_logprobs(a, t == at::kBFloat16 ? LOGITS_BF16 : t == at::kHalf ? LOGITS_FP16 : LOGITS_FP32,
-                                                 at::cuda::getCurrentCUDAStream().stream());
+    int sms = 0;
+    cudaError_t rc = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, logits.get_device());
+    if (rc == cudaSuccess)
+      rc = launch_token_logprobs(a, t == at::kBFloat16 ? LOGITS_BF16 : t == at::kHalf ? LOGITS_FP16 : LOGITS_FP32, sms,
+                                 at::cuda::getCurrentCUDAStream().stream());
     TORCH_CHECK(rc == cudaSuccess, "penny: token_logprobs: ", cudaGetErrorString(rc));
     return std::make_tuple(both[0], both[1], top_logprobs, top_ids);
   }, py::arg("logits"), py::arg("tokens"), py::arg("top") = 0);

@@ -1,8 +1,10 @@
 // Log probabilities of given tokens under the softmax of their logits, its entropy, and its likeliest tokens.
 //
-// With m = max x, Z = sum exp(x - m):  log p(t) = x_t - m - log Z,  entropy = log Z - (sum exp(x - m) (x - m)) / Z.
-// One pass over the logits: every thread keeps the two sums (fp32) against a maximum that it has seen, and scales them when it meets one that
-// is e^8 times as likely; threads, warps and the CTAs of a row's cluster are joined by the same rule.  The sums are taken of x - m and not of x, so that an
+// With m a logit of the row, Z = sum exp(x - m):  log p(t) = x_t - m - log Z,  entropy = log Z - (sum exp(x - m) (x - m)) / Z.
+// One pass over the logits: every thread keeps the two sums (fp32) against the largest of its first values, or one that it has met since
+// and that is over e^8 times as likely, and scales them then; threads, warps and the CTAs of a row's cluster are joined against the larger of two.  So
+// m is the row's largest logit or one up to 8 below it.  (No log p is above zero for that, nor an entropy below: where m is not the largest, it keeps
+// every p under 1 / (1 + e^-8), far more than two roundings from one.)  The sums are taken of x - m and not of x, so that an
 // fp32 logit loses nothing against a far maximum.
 //
 // The likeliest tokens are found in the same pass.  Of a CTA's first values the largest ones of 64 groups of lanes are ranked: at least

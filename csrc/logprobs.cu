@@ -16,8 +16,12 @@
 //
 // Few rows: a row's cluster has up to eight CTAs, whose sums and lists meet in the first one's shared memory.
 //
-// Many rows are bound by instructions and exponentials, near the copy rate: 2047 rows of 128256 in bf16 101 us (5.2 TB/s), with the 20 likeliest
-// 145; 1000 in fp32 87 (5.9 TB/s).  Few by latency: 64 rows 8.6 us, with the 20 likeliest 13.5; one 4.8.
+// Many rows: 2047 of 128256 in bf16 100 us in a graph (5.2 TB/s), 113 called one after another; with the 20 likeliest 145; 1000 in fp32 87 (5.9 TB/s).
+// No pipe is at its bound (1480 rows: issue slots 71 % of active cycles, exponentials' pipe 59 %, ALU 48 %, HBM 4.8 TB/s; warps wait for fixed latencies, for
+// each other and for loads in equal parts; with the likeliest tokens as much for barriers).  Few by latency: 64 rows 8.6 us, with the 20 likeliest
+// 13.5; one 4.8.
+// A vector with minus infinity in it goes value by value: with a tenth of the tokens left 2047 rows take 379 us, the 20 likeliest 407.  Where so few are left
+// that groups of lanes have none, there is no bound, and all of the row comes on the list, which runs over: ten tokens left, 20 likeliest, 1175 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>

@@ -16,7 +16,9 @@
 //
 // All but the copy are latency: a few reads one after another, prefix sums, barriers.  One CTA for a small state, a cluster of up
 // to sixteen for a large one: 64 forks of 62 pages each and their leaving 17 us (fork 8 of 12 pages 5), 600 pages moved together 5.5 (and 78 for 143
-// copies in 48 pools, 5.6 TB/s), groups of 64 rows 7.4, of 4000 25.
+// copies in 48 pools, 5.6 TB/s), groups of 64 rows 7.4, of 4000 25 (one CTA sorts, the others have returned).
+// Copies of small pages are held up by the index arithmetic of their vectors: 1000 of 4 KB in 48 pools 5.2 TB/s with 63 % of the issue slots used, warps waiting
+// for fixed latencies more than for loads.
 #include "kernel_setup.h"
 #include "paged_kernels.h"
 #include "paged_plan.h"
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(kThreads) k_page_compact(const PageCompact a, 
 }
 
 // A CTA takes pieces of a page, or the same page of `group` pools where pages are small; (copy, pools, piece) in a line, the pools of a copy one
-// behind the other.  (A pool of small pages, one by one, 880 GB/s, so 4000.)
+// behind the other.  (A pool of small pages, one by one, 880 GB/s, so 4000; 48 pools 5200.)
 constexpr int kCopyThreads = 256, kAhead = 8, kPiece = kCopyThreads * kAhead;  // vectors of 16 bytes
 __global__ void __launch_bounds__(kCopyThreads) k_page_copy(const __grid_constant__ PageCopy a, int pieces, int group) {
   pdl_launch_dependents();

@@ -14,7 +14,7 @@
 //   * Keys and values are staged by TMA, boxes of 8 to 32 positions of a page; a warp zeroes what values of a tile lie behind its ends (stale
 //     rows may hold NaN).  Pages of no multiple of 8 positions come by cp.async, 16 bytes at a time through a list of places, which
 //     any page size and strides will do for.  e4m3 pages are converted on the way to fp16, which is exact, and bf16 queries meet them as fp16 times
-//     a power of two (four conversions for a pair of values in place of one were the bound: 91 us for 130 rows of nine prompts).
+//     a power of two (four conversions for a pair of values in place of one were the bound).
 //   * All items (a KV head of a group, or of a row) lie in a line that is cut into equal shares, a CTA to an SM
 //     (paged_shared_plan.h).  A warp walks the line and hands the pieces to the others; loads run ahead across pieces.  Pieces leave unnormalised
 //     fp32 outputs in a workspace, a second kernel joins them.  No counters: a workspace holds nothing between calls.
@@ -24,8 +24,9 @@
 //     roundings of many weights leave, about one of its own.
 //
 // Bound by chains of waits, not by a pipe: a tile of 128 positions of two times 128 queries takes 4200 clocks, 2050 of softmax and 1600 of products
-// that wait for each other, in two streams; one of a row's own positions 2600.  64 rows of 4000 shared and 300 own positions, 32 of 8 heads of 128,
-// bf16, 55 us; 100 of 16000 and 500 97; 130 of nine prompts, e4m3, 89.
+// that wait for each other, in two streams; one of a row's own positions 2600, with a row's few queries of 128.  64 rows of 4000 shared and 300 own
+// positions, 32 of 8 heads of 128, bf16, 56 us called one after another and 55 in a graph; 100 of 16000 and 500 104 and 97; 130 of nine prompts, e4m3,
+// 93 and 89 (each row by itself 91); 64 of 2048 that share nothing 107 (each by itself 84).
 //
 // Every wait is bounded; one that ran out sets the error word that all tcgen05 kernels here share, and the CTA ends.
 #include <cuda_bf16.h>

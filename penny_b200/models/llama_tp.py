@@ -88,7 +88,9 @@ class LlamaTPDecoder:
         of max_len), of cache_dtype (bf16 or e4m3; cache_scales: its (k_scale, v_scale), as PagedKVCache takes them).  `positions` are
         that cache's lengths then; every step lets one token come to every
         row.  A row for which there is no page is left out of a step, which raises OutOfPages when it has waited for the device.
-        sharing: rows may be forked (`fork`); a step finds the rows that have pages in common and reads those once."""
+        sharing: rows may be forked (`fork`); a step finds the rows that have pages in common and reads those once, if rows of max_len would hold
+        over 512 MB of keys and values a layer.  That pays for rows that share most of what they hold: 64 rows of 2048 positions, max_len 2560, 8 layers, a step
+        1577 us without sharing, 1227 with all forked from one, 1823 with none forked; of 500 positions 1121, 1223 and 1281."""
         if page_size < 0 or (page_size == 0 and (pages is not None or cache_dtype is not None or cache_scales is not None or sharing)):
             raise ValueError("pages, cache_dtype, cache_scales and sharing belong to a cache in pages: page_size above 0")
         if cache_dtype not in (None, torch.bfloat16, torch.float8_e4m3fn):

@@ -44,7 +44,7 @@ PENNY_ATTN_HD int cta_of(int begin, int tile, bool pair, int share) { return (be
 //   20 of 20 of 64 fp16   0.82 0.92 -        0.77 0.79 2.23     0.68 0.69 1.77     0.65 0.59 1.58     0.58 0.51 1.33     0.54 0.56 1.07     0.50 0.45 0.81
 // With 80 % shared 0.8 to 1.4 at 1100 MB, with 30 % 1.1 to 3.1 at any size: a row's own positions take longer here, so such rows go without groups.
 inline bool shared_pays(long long rows, long long positions, int kv_heads, int dim, int value_bytes) {
-  return rows * positions * kv_heads * dim * 2 * value_bytes > 512ll << 20;
+  return (double)rows * positions * kv_heads * dim * 2 * value_bytes > 512ll << 20;  // (heads of stride zero: more than 64 bits hold)
 }
 // A row takes what its group shares, the group's first `shared` positions, if it sees all of it; one whose window leaves some out, or that was cut
 // back since, reads what it sees by itself.  (A weight of zero does not take a value that is not finite out of a product.)

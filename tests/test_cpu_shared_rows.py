@@ -34,3 +34,6 @@ def test_what_is_read_each_row_by_itself():
                                                        (16, 8292, 8, 128, 2, True), (64, 2112, 8, 128, 2, True), (64, 8292, 8, 128, 2, True),  # 48.1 / 164.9
                                                        (64, 8292, 8, 128, 1, True), (16, 8292, 20, 64, 2, True), (4, 220, 1, 128, 2, False)):
         assert schedule.shared_pays(rows, positions, kv_heads, dim, size) == pays, (rows, positions)
+    # (the bound itself, and more bytes than 64 bits hold: heads may be one head's memory)
+    assert not schedule.shared_pays(64, 2048, 8, 128, 2) and schedule.shared_pays(64, 2049, 8, 128, 2)
+    assert schedule.shared_pays(8192, 2 ** 31 - 65536, 2 ** 19, 256, 2) and schedule.shared_pays(8192, 2 ** 30, 2 ** 13, 256, 2)
